@@ -18,7 +18,8 @@ _PUBLIC = {
     "GaussianStore": "retinags_b200.models.gaussians", "GaussianModel": "retinags_b200.models.gaussian_model",
     "Scene": "retinags_b200.scene", "render": "retinags_b200.gaussian_renderer", "StepEngine": "retinags_b200.engine",
     "Trainer": "retinags_b200.trainer", "BvhTree": "retinags_b200.parallel.partition", "Camera": "retinags_b200.data.cameras",
-    "ViewerServer": "retinags_b200.viewer_server",
+    "ViewerServer": "retinags_b200.viewer_server", "label_loss": "retinags_b200.ops.label_loss",
+    "layer_norm": "retinags_b200.ops.layer_norm", "pack8": "retinags_b200.ops.pack8", "Packed8": "retinags_b200.ops.pack8",
 }
 
 

@@ -18,7 +18,7 @@ ROOT = Path(__file__).resolve().parent
 CSRC = ROOT / "csrc"
 LIB = ROOT / "lib"
 
-CPU_SOURCES = ["rgs_cpu.cpp"]
+CPU_SOURCES = ["rgs_cpu.cpp", "rgs_fields_cpu.cpp"]
 CUDA_SOURCES = [
     "rgs_raster.cu",
     "rgs_sort.cu",
@@ -31,6 +31,8 @@ CUDA_SOURCES = [
     "rgs_surgery.cu",
     "rgs_ssim_tc.cu",
     "rgs_noalloc.cu",
+    "rgs_label.cu",
+    "rgs_norm.cu",
 ]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

@@ -1,0 +1,114 @@
+"""Softmax cross entropy of linear scores against a vocabulary of labels, without the scores in memory.
+
+The loss of a label field: rendered features (..., C) are scored against V labels (classes, instances, entries of a
+codebook) by ``features @ weight.T + bias``.  At 1600 x 1036 pixels the scores of 1024 labels are 6.8 GB in 32 bits;
+the kernels (``csrc/rgs_label.cu``) walk the vocabulary in pieces, keep two numbers per pixel for the backward pass
+(the largest score and the logarithm of the sum of exponentials below it) and compute the scores anew there.  Stands beside the photometric loss of
+``ops.loss``; the readable definition is ``utils.loss.label_loss``.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import native
+from .pack8 import DTYPES, as_rows, dtype_code
+
+MAX_CHANNELS = 1024
+_REDUCTIONS = ("mean", "sum", "none")
+_LIMIT = 2 ** 31 - 1
+
+
+def _scratch(device: torch.device, n: int, c: int, v: int, dtype: int, backward: int) -> torch.Tensor:
+    kind = "cuda" if device.type == "cuda" else "cpu"
+    fn = getattr(native.lib(kind), f"rgs_{kind}_label_scratch_bytes")
+    fn.argtypes, fn.restype = [ctypes.c_int64] * 5, ctypes.c_int64
+    with torch.cuda.device(device) if kind == "cuda" else torch.no_grad():
+        return torch.empty(int(fn(n, c, v, dtype, backward)), dtype=torch.uint8, device=device)
+
+
+class _LabelLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, features, weight, bias, labels, reduction):
+        dev = features.device
+        x, ldx, _ = as_rows(features, "label_loss", planes_ok=False)
+        w, ldw, _ = as_rows(weight, "label_loss", planes_ok=False)
+        y = labels.reshape(-1).contiguous()
+        n, c = x.shape
+        v = w.shape[0]
+        per_row = reduction == "none"
+        new = torch.empty if n else torch.zeros
+        lse = torch.empty(2, n, dtype=torch.float32, device=dev)
+        losses = torch.empty(n, dtype=torch.float32, device=dev) if per_row else None
+        result = None if per_row else new((), dtype=torch.float32, device=dev)
+        count = new(1, dtype=torch.float32, device=dev)
+        b_code = DTYPES[bias.dtype] if bias is not None else 0
+        if n:
+            native.call("label_fwd", dev, x, ldx, w, ldw, bias, y, y.element_size(), n, c, v, DTYPES[x.dtype], b_code,
+                        int(reduction == "mean"), _scratch(dev, n, c, v, DTYPES[x.dtype], 0), lse, losses, result, count)
+        ctx.save_for_backward(x, w, bias, y, lse, count)
+        ctx.args = (tuple(features.shape), tuple(weight.shape), ldx, ldw, b_code, reduction)
+        return losses.view(features.shape[:-1]) if per_row else result
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gout):
+        x, w, bias, y, lse, count = ctx.saved_tensors
+        x_shape, w_shape, ldx, ldw, b_code, reduction = ctx.args
+        dev = x.device
+        n, c = x.shape
+        v = w.shape[0]
+        g = gout.reshape(-1).contiguous()
+        new = torch.empty if n else torch.zeros
+        dx = torch.empty(x_shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
+        dw = new(w_shape, dtype=w.dtype, device=dev) if ctx.needs_input_grad[1] else None
+        db = new(v, dtype=bias.dtype, device=dev) if ctx.needs_input_grad[2] else None
+        if n and (dx is not None or dw is not None or db is not None):
+            native.call("label_bwd", dev, x, ldx, w, ldw, bias, y, y.element_size(), n, c, v, DTYPES[x.dtype], b_code, lse, g,
+                        int(reduction == "none"), count if reduction == "mean" else None,
+                        _scratch(dev, n, c, v, DTYPES[x.dtype], 1), dx, dw, db)
+        return dx, dw, db, None, None
+
+
+def label_loss(features: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, bias: torch.Tensor | None = None,
+               reduction: str = "mean") -> torch.Tensor:
+    """Cross entropy (float32) of ``features @ weight.T + bias`` against ``labels``.
+
+    ``features`` (..., C) and ``weight`` (V, C) are float32 or bfloat16, both of one type, with C up to 1024;
+    ``labels`` (...) int64 or int32; ``bias`` (V) of the features' type or float32 (``-inf`` takes a label out).  A label
+    outside [0, V) marks a pixel without one: its loss and gradient are zero, whatever its features hold, and it does not
+    count in the mean.  ``reduction``: ``"mean"`` over the pixels that count (0 if none does), ``"sum"``, ``"none"``
+    (one loss per pixel).  Differentiable (once) in features, weight and bias.
+
+    Products of bfloat16 inputs are exact and summed in 32 bits; ``exp(score - lse) - [label]`` is rounded to bfloat16
+    for the products with features and weight.  float32 inputs go through the same tensor-core products in three
+    bfloat16 pieces each, with the results of 32-bit arithmetic.
+    """
+    code = dtype_code(features, "label_loss features")
+    if weight.dtype != features.dtype:
+        raise TypeError(f"label_loss: weight of type {features.dtype} expected, got {weight.dtype}")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"label_loss: reduction is one of {_REDUCTIONS}, got {reduction!r}")
+    if features.dim() < 1 or weight.dim() != 2 or features.shape[-1] != weight.shape[1]:
+        raise ValueError(f"label_loss: features (..., C) and weight (V, C) expected, got {tuple(features.shape)} and {tuple(weight.shape)}")
+    c, v = features.shape[-1], weight.shape[0]
+    if not 1 <= c <= MAX_CHANNELS:
+        raise ValueError(f"label_loss: 1 to {MAX_CHANNELS} channels expected, got {c}")
+    if v < 1:
+        raise ValueError("label_loss: the vocabulary is empty")
+    if labels.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"label_loss: int64 or int32 labels expected, got {labels.dtype}")
+    if labels.shape != features.shape[:-1]:
+        raise ValueError(f"label_loss: labels of shape {tuple(features.shape[:-1])} expected, got {tuple(labels.shape)}")
+    if labels.numel() > _LIMIT or v > _LIMIT:
+        raise ValueError("label_loss: at most 2^31 - 1 pixels and labels")
+    if bias is not None:
+        if bias.shape != (v,):
+            raise ValueError(f"label_loss: bias of shape ({v},) expected, got {tuple(bias.shape)}")
+        if DTYPES.get(bias.dtype, -1) not in (0, code):
+            raise TypeError(f"label_loss: bias of type {features.dtype} or float32 expected, got {bias.dtype}")
+    for name, t in (("weight", weight), ("labels", labels), ("bias", bias)):
+        if t is not None and t.device != features.device:
+            raise ValueError(f"label_loss: {name} on {features.device} expected, got {t.device}")
+    return _LabelLoss.apply(features, weight, bias.contiguous() if bias is not None else None, labels, reduction)

@@ -1,0 +1,92 @@
+"""Layer norm over the channels of rendered features, with its backward pass.
+
+Blended features are weighted sums over the splats of a pixel, so their size follows the pixel's coverage; the norm
+takes that out ahead of a classifier (``ops.label_loss``).  The input may be rows (..., C) or, as the renderer writes an
+image, channel planes (``image.permute(1, 2, 0)`` of a (C,H,W) image), both read where they lie; the output is dense
+rows in ``out_dtype``.  Sums are held in 32 bits whatever the types.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import native
+from .pack8 import DTYPES, alloc_codes, as_rows, dtype_code, empty_like_layout
+
+
+def _scratch(device: torch.device, n: int, c: int) -> torch.Tensor:
+    kind = "cuda" if device.type == "cuda" else "cpu"
+    fn = getattr(native.lib(kind), f"rgs_{kind}_norm_scratch_bytes")
+    fn.argtypes, fn.restype = [ctypes.c_int64, ctypes.c_int64], ctypes.c_int64
+    return torch.empty(int(fn(n, c)), dtype=torch.uint8, device=device)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, out_dtype, keep):
+        flat, ld, planes = as_rows(x, "layer_norm")
+        n, c = flat.shape
+        y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+        p_code = DTYPES[weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32]
+        codes = exponents = None
+        # bias alone needs no input in the backward pass
+        if keep == "int8" and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]):
+            codes, exponents = alloc_codes(x.shape, planes, x.device)
+        if n:
+            native.call("norm_fwd", x.device, flat, DTYPES[x.dtype], ld, planes, weight, bias, p_code, n, c, eps, y, DTYPES[out_dtype],
+                        codes, exponents)
+        ctx.save_for_backward(flat if codes is None else None, codes, exponents, weight)
+        ctx.layout = (tuple(x.shape), x.dtype, ld, planes, n, c, p_code, eps)
+        ctx.param_dtypes = (weight.dtype if weight is not None else None, bias.dtype if bias is not None else None)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        flat, codes, exponents, weight = ctx.saved_tensors
+        shape, x_dtype, ld, planes, n, c, p_code, eps = ctx.layout
+        dev = dy.device
+        dyf, ldy, _ = as_rows(dy, "layer_norm", planes_ok=False)
+        dx = empty_like_layout(shape, planes, x_dtype, dev) if ctx.needs_input_grad[0] else None
+        new = torch.empty if n else torch.zeros
+        dw = new(c, dtype=ctx.param_dtypes[0], device=dev) if ctx.needs_input_grad[1] else None
+        db = new(c, dtype=ctx.param_dtypes[1], device=dev) if ctx.needs_input_grad[2] else None
+        if n:
+            native.call("norm_bwd", dev, flat, DTYPES[x_dtype], ld, planes, codes, exponents, dyf, DTYPES[dyf.dtype], ldy, weight, p_code,
+                        n, c, eps, _scratch(dev, n, c), dx, dw, db)
+        return dx, dw, db, None, None, None
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
+               out_dtype: torch.dtype | None = None, keep: str = "input") -> torch.Tensor:
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension of ``x`` (..., C), as dense rows.
+
+    ``x`` and ``out_dtype`` (default: that of ``x``) are float32 or bfloat16; ``weight`` and ``bias`` (C) are of one of
+    these types, both of the same.  ``keep`` says what waits for the backward pass: ``"input"`` the tensor itself,
+    ``"int8"`` its 8-bit form (``ops.pack8``); the gradients are then those of the norm at the restored values, and the
+    input's memory is free as soon as nothing else holds it.
+    """
+    dtype_code(x, "layer_norm")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in DTYPES:
+        raise TypeError(f"layer_norm: out_dtype float32 or bfloat16 expected, got {out_dtype}")
+    if keep not in ("input", "int8"):
+        raise ValueError(f"layer_norm: keep is 'input' or 'int8', got {keep!r}")
+    if not eps >= 0.0:
+        raise ValueError(f"layer_norm: eps >= 0 expected, got {eps}")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"layer_norm: shape (..., C) with at least one channel expected, got {tuple(x.shape)}")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        dtype_code(p, f"layer_norm {name}")
+        if p.shape != (x.shape[-1],):
+            raise ValueError(f"layer_norm: {name} of shape ({x.shape[-1]},) expected, got {tuple(p.shape)}")
+        if p.device != x.device:
+            raise ValueError(f"layer_norm: {name} on {x.device} expected, got {p.device}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"layer_norm: weight and bias of one type expected, got {weight.dtype} and {bias.dtype}")
+    weight = weight.contiguous() if weight is not None else None
+    bias = bias.contiguous() if bias is not None else None
+    return _LayerNorm.apply(x, weight, bias, float(eps), out_dtype, keep)

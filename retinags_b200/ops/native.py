@@ -45,6 +45,12 @@ SIGNATURES = {
     "densify_gather": "pppiippppppiipp",
     "records_pack": "pppipiipp",
     "records_unpack": "pipppiip",
+    "label_fwd": "pipippiiiiiiipppppp",
+    "label_bwd": "pipippiiiiiippippppp" "p",
+    "norm_fwd": "piiippiiifpippp",
+    "norm_bwd": "piiipppiipiiifppppp",
+    "pack8": "piiiiippp",
+    "unpack8": "ppiiipip",
 }
 
 _CTYPE = {"p": ctypes.c_void_p, "i": ctypes.c_int64, "f": ctypes.c_double}

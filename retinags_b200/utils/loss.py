@@ -2,7 +2,7 @@
 
 Counterparts of the reference's ``utils/loss_utils.py:17-63`` (``l1_loss``, ``l2_loss``, ``ssim`` with the 11x11
 sigma-1.5 window, zero padding, C1 = 0.01^2, C2 = 0.03^2) and ``utils/image_utils.py:14-19`` (``mse``, ``psnr``).
-Training and evaluation use the fused kernels of ``csrc/rgs_loss.cu``; these are the readable definitions, the oracle
+Training and evaluation use the fused kernels of ``csrc/rgs_loss.cu`` (``csrc/rgs_label.cu`` for labels); these are the readable definitions, the oracle
 of the kernel tests, and what scripts call on arbitrary tensors (they are differentiable through autograd).
 """
 from __future__ import annotations
@@ -51,6 +51,24 @@ def mse(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
 
 def psnr(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     return 20.0 * torch.log10(1.0 / torch.sqrt(mse(a, b)))
+
+
+def label_loss(features: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, bias: torch.Tensor | None = None,
+               reduction: str = "mean") -> torch.Tensor:
+    """Cross entropy of ``features @ weight.T + bias`` (..., V) against ``labels`` (...); labels outside [0, V) do not count.
+
+    The definition of ``ops.label_loss``, with all scores in memory; computed in the features' type."""
+    x, y, v = features.reshape(-1, features.shape[-1]), labels.reshape(-1).long(), weight.shape[0]
+    counts = (y >= 0) & (y < v)
+    rows = counts.nonzero()[:, 0]
+    scores = x[rows] @ weight.t()
+    if bias is not None:
+        scores = scores + bias.to(scores.dtype)
+    loss = torch.logsumexp(scores, 1) - scores.gather(1, y[rows, None])[:, 0]
+    if reduction == "none":
+        return torch.zeros(x.shape[0], dtype=loss.dtype, device=x.device).index_put((rows,), loss).view(labels.shape)
+    total = loss.sum()
+    return total / max(rows.numel(), 1) if reduction == "mean" else total
 
 
 def training_loss(image: torch.Tensor, gt: torch.Tensor, lambda_dssim: float = 0.2) -> torch.Tensor:
