@@ -9,7 +9,7 @@ static inline int64_t field_at(int64_t n, int64_t c, int64_t ld, int64_t planes)
 extern "C" {
 
 int64_t rgs_cpu_norm_scratch_bytes(int64_t, int64_t) { return 16; }
-int64_t rgs_cpu_label_scratch_bytes(int64_t, int64_t, int64_t, int64_t, int64_t) { return 16; }
+int64_t rgs_cpu_label_scratch_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) { return 16; }
 
 int rgs_cpu_pack8(const void* x, int64_t dtype, int64_t ld, int64_t planes, int64_t n, int64_t c, int8_t* codes, uint8_t* expo, void*) {
     const int64_t blocks = (c + RGS_PACK_BLOCK - 1) / RGS_PACK_BLOCK;
@@ -149,11 +149,11 @@ int rgs_cpu_label_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, co
     return 0;
 }
 
-// gout: one gradient for all rows (per_row = 0; divided by max(count, 1) when mean) or one per row
+// gout: one gradient for all rows (per_row = 0; divided by max(count, 1) for the mean) or one per row
 int rgs_cpu_label_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* labels, int64_t label_bytes,
                       int64_t n, int64_t c, int64_t vocab, int64_t dtype, int64_t b_dtype, const float* lse, const float* gout,
-                      int64_t per_row, const float* count, void*, void* dx, void* dw, void* db, void*) {
-    const double scale = count ? 1.0 / (*count > 1.f ? *count : 1.f) : 1.0;
+                      int64_t per_row, int64_t mean, const float* count, void*, void* dx, void* dw, void* db, void*) {
+    const double scale = mean ? 1.0 / (*count > 1.f ? *count : 1.f) : 1.0;
     auto grad = [&](int64_t i, int64_t v, int64_t y) -> double {
         double l = bias ? rgs_load_as_float(bias, v, (int)b_dtype) : 0.f;
         for (int64_t j = 0; j < c; ++j)

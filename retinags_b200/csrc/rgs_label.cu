@@ -1,132 +1,1004 @@
 // Label loss: softmax cross entropy of linear scores over a vocabulary, without the scores in memory.
 //
-//   s_nv = x_n . w_v + b_v,  lse_n = log sum_v exp s_nv,  loss_n = lse_n - s_n,y_n
-//   G_nv = g_n (exp(s_nv - lse_n) - [v = y_n]),  dX = G W,  dW = G^T X,  db_v = sum_n G_nv
+//   s_nv = x_n . w_v + b_v,  m_n = max_v s_nv,  z_n = sum_v exp(s_nv - m_n),  loss_n = log z_n + (m_n - s_n,y_n)
+//   G_nv = exp(s_nv - m_n) / z_n - [v = y_n],  dX = g G W,  dW = (g G)^T X,  db_v = sum_n g_n G_nv
 //
-// First form: a warp owns a row (of X, or of W for the gradients of W and b) and walks the rows of the other matrix;
-// the scores are recomputed in the backward pass from the kept lse.
+// One persistent kernel on the fifth-generation tensor cores does all the products.  A CTA holds a tile of 128 rows of
+// one matrix (A: rows of X for the loss and dX, rows of W for dW) and walks tiles of 128 rows of the other (B):
+//   TMA brings tiles of 128 rows x 64 channels (bf16, 128-byte swizzle) into a ring in shared memory
+//   S = A B^T: tcgen05.mma into one of two score buffers in TMEM
+//   two warpgroups take the score buffers in turn (one thread per row of A: no shuffles), form the running maximum and
+//   sum (forward) or G (backward); G goes back over the scores in TMEM as a bf16 operand
+//   O += G B: tcgen05.mma with G from TMEM and the same B tile, read with its channels as the N side
+// so a B tile is fetched once for both products and the scores never leave the SM.  The gradient kernel walks the items of
+// dX and dW in one launch.  For dW the roles are swapped (rows of A are labels, columns are pixels); the scores are
+// computed anew there: five products of 2NVC operations in all against four with scores kept, and no N x V traffic.
+//
+// 32-bit inputs: every operand is split into three bf16 pieces (8 + 8 + 8 bits of mantissa) and six of the nine piece
+// products are kept; what is dropped is below 2^-24 of a product.  G is split the same way in registers.
+//
+// Bounds per 128 x 128 scores: 1024 clocks for the exponentials (16 per clock and SM), 4 C clocks for a product.
+//
+// All waits are bounded; when one runs out the CTA stops waiting, writes NaN into what it still owes and frees its TMEM.
+#include <cuda.h>
+#include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <string.h>
+#include <atomic>
 #include "rgs_cuda_common.cuh"
 #include "rgs_field_math.h"
 
-#define LB_WARPS 8
+#define LT 128                      // rows of a tile of either matrix
+#define LTILE 16384                 // bytes of a staged tile: 128 rows x 64 channels bf16
+#define LSLOTS 13                   // staged tiles in shared memory
+#define LKSLOTS 4                   // staged blocks of column constants
+#define LKBYTES 2048
+#define LTHREADS 384                // warp 0 TMA, warp 1 MMA, warp 2 TMEM, warps 4-11 two warpgroups on the scores
+#define LWAIT (1u << 20)
+#define LOG2E 1.4426950408889634f
+#define LN2 0.6931471805599453f
 
-__device__ __forceinline__ float warp_sum(float v) {
+struct LabelArgs {
+    int64_t n, v;
+    int c, nk;                       // channels, chunks of 64 channels
+    int noc, nrange;                 // chunks of output channels per item, ranges of them
+    int a_slots, b_res, ring;        // slots of resident A tiles (0: A goes through the ring), B kept for both products, ring slots
+    int nob;                         // output buffers in TMEM
+    int nmx, nmw;                    // tiles of 128 pixels, of 128 labels
+    int nsx, nsw;                    // pieces of the walk over labels (forward, dX) and over pixels (dW)
+    int64_t items_x, items_w;
+    const float* b2;                 // (nmw * 128) bias * log2 e; -inf behind the last label
+    const float* kn;                 // (nmx, 4, 128) per pixel: m * log2 e, g / z, g, label (bits); backward only
+    const float* lse;                // (2, n) m and log z, both in units of log 2
+    const void* labels; int label_bytes;
+    const float* flags;              // [1] != 0: a pixel without a label holds something that is not finite
+    float* pm; float* ps; float* at; // forward: (2 nsx, n) partial maximum and sum, (n) score of the label
+    float* part_x; float* part_w;    // (nsx, nmx*128, cq), (nsw, nmw*128, cq) when split
+    float* part_b;                   // (2 nsw, nmw*128)
+    int cq;
+    void* dx; void* dw; int dtype;
+};
+
+// ---------------------------------------------------------------------------------------------------------------------
+// PTX
+// ---------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
+__device__ __forceinline__ bool lb_wait(unsigned long long* bar, uint32_t parity, volatile int* fail) {
+    const uint32_t addr = rgs_smem_addr(bar);
+    for (uint32_t it = 0; it < LWAIT; ++it) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(addr), "r"(parity) : "memory");
+        if (ok) return true;
+        if ((it & 15u) == 15u && *fail) return false;
+    }
+    *fail = 1;
+    return false;
+}
+__device__ __forceinline__ void lb_tma(void* dst, const CUtensorMap* map, int x, int y, int z, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+                 "r"(rgs_smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(rgs_smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void lb_commit(unsigned long long* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(rgs_smem_addr(bar)) : "memory");
+}
+// shared-memory descriptors, 128-byte swizzle: rows of 64 channels, eight rows (1024 bytes) to a pattern
+__device__ __forceinline__ uint64_t lb_desc(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(1024 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void lb_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::
+                 "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void lb_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::
+                 "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+#define LB_R16(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7]), \
+    "+r"(r[o + 8]), "+r"(r[o + 9]), "+r"(r[o + 10]), "+r"(r[o + 11]), "+r"(r[o + 12]), "+r"(r[o + 13]), "+r"(r[o + 14]), "+r"(r[o + 15])
+#define LB_O16(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7]), \
+    "=r"(r[o + 8]), "=r"(r[o + 9]), "=r"(r[o + 10]), "=r"(r[o + 11]), "=r"(r[o + 12]), "=r"(r[o + 13]), "=r"(r[o + 14]), "=r"(r[o + 15])
+#define LB_I16(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7]), \
+    "r"(r[o + 8]), "r"(r[o + 9]), "r"(r[o + 10]), "r"(r[o + 11]), "r"(r[o + 12]), "r"(r[o + 13]), "r"(r[o + 14]), "r"(r[o + 15])
+
+__device__ __forceinline__ void tm_ld32(uint32_t a, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+                 "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : LB_O16(r, 0), LB_O16(r, 16) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void tm_wait_ld32(uint32_t (&r)[32]) {  // the registers pass through, so nothing reads them before
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : LB_R16(r, 0), LB_R16(r, 16)::"memory");
+}
+__device__ __forceinline__ void tm_ld16(uint32_t a, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : LB_O16(r, 0) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void tm_wait_ld16(uint32_t (&r)[16]) { asm volatile("tcgen05.wait::ld.sync.aligned;" : LB_R16(r, 0)::"memory"); }
+__device__ __forceinline__ void tm_st16(uint32_t a, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::
+                 LB_I16(r, 0), "r"(a) : "memory");
+}
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float bf_lo(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+
+// ---------------------------------------------------------------------------------------------------------------------
+// items of the persistent loop: rows of A, range of output channels, piece of the walk over B
+// ---------------------------------------------------------------------------------------------------------------------
+struct LabelItem { int dw, m, oc0, noc, split, j0, j1; };
+
+__device__ __forceinline__ LabelItem lb_item(const LabelArgs& a, int64_t i) {
+    LabelItem it;
+    it.dw = i >= a.items_x;
+    if (it.dw) i -= a.items_x;
+    const int nm = it.dw ? a.nmw : a.nmx, nj = it.dw ? a.nmx : a.nmw, ns = it.dw ? a.nsw : a.nsx;
+    it.m = (int)(i % nm);
+    i /= nm;
+    it.oc0 = (int)(i % a.nrange) * a.noc;
+    it.noc = min(a.noc, a.nk - it.oc0);
+    it.split = (int)(i / a.nrange);
+    it.j0 = (int)((int64_t)nj * it.split / ns);
+    it.j1 = (int)((int64_t)nj * (it.split + 1) / ns);
+    return it;
+}
+
+// sixteen channels of a row of the output, rounded to its type; vector stores where rows keep their alignment
+__device__ __forceinline__ void lb_store16(void* out, int64_t r, int c, int channels, int dtype, const float (&f)[16]) {
+    if (dtype == RGS_BF16) {
+        __nv_bfloat16* p = static_cast<__nv_bfloat16*>(out) + r * channels + c;
+        if ((channels & 7) == 0) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    return v;
-}
-
-__device__ __forceinline__ float row_dot(const void* a, int64_t ia, const void* b, int64_t ib, int c, int dtype, int lane) {
-    float s = 0.f;
-    for (int j = lane; j < c; j += 32) s = fmaf(rgs_load_as_float(a, ia + j, dtype), rgs_load_as_float(b, ib + j, dtype), s);
-    return warp_sum(s);
-}
-
-__global__ void __launch_bounds__(LB_WARPS * 32) rgs_label_fwd_kernel(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
-                                                                      const void* labels, int label_bytes, int64_t n, int c, int64_t vocab,
-                                                                      int dtype, int b_dtype, float* lse, float* losses) {
-    const int lane = threadIdx.x & 31;
-    for (int64_t i = (int64_t)blockIdx.x * LB_WARPS + (threadIdx.x >> 5); i < n; i += (int64_t)gridDim.x * LB_WARPS) {
-        const int64_t y = rgs_label(labels, i, label_bytes, vocab);
-        float m = -INFINITY, s = 0.f, at = 0.f;
-        for (int64_t v = 0; v < vocab; ++v) {
-            const float l = row_dot(x, i * ldx, w, v * ldw, c, dtype, lane) + (bias ? rgs_load_as_float(bias, v, b_dtype) : 0.f);
-            if (v == y) at = l;
-            if (l > m || l != l) { s *= expf(m - l); m = l; }
-            if (!(l == -INFINITY && m == -INFINITY)) s += expf(l - m);
+            for (int q = 0; q < 16; q += 8)
+                if (c + q < channels)
+                    *reinterpret_cast<uint4*>(p + q) = make_uint4(bf16x2(f[q], f[q + 1]), bf16x2(f[q + 2], f[q + 3]), bf16x2(f[q + 4], f[q + 5]), bf16x2(f[q + 6], f[q + 7]));
+        } else {
+#pragma unroll
+            for (int q = 0; q < 16; ++q)
+                if (c + q < channels) p[q] = __float2bfloat16_rn(f[q]);
         }
+    } else {
+        float* p = static_cast<float*>(out) + r * channels + c;
+        if ((channels & 3) == 0) {
+#pragma unroll
+            for (int q = 0; q < 16; q += 4)
+                if (c + q < channels) *reinterpret_cast<float4*>(p + q) = make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 16; ++q)
+                if (c + q < channels) p[q] = f[q];
+        }
+    }
+}
+
+struct LabelShared {
+    unsigned long long full[LSLOTS], empty[LSLOTS], a_full[2], a_empty[2], k_full[LKSLOTS], k_empty[LKSLOTS];
+    unsigned long long s_full[2], s_done[2], o_full[2], o_free[2], drain;
+    uint32_t tmem;
+    int fail;
+};
+#define LSMEM (1024 + LSLOTS * LTILE + LKSLOTS * LKBYTES + (int)sizeof(LabelShared))
+
+template <int P, bool GRAD>
+__global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                                                                   const __grid_constant__ LabelArgs a) {
+    constexpr int SB = P == 1 ? 128 : 192;        // TMEM columns of a score buffer (scores; over them G, its third piece behind)
+    constexpr int OUT = 2 * SB;                   // first column of the outputs
+    constexpr int OB = P == 1 ? 128 : 64;         // columns of an output buffer when there are two
+    constexpr int COMBOS = P == 1 ? 1 : 6;
+    constexpr int CA[6] = {P == 1 ? 0 : 2, 0, 1, 1, 0, 0}, CB[6] = {0, 2, 1, 0, 1, 0};  // smallest products first
+    extern __shared__ unsigned char raw[];
+    unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    float* kbuf = reinterpret_cast<float*>(tiles + LSLOTS * LTILE);
+    LabelShared* sh = reinterpret_cast<LabelShared*>(tiles + LSLOTS * LTILE + LKSLOTS * LKBYTES);
+    volatile int* fail = &sh->fail;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int na = P * a.nk;                      // tiles of one A or B row block
+    unsigned char* ring = tiles + (size_t)a.a_slots * na * LTILE;
+
+    if (tid == 0) {
+        for (int i = 0; i < LSLOTS; ++i) { rgs_mbar_init(&sh->full[i], 1); rgs_mbar_init(&sh->empty[i], 1); }
+        for (int i = 0; i < 2; ++i) {
+            rgs_mbar_init(&sh->a_full[i], 1); rgs_mbar_init(&sh->a_empty[i], 1);
+            rgs_mbar_init(&sh->s_full[i], 1); rgs_mbar_init(&sh->s_done[i], 128);
+            rgs_mbar_init(&sh->o_full[i], 1); rgs_mbar_init(&sh->o_free[i], 256);
+        }
+        for (int i = 0; i < LKSLOTS; ++i) { rgs_mbar_init(&sh->k_full[i], 1); rgs_mbar_init(&sh->k_empty[i], 128); }
+        rgs_mbar_init(&sh->drain, 1);
+        sh->fail = 0;
+        rgs_fence_mbar_init();
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(rgs_smem_addr(&sh->tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = sh->tmem;
+    const int64_t items = a.items_x + a.items_w;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------------------------------------ TMA
         if (lane == 0) {
-            const float z = logf(s);
-            lse[i] = m;
-            lse[n + i] = z;
-            losses[i] = y < 0 ? 0.f : z + (m - at);
+            uint32_t cnt = 0, kc = 0, ai = 0;
+            bool ok = true;
+            auto tile = [&](const CUtensorMap* map, int chunk, int row, int piece) {
+                const uint32_t s = cnt % a.ring;
+                ok = ok && lb_wait(&sh->empty[s], ((cnt / a.ring) & 1) ^ 1, fail);
+                if (!ok) return;
+                rgs_mbar_expect_tx(&sh->full[s], LTILE);
+                lb_tma(ring + (size_t)s * LTILE, map, chunk * 64, row * LT, piece, &sh->full[s]);
+                ++cnt;
+            };
+            // the order of tiles is the order in which the MMA warp takes them: S(0), S(1), O(0), S(2), O(1), ...; with B
+            // kept for both products O takes nothing from the ring
+            bool have_prev = false;
+            int prev_j = 0, prev_oc0 = 0, prev_noc = 0, prev_dw = 0;
+            auto out_tiles = [&]() {
+                if (!GRAD || a.b_res || !have_prev) return;
+                const CUtensorMap* mb = prev_dw ? &map_x : &map_w;
+                for (int oc = 0; oc < prev_noc && ok; ++oc)
+                    for (int p = 0; p < P && ok; ++p) tile(mb, prev_oc0 + oc, prev_j, p);
+            };
+            for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x, ++ai) {
+                const LabelItem it = lb_item(a, i);
+                const CUtensorMap *ma = it.dw ? &map_w : &map_x, *mb = it.dw ? &map_x : &map_w;
+                if (a.a_slots) {
+                    const uint32_t s = ai % a.a_slots;
+                    ok = lb_wait(&sh->a_empty[s], ((ai / a.a_slots) & 1) ^ 1, fail);
+                    if (!ok) break;
+                    rgs_mbar_expect_tx(&sh->a_full[s], na * LTILE);
+                    for (int k = 0; k < na; ++k) lb_tma(tiles + (size_t)(s * na + k) * LTILE, ma, (k / P) * 64, it.m * LT, k % P, &sh->a_full[s]);
+                }
+                for (int j = it.j0; j < it.j1 && ok; ++j) {
+                    const uint32_t s = kc % LKSLOTS;
+                    ok = lb_wait(&sh->k_empty[s], ((kc / LKSLOTS) & 1) ^ 1, fail);
+                    if (!ok) break;
+                    const uint32_t bytes = it.dw ? LT * 16 : LT * 4;
+                    rgs_mbar_expect_tx(&sh->k_full[s], bytes);
+                    rgs_bulk_g2s(kbuf + s * (LKBYTES / 4), it.dw ? a.kn + (size_t)j * (LT * 4) : a.b2 + (size_t)j * LT, bytes, &sh->k_full[s]);
+                    ++kc;
+                    for (int k = 0; k < a.nk && ok; ++k) {
+                        if (!a.a_slots)
+                            for (int p = 0; p < P && ok; ++p) tile(ma, k, it.m, p);
+                        for (int p = 0; p < P && ok; ++p) tile(mb, k, j, p);
+                    }
+                    out_tiles();
+                    have_prev = true; prev_j = j; prev_oc0 = it.oc0; prev_noc = it.noc; prev_dw = it.dw;
+                }
+            }
+            if (ok) out_tiles();
+            // copies still in flight land before the CTA leaves (all were consumed unless a wait ran out)
+            if (*fail) {
+                for (uint32_t k = cnt > (uint32_t)a.ring ? cnt - a.ring : 0; k < cnt; ++k) rgs_mbar_wait(&sh->full[k % a.ring], (k / a.ring) & 1, 1u << 16);
+                for (uint32_t k = kc > LKSLOTS ? kc - LKSLOTS : 0; k < kc; ++k) rgs_mbar_wait(&sh->k_full[k % LKSLOTS], (k / LKSLOTS) & 1, 1u << 16);
+                if (a.a_slots)
+                    for (uint32_t k = ai > (uint32_t)a.a_slots ? ai - a.a_slots : 0; k <= ai; ++k)
+                        rgs_mbar_wait(&sh->a_full[k % a.a_slots], (k / a.a_slots) & 1, 1u << 10);
+            }
         }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------------------------------------ MMA
+        if (lane == 0) {
+            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(LT >> 4) << 24);
+            uint32_t cnt = 0, ai = 0, ob = 0;  // ring tiles taken, items begun, outputs begun
+            bool ok = true;
+            auto take = [&](uint32_t k) {
+                ok = ok && lb_wait(&sh->full[k % a.ring], (k / a.ring) & 1, fail);
+                return rgs_smem_addr(ring + (size_t)(k % a.ring) * LTILE);
+            };
+            auto issue_s = [&](const LabelItem& it, int j, uint32_t t) {
+                if (a.a_slots && j == it.j0) ok = ok && lb_wait(&sh->a_full[ai % a.a_slots], (ai / a.a_slots) & 1, fail);
+                const uint32_t d = tmem + (t & 1) * SB;
+                uint32_t acc = 0;
+                for (int k = 0; k < a.nk && ok; ++k) {
+                    uint32_t at[P], bt[P];
+                    const uint32_t first = cnt;
+                    if (a.a_slots) {
+#pragma unroll
+                        for (int p = 0; p < P; ++p) at[p] = rgs_smem_addr(tiles + (size_t)((ai % a.a_slots) * na + k * P + p) * LTILE);
+                    } else {
+#pragma unroll
+                        for (int p = 0; p < P; ++p) at[p] = take(cnt++);
+                    }
+#pragma unroll
+                    for (int p = 0; p < P; ++p) bt[p] = take(cnt++);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const int steps = min(4, (a.c - k * 64 + 15) >> 4);
+#pragma unroll
+                    for (int q = 0; q < COMBOS; ++q)
+                        for (int ks = 0; ks < steps; ++ks) {
+                            lb_mma_ss(d, lb_desc(at[CA[q]] + ks * 32), lb_desc(bt[CB[q]] + ks * 32), idesc | ((LT >> 3) << 17), acc);
+                            acc = 1;
+                        }
+                    if (!a.b_res)
+                        for (uint32_t u = first; u < cnt; ++u) lb_commit(&sh->empty[u % a.ring]);
+                }
+                if (!ok) return;
+                lb_commit(&sh->s_full[t & 1]);
+                if (j == it.j1 - 1) {
+                    if (a.a_slots) lb_commit(&sh->a_empty[ai % a.a_slots]);
+                    ++ai;
+                }
+            };
+            // G B for score buffer t; first: ring index of its B tiles when they are kept
+            auto issue_o = [&](const LabelItem& it, int j, uint32_t t, uint32_t first) {
+                ok = ok && lb_wait(&sh->s_done[t & 1], (t >> 1) & 1, fail);
+                if (j == it.j0) ok = ok && lb_wait(&sh->o_free[ob % a.nob], ((ob / a.nob) & 1) ^ 1, fail);
+                const uint32_t s = tmem + (t & 1) * SB, o = tmem + OUT + (ob % a.nob) * OB;
+                for (int oc = 0; oc < it.noc && ok; ++oc) {
+                    uint32_t bt[P];
+                    const uint32_t begin = cnt;
+#pragma unroll
+                    for (int p = 0; p < P; ++p) bt[p] = a.b_res ? rgs_smem_addr(ring + (size_t)((first + (it.oc0 + oc) * P + p) % a.ring) * LTILE) : take(cnt++);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t cols = min(64, (a.c - (it.oc0 + oc) * 64 + 15) & ~15);
+                    const uint32_t id = idesc | (1u << 16) | ((cols >> 3) << 17);
+#pragma unroll
+                    for (int q = 0; q < COMBOS; ++q)
+#pragma unroll
+                        for (int ks = 0; ks < 8; ++ks) {
+                            // 16 columns of G are 8 words: two such runs per group of 32 scores, the pieces behind one another
+                            const uint32_t g = CA[q] == 2 ? s + 128 + ks * 8 : s + (ks >> 1) * 32 + CA[q] * 16 + (ks & 1) * 8;
+                            lb_mma_ts(o + oc * 64, g, lb_desc(bt[CB[q]] + ks * 2048), id, !(j == it.j0 && q == 0 && ks == 0));
+                        }
+                    if (!a.b_res)
+                        for (uint32_t u = begin; u < cnt; ++u) lb_commit(&sh->empty[u % a.ring]);
+                }
+                if (!ok) return;
+                if (a.b_res)
+                    for (int u = 0; u < na; ++u) lb_commit(&sh->empty[(first + u) % a.ring]);
+                if (j == it.j1 - 1) lb_commit(&sh->o_full[ob++ % a.nob]);
+            };
+            uint32_t t = 0, prev_first = 0;
+            LabelItem prev;
+            int prev_j = 0;
+            bool have_prev = false;
+            for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+                const LabelItem it = lb_item(a, i);
+                for (int j = it.j0; j < it.j1 && ok; ++j, ++t) {
+                    // forward: the scores of t-2 have been read; backward: G(t-2) B was issued before, and runs before
+                    if (!GRAD && t >= 2) ok = lb_wait(&sh->s_done[t & 1], ((t >> 1) & 1) ^ 1, fail);
+                    if (!ok) break;
+                    const uint32_t first = cnt;
+                    issue_s(it, j, t);
+                    if (GRAD) {
+                        if (have_prev && ok) issue_o(prev, prev_j, t - 1, prev_first);
+                        prev = it; prev_j = j; prev_first = first; have_prev = true;
+                    }
+                }
+            }
+            if (GRAD && have_prev && ok) issue_o(prev, prev_j, t - 1, prev_first);
+            lb_commit(&sh->drain);
+            rgs_mbar_wait(&sh->drain, 0, LWAIT);
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------------------------------------------ scores
+        const int g = (warp - 4) >> 2;                       // warpgroup: takes the score tiles t with t % 2 == g
+        const int wrow = (warp & 3) * 32, row = wrow + lane; // row of A
+        const uint32_t lanes = (uint32_t)wrow << 16;
+        const float nan = __int_as_float(0x7fc00000);
+        uint32_t t = 0, ob = 0;
+        bool dead = false;
+        int64_t out_i = blockIdx.x;                          // next item whose output this warpgroup writes
+        auto write_out = [&](int64_t i) {
+            const LabelItem it = lb_item(a, i);
+            if (!dead) dead = __any_sync(0xffffffffu, !lb_wait(&sh->o_full[ob % a.nob], (ob / a.nob) & 1, fail));
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t o = tmem + lanes + OUT + (ob % a.nob) * OB;
+            const int64_t r = (int64_t)it.m * LT + row, rows = it.dw ? a.v : a.n;
+            const int ns = it.dw ? a.nsw : a.nsx;
+            float scale = 1.f;
+            bool zero = false;
+            if (!it.dw) {
+                const float* k = a.kn + (size_t)it.m * (LT * 4);
+                scale = k[2 * LT + row];
+                zero = __float_as_int(k[3 * LT + row]) < 0;
+            }
+            for (int c0 = g * 16; c0 < it.noc * 64; c0 += 32) {
+                const int c = it.oc0 * 64 + c0;
+                if (c >= a.c) break;
+                uint32_t u[16];
+                tm_ld16(o + c0, u);
+                tm_wait_ld16(u);
+                if (r < rows && (!it.dw || a.dw)) {
+                    float f[16];
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) f[q] = dead ? nan : __uint_as_float(u[q]);
+                    if (ns > 1) {
+                        float* p = (it.dw ? a.part_w : a.part_x) + ((int64_t)it.split * (it.dw ? a.nmw : a.nmx) * LT + r) * a.cq + c;
+#pragma unroll
+                        for (int q = 0; q < 16; q += 4) *reinterpret_cast<float4*>(p + q) = make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) f[q] = zero ? 0.f : f[q] * scale;
+                        lb_store16(it.dw ? a.dw : a.dx, r, c, a.c, a.dtype, f);
+                    }
+                }
+                __syncwarp();
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            rgs_mbar_arrive(&sh->o_free[ob % a.nob]);
+            ++ob;
+        };
+        const bool dirty = GRAD && P == 1 && a.b_res && a.flags[1] != 0.f;
+        for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+            const LabelItem it = lb_item(a, i);
+            const int64_t r = (int64_t)it.m * LT + row;
+            // per-row values
+            int64_t y = -1;
+            float m2 = -INFINITY, inv_z = 0.f, sum = 0.f, b2row = 0.f;
+            if (!it.dw) {
+                if (r < a.n) {
+                    y = rgs_label(a.labels, r, a.label_bytes, a.v);
+                    if (GRAD) { m2 = a.lse[r]; inv_z = ex2(-a.lse[a.n + r]); }
+                } else if (GRAD) {
+                    m2 = INFINITY;
+                }
+            } else {
+                b2row = a.b2[r];
+            }
+            for (int j = it.j0; j < it.j1; ++j, ++t) {
+                if ((int)(t & 1) != g) continue;
+                const uint32_t s = tmem + lanes + (t & 1) * SB;
+                const uint32_t ks = t % LKSLOTS;
+                if (!dead) {  // the whole warp goes on or none of it: TMEM accesses are warp-wide
+                    dead = !lb_wait(&sh->k_full[ks], (t / LKSLOTS) & 1, fail) || !lb_wait(&sh->s_full[t & 1], (t >> 1) & 1, fail);
+                    dead = __any_sync(0xffffffffu, dead);
+                }
+                if (dead) continue;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const float* kb = kbuf + ks * (LKBYTES / 4);
+                const int64_t yt = y - (int64_t)j * LT;
+                const int yl = yt >= 0 && yt < LT ? (int)yt : -1024;  // label within the tile (forward, dX)
+                const int vrow = it.dw ? (int)r : 0;
+                uint32_t u[32];
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    __syncwarp();
+                    tm_ld32(s + c * 32, u);
+                    tm_wait_ld32(u);
+                    float f[32];
+                    if (!GRAD || !it.dw) {
+#pragma unroll
+                        for (int q = 0; q < 32; q += 4) {
+                            const float4 b = *reinterpret_cast<const float4*>(kb + c * 32 + q);
+                            f[q] = fmaf(__uint_as_float(u[q]), LOG2E, b.x);
+                            f[q + 1] = fmaf(__uint_as_float(u[q + 1]), LOG2E, b.y);
+                            f[q + 2] = fmaf(__uint_as_float(u[q + 2]), LOG2E, b.z);
+                            f[q + 3] = fmaf(__uint_as_float(u[q + 3]), LOG2E, b.w);
+                        }
+                    }
+                    if (!GRAD) {
+                        float top = f[0];
+#pragma unroll
+                        for (int q = 1; q < 32; ++q) top = fmaxf(top, f[q]);
+                        if ((unsigned)(yl - c * 32) < 32u) {
+#pragma unroll
+                            for (int q = 0; q < 32; ++q)
+                                if (yl - c * 32 == q) a.at[r] = f[q];
+                        }
+                        top = fmaxf(m2, top);
+                        const float ref = top == -INFINITY ? 0.f : top;
+                        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) acc[q & 3] += ex2(f[q] - ref);
+                        sum = fmaf(sum, ex2(m2 - ref), (acc[0] + acc[1]) + (acc[2] + acc[3]));
+                        m2 = top;
+                        continue;
+                    }
+                    if (!it.dw) {
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) f[q] = ex2(f[q] - m2) * inv_z;
+                        if ((unsigned)(yl - c * 32) < 32u) {
+#pragma unroll
+                            for (int q = 0; q < 32; ++q)
+                                if (yl - c * 32 == q) f[q] -= 1.f;
+                        }
+                    } else {
+                        float acc = 0.f;
+#pragma unroll
+                        for (int q = 0; q < 32; q += 4) {
+                            const float4 m = *reinterpret_cast<const float4*>(kb + c * 32 + q);
+                            const float4 z = *reinterpret_cast<const float4*>(kb + LT + c * 32 + q);
+                            const int4 l = *reinterpret_cast<const int4*>(kb + 3 * LT + c * 32 + q);
+                            f[q] = ex2(fmaf(__uint_as_float(u[q]), LOG2E, b2row) - m.x) * z.x;
+                            f[q + 1] = ex2(fmaf(__uint_as_float(u[q + 1]), LOG2E, b2row) - m.y) * z.y;
+                            f[q + 2] = ex2(fmaf(__uint_as_float(u[q + 2]), LOG2E, b2row) - m.z) * z.z;
+                            f[q + 3] = ex2(fmaf(__uint_as_float(u[q + 3]), LOG2E, b2row) - m.w) * z.w;
+                            if (l.x == vrow) f[q] -= kb[2 * LT + c * 32 + q];
+                            if (l.y == vrow) f[q + 1] -= kb[2 * LT + c * 32 + q + 1];
+                            if (l.z == vrow) f[q + 2] -= kb[2 * LT + c * 32 + q + 2];
+                            if (l.w == vrow) f[q + 3] -= kb[2 * LT + c * 32 + q + 3];
+                            if (P == 1 && dirty) {
+                                if (l.x < 0) f[q] = 0.f;
+                                if (l.y < 0) f[q + 1] = 0.f;
+                                if (l.z < 0) f[q + 2] = 0.f;
+                                if (l.w < 0) f[q + 3] = 0.f;
+                            }
+                            acc += (f[q] + f[q + 1]) + (f[q + 2] + f[q + 3]);
+                        }
+                        sum += acc;
+                    }
+                    uint32_t w0[16];
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) w0[q] = bf16x2(f[2 * q], f[2 * q + 1]);
+                    __syncwarp();
+                    tm_st16(s + c * 32, w0);
+                    if (P == 3) {
+                        uint32_t w1[16];
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) {
+                            f[2 * q] -= bf_lo(w0[q]);
+                            f[2 * q + 1] -= bf_hi(w0[q]);
+                            w1[q] = bf16x2(f[2 * q], f[2 * q + 1]);
+                        }
+                        tm_st16(s + c * 32 + 16, w1);
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) w0[q] = bf16x2(f[2 * q] - bf_lo(w1[q]), f[2 * q + 1] - bf_hi(w1[q]));
+                        tm_st16(s + 128 + c * 16, w0);
+                    }
+                }
+                if (P == 1 && dirty && it.dw) {
+                    // pixels without a label whose features are not finite: 0 * inf must not reach dW, so their rows of the
+                    // staged tile are cleared (row n of every chunk; a whole 128-byte row, whatever the swizzle)
+                    if (__float_as_int(kb[3 * LT + row]) < 0) {
+                        for (int k = 0; k < a.nk; ++k) {
+                            uint4* p = reinterpret_cast<uint4*>(ring + (size_t)(((uint64_t)t * na + k) % a.ring) * LTILE + row * 128);
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) p[q] = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    rgs_fence_proxy_async();
+                }
+                if (GRAD) asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                rgs_mbar_arrive(&sh->k_empty[ks]);
+                rgs_mbar_arrive(&sh->s_done[t & 1]);
+                if (GRAD)
+                    for (; out_i < i; out_i += gridDim.x) write_out(out_i);  // outputs of earlier items, behind the first scores of this one
+            }
+            if (!GRAD) {
+                if (r < a.n) {
+                    a.pm[((int64_t)it.split * 2 + g) * a.n + r] = dead ? nan : m2;
+                    a.ps[((int64_t)it.split * 2 + g) * a.n + r] = dead ? nan : sum;
+                }
+            } else if (it.dw && a.part_b && it.oc0 == 0) {
+                a.part_b[((int64_t)it.split * 2 + g) * a.nmw * LT + r] = dead ? nan : sum;
+            }
+        }
+        if (GRAD)
+            for (; out_i < items; out_i += gridDim.x) write_out(out_i);
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// before: operands that TMA cannot read as they are, column constants
+// ---------------------------------------------------------------------------------------------------------------------
+struct LabelPrep {
+    const void* x; int64_t ldx; const void* w; int64_t ldw; const void* bias; const void* labels;
+    int label_bytes, dtype, b_dtype, backward, per_row, pieces;
+    int64_t n, v;
+    int c, cp, nmx, nmw;
+    __nv_bfloat16* xs; __nv_bfloat16* ws;  // (pieces, rows, cp) or null where the tensor itself is read
+    float* b2; float* kn;
+    const float* lse; const float* gout; const float* count;
+    unsigned* ticket;
+};
+
+// eight channels of a row in one or three bf16 pieces whose sum is the value (to 2^-25 of it; infinities in the first alone)
+__device__ __forceinline__ void lb_split8(const void* src, int64_t ld, int dtype, int64_t rows, int64_t r, int c0, int c, int cp, int pieces,
+                                          bool clear, __nv_bfloat16* dst) {
+    float f[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) f[q] = !clear && c0 + q < c ? rgs_load_as_float(src, r * ld + c0 + q, dtype) : 0.f;
+    for (int p = 0; p < pieces; ++p) {
+        uint32_t u[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            u[q] = bf16x2(f[2 * q], f[2 * q + 1]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float& e = f[2 * q + h];
+                float k = h ? bf_hi(u[q]) : bf_lo(u[q]);
+                if (!(fabsf(k) <= 3.3e38f)) {      // infinity, NaN, or a finite value that rounds up to infinity
+                    if (fabsf(e) <= 3.402823466e38f) {
+                        k = __uint_as_float(__float_as_uint(e) & 0xffff0000u);
+                        u[q] = h ? (u[q] & 0xffffu) | (__float_as_uint(k) & 0xffff0000u) : (u[q] & 0xffff0000u) | (__float_as_uint(k) >> 16);
+                    } else {
+                        k = 0.f;
+                        e = 0.f;
+                    }
+                }
+                e -= k;
+            }
+        }
+        *reinterpret_cast<uint4*>(dst + ((int64_t)p * rows + r) * cp + c0) = make_uint4(u[0], u[1], u[2], u[3]);
     }
 }
 
-__global__ void __launch_bounds__(1024) rgs_label_sum_kernel(const float* losses, const void* labels, int label_bytes, int64_t n,
-                                                             int64_t vocab, int mean, float* result, float* count) {
-    __shared__ double part[32];
-    __shared__ unsigned long long rows[32];
-    double t = 0;
-    unsigned long long k = 0;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) {
-        t += losses[i];
-        k += rgs_label(labels, i, label_bytes, vocab) >= 0;
+__global__ void __launch_bounds__(256) rgs_label_prep_kernel(const __grid_constant__ LabelPrep a) {
+    const int groups = a.cp / 8;
+    const int64_t gx = a.xs ? a.n * groups : 0, gw = a.ws ? a.v * groups : 0, gb = (int64_t)a.nmw * LT;
+    const int64_t gk = a.backward ? (int64_t)a.nmx * LT : 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.ticket) *a.ticket = 0u;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < gx + gw + gb + gk; i += (int64_t)gridDim.x * 256) {
+        int64_t k = i;
+        if (k < gx) {
+            const int64_t r = k / groups;
+            const bool clear = a.backward && rgs_label(a.labels, r, a.label_bytes, a.v) < 0;
+            lb_split8(a.x, a.ldx, a.dtype, a.n, r, (int)(k - r * groups) * 8, a.c, a.cp, a.pieces, clear, a.xs);
+            continue;
+        }
+        k -= gx;
+        if (k < gw) {
+            const int64_t r = k / groups;
+            lb_split8(a.w, a.ldw, a.dtype, a.v, r, (int)(k - r * groups) * 8, a.c, a.cp, a.pieces, false, a.ws);
+            continue;
+        }
+        k -= gw;
+        if (k < gb) {
+            float b = k < a.v ? 0.f : -INFINITY;
+            if (k < a.v && a.bias) {
+                const float raw = rgs_load_as_float(a.bias, k, a.b_dtype);
+                b = raw * LOG2E;  // a finite bias stays finite: the lowest value of the type is no -inf
+                if (fabsf(raw) <= 3.402823466e38f) b = fminf(fmaxf(b, -3.402823466e38f), 3.402823466e38f);
+            }
+            a.b2[k] = b;
+            continue;
+        }
+        k -= gb;
+        const int64_t y = k < a.n ? rgs_label(a.labels, k, a.label_bytes, a.v) : -1;
+        float m = INFINITY, z = 0.f, g = 0.f;
+        if (y >= 0) {
+            g = a.gout[a.per_row ? k : 0] * (a.count ? 1.f / fmaxf(a.count[0], 1.f) : 1.f);
+            m = a.lse[k];
+            z = g * exp2f(-a.lse[a.n + k]);
+        }
+        float* o = a.kn + (k / LT) * (4 * LT) + k % LT;
+        o[0] = m; o[LT] = z; o[2 * LT] = g; o[3 * LT] = __int_as_float((int)y);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// after the forward pass: joins the pieces of the walk over the labels; the last block adds up the blocks in order
+// ---------------------------------------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) rgs_label_join_kernel(const float* __restrict__ pm, const float* __restrict__ ps, const float* __restrict__ at,
+                                                             const void* labels, int label_bytes, int64_t n, int64_t vocab, int parts, int mean,
+                                                             float* lse, float* losses, float* result, float* count, double* bsum,
+                                                             unsigned long long* bcount, unsigned* ticket) {
+    __shared__ double ssum[8];
+    __shared__ unsigned long long scount[8];
+    __shared__ int sdirty, last;
+    double total = 0;
+    unsigned long long rows = 0;
+    int dirty = 0;
+    if (threadIdx.x == 0) sdirty = 0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t y = rgs_label(labels, i, label_bytes, vocab);
+        float m = pm[i];
+        for (int k = 1; k < parts; ++k) m = fmaxf(m, pm[(int64_t)k * n + i]);
+        const float ref = m == -INFINITY ? 0.f : m;
+        float z = 0.f;
+        for (int k = 0; k < parts; ++k) z = fmaf(ps[(int64_t)k * n + i], exp2f(pm[(int64_t)k * n + i] - ref), z);
+        const float lz = log2f(z);
+        lse[i] = m;
+        lse[n + i] = lz;
+        float loss = 0.f;
+        if (y >= 0) {
+            loss = (lz + (m - at[i])) * LN2;
+            ++rows;
+        } else if (!(fabsf(m) <= 3.402823466e38f) || !(fabsf(lz) <= 3.402823466e38f)) {
+            dirty = 1;
+        }
+        if (losses) losses[i] = loss;
+        total += (double)loss;
     }
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) { t += __shfl_xor_sync(0xffffffffu, t, d); k += __shfl_xor_sync(0xffffffffu, k, d); }
-    if ((threadIdx.x & 31) == 0) { part[threadIdx.x >> 5] = t; rows[threadIdx.x >> 5] = k; }
+    for (int d = 16; d > 0; d >>= 1) { total += __shfl_xor_sync(0xffffffffu, total, d); rows += __shfl_xor_sync(0xffffffffu, rows, d); }
+    __syncthreads();
+    if (dirty) sdirty = 1;
+    if ((threadIdx.x & 31) == 0) { ssum[threadIdx.x >> 5] = total; scount[threadIdx.x >> 5] = rows; }
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int i = 1; i < 32; ++i) { t += part[i]; k += rows[i]; }
-        *count = (float)k;
-        if (result) *result = (float)(mean ? t / (double)(k > 0 ? k : 1) : t);
+        total = 0; rows = 0;
+        for (int k = 0; k < 8; ++k) { total += ssum[k]; rows += scount[k]; }
+        bsum[blockIdx.x] = total;
+        bcount[blockIdx.x] = rows * 2 + (unsigned)sdirty;
+        __threadfence();
+        last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    total = 0; rows = 0; dirty = 0;
+    for (unsigned k = threadIdx.x; k < gridDim.x; k += 256) {
+        total += __ldcg(&bsum[k]);
+        const unsigned long long u = __ldcg(&bcount[k]);
+        rows += u >> 1;
+        dirty |= (int)(u & 1);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) { total += __shfl_xor_sync(0xffffffffu, total, d); rows += __shfl_xor_sync(0xffffffffu, rows, d); }
+    if ((threadIdx.x & 31) == 0) { ssum[threadIdx.x >> 5] = total; scount[threadIdx.x >> 5] = rows; }
+    dirty = __syncthreads_or(dirty);
+    if (threadIdx.x == 0) {
+        total = 0; rows = 0;
+        for (int k = 0; k < 8; ++k) { total += ssum[k]; rows += scount[k]; }
+        count[0] = (float)rows;
+        count[1] = dirty ? 1.f : 0.f;
+        if (result) *result = (float)(mean ? total / (double)(rows > 0 ? rows : 1) : total);
     }
 }
 
-// rows_of_w = 0: out = dX, walks W; 1: out = dW (and db), walks X
-__global__ void __launch_bounds__(LB_WARPS * 32) rgs_label_bwd_kernel(const void* a, int64_t lda, const void* b, int64_t ldb, const void* bias,
-                                                                      const void* labels, int label_bytes, int64_t na, int64_t nb, int c,
-                                                                      int64_t vocab, int dtype, int b_dtype, const float* lse,
-                                                                      const float* gout, int per_row, const float* count, int rows_of_w,
-                                                                      void* out, void* db) {
-    extern __shared__ float acc_all[];
-    const int lane = threadIdx.x & 31;
-    float* acc = acc_all + (size_t)(threadIdx.x >> 5) * c;
-    const float scale = count ? 1.f / fmaxf(*count, 1.f) : 1.f;
-    for (int64_t i = (int64_t)blockIdx.x * LB_WARPS + (threadIdx.x >> 5); i < na; i += (int64_t)gridDim.x * LB_WARPS) {
-        for (int j = lane; j < c; j += 32) acc[j] = 0.f;
-        float sb = 0.f;
-        const int64_t ya = rows_of_w ? 0 : rgs_label(labels, i, label_bytes, vocab);
-        for (int64_t k = 0; k < nb && ya >= 0; ++k) {
-            const int64_t n = rows_of_w ? k : i, v = rows_of_w ? i : k;
-            const int64_t y = rows_of_w ? rgs_label(labels, k, label_bytes, vocab) : ya;
-            if (y < 0) continue;
-            const float l = row_dot(a, i * lda, b, k * ldb, c, dtype, lane) + (bias ? rgs_load_as_float(bias, v, b_dtype) : 0.f);
-            const float g = (expf((l - lse[n]) - lse[(rows_of_w ? nb : na) + n]) - (v == y ? 1.f : 0.f)) * gout[per_row ? n : 0] * scale;
-            sb += g;
-            for (int j = lane; j < c; j += 32) acc[j] = fmaf(g, rgs_load_as_float(b, k * ldb + j, dtype), acc[j]);
+// after the backward pass: adds up the pieces in order
+__global__ void __launch_bounds__(256) rgs_label_reduce_kernel(const __grid_constant__ LabelArgs a, void* db, int b_dtype) {
+    const int64_t tx = a.part_x ? a.n * (a.cq / 4) : 0, tw = a.part_w ? a.v * (a.cq / 4) : 0, tb = db ? a.v : 0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < tx + tw + tb; i += (int64_t)gridDim.x * 256) {
+        if (i >= tx + tw) {
+            const int64_t v = i - tx - tw;
+            float s = 0.f;
+            for (int k = 0; k < 2 * a.nsw; ++k) s += a.part_b[((int64_t)k * a.nmw) * LT + v];
+            rgs_store_float(db, v, b_dtype, s);
+            continue;
         }
-        if (out)
-            for (int j = lane; j < c; j += 32) rgs_store_float(out, i * c + j, dtype, acc[j]);
-        if (db && lane == 0) rgs_store_float(db, i, b_dtype, sb);
+        const bool is_w = i >= tx;
+        const int64_t e = is_w ? i - tx : i, r = e / (a.cq / 4);
+        const int c = (int)(e - r * (a.cq / 4)) * 4;
+        if (c >= a.c) continue;
+        const int ns = is_w ? a.nsw : a.nsx;
+        const int64_t stride = (int64_t)(is_w ? a.nmw : a.nmx) * LT * a.cq;
+        const float* p = (is_w ? a.part_w : a.part_x) + r * a.cq + c;
+        float4 s = *reinterpret_cast<const float4*>(p);
+        for (int k = 1; k < ns; ++k) {
+            const float4 t = *reinterpret_cast<const float4*>(p + k * stride);
+            s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
+        }
+        float f[4] = {s.x, s.y, s.z, s.w};
+        if (!is_w) {
+            const float* k = a.kn + (r / LT) * (4 * LT) + r % LT;
+            const float scale = k[2 * LT];
+            const bool zero = __float_as_int(k[3 * LT]) < 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) f[q] = zero ? 0.f : f[q] * scale;
+        }
+        void* out = is_w ? a.dw : a.dx;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (c + q < a.c) rgs_store_float(out, r * a.c + c + q, a.dtype, f[q]);
     }
 }
 
-static inline unsigned label_grid(int64_t rows) {
-    const int64_t want = (rows + LB_WARPS - 1) / LB_WARPS, most = RGS_SMS * 8;
+// ---------------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------------
+typedef CUresult (*LabelEncode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static LabelEncode label_encode() {
+    static std::atomic<LabelEncode> cached{nullptr};
+    LabelEncode fn = cached.load();
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
+        fn = reinterpret_cast<LabelEncode>(p);
+        cached.store(fn);
+    }
+    return fn;
+}
+
+// (channels, rows, pieces) of bf16; boxes of 64 channels x 128 rows; what lies outside reads as zero
+static int label_map(CUtensorMap* map, const void* base, int64_t c, int64_t rows, int64_t ld, int64_t pieces) {
+    LabelEncode enc = label_encode();
+    if (!enc) return 20;
+    const cuuint64_t dims[3] = {(cuuint64_t)c, (cuuint64_t)rows, (cuuint64_t)pieces};
+    const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)ld * 2 * (cuuint64_t)rows};
+    const cuuint32_t box[3] = {64, LT, 1}, estr[3] = {1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : 21;
+}
+
+static inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+// Number of pieces of a walk over nj tiles made by `tiles` row tiles: none where there are three row tiles or more to an
+// SM; else pieces short enough for six items to an SM.  `run` bounds the tiles that one accumulator sums, `most` the pieces.
+static int label_pieces(int64_t tiles, int64_t nj, int64_t sms, int64_t run, int64_t most) {
+    int64_t per = nj;
+    if (tiles < 3 * sms) per = (tiles * nj + sms * 6 - 1) / (sms * 6);
+    if (per > run) per = run;
+    if (per < 1) per = 1;
+    int64_t ns = (nj + per - 1) / per;
+    if (ns > most) ns = most;
+    return (int)(ns < 1 ? 1 : ns);
+}
+
+struct LabelPlan {
+    LabelArgs a;
+    int pieces, direct_x, direct_w, cp;
+    int64_t o_xs, o_ws, o_b2, o_kn, o_pm, o_ps, o_at, o_px, o_pw, o_pb, o_bsum, o_bcount, o_ticket, bytes;
+};
+
+#define LJOIN 592  // most blocks of the joining kernel
+
+static void label_plan(LabelPlan& p, int64_t n, int64_t c, int64_t v, int dtype, int direct, int backward) {
+    LabelArgs& a = p.a;
+    memset(&p, 0, sizeof(p));
+    const int64_t sms = RGS_SMS;
+    p.pieces = dtype == RGS_BF16 ? 1 : 3;
+    a.n = n; a.v = v; a.c = (int)c; a.nk = (int)((c + 63) / 64);
+    a.nmx = (int)((n + LT - 1) / LT); a.nmw = (int)((v + LT - 1) / LT);
+    a.dtype = dtype;
+    const int na = p.pieces * a.nk;
+    // tiles of A stay where eight of them fit; two blocks of them where that leaves two blocks of B
+    a.a_slots = na > 8 ? 0 : (LSLOTS - 2 * na >= 2 * na ? 2 : 1);
+    a.ring = LSLOTS - a.a_slots * na;
+    a.b_res = backward && a.a_slots && a.ring >= 2 * na;
+    const int cols = p.pieces == 1 ? 4 : 2;  // chunks of output channels that TMEM holds beside the scores
+    a.noc = a.nk < cols ? a.nk : cols;
+    a.nrange = backward ? (a.nk + a.noc - 1) / a.noc : 1;
+    a.nob = 2 * a.noc <= cols ? 2 : 1;
+    a.cq = (int)up(c, 16);
+    // where B is fetched anew for the second product its rows cannot be cleared in place: X goes through the copy
+    p.direct_x = p.pieces == 1 && (direct & 1) && (!backward || a.b_res);
+    p.direct_w = p.pieces == 1 && (direct & 2);
+    p.cp = (int)up(c, 8);
+    const int64_t run = p.pieces == 1 ? 512 : 32;
+    const int64_t rows_x = (int64_t)a.nmx * LT, rows_w = (int64_t)a.nmw * LT;
+    if (backward) {
+        const int64_t room = (int64_t)1 << 31;  // bytes of partial sums
+        a.nsx = label_pieces((int64_t)a.nmx * a.nrange, a.nmw, sms, run, room / (rows_x * a.cq * 4) + 1);
+        a.nsw = label_pieces((int64_t)a.nmw * a.nrange, a.nmx, sms, run, room / (rows_w * a.cq * 4) + 1);
+    } else {
+        a.nsx = label_pieces(a.nmx, a.nmw, sms, a.nmw, a.nmw);
+        a.nsw = 1;
+    }
+    int64_t o = 0;
+    auto take = [&](int64_t bytes) { const int64_t at = o; o = up(o + bytes, 1024); return at; };
+    p.o_xs = p.direct_x ? -1 : take(n * p.cp * 2 * p.pieces);
+    p.o_ws = p.direct_w ? -1 : take(v * p.cp * 2 * p.pieces);
+    p.o_b2 = take(rows_w * 4);
+    if (backward) {
+        p.o_kn = take(rows_x * 16);
+        p.o_px = a.nsx > 1 ? take(a.nsx * rows_x * a.cq * 4) : -1;
+        p.o_pw = a.nsw > 1 ? take(a.nsw * rows_w * a.cq * 4) : -1;
+        p.o_pb = take(2 * a.nsw * rows_w * 4);
+    } else {
+        p.o_pm = take(2 * a.nsx * n * 4);
+        p.o_ps = take(2 * a.nsx * n * 4);
+        p.o_at = take(n * 4);
+        p.o_bsum = take(LJOIN * 8);
+        p.o_bcount = take(LJOIN * 8);
+        p.o_ticket = take(4);
+    }
+    p.bytes = o + 1024;
+}
+
+static int label_direct(const void* x, int64_t ldx, const void* w, int64_t ldw) {
+    const int dx = ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0, dw = ldw % 8 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+    return dx | (dw << 1);
+}
+
+template <int P, bool GRAD>
+static int label_run(const CUtensorMap& mx, const CUtensorMap& mw, const LabelArgs& a, cudaStream_t stream) {
+    static std::atomic<uint64_t> ready{0};  // devices whose limit on dynamic shared memory was raised
+    int dev = 0;
+    RGS_CUDA_CHECK(cudaGetDevice(&dev));
+    if (dev > 63 || !((ready.load() >> dev) & 1)) {
+        RGS_CUDA_CHECK(cudaFuncSetAttribute(rgs_label_tc_kernel<P, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, LSMEM));
+        if (dev <= 63) ready.fetch_or((uint64_t)1 << dev);
+    }
+    const int64_t items = a.items_x + a.items_w, sms = RGS_SMS;
+    rgs_label_tc_kernel<P, GRAD><<<(unsigned)(items < sms ? items : sms), LTHREADS, LSMEM, stream>>>(mx, mw, a);
+    return (int)cudaGetLastError();
+}
+
+static inline unsigned label_grid(int64_t work, int64_t most) {
+    const int64_t want = (work + 255) / 256;
     return (unsigned)(want < 1 ? 1 : (want > most ? most : want));
+}
+
+static int label_operands(const LabelPlan& p, const LabelPrep& q, CUtensorMap* mx, CUtensorMap* mw) {
+    // autograd runs the backward pass on a thread of its own, where the driver has no context yet: cudaSetDevice binds it
+    int dev = 0;
+    RGS_CUDA_CHECK(cudaGetDevice(&dev));
+    RGS_CUDA_CHECK(cudaSetDevice(dev));
+    int rc = p.direct_x ? label_map(mx, q.x, q.c, q.n, q.ldx, 1) : label_map(mx, q.xs, p.cp, q.n, p.cp, p.pieces);
+    if (rc) return rc;
+    return p.direct_w ? label_map(mw, q.w, q.c, q.v, q.ldw, 1) : label_map(mw, q.ws, p.cp, q.v, p.cp, p.pieces);
+}
+
+static void label_prep(const LabelPlan& p, const LabelPrep& q, cudaStream_t stream) {
+    const int64_t work = ((q.xs ? q.n : 0) + (q.ws ? q.v : 0)) * (q.cp / 8) + (int64_t)q.nmw * LT + (q.backward ? (int64_t)q.nmx * LT : 0);
+    rgs_label_prep_kernel<<<label_grid(work, RGS_SMS * 16), 256, 0, stream>>>(q);
 }
 
 extern "C" {
 
-int64_t rgs_cuda_label_scratch_bytes(int64_t n, int64_t, int64_t, int64_t, int64_t) { return n * 4 + 16; }
+// direct: bit 0 / 1: rows of x / w start on 16-byte boundaries
+int64_t rgs_cuda_label_scratch_bytes(int64_t n, int64_t c, int64_t vocab, int64_t dtype, int64_t direct, int64_t backward) {
+    LabelPlan p;
+    label_plan(p, n, c, vocab, (int)dtype, (int)direct, (int)backward);
+    return p.bytes;
+}
 
 int rgs_cuda_label_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* labels, int64_t label_bytes,
                        int64_t n, int64_t c, int64_t vocab, int64_t dtype, int64_t b_dtype, int64_t mean, void* scratch, float* lse,
                        float* losses, float* result, float* count, void* stream) {
-    float* row_loss = losses ? losses : static_cast<float*>(scratch);
-    rgs_label_fwd_kernel<<<label_grid(n), LB_WARPS * 32, 0, (cudaStream_t)stream>>>(x, ldx, w, ldw, bias, labels, (int)label_bytes, n, (int)c,
-                                                                                    vocab, (int)dtype, (int)b_dtype, lse, row_loss);
-    rgs_label_sum_kernel<<<1, 1024, 0, (cudaStream_t)stream>>>(row_loss, labels, (int)label_bytes, n, vocab, (int)mean, result, count);
+    cudaStream_t st = (cudaStream_t)stream;
+    LabelPlan p;
+    label_plan(p, n, c, vocab, (int)dtype, label_direct(x, ldx, w, ldw), 0);
+    LabelArgs& a = p.a;
+    unsigned char* s = reinterpret_cast<unsigned char*>(up((int64_t)reinterpret_cast<uintptr_t>(scratch), 1024));
+    LabelPrep q{x, ldx, w, ldw, bias, labels, (int)label_bytes, (int)dtype, (int)b_dtype, 0, 0, p.pieces, n, vocab, (int)c, p.cp, a.nmx, a.nmw,
+                p.direct_x ? nullptr : reinterpret_cast<__nv_bfloat16*>(s + p.o_xs), p.direct_w ? nullptr : reinterpret_cast<__nv_bfloat16*>(s + p.o_ws),
+                reinterpret_cast<float*>(s + p.o_b2), nullptr, nullptr, nullptr, nullptr, reinterpret_cast<unsigned*>(s + p.o_ticket)};
+    CUtensorMap mx, mw;
+    int rc = label_operands(p, q, &mx, &mw);
+    if (rc) return rc;
+    label_prep(p, q, st);
+    RGS_CUDA_CHECK(cudaGetLastError());
+    a.items_x = (int64_t)a.nmx * a.nsx;
+    a.b2 = q.b2;
+    a.labels = labels; a.label_bytes = (int)label_bytes;
+    a.flags = count;
+    a.pm = reinterpret_cast<float*>(s + p.o_pm);
+    a.ps = reinterpret_cast<float*>(s + p.o_ps);
+    a.at = reinterpret_cast<float*>(s + p.o_at);
+    rc = p.pieces == 1 ? label_run<1, false>(mx, mw, a, st) : label_run<3, false>(mx, mw, a, st);
+    if (rc) return rc;
+    rgs_label_join_kernel<<<label_grid(n, LJOIN), 256, 0, st>>>(a.pm, a.ps, a.at, labels, (int)label_bytes, n, vocab, 2 * a.nsx, (int)mean, lse, losses,
+                                                                result, count, reinterpret_cast<double*>(s + p.o_bsum),
+                                                                reinterpret_cast<unsigned long long*>(s + p.o_bcount), q.ticket);
     return (int)cudaGetLastError();
 }
 
 int rgs_cuda_label_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* labels, int64_t label_bytes,
                        int64_t n, int64_t c, int64_t vocab, int64_t dtype, int64_t b_dtype, const float* lse, const float* gout,
-                       int64_t per_row, const float* count, void* scratch, void* dx, void* dw, void* db, void* stream) {
-    const size_t smem = (size_t)LB_WARPS * c * 4;
-    if (dx)
-        rgs_label_bwd_kernel<<<label_grid(n), LB_WARPS * 32, smem, (cudaStream_t)stream>>>(
-            x, ldx, w, ldw, bias, labels, (int)label_bytes, n, vocab, (int)c, vocab, (int)dtype, (int)b_dtype, lse, gout, (int)per_row, count,
-            0, dx, nullptr);
-    if (dw || db)
-        rgs_label_bwd_kernel<<<label_grid(vocab), LB_WARPS * 32, smem, (cudaStream_t)stream>>>(
-            w, ldw, x, ldx, bias, labels, (int)label_bytes, vocab, n, (int)c, vocab, (int)dtype, (int)b_dtype, lse, gout, (int)per_row, count,
-            1, dw, db);
+                       int64_t per_row, int64_t mean, const float* count, void* scratch, void* dx, void* dw, void* db, void* stream) {
+    cudaStream_t st = (cudaStream_t)stream;
+    LabelPlan p;
+    label_plan(p, n, c, vocab, (int)dtype, label_direct(x, ldx, w, ldw), 1);
+    LabelArgs& a = p.a;
+    unsigned char* s = reinterpret_cast<unsigned char*>(up((int64_t)reinterpret_cast<uintptr_t>(scratch), 1024));
+    LabelPrep q{x, ldx, w, ldw, bias, labels, (int)label_bytes, (int)dtype, (int)b_dtype, 1, (int)per_row, p.pieces, n, vocab, (int)c, p.cp, a.nmx,
+                a.nmw, p.direct_x ? nullptr : reinterpret_cast<__nv_bfloat16*>(s + p.o_xs),
+                p.direct_w ? nullptr : reinterpret_cast<__nv_bfloat16*>(s + p.o_ws), reinterpret_cast<float*>(s + p.o_b2),
+                reinterpret_cast<float*>(s + p.o_kn), lse, gout, mean ? count : nullptr, nullptr};
+    CUtensorMap mx, mw;
+    int rc = label_operands(p, q, &mx, &mw);
+    if (rc) return rc;
+    label_prep(p, q, st);
+    RGS_CUDA_CHECK(cudaGetLastError());
+    a.items_x = dx ? (int64_t)a.nmx * a.nrange * a.nsx : 0;
+    a.items_w = dw || db ? (int64_t)a.nmw * a.nrange * a.nsw : 0;
+    a.b2 = q.b2; a.kn = q.kn; a.lse = lse;
+    a.labels = labels; a.label_bytes = (int)label_bytes;
+    a.flags = count;
+    a.part_x = dx && a.nsx > 1 ? reinterpret_cast<float*>(s + p.o_px) : nullptr;
+    a.part_w = dw && a.nsw > 1 ? reinterpret_cast<float*>(s + p.o_pw) : nullptr;
+    a.part_b = db ? reinterpret_cast<float*>(s + p.o_pb) : nullptr;
+    a.dx = dx; a.dw = dw;
+    rc = p.pieces == 1 ? label_run<1, true>(mx, mw, a, st) : label_run<3, true>(mx, mw, a, st);
+    if (rc) return rc;
+    if (a.part_x || a.part_w || db) {
+        const int64_t work = (a.part_x ? n * (a.cq / 4) : 0) + (a.part_w ? vocab * (a.cq / 4) : 0) + (db ? vocab : 0);
+        rgs_label_reduce_kernel<<<label_grid(work, RGS_SMS * 16), 256, 0, st>>>(a, db, (int)b_dtype);
+    }
     return (int)cudaGetLastError();
 }
 

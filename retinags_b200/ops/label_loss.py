@@ -20,12 +20,15 @@ _REDUCTIONS = ("mean", "sum", "none")
 _LIMIT = 2 ** 31 - 1
 
 
-def _scratch(device: torch.device, n: int, c: int, v: int, dtype: int, backward: int) -> torch.Tensor:
+def _scratch(x: torch.Tensor, ldx: int, w: torch.Tensor, ldw: int, backward: int) -> torch.Tensor:
+    """Workspace of one pass; it depends on whether the kernels can read the rows as they lie (16-byte boundaries)."""
+    device = x.device
+    direct = sum((ld % 8 == 0 and t.data_ptr() % 16 == 0) << k for k, (t, ld) in enumerate(((x, ldx), (w, ldw))))
     kind = "cuda" if device.type == "cuda" else "cpu"
     fn = getattr(native.lib(kind), f"rgs_{kind}_label_scratch_bytes")
-    fn.argtypes, fn.restype = [ctypes.c_int64] * 5, ctypes.c_int64
+    fn.argtypes, fn.restype = [ctypes.c_int64] * 6, ctypes.c_int64
     with torch.cuda.device(device) if kind == "cuda" else torch.no_grad():
-        return torch.empty(int(fn(n, c, v, dtype, backward)), dtype=torch.uint8, device=device)
+        return torch.empty(int(fn(*x.shape, w.shape[0], DTYPES[x.dtype], direct, backward)), dtype=torch.uint8, device=device)
 
 
 class _LabelLoss(torch.autograd.Function):
@@ -42,11 +45,11 @@ class _LabelLoss(torch.autograd.Function):
         lse = torch.empty(2, n, dtype=torch.float32, device=dev)
         losses = torch.empty(n, dtype=torch.float32, device=dev) if per_row else None
         result = None if per_row else new((), dtype=torch.float32, device=dev)
-        count = new(1, dtype=torch.float32, device=dev)
+        count = new(2, dtype=torch.float32, device=dev)
         b_code = DTYPES[bias.dtype] if bias is not None else 0
         if n:
             native.call("label_fwd", dev, x, ldx, w, ldw, bias, y, y.element_size(), n, c, v, DTYPES[x.dtype], b_code,
-                        int(reduction == "mean"), _scratch(dev, n, c, v, DTYPES[x.dtype], 0), lse, losses, result, count)
+                        int(reduction == "mean"), _scratch(x, ldx, w, ldw, 0), lse, losses, result, count)
         ctx.save_for_backward(x, w, bias, y, lse, count)
         ctx.args = (tuple(features.shape), tuple(weight.shape), ldx, ldw, b_code, reduction)
         return losses.view(features.shape[:-1]) if per_row else result
@@ -66,8 +69,8 @@ class _LabelLoss(torch.autograd.Function):
         db = new(v, dtype=bias.dtype, device=dev) if ctx.needs_input_grad[2] else None
         if n and (dx is not None or dw is not None or db is not None):
             native.call("label_bwd", dev, x, ldx, w, ldw, bias, y, y.element_size(), n, c, v, DTYPES[x.dtype], b_code, lse, g,
-                        int(reduction == "none"), count if reduction == "mean" else None,
-                        _scratch(dev, n, c, v, DTYPES[x.dtype], 1), dx, dw, db)
+                        int(reduction == "none"), int(reduction == "mean"), count,
+                        _scratch(x, ldx, w, ldw, 1), dx, dw, db)
         return dx, dw, db, None, None
 
 

@@ -46,7 +46,7 @@ SIGNATURES = {
     "records_pack": "pppipiipp",
     "records_unpack": "pipppiip",
     "label_fwd": "pipippiiiiiiipppppp",
-    "label_bwd": "pipippiiiiiippippppp" "p",
+    "label_bwd": "pipippiiiiiippiipppppp",
     "norm_fwd": "piiippiiifpippp",
     "norm_bwd": "piiipppiipiiifppppp",
     "pack8": "piiiiippp",
