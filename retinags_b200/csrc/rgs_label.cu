@@ -7,8 +7,8 @@
 // one matrix (A: rows of X for the loss and dX, rows of W for dW) and walks tiles of 128 rows of the other (B):
 //   TMA brings tiles of 128 rows x 64 channels (bf16, 128-byte swizzle) into a ring in shared memory
 //   S = A B^T: tcgen05.mma into one of two score buffers in TMEM
-//   two warpgroups take the score buffers in turn (one thread per row of A: no shuffles), form the running maximum and
-//   sum (forward) or G (backward); G goes back over the scores in TMEM as a bf16 operand
+//   four warpgroups, two to a score buffer with 64 of its columns each (one thread per row of A: no shuffles), form the
+//   running maximum and sum (forward) or G (backward); G goes back over the scores in TMEM as a bf16 operand
 //   O += G B: tcgen05.mma with G from TMEM and the same B tile, read with its channels as the N side
 // so a B tile is fetched once for both products and the scores never leave the SM.  The gradient kernel walks the items of
 // dX and dW in one launch.  For dW the roles are swapped (rows of A are labels, columns are pixels); the scores are
@@ -30,32 +30,34 @@
 #include "rgs_field_math.h"
 
 #define LT 128                      // rows of a tile of either matrix
-#define LTILE 16384                 // bytes of a staged tile: 128 rows x 64 channels bf16
-#define LSLOTS 13                   // staged tiles in shared memory
+#define LROOM (13 * 16384)          // bytes of staged tiles: 128 rows x 64 (or 32) channels bf16 each
+#define LSTAGES 13                  // most stages of the ring
 #define LKSLOTS 4                   // staged blocks of column constants
 #define LKBYTES 2048
-#define LTHREADS 384                // warp 0 TMA, warp 1 MMA, warp 2 TMEM, warps 4-11 two warpgroups on the scores
+#define LTHREADS 576                // warp 0 TMA, warp 1 MMA, warps 2-17 four warpgroups on the scores
 #define LWAIT (1u << 20)
 #define LOG2E 1.4426950408889634f
 #define LN2 0.6931471805599453f
 
 struct LabelArgs {
     int64_t n, v;
-    int c, nk;                       // channels, chunks of 64 channels
+    int c, nk;                       // channels, chunks of 64 (32) channels
     int noc, nrange;                 // chunks of output channels per item, ranges of them
-    int a_slots, b_res, ring;        // slots of resident A tiles (0: A goes through the ring), B kept for both products, ring slots
+    int a_slots;                     // blocks of A that stay in shared memory (0: A goes through the ring)
+    int whole, gs, stages;           // a stage holds a whole block of B, kept for both products; tiles of a stage; stages
     int nob;                         // output buffers in TMEM
     int nmx, nmw;                    // tiles of 128 pixels, of 128 labels
     int nsx, nsw;                    // pieces of the walk over labels (forward, dX) and over pixels (dW)
-    int64_t items_x, items_w;
+    int perx, restx, perw, restw;    // tiles of a piece: per, one more in the first rest pieces
+    unsigned items_x, items_w;
     const float* b2;                 // (nmw * 128) bias * log2 e; -inf behind the last label
-    const float* kn;                 // (nmx, 4, 128) per pixel: m * log2 e, g / z, g, label (bits); backward only
+    const float* kn;                 // (nmx, 4, 128) per pixel: -m * log2 e, g / z, g, label (bits); backward only
     const float* lse;                // (2, n) m and log z, both in units of log 2
     const void* labels; int label_bytes;
     const float* flags;              // [1] != 0: a pixel without a label holds something that is not finite
-    float* pm; float* ps; float* at; // forward: (2 nsx, n) partial maximum and sum, (n) score of the label
+    float* pm; float* ps; float* at; // forward: (4 nsx, n) partial maximum and sum, (n) score of the label
     float* part_x; float* part_w;    // (nsx, nmx*128, cq), (nsw, nmw*128, cq) when split
-    float* part_b;                   // (2 nsw, nmw*128)
+    float* part_b;                   // (4 nsw, nmw*128)
     int cq;
     void* dx; void* dw; int dtype;
 };
@@ -77,6 +79,22 @@ __device__ __forceinline__ bool lb_wait(unsigned long long* bar, uint32_t parity
     *fail = 1;
     return false;
 }
+// the same by a whole warp, with one answer for all of it
+__device__ __forceinline__ bool lb_wait_warp(unsigned long long* bar, uint32_t parity, volatile int* fail) {
+    return __all_sync(0xffffffffu, lb_wait(bar, parity, fail));
+}
+__device__ __forceinline__ void lb_wait_quiet(unsigned long long* bar, uint32_t parity, volatile int* fail) {
+    lb_wait(bar, parity, fail);
+    __syncwarp();
+}
+// One lane of a converged warp.  The producer and MMA warps run their loops with all lanes and let this one issue: the
+// addresses and descriptors then stay in uniform registers, which TMA and MMA instructions take (with a single thread
+// in the loop every instruction moved its operands there first: 2530 -> see below).
+__device__ __forceinline__ bool lb_elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ void lb_tma(void* dst, const CUtensorMap* map, int x, int y, int z, unsigned long long* bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
                  "r"(rgs_smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(rgs_smem_addr(bar)) : "memory");
@@ -84,9 +102,12 @@ __device__ __forceinline__ void lb_tma(void* dst, const CUtensorMap* map, int x,
 __device__ __forceinline__ void lb_commit(unsigned long long* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(rgs_smem_addr(bar)) : "memory");
 }
-// shared-memory descriptors, 128-byte swizzle: rows of 64 channels, eight rows (1024 bytes) to a pattern
-__device__ __forceinline__ uint64_t lb_desc(uint32_t addr) {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(1024 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// shared-memory descriptor of a tile at address 0: rows of KC channels under the swizzle of their length (128 or 64 bytes),
+// eight rows to a pattern; both strides are that of the pattern, so it reads rows as K-major or as steps of K
+template <int KC>
+__device__ __forceinline__ uint64_t lb_desc() {
+    constexpr uint64_t pattern = (KC * 16) >> 4;
+    return (pattern << 16) | (pattern << 32) | ((uint64_t)1 << 46) | ((uint64_t)(KC == 64 ? 2 : 4) << 61);
 }
 __device__ __forceinline__ void lb_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::
@@ -100,8 +121,6 @@ __device__ __forceinline__ void lb_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
     "+r"(r[o + 8]), "+r"(r[o + 9]), "+r"(r[o + 10]), "+r"(r[o + 11]), "+r"(r[o + 12]), "+r"(r[o + 13]), "+r"(r[o + 14]), "+r"(r[o + 15])
 #define LB_O16(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7]), \
     "=r"(r[o + 8]), "=r"(r[o + 9]), "=r"(r[o + 10]), "=r"(r[o + 11]), "=r"(r[o + 12]), "=r"(r[o + 13]), "=r"(r[o + 14]), "=r"(r[o + 15])
-#define LB_I16(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7]), \
-    "r"(r[o + 8]), "r"(r[o + 9]), "r"(r[o + 10]), "r"(r[o + 11]), "r"(r[o + 12]), "r"(r[o + 13]), "r"(r[o + 14]), "r"(r[o + 15])
 
 __device__ __forceinline__ void tm_ld32(uint32_t a, uint32_t (&r)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
@@ -116,14 +135,27 @@ __device__ __forceinline__ void tm_ld16(uint32_t a, uint32_t (&r)[16]) {
                  : LB_O16(r, 0) : "r"(a) : "memory");
 }
 __device__ __forceinline__ void tm_wait_ld16(uint32_t (&r)[16]) { asm volatile("tcgen05.wait::ld.sync.aligned;" : LB_R16(r, 0)::"memory"); }
-__device__ __forceinline__ void tm_st16(uint32_t a, const uint32_t (&r)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::
-                 LB_I16(r, 0), "r"(a) : "memory");
-}
 __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
+}
+__device__ __forceinline__ void tm_st8(uint32_t a, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(a) : "memory");
+}
+// two floats to a register pair: one instruction for both
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 mk2(float a, float b) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ f2 mk2u(uint32_t a, uint32_t b) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b)); return r; }
+__device__ __forceinline__ void un2(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+// v -= g where a == b.  Written out: the compiler turns a chain of such conditions over an array into an index, and the
+// array into local memory (the backward pass then took twice as long).
+__device__ __forceinline__ void sub_if(float& v, float g, int a, int b) {
+    asm("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %2, %3;\n\t@p sub.f32 %0, %0, %1;\n\t}" : "+f"(v) : "f"(g), "r"(a), "r"(b));
 }
 __device__ __forceinline__ float bf_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
@@ -133,20 +165,32 @@ __device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 
 // ---------------------------------------------------------------------------------------------------------------------
 struct LabelItem { int dw, m, oc0, noc, split, j0, j1; };
 
-__device__ __forceinline__ LabelItem lb_item(const LabelArgs& a, int64_t i) {
+// single threads run this between products: no division where there is nothing to divide
+__device__ __forceinline__ LabelItem lb_item(const LabelArgs& a, unsigned i) {
     LabelItem it;
     it.dw = i >= a.items_x;
     if (it.dw) i -= a.items_x;
-    const int nm = it.dw ? a.nmw : a.nmx, nj = it.dw ? a.nmx : a.nmw, ns = it.dw ? a.nsw : a.nsx;
-    it.m = (int)(i % nm);
-    i /= nm;
-    it.oc0 = (int)(i % a.nrange) * a.noc;
+    const unsigned nm = it.dw ? a.nmw : a.nmx, base = it.dw ? a.perw : a.perx, rest = it.dw ? a.restw : a.restx;
+    unsigned q = 0;
+    if (i >= nm) { q = i / nm; i -= q * nm; }
+    it.m = (int)i;
+    unsigned range = 0;
+    if (a.nrange > 1) { range = q % (unsigned)a.nrange; q /= (unsigned)a.nrange; }
+    it.oc0 = (int)range * a.noc;
     it.noc = min(a.noc, a.nk - it.oc0);
-    it.split = (int)(i / a.nrange);
-    it.j0 = (int)((int64_t)nj * it.split / ns);
-    it.j1 = (int)((int64_t)nj * (it.split + 1) / ns);
+    it.split = (int)q;
+    it.j0 = (int)(q * base + min(q, rest));  // the first `rest` pieces are one tile longer
+    it.j1 = it.j0 + (int)base + (q < rest);
     return it;
 }
+
+// place in a ring of buffers and the parity of its current use
+struct LabelCursor {
+    uint32_t slot = 0, phase = 0;
+    __device__ __forceinline__ void next(uint32_t size) {
+        if (++slot == size) { slot = 0; phase ^= 1; }
+    }
+};
 
 // sixteen channels of a row of the output, rounded to its type; vector stores where rows keep their alignment
 __device__ __forceinline__ void lb_store16(void* out, int64_t r, int c, int channels, int dtype, const float (&f)[16]) {
@@ -177,14 +221,14 @@ __device__ __forceinline__ void lb_store16(void* out, int64_t r, int c, int chan
 }
 
 struct LabelShared {
-    unsigned long long full[LSLOTS], empty[LSLOTS], a_full[2], a_empty[2], k_full[LKSLOTS], k_empty[LKSLOTS];
+    unsigned long long full[LSTAGES], empty[LSTAGES], a_full[2], a_empty[2], k_full[LKSLOTS], k_empty[LKSLOTS];
     unsigned long long s_full[2], s_done[2], o_full[2], o_free[2], drain;
     uint32_t tmem;
     int fail;
 };
-#define LSMEM (1024 + LSLOTS * LTILE + LKSLOTS * LKBYTES + (int)sizeof(LabelShared))
+#define LSMEM (1024 + LROOM + LKSLOTS * LKBYTES + (int)sizeof(LabelShared))
 
-template <int P, bool GRAD>
+template <int P, bool GRAD, int KC>
 __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                                                                    const __grid_constant__ LabelArgs a) {
     constexpr int SB = P == 1 ? 128 : 192;        // TMEM columns of a score buffer (scores; over them G, its third piece behind)
@@ -192,28 +236,31 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
     constexpr int OB = P == 1 ? 128 : 64;         // columns of an output buffer when there are two
     constexpr int COMBOS = P == 1 ? 1 : 6;
     constexpr int CA[6] = {P == 1 ? 0 : 2, 0, 1, 1, 0, 0}, CB[6] = {0, 2, 1, 0, 1, 0};  // smallest products first
+    constexpr int TB = KC * 2 * LT;               // bytes of a staged tile
     extern __shared__ unsigned char raw[];
     unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    float* kbuf = reinterpret_cast<float*>(tiles + LSLOTS * LTILE);
-    LabelShared* sh = reinterpret_cast<LabelShared*>(tiles + LSLOTS * LTILE + LKSLOTS * LKBYTES);
+    float* kbuf = reinterpret_cast<float*>(tiles + LROOM);
+    LabelShared* sh = reinterpret_cast<LabelShared*>(tiles + LROOM + LKSLOTS * LKBYTES);
     volatile int* fail = &sh->fail;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int na = P * a.nk;                      // tiles of one A or B row block
-    unsigned char* ring = tiles + (size_t)a.a_slots * na * LTILE;
+    const uint32_t na = P * a.nk;                 // tiles of one block of 128 rows, chunk by chunk, its pieces together
+    unsigned char* ring = tiles + a.a_slots * na * TB;
+    const uint32_t stage = a.gs * TB;             // bytes of a stage of the ring: a whole block of B, or one chunk of A or B
 
-    if (tid == 0) {
-        for (int i = 0; i < LSLOTS; ++i) { rgs_mbar_init(&sh->full[i], 1); rgs_mbar_init(&sh->empty[i], 1); }
-        for (int i = 0; i < 2; ++i) {
-            rgs_mbar_init(&sh->a_full[i], 1); rgs_mbar_init(&sh->a_empty[i], 1);
-            rgs_mbar_init(&sh->s_full[i], 1); rgs_mbar_init(&sh->s_done[i], 128);
-            rgs_mbar_init(&sh->o_full[i], 1); rgs_mbar_init(&sh->o_free[i], 256);
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int i = 0; i < LSTAGES; ++i) { rgs_mbar_init(&sh->full[i], 1); rgs_mbar_init(&sh->empty[i], 1); }
+            for (int i = 0; i < 2; ++i) {
+                rgs_mbar_init(&sh->a_full[i], 1); rgs_mbar_init(&sh->a_empty[i], 1);
+                rgs_mbar_init(&sh->s_full[i], 1); rgs_mbar_init(&sh->s_done[i], 256);
+                rgs_mbar_init(&sh->o_full[i], 1); rgs_mbar_init(&sh->o_free[i], 512);
+            }
+            for (int i = 0; i < LKSLOTS; ++i) { rgs_mbar_init(&sh->k_full[i], 1); rgs_mbar_init(&sh->k_empty[i], 256); }
+            rgs_mbar_init(&sh->drain, 1);
+            sh->fail = 0;
+            rgs_fence_mbar_init();
         }
-        for (int i = 0; i < LKSLOTS; ++i) { rgs_mbar_init(&sh->k_full[i], 1); rgs_mbar_init(&sh->k_empty[i], 128); }
-        rgs_mbar_init(&sh->drain, 1);
-        sh->fail = 0;
-        rgs_fence_mbar_init();
-    }
-    if (warp == 2) {
+        __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(rgs_smem_addr(&sh->tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -221,192 +268,230 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = sh->tmem;
-    const int64_t items = a.items_x + a.items_w;
+    const unsigned items = a.items_x + a.items_w;
 
     if (warp == 0) {
         // ------------------------------------------------------------------------------------------------ TMA
-        if (lane == 0) {
-            uint32_t cnt = 0, kc = 0, ai = 0;
-            bool ok = true;
-            auto tile = [&](const CUtensorMap* map, int chunk, int row, int piece) {
-                const uint32_t s = cnt % a.ring;
-                ok = ok && lb_wait(&sh->empty[s], ((cnt / a.ring) & 1) ^ 1, fail);
-                if (!ok) return;
-                rgs_mbar_expect_tx(&sh->full[s], LTILE);
-                lb_tma(ring + (size_t)s * LTILE, map, chunk * 64, row * LT, piece, &sh->full[s]);
-                ++cnt;
-            };
-            // the order of tiles is the order in which the MMA warp takes them: S(0), S(1), O(0), S(2), O(1), ...; with B
-            // kept for both products O takes nothing from the ring
-            bool have_prev = false;
-            int prev_j = 0, prev_oc0 = 0, prev_noc = 0, prev_dw = 0;
-            auto out_tiles = [&]() {
-                if (!GRAD || a.b_res || !have_prev) return;
-                const CUtensorMap* mb = prev_dw ? &map_x : &map_w;
-                for (int oc = 0; oc < prev_noc && ok; ++oc)
-                    for (int p = 0; p < P && ok; ++p) tile(mb, prev_oc0 + oc, prev_j, p);
-            };
-            for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x, ++ai) {
-                const LabelItem it = lb_item(a, i);
-                const CUtensorMap *ma = it.dw ? &map_w : &map_x, *mb = it.dw ? &map_x : &map_w;
-                if (a.a_slots) {
-                    const uint32_t s = ai % a.a_slots;
-                    ok = lb_wait(&sh->a_empty[s], ((ai / a.a_slots) & 1) ^ 1, fail);
-                    if (!ok) break;
-                    rgs_mbar_expect_tx(&sh->a_full[s], na * LTILE);
-                    for (int k = 0; k < na; ++k) lb_tma(tiles + (size_t)(s * na + k) * LTILE, ma, (k / P) * 64, it.m * LT, k % P, &sh->a_full[s]);
+        const bool lead = lb_elect();
+        LabelCursor rc, ac, kc;
+        uint32_t loads = 0;
+        bool ok = true;
+        // one stage: gs tiles from chunk k on, all pieces of a chunk before the next
+        auto load = [&](const CUtensorMap* map, int k, int row) {
+            ok = ok && lb_wait_warp(&sh->empty[rc.slot], rc.phase ^ 1, fail);
+            if (!ok) return;
+            if (lead) {
+                unsigned char* dst = ring + rc.slot * stage;
+                rgs_mbar_expect_tx(&sh->full[rc.slot], stage);
+                for (int u = 0; u < a.gs; u += P, ++k)
+#pragma unroll
+                    for (int p = 0; p < P; ++p) lb_tma(dst + (u + p) * TB, map, k * KC, row * LT, p, &sh->full[rc.slot]);
+            }
+            rc.next(a.stages);
+            ++loads;
+        };
+        // the order of stages is the order in which the MMA warp takes them: S(0), S(1), O(0), S(2), O(1), ...; with B kept
+        // for both products O takes nothing from the ring
+        bool have_prev = false;
+        int prev_j = 0, prev_oc0 = 0, prev_noc = 0, prev_dw = 0;
+        auto out_tiles = [&]() {
+            if (!GRAD || a.whole || !have_prev) return;
+            for (int oc = 0; oc < prev_noc && ok; ++oc) load(prev_dw ? &map_x : &map_w, prev_oc0 + oc, prev_j);
+        };
+        for (unsigned i = blockIdx.x; i < items && ok; i += gridDim.x) {
+            const LabelItem it = lb_item(a, i);
+            const CUtensorMap *ma = it.dw ? &map_w : &map_x, *mb = it.dw ? &map_x : &map_w;
+            if (a.a_slots) {
+                ok = lb_wait_warp(&sh->a_empty[ac.slot], ac.phase ^ 1, fail);
+                if (!ok) break;
+                if (lead) {
+                    unsigned char* dst = tiles + ac.slot * na * TB;
+                    rgs_mbar_expect_tx(&sh->a_full[ac.slot], na * TB);
+                    for (int k = 0; k < a.nk; ++k)
+#pragma unroll
+                        for (int p = 0; p < P; ++p) lb_tma(dst + (k * P + p) * TB, ma, k * KC, it.m * LT, p, &sh->a_full[ac.slot]);
                 }
-                for (int j = it.j0; j < it.j1 && ok; ++j) {
-                    const uint32_t s = kc % LKSLOTS;
-                    ok = lb_wait(&sh->k_empty[s], ((kc / LKSLOTS) & 1) ^ 1, fail);
-                    if (!ok) break;
+                ac.next(a.a_slots);
+            }
+            for (int j = it.j0; j < it.j1 && ok; ++j) {
+                ok = lb_wait_warp(&sh->k_empty[kc.slot], kc.phase ^ 1, fail);
+                if (!ok) break;
+                if (lead) {
                     const uint32_t bytes = it.dw ? LT * 16 : LT * 4;
-                    rgs_mbar_expect_tx(&sh->k_full[s], bytes);
-                    rgs_bulk_g2s(kbuf + s * (LKBYTES / 4), it.dw ? a.kn + (size_t)j * (LT * 4) : a.b2 + (size_t)j * LT, bytes, &sh->k_full[s]);
-                    ++kc;
+                    rgs_mbar_expect_tx(&sh->k_full[kc.slot], bytes);
+                    rgs_bulk_g2s(kbuf + kc.slot * (LKBYTES / 4), it.dw ? a.kn + (size_t)j * (LT * 4) : a.b2 + (size_t)j * LT, bytes, &sh->k_full[kc.slot]);
+                }
+                kc.next(LKSLOTS);
+                if (a.whole) {
+                    load(mb, 0, j);
+                } else {
                     for (int k = 0; k < a.nk && ok; ++k) {
-                        if (!a.a_slots)
-                            for (int p = 0; p < P && ok; ++p) tile(ma, k, it.m, p);
-                        for (int p = 0; p < P && ok; ++p) tile(mb, k, j, p);
+                        if (!a.a_slots) load(ma, k, it.m);
+                        load(mb, k, j);
                     }
                     out_tiles();
                     have_prev = true; prev_j = j; prev_oc0 = it.oc0; prev_noc = it.noc; prev_dw = it.dw;
                 }
             }
-            if (ok) out_tiles();
-            // copies still in flight land before the CTA leaves (all were consumed unless a wait ran out)
-            if (*fail) {
-                for (uint32_t k = cnt > (uint32_t)a.ring ? cnt - a.ring : 0; k < cnt; ++k) rgs_mbar_wait(&sh->full[k % a.ring], (k / a.ring) & 1, 1u << 16);
-                for (uint32_t k = kc > LKSLOTS ? kc - LKSLOTS : 0; k < kc; ++k) rgs_mbar_wait(&sh->k_full[k % LKSLOTS], (k / LKSLOTS) & 1, 1u << 16);
-                if (a.a_slots)
-                    for (uint32_t k = ai > (uint32_t)a.a_slots ? ai - a.a_slots : 0; k <= ai; ++k)
-                        rgs_mbar_wait(&sh->a_full[k % a.a_slots], (k / a.a_slots) & 1, 1u << 10);
+        }
+        if (ok) out_tiles();
+        if (*fail) {  // copies still in flight land before the CTA leaves (all were consumed unless a wait ran out)
+            const uint32_t live = loads < (uint32_t)a.stages ? loads : a.stages;
+            for (uint32_t k = 0; k < live; ++k) {
+                if (rc.slot == 0) { rc.slot = a.stages; rc.phase ^= 1; }
+                --rc.slot;
+                rgs_mbar_wait(&sh->full[rc.slot], rc.phase, 1u << 12);
+            }
+            for (int k = 0; k < LKSLOTS; ++k) {
+                if (kc.slot == 0) { kc.slot = LKSLOTS; kc.phase ^= 1; }
+                --kc.slot;
+                rgs_mbar_wait(&sh->k_full[kc.slot], kc.phase, 1u << 12);
+            }
+            for (int k = 0; k < a.a_slots; ++k) {
+                if (ac.slot == 0) { ac.slot = a.a_slots; ac.phase ^= 1; }
+                --ac.slot;
+                rgs_mbar_wait(&sh->a_full[ac.slot], ac.phase, 1u << 12);
             }
         }
-        __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------------------------------------------ MMA
-        if (lane == 0) {
-            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(LT >> 4) << 24);
-            uint32_t cnt = 0, ai = 0, ob = 0;  // ring tiles taken, items begun, outputs begun
-            bool ok = true;
-            auto take = [&](uint32_t k) {
-                ok = ok && lb_wait(&sh->full[k % a.ring], (k / a.ring) & 1, fail);
-                return rgs_smem_addr(ring + (size_t)(k % a.ring) * LTILE);
-            };
-            auto issue_s = [&](const LabelItem& it, int j, uint32_t t) {
-                if (a.a_slots && j == it.j0) ok = ok && lb_wait(&sh->a_full[ai % a.a_slots], (ai / a.a_slots) & 1, fail);
-                const uint32_t d = tmem + (t & 1) * SB;
-                uint32_t acc = 0;
-                for (int k = 0; k < a.nk && ok; ++k) {
-                    uint32_t at[P], bt[P];
-                    const uint32_t first = cnt;
-                    if (a.a_slots) {
+        // once a wait has run out the others return at once: the loop goes through its (bounded) motions on whatever lies in
+        // shared memory and TMEM, and the warpgroups write NaN
+        const bool lead = lb_elect();
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(LT >> 4) << 24);
+        LabelCursor rc, ac, oc_, gc;                         // ring, A, outputs; oldest stage not given back
+        const uint64_t dbase = lb_desc<KC>(), ring16 = rgs_smem_addr(ring) >> 4, tiles16 = rgs_smem_addr(tiles) >> 4;
+        constexpr uint32_t T16 = TB >> 4;
+        const uint32_t stage16 = stage >> 4;
+        const uint32_t last_steps = (uint32_t)(a.c - (a.nk - 1) * KC + 15) >> 4;  // of 16 channels, in the last chunk
+        auto take = [&]() {
+            lb_wait_quiet(&sh->full[rc.slot], rc.phase, fail);
+            const uint64_t d = dbase + ring16 + rc.slot * stage16;
+            rc.next(a.stages);
+            return d;
+        };
+        auto give = [&]() {
+            if (lead) lb_commit(&sh->empty[gc.slot]);
+            gc.next(a.stages);
+        };
+        // one chunk of S: the six products of pieces, up to KC / 16 steps each
+        auto chunk_s = [&](uint32_t d, uint64_t at, uint64_t bt, int k) {
+            const uint32_t steps = k == a.nk - 1 ? last_steps : KC / 16;
 #pragma unroll
-                        for (int p = 0; p < P; ++p) at[p] = rgs_smem_addr(tiles + (size_t)((ai % a.a_slots) * na + k * P + p) * LTILE);
-                    } else {
+            for (int q = 0; q < COMBOS; ++q)
 #pragma unroll
-                        for (int p = 0; p < P; ++p) at[p] = take(cnt++);
-                    }
-#pragma unroll
-                    for (int p = 0; p < P; ++p) bt[p] = take(cnt++);
-                    if (!ok) break;
+                for (uint32_t ks = 0; ks < KC / 16; ++ks)
+                    if (ks < steps) lb_mma_ss(d, at + CA[q] * T16 + ks * 2, bt + CB[q] * T16 + ks * 2, idesc | ((LT >> 3) << 17), !(k == 0 && q == 0 && ks == 0));
+        };
+        auto issue_s = [&](const LabelItem& it, int j, uint32_t t) {
+            const uint32_t d = tmem + (t & 1) * SB;
+            if (a.a_slots && j == it.j0) lb_wait_quiet(&sh->a_full[ac.slot], ac.phase, fail);
+            const uint64_t abase = dbase + tiles16 + ac.slot * (na * T16);
+            if (a.whole) {
+                const uint64_t bt = take();
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (lead)
+                    for (int k = 0; k < a.nk; ++k) chunk_s(d, abase + k * (P * T16), bt + k * (P * T16), k);
+                if (!GRAD) give();
+            } else {
+                for (int k = 0; k < a.nk; ++k) {
+                    const uint64_t at = a.a_slots ? abase + k * (P * T16) : take();
+                    const uint64_t bt = take();
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const int steps = min(4, (a.c - k * 64 + 15) >> 4);
-#pragma unroll
-                    for (int q = 0; q < COMBOS; ++q)
-                        for (int ks = 0; ks < steps; ++ks) {
-                            lb_mma_ss(d, lb_desc(at[CA[q]] + ks * 32), lb_desc(bt[CB[q]] + ks * 32), idesc | ((LT >> 3) << 17), acc);
-                            acc = 1;
-                        }
-                    if (!a.b_res)
-                        for (uint32_t u = first; u < cnt; ++u) lb_commit(&sh->empty[u % a.ring]);
-                }
-                if (!ok) return;
-                lb_commit(&sh->s_full[t & 1]);
-                if (j == it.j1 - 1) {
-                    if (a.a_slots) lb_commit(&sh->a_empty[ai % a.a_slots]);
-                    ++ai;
-                }
-            };
-            // G B for score buffer t; first: ring index of its B tiles when they are kept
-            auto issue_o = [&](const LabelItem& it, int j, uint32_t t, uint32_t first) {
-                ok = ok && lb_wait(&sh->s_done[t & 1], (t >> 1) & 1, fail);
-                if (j == it.j0) ok = ok && lb_wait(&sh->o_free[ob % a.nob], ((ob / a.nob) & 1) ^ 1, fail);
-                const uint32_t s = tmem + (t & 1) * SB, o = tmem + OUT + (ob % a.nob) * OB;
-                for (int oc = 0; oc < it.noc && ok; ++oc) {
-                    uint32_t bt[P];
-                    const uint32_t begin = cnt;
-#pragma unroll
-                    for (int p = 0; p < P; ++p) bt[p] = a.b_res ? rgs_smem_addr(ring + (size_t)((first + (it.oc0 + oc) * P + p) % a.ring) * LTILE) : take(cnt++);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t cols = min(64, (a.c - (it.oc0 + oc) * 64 + 15) & ~15);
-                    const uint32_t id = idesc | (1u << 16) | ((cols >> 3) << 17);
-#pragma unroll
-                    for (int q = 0; q < COMBOS; ++q)
-#pragma unroll
-                        for (int ks = 0; ks < 8; ++ks) {
-                            // 16 columns of G are 8 words: two such runs per group of 32 scores, the pieces behind one another
-                            const uint32_t g = CA[q] == 2 ? s + 128 + ks * 8 : s + (ks >> 1) * 32 + CA[q] * 16 + (ks & 1) * 8;
-                            lb_mma_ts(o + oc * 64, g, lb_desc(bt[CB[q]] + ks * 2048), id, !(j == it.j0 && q == 0 && ks == 0));
-                        }
-                    if (!a.b_res)
-                        for (uint32_t u = begin; u < cnt; ++u) lb_commit(&sh->empty[u % a.ring]);
-                }
-                if (!ok) return;
-                if (a.b_res)
-                    for (int u = 0; u < na; ++u) lb_commit(&sh->empty[(first + u) % a.ring]);
-                if (j == it.j1 - 1) lb_commit(&sh->o_full[ob++ % a.nob]);
-            };
-            uint32_t t = 0, prev_first = 0;
-            LabelItem prev;
-            int prev_j = 0;
-            bool have_prev = false;
-            for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
-                const LabelItem it = lb_item(a, i);
-                for (int j = it.j0; j < it.j1 && ok; ++j, ++t) {
-                    // forward: the scores of t-2 have been read; backward: G(t-2) B was issued before, and runs before
-                    if (!GRAD && t >= 2) ok = lb_wait(&sh->s_done[t & 1], ((t >> 1) & 1) ^ 1, fail);
-                    if (!ok) break;
-                    const uint32_t first = cnt;
-                    issue_s(it, j, t);
-                    if (GRAD) {
-                        if (have_prev && ok) issue_o(prev, prev_j, t - 1, prev_first);
-                        prev = it; prev_j = j; prev_first = first; have_prev = true;
-                    }
+                    if (lead) chunk_s(d, at, bt, k);
+                    if (!a.a_slots) give();
+                    give();
                 }
             }
-            if (GRAD && have_prev && ok) issue_o(prev, prev_j, t - 1, prev_first);
-            lb_commit(&sh->drain);
-            rgs_mbar_wait(&sh->drain, 0, LWAIT);
+            if (lead) lb_commit(&sh->s_full[t & 1]);
+            if (j == it.j1 - 1 && a.a_slots) {
+                if (lead) lb_commit(&sh->a_empty[ac.slot]);
+                ac.next(a.a_slots);
+            }
+        };
+        // G B of score buffer t; B as the K x N operand with its channels as N, 16 rows a step
+        auto chunk_o = [&](uint32_t s, uint32_t o, uint64_t bt, int chunk, bool fresh) {
+            const uint32_t cols = min(KC, (a.c - chunk * KC + 15) & ~15);
+            const uint32_t id = idesc | (1u << 16) | ((cols >> 3) << 17);
+#pragma unroll
+            for (int q = 0; q < COMBOS; ++q)
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) {
+                    // 16 columns of G are 8 words: the first two pieces lie over the 16 scores, the third behind all
+                    const uint32_t g = CA[q] == 2 ? s + 128 + ks * 8 : s + ks * 16 + CA[q] * 8;
+                    lb_mma_ts(o, g, bt + CB[q] * T16 + ks * (KC * 2), id, !(fresh && q == 0 && ks == 0));
+                }
+        };
+        auto issue_o = [&](const LabelItem& it, int j, uint32_t t) {
+            lb_wait_quiet(&sh->s_done[t & 1], (t >> 1) & 1, fail);
+            if (j == it.j0) lb_wait_quiet(&sh->o_free[oc_.slot], oc_.phase ^ 1, fail);
+            const uint32_t s = tmem + (t & 1) * SB, o = tmem + OUT + oc_.slot * OB;
+            if (a.whole) {  // the stage that S(t) took is the oldest one still held
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t bt = dbase + ring16 + gc.slot * stage16;
+                if (lead)
+                    for (int oc = 0; oc < it.noc; ++oc) chunk_o(s, o + oc * KC, bt + (it.oc0 + oc) * (P * T16), it.oc0 + oc, j == it.j0);
+                give();
+            } else {
+                for (int oc = 0; oc < it.noc; ++oc) {
+                    const uint64_t bt = take();
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (lead) chunk_o(s, o + oc * KC, bt, it.oc0 + oc, j == it.j0);
+                    give();
+                }
+            }
+            if (j == it.j1 - 1) {
+                if (lead) lb_commit(&sh->o_full[oc_.slot]);
+                oc_.next(a.nob);
+            }
+        };
+        uint32_t t = 0;
+        LabelItem prev;
+        int prev_j = 0;
+        bool have_prev = false;
+        for (unsigned i = blockIdx.x; i < items; i += gridDim.x) {
+            const LabelItem it = lb_item(a, i);
+            for (int j = it.j0; j < it.j1; ++j, ++t) {
+                // forward: the scores of t-2 have been read; backward: G(t-2) B was issued before, and runs before
+                if (!GRAD && t >= 2) lb_wait_quiet(&sh->s_done[t & 1], ((t >> 1) & 1) ^ 1, fail);
+                issue_s(it, j, t);
+                if (GRAD) {
+                    if (have_prev) issue_o(prev, prev_j, t - 1);
+                    prev = it; prev_j = j; have_prev = true;
+                }
+            }
         }
-        __syncwarp();
-    } else if (warp >= 4) {
+        if (GRAD && have_prev) issue_o(prev, prev_j, t - 1);
+        if (lead) lb_commit(&sh->drain);
+        rgs_mbar_wait(&sh->drain, 0, LWAIT);
+    } else {
         // ------------------------------------------------------------------------------------------------ scores
-        const int g = (warp - 4) >> 2;                       // warpgroup: takes the score tiles t with t % 2 == g
+        const int wg = (warp - 2) >> 2;                      // warpgroup: score tiles t with t % 2 == wg % 2,
+        const int half = (wg >> 1) * 64;                     // 64 of their columns
         const int wrow = (warp & 3) * 32, row = wrow + lane; // row of A
         const uint32_t lanes = (uint32_t)wrow << 16;
         const float nan = __int_as_float(0x7fc00000);
-        uint32_t t = 0, ob = 0;
+        const f2 log2e = mk2(LOG2E, LOG2E);
+        uint32_t t = 0, kept = 0;                            // score tiles seen; ring stage of the B block of tile t
+        LabelCursor oc_;
         bool dead = false;
-        int64_t out_i = blockIdx.x;                          // next item whose output this warpgroup writes
-        auto write_out = [&](int64_t i) {
+        unsigned out_i = blockIdx.x;                         // next item whose output this warpgroup writes
+        auto write_out = [&](unsigned i) {
             const LabelItem it = lb_item(a, i);
-            if (!dead) dead = __any_sync(0xffffffffu, !lb_wait(&sh->o_full[ob % a.nob], (ob / a.nob) & 1, fail));
+            if (!dead) dead = __any_sync(0xffffffffu, !lb_wait(&sh->o_full[oc_.slot], oc_.phase, fail));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t o = tmem + lanes + OUT + (ob % a.nob) * OB;
+            const uint32_t o = tmem + lanes + OUT + oc_.slot * OB;
             const int64_t r = (int64_t)it.m * LT + row, rows = it.dw ? a.v : a.n;
             const int ns = it.dw ? a.nsw : a.nsx;
             float scale = 1.f;
-            bool zero = false;
+            int label = 0;
             if (!it.dw) {
                 const float* k = a.kn + (size_t)it.m * (LT * 4);
                 scale = k[2 * LT + row];
-                zero = __float_as_int(k[3 * LT + row]) < 0;
+                label = __float_as_int(k[3 * LT + row]);
             }
-            for (int c0 = g * 16; c0 < it.noc * 64; c0 += 32) {
-                const int c = it.oc0 * 64 + c0;
+            for (int c0 = wg * 16; c0 < it.noc * KC; c0 += 64) {
+                const int c = it.oc0 * KC + c0;
                 if (c >= a.c) break;
                 uint32_t u[16];
                 tm_ld16(o + c0, u);
@@ -421,160 +506,215 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                         for (int q = 0; q < 16; q += 4) *reinterpret_cast<float4*>(p + q) = make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]);
                     } else {
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) f[q] = zero ? 0.f : f[q] * scale;
+                        for (int q = 0; q < 16; ++q) f[q] = label < 0 ? 0.f : f[q] * scale;
                         lb_store16(it.dw ? a.dw : a.dx, r, c, a.c, a.dtype, f);
                     }
                 }
                 __syncwarp();
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            rgs_mbar_arrive(&sh->o_free[ob % a.nob]);
-            ++ob;
+            rgs_mbar_arrive(&sh->o_free[oc_.slot]);
+            oc_.next(a.nob);
         };
-        const bool dirty = GRAD && P == 1 && a.b_res && a.flags[1] != 0.f;
-        for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+        const bool dirty = GRAD && P == 1 && a.whole && a.flags[1] != 0.f;
+        for (unsigned i = blockIdx.x; i < items; i += gridDim.x) {
             const LabelItem it = lb_item(a, i);
             const int64_t r = (int64_t)it.m * LT + row;
             // per-row values
             int64_t y = -1;
             float m2 = -INFINITY, inv_z = 0.f, sum = 0.f, b2row = 0.f;
             if (!it.dw) {
-                if (r < a.n) {
-                    y = rgs_label(a.labels, r, a.label_bytes, a.v);
-                    if (GRAD) { m2 = a.lse[r]; inv_z = ex2(-a.lse[a.n + r]); }
-                } else if (GRAD) {
+                if (GRAD) {
                     m2 = INFINITY;
+                    if (r < a.n) { m2 = a.lse[r]; inv_z = ex2(-a.lse[a.n + r]); }
+                    y = __float_as_int(a.kn[(size_t)it.m * (LT * 4) + 3 * LT + row]);
+                } else if (r < a.n) {
+                    y = rgs_label(a.labels, r, a.label_bytes, a.v);
                 }
             } else {
                 b2row = a.b2[r];
             }
             for (int j = it.j0; j < it.j1; ++j, ++t) {
-                if ((int)(t & 1) != g) continue;
-                const uint32_t s = tmem + lanes + (t & 1) * SB;
-                const uint32_t ks = t % LKSLOTS;
+                const uint32_t bstage = kept;
+                if (GRAD && P == 1 && ++kept == (uint32_t)a.stages) kept = 0;
+                if ((int)(t & 1) != (wg & 1)) continue;
+                const uint32_t s = tmem + lanes + (t & 1) * SB + half;
+                const uint32_t ks = t & (LKSLOTS - 1);
                 if (!dead) {  // the whole warp goes on or none of it: TMEM accesses are warp-wide
                     dead = !lb_wait(&sh->k_full[ks], (t / LKSLOTS) & 1, fail) || !lb_wait(&sh->s_full[t & 1], (t >> 1) & 1, fail);
                     dead = __any_sync(0xffffffffu, dead);
                 }
                 if (dead) continue;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const float* kb = kbuf + ks * (LKBYTES / 4);
-                const int64_t yt = y - (int64_t)j * LT;
-                const int yl = yt >= 0 && yt < LT ? (int)yt : -1024;  // label within the tile (forward, dX)
-                const int vrow = it.dw ? (int)r : 0;
-                uint32_t u[32];
-#pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    __syncwarp();
-                    tm_ld32(s + c * 32, u);
-                    tm_wait_ld32(u);
-                    float f[32];
-                    if (!GRAD || !it.dw) {
+                const float* kb = kbuf + ks * (LKBYTES / 4) + half;
+                const int64_t yt = y - (int64_t)j * LT - half;
+                const int yl = y >= 0 && yt >= 0 && yt < 64 ? (int)yt : -1;  // the row's label among these columns
+                if (!GRAD) {
+                    uint32_t u[2][32];
+                    tm_ld32(s, u[0]);
+                    tm_ld32(s + 32, u[1]);
+                    tm_wait_ld32(u[0]);
+                    tm_wait_ld32(u[1]);
+                    // all scores are in registers: the buffer is free for the product after the next
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    rgs_mbar_arrive(&sh->s_done[t & 1]);
 #pragma unroll
-                        for (int q = 0; q < 32; q += 4) {
-                            const float4 b = *reinterpret_cast<const float4*>(kb + c * 32 + q);
-                            f[q] = fmaf(__uint_as_float(u[q]), LOG2E, b.x);
-                            f[q + 1] = fmaf(__uint_as_float(u[q + 1]), LOG2E, b.y);
-                            f[q + 2] = fmaf(__uint_as_float(u[q + 2]), LOG2E, b.z);
-                            f[q + 3] = fmaf(__uint_as_float(u[q + 3]), LOG2E, b.w);
+                    for (int h = 0; h < 2; ++h) {
+                        f2 v[16];
+                        float f[32];
+#pragma unroll
+                        for (int q = 0; q < 16; q += 2) {
+                            const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(kb + h * 32 + 2 * q);
+                            v[q] = fma2(mk2u(u[h][2 * q], u[h][2 * q + 1]), log2e, b.x);
+                            v[q + 1] = fma2(mk2u(u[h][2 * q + 2], u[h][2 * q + 3]), log2e, b.y);
                         }
-                    }
-                    if (!GRAD) {
-                        float top = f[0];
 #pragma unroll
-                        for (int q = 1; q < 32; ++q) top = fmaxf(top, f[q]);
-                        if ((unsigned)(yl - c * 32) < 32u) {
+                        for (int q = 0; q < 16; ++q) un2(v[q], f[2 * q], f[2 * q + 1]);
+                        float top[4];
 #pragma unroll
-                            for (int q = 0; q < 32; ++q)
-                                if (yl - c * 32 == q) a.at[r] = f[q];
+                        for (int q = 0; q < 4; ++q) {
+                            top[q] = fmaxf(f[q], f[q + 4]);
+#pragma unroll
+                            for (int e = 8; e < 32; e += 8) top[q] = fmaxf(top[q], fmaxf(f[q + e], f[q + e + 4]));
                         }
-                        top = fmaxf(m2, top);
-                        const float ref = top == -INFINITY ? 0.f : top;
-                        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                        if ((yl >> 5) == h) {  // one of the 32 by the bits of its index
+                            float z[16];
 #pragma unroll
-                        for (int q = 0; q < 32; ++q) acc[q & 3] += ex2(f[q] - ref);
-                        sum = fmaf(sum, ex2(m2 - ref), (acc[0] + acc[1]) + (acc[2] + acc[3]));
-                        m2 = top;
-                        continue;
-                    }
-                    if (!it.dw) {
+                            for (int q = 0; q < 16; ++q) z[q] = yl & 16 ? f[q + 16] : f[q];
 #pragma unroll
-                        for (int q = 0; q < 32; ++q) f[q] = ex2(f[q] - m2) * inv_z;
-                        if ((unsigned)(yl - c * 32) < 32u) {
+                            for (int w = 8; w > 0; w >>= 1)
 #pragma unroll
-                            for (int q = 0; q < 32; ++q)
-                                if (yl - c * 32 == q) f[q] -= 1.f;
+                                for (int q = 0; q < w; ++q) z[q] = yl & w ? z[q + w] : z[q];
+                            a.at[r] = z[0];
                         }
-                    } else {
-                        float acc = 0.f;
-#pragma unroll
-                        for (int q = 0; q < 32; q += 4) {
-                            const float4 m = *reinterpret_cast<const float4*>(kb + c * 32 + q);
-                            const float4 z = *reinterpret_cast<const float4*>(kb + LT + c * 32 + q);
-                            const int4 l = *reinterpret_cast<const int4*>(kb + 3 * LT + c * 32 + q);
-                            f[q] = ex2(fmaf(__uint_as_float(u[q]), LOG2E, b2row) - m.x) * z.x;
-                            f[q + 1] = ex2(fmaf(__uint_as_float(u[q + 1]), LOG2E, b2row) - m.y) * z.y;
-                            f[q + 2] = ex2(fmaf(__uint_as_float(u[q + 2]), LOG2E, b2row) - m.z) * z.z;
-                            f[q + 3] = ex2(fmaf(__uint_as_float(u[q + 3]), LOG2E, b2row) - m.w) * z.w;
-                            if (l.x == vrow) f[q] -= kb[2 * LT + c * 32 + q];
-                            if (l.y == vrow) f[q + 1] -= kb[2 * LT + c * 32 + q + 1];
-                            if (l.z == vrow) f[q + 2] -= kb[2 * LT + c * 32 + q + 2];
-                            if (l.w == vrow) f[q + 3] -= kb[2 * LT + c * 32 + q + 3];
-                            if (P == 1 && dirty) {
-                                if (l.x < 0) f[q] = 0.f;
-                                if (l.y < 0) f[q + 1] = 0.f;
-                                if (l.z < 0) f[q + 2] = 0.f;
-                                if (l.w < 0) f[q + 3] = 0.f;
-                            }
-                            acc += (f[q] + f[q + 1]) + (f[q + 2] + f[q + 3]);
-                        }
-                        sum += acc;
-                    }
-                    uint32_t w0[16];
-#pragma unroll
-                    for (int q = 0; q < 16; ++q) w0[q] = bf16x2(f[2 * q], f[2 * q + 1]);
-                    __syncwarp();
-                    tm_st16(s + c * 32, w0);
-                    if (P == 3) {
-                        uint32_t w1[16];
+                        const float best = fmaxf(m2, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+                        const float ref = best == -INFINITY ? 0.f : best;
+                        const f2 minus = mk2(-ref, -ref);
+                        f2 acc[2] = {0ull, 0ull};
 #pragma unroll
                         for (int q = 0; q < 16; ++q) {
-                            f[2 * q] -= bf_lo(w0[q]);
-                            f[2 * q + 1] -= bf_hi(w0[q]);
-                            w1[q] = bf16x2(f[2 * q], f[2 * q + 1]);
+                            float e0, e1;
+                            un2(add2(v[q], minus), e0, e1);
+                            acc[q & 1] = add2(acc[q & 1], mk2(ex2(e0), ex2(e1)));
                         }
-                        tm_st16(s + c * 32 + 16, w1);
+                        float s0, s1;
+                        un2(add2(acc[0], acc[1]), s0, s1);
+                        sum = fmaf(sum, ex2(m2 - ref), s0 + s1);
+                        m2 = best;
+                    }
+                    rgs_mbar_arrive(&sh->k_empty[ks]);
+                    continue;
+                }
+#pragma unroll 1
+                for (int h = 0; h < 64; h += 32) {
+                    uint32_t u[32];
+                    __syncwarp();
+                    tm_ld32(s + h, u);
+                    tm_wait_ld32(u);
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) w0[q] = bf16x2(f[2 * q] - bf_lo(w1[q]), f[2 * q + 1] - bf_hi(w1[q]));
-                        tm_st16(s + 128 + c * 16, w0);
+                    for (int o = 0; o < 32; o += 16) {  // 16 columns: one step of the product's inner dimension
+                        float e[16];
+                        if (!it.dw) {
+                            const f2 minus = mk2(-m2, -m2), factor = mk2(inv_z, inv_z);
+#pragma unroll
+                            for (int q = 0; q < 16; q += 4) {
+                                const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(kb + h + o + q);
+                                un2(add2(fma2(mk2u(u[o + q], u[o + q + 1]), log2e, b.x), minus), e[q], e[q + 1]);
+                                un2(add2(fma2(mk2u(u[o + q + 2], u[o + q + 3]), log2e, b.y), minus), e[q + 2], e[q + 3]);
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) e[q + k] = ex2(e[q + k]);
+                                un2(mul2(mk2(e[q], e[q + 1]), factor), e[q], e[q + 1]);
+                                un2(mul2(mk2(e[q + 2], e[q + 3]), factor), e[q + 2], e[q + 3]);
+                            }
+                            if ((yl >> 4) == ((h + o) >> 4)) {  // before the rounding: p - 1 of a pixel that is nearly certain is small
+#pragma unroll
+                                for (int q = 0; q < 16; ++q) sub_if(e[q], 1.f, yl & 15, q);
+                            }
+                        } else {
+                            const f2 b2 = mk2(b2row, b2row);
+#pragma unroll
+                            for (int q = 0; q < 16; q += 4) {  // the constants hold -m: one addition
+                                const ulonglong2 m = *reinterpret_cast<const ulonglong2*>(kb + h + o + q);
+                                const ulonglong2 z = *reinterpret_cast<const ulonglong2*>(kb + LT + h + o + q);
+                                un2(add2(fma2(mk2u(u[o + q], u[o + q + 1]), log2e, b2), m.x), e[q], e[q + 1]);
+                                un2(add2(fma2(mk2u(u[o + q + 2], u[o + q + 3]), log2e, b2), m.y), e[q + 2], e[q + 3]);
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) e[q + k] = ex2(e[q + k]);
+                                un2(mul2(mk2(e[q], e[q + 1]), z.x), e[q], e[q + 1]);
+                                un2(mul2(mk2(e[q + 2], e[q + 3]), z.y), e[q + 2], e[q + 3]);
+                            }
+                            // pixels of these 16 whose label is one of the warp's 32 rows
+                            const int* lab = reinterpret_cast<const int*>(kb + 3 * LT + h + o);
+                            if (__any_sync(0xffffffffu, (unsigned)(lab[lane & 15] - it.m * LT - wrow) < 32u)) {
+#pragma unroll
+                                for (int q = 0; q < 16; q += 4) {
+                                    const int4 l = *reinterpret_cast<const int4*>(lab + q);
+                                    const float4 g = *reinterpret_cast<const float4*>(kb + 2 * LT + h + o + q);
+                                    sub_if(e[q], g.x, l.x, (int)r);
+                                    sub_if(e[q + 1], g.y, l.y, (int)r);
+                                    sub_if(e[q + 2], g.z, l.z, (int)r);
+                                    sub_if(e[q + 3], g.w, l.w, (int)r);
+                                }
+                            }
+                            if (P == 1 && dirty) {
+#pragma unroll
+                                for (int q = 0; q < 16; ++q)
+                                    if (lab[q] < 0) e[q] = 0.f;
+                            }
+                            if (a.part_b) {
+                                f2 acc = mk2(e[0], e[1]);
+#pragma unroll
+                                for (int q = 2; q < 16; q += 2) acc = add2(acc, mk2(e[q], e[q + 1]));
+                                float s0, s1;
+                                un2(acc, s0, s1);
+                                sum += s0 + s1;
+                            }
+                        }
+                        uint32_t w0[8];
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) w0[q] = bf16x2(e[2 * q], e[2 * q + 1]);
+                        __syncwarp();
+                        tm_st8(s + h + o, w0);
+                        if (P == 3) {
+                            uint32_t w1[8];
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) {
+                                e[2 * q] -= bf_lo(w0[q]);
+                                e[2 * q + 1] -= bf_hi(w0[q]);
+                                w1[q] = bf16x2(e[2 * q], e[2 * q + 1]);
+                            }
+                            tm_st8(s + h + o + 8, w1);
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) w0[q] = bf16x2(e[2 * q] - bf_lo(w1[q]), e[2 * q + 1] - bf_hi(w1[q]));
+                            tm_st8(s - half + 128 + ((half + h + o) >> 1), w0);
+                        }
                     }
                 }
                 if (P == 1 && dirty && it.dw) {
                     // pixels without a label whose features are not finite: 0 * inf must not reach dW, so their rows of the
-                    // staged tile are cleared (row n of every chunk; a whole 128-byte row, whatever the swizzle)
-                    if (__float_as_int(kb[3 * LT + row]) < 0) {
+                    // staged block are cleared (row n of every chunk, whole, whatever the swizzle)
+                    if (__float_as_int(kb[3 * LT + row - half]) < 0) {
                         for (int k = 0; k < a.nk; ++k) {
-                            uint4* p = reinterpret_cast<uint4*>(ring + (size_t)(((uint64_t)t * na + k) % a.ring) * LTILE + row * 128);
+                            uint4* p = reinterpret_cast<uint4*>(ring + bstage * stage + k * TB + row * (KC * 2));
 #pragma unroll
-                            for (int q = 0; q < 8; ++q) p[q] = make_uint4(0, 0, 0, 0);
+                            for (int q = 0; q < KC / 8; ++q) p[q] = make_uint4(0, 0, 0, 0);
                         }
                     }
                     rgs_fence_proxy_async();
                 }
-                if (GRAD) asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 rgs_mbar_arrive(&sh->k_empty[ks]);
                 rgs_mbar_arrive(&sh->s_done[t & 1]);
-                if (GRAD)
-                    for (; out_i < i; out_i += gridDim.x) write_out(out_i);  // outputs of earlier items, behind the first scores of this one
+                for (; out_i < i; out_i += gridDim.x) write_out(out_i);  // outputs of earlier items, behind the first scores of this one
             }
             if (!GRAD) {
                 if (r < a.n) {
-                    a.pm[((int64_t)it.split * 2 + g) * a.n + r] = dead ? nan : m2;
-                    a.ps[((int64_t)it.split * 2 + g) * a.n + r] = dead ? nan : sum;
+                    a.pm[((int64_t)it.split * 4 + wg) * a.n + r] = dead ? nan : m2;
+                    a.ps[((int64_t)it.split * 4 + wg) * a.n + r] = dead ? nan : sum;
                 }
             } else if (it.dw && a.part_b && it.oc0 == 0) {
-                a.part_b[((int64_t)it.split * 2 + g) * a.nmw * LT + r] = dead ? nan : sum;
+                a.part_b[((int64_t)it.split * 4 + wg) * a.nmw * LT + r] = dead ? nan : sum;
             }
         }
         if (GRAD)
@@ -583,7 +723,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -663,14 +803,14 @@ __global__ void __launch_bounds__(256) rgs_label_prep_kernel(const __grid_consta
         }
         k -= gb;
         const int64_t y = k < a.n ? rgs_label(a.labels, k, a.label_bytes, a.v) : -1;
-        float m = INFINITY, z = 0.f, g = 0.f;
+        float m = INFINITY, z = 0.f, g = 0.f;  // -m is what is kept: a pixel without a label has exp(-inf) = 0
         if (y >= 0) {
             g = a.gout[a.per_row ? k : 0] * (a.count ? 1.f / fmaxf(a.count[0], 1.f) : 1.f);
             m = a.lse[k];
             z = g * exp2f(-a.lse[a.n + k]);
         }
         float* o = a.kn + (k / LT) * (4 * LT) + k % LT;
-        o[0] = m; o[LT] = z; o[2 * LT] = g; o[3 * LT] = __int_as_float((int)y);
+        o[0] = -m; o[LT] = z; o[2 * LT] = g; o[3 * LT] = __int_as_float((int)y);
     }
 }
 
@@ -752,7 +892,7 @@ __global__ void __launch_bounds__(256) rgs_label_reduce_kernel(const __grid_cons
         if (i >= tx + tw) {
             const int64_t v = i - tx - tw;
             float s = 0.f;
-            for (int k = 0; k < 2 * a.nsw; ++k) s += a.part_b[((int64_t)k * a.nmw) * LT + v];
+            for (int k = 0; k < 4 * a.nsw; ++k) s += a.part_b[((int64_t)k * a.nmw) * LT + v];
             rgs_store_float(db, v, b_dtype, s);
             continue;
         }
@@ -802,15 +942,15 @@ static LabelEncode label_encode() {
     return fn;
 }
 
-// (channels, rows, pieces) of bf16; boxes of 64 channels x 128 rows; what lies outside reads as zero
-static int label_map(CUtensorMap* map, const void* base, int64_t c, int64_t rows, int64_t ld, int64_t pieces) {
+// (channels, rows, pieces) of bf16; boxes of kc channels x 128 rows; what lies outside reads as zero
+static int label_map(CUtensorMap* map, const void* base, int64_t c, int64_t rows, int64_t ld, int64_t pieces, int kc) {
     LabelEncode enc = label_encode();
     if (!enc) return 20;
     const cuuint64_t dims[3] = {(cuuint64_t)c, (cuuint64_t)rows, (cuuint64_t)pieces};
     const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)ld * 2 * (cuuint64_t)rows};
-    const cuuint32_t box[3] = {64, LT, 1}, estr[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {(cuuint32_t)kc, LT, 1}, estr[3] = {1, 1, 1};
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : 21;
+               kc == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : 21;
 }
 
 static inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
@@ -829,7 +969,7 @@ static int label_pieces(int64_t tiles, int64_t nj, int64_t sms, int64_t run, int
 
 struct LabelPlan {
     LabelArgs a;
-    int pieces, direct_x, direct_w, cp;
+    int pieces, kc, direct_x, direct_w, cp;
     int64_t o_xs, o_ws, o_b2, o_kn, o_pm, o_ps, o_at, o_px, o_pw, o_pb, o_bsum, o_bcount, o_ticket, bytes;
 };
 
@@ -840,21 +980,26 @@ static void label_plan(LabelPlan& p, int64_t n, int64_t c, int64_t v, int dtype,
     memset(&p, 0, sizeof(p));
     const int64_t sms = RGS_SMS;
     p.pieces = dtype == RGS_BF16 ? 1 : 3;
-    a.n = n; a.v = v; a.c = (int)c; a.nk = (int)((c + 63) / 64);
+    p.kc = c <= 32 ? 32 : 64;
+    a.n = n; a.v = v; a.c = (int)c; a.nk = (int)((c + p.kc - 1) / p.kc);
     a.nmx = (int)((n + LT - 1) / LT); a.nmw = (int)((v + LT - 1) / LT);
     a.dtype = dtype;
-    const int na = p.pieces * a.nk;
-    // tiles of A stay where eight of them fit; two blocks of them where that leaves two blocks of B
-    a.a_slots = na > 8 ? 0 : (LSLOTS - 2 * na >= 2 * na ? 2 : 1);
-    a.ring = LSLOTS - a.a_slots * na;
-    a.b_res = backward && a.a_slots && a.ring >= 2 * na;
-    const int cols = p.pieces == 1 ? 4 : 2;  // chunks of output channels that TMEM holds beside the scores
+    const int na = p.pieces * a.nk, room = LROOM / (256 * p.kc);
+    // whole blocks of B where a block of A (better two) leaves room for two (three) of them; else chunk by chunk, A staying
+    // where half of the room holds it
+    a.whole = 1; a.gs = na;
+    if (room >= 5 * na) a.a_slots = 2;
+    else if (room >= 3 * na) a.a_slots = 1;
+    else { a.whole = 0; a.gs = p.pieces; a.a_slots = na <= 8 ? 1 : 0; }
+    a.stages = (room - a.a_slots * na) / a.gs;
+    if (a.stages > LSTAGES) a.stages = LSTAGES;
+    const int cols = (p.pieces == 1 ? 256 : 128) / p.kc;  // chunks of output channels that TMEM holds beside the scores
     a.noc = a.nk < cols ? a.nk : cols;
     a.nrange = backward ? (a.nk + a.noc - 1) / a.noc : 1;
     a.nob = 2 * a.noc <= cols ? 2 : 1;
     a.cq = (int)up(c, 16);
     // where B is fetched anew for the second product its rows cannot be cleared in place: X goes through the copy
-    p.direct_x = p.pieces == 1 && (direct & 1) && (!backward || a.b_res);
+    p.direct_x = p.pieces == 1 && (direct & 1) && (!backward || a.whole);
     p.direct_w = p.pieces == 1 && (direct & 2);
     p.cp = (int)up(c, 8);
     const int64_t run = p.pieces == 1 ? 512 : 32;
@@ -867,6 +1012,8 @@ static void label_plan(LabelPlan& p, int64_t n, int64_t c, int64_t v, int dtype,
         a.nsx = label_pieces(a.nmx, a.nmw, sms, a.nmw, a.nmw);
         a.nsw = 1;
     }
+    a.perx = a.nmw / a.nsx; a.restx = a.nmw % a.nsx;
+    a.perw = a.nmx / a.nsw; a.restw = a.nmx % a.nsw;
     int64_t o = 0;
     auto take = [&](int64_t bytes) { const int64_t at = o; o = up(o + bytes, 1024); return at; };
     p.o_xs = p.direct_x ? -1 : take(n * p.cp * 2 * p.pieces);
@@ -876,10 +1023,10 @@ static void label_plan(LabelPlan& p, int64_t n, int64_t c, int64_t v, int dtype,
         p.o_kn = take(rows_x * 16);
         p.o_px = a.nsx > 1 ? take(a.nsx * rows_x * a.cq * 4) : -1;
         p.o_pw = a.nsw > 1 ? take(a.nsw * rows_w * a.cq * 4) : -1;
-        p.o_pb = take(2 * a.nsw * rows_w * 4);
+        p.o_pb = take(4 * a.nsw * rows_w * 4);
     } else {
-        p.o_pm = take(2 * a.nsx * n * 4);
-        p.o_ps = take(2 * a.nsx * n * 4);
+        p.o_pm = take(4 * a.nsx * n * 4);
+        p.o_ps = take(4 * a.nsx * n * 4);
         p.o_at = take(n * 4);
         p.o_bsum = take(LJOIN * 8);
         p.o_bcount = take(LJOIN * 8);
@@ -893,18 +1040,24 @@ static int label_direct(const void* x, int64_t ldx, const void* w, int64_t ldw) 
     return dx | (dw << 1);
 }
 
-template <int P, bool GRAD>
-static int label_run(const CUtensorMap& mx, const CUtensorMap& mw, const LabelArgs& a, cudaStream_t stream) {
+template <int P, bool GRAD, int KC>
+static int label_launch(const CUtensorMap& mx, const CUtensorMap& mw, const LabelArgs& a, cudaStream_t stream) {
     static std::atomic<uint64_t> ready{0};  // devices whose limit on dynamic shared memory was raised
     int dev = 0;
     RGS_CUDA_CHECK(cudaGetDevice(&dev));
     if (dev > 63 || !((ready.load() >> dev) & 1)) {
-        RGS_CUDA_CHECK(cudaFuncSetAttribute(rgs_label_tc_kernel<P, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, LSMEM));
+        RGS_CUDA_CHECK(cudaFuncSetAttribute(rgs_label_tc_kernel<P, GRAD, KC>, cudaFuncAttributeMaxDynamicSharedMemorySize, LSMEM));
         if (dev <= 63) ready.fetch_or((uint64_t)1 << dev);
     }
-    const int64_t items = a.items_x + a.items_w, sms = RGS_SMS;
-    rgs_label_tc_kernel<P, GRAD><<<(unsigned)(items < sms ? items : sms), LTHREADS, LSMEM, stream>>>(mx, mw, a);
+    const int64_t items = (int64_t)a.items_x + a.items_w, sms = RGS_SMS;
+    rgs_label_tc_kernel<P, GRAD, KC><<<(unsigned)(items < sms ? items : sms), LTHREADS, LSMEM, stream>>>(mx, mw, a);
     return (int)cudaGetLastError();
+}
+
+template <bool GRAD>
+static int label_run(const LabelPlan& p, const CUtensorMap& mx, const CUtensorMap& mw, cudaStream_t stream) {
+    if (p.pieces == 1) return p.kc == 64 ? label_launch<1, GRAD, 64>(mx, mw, p.a, stream) : label_launch<1, GRAD, 32>(mx, mw, p.a, stream);
+    return p.kc == 64 ? label_launch<3, GRAD, 64>(mx, mw, p.a, stream) : label_launch<3, GRAD, 32>(mx, mw, p.a, stream);
 }
 
 static inline unsigned label_grid(int64_t work, int64_t most) {
@@ -917,9 +1070,9 @@ static int label_operands(const LabelPlan& p, const LabelPrep& q, CUtensorMap* m
     int dev = 0;
     RGS_CUDA_CHECK(cudaGetDevice(&dev));
     RGS_CUDA_CHECK(cudaSetDevice(dev));
-    int rc = p.direct_x ? label_map(mx, q.x, q.c, q.n, q.ldx, 1) : label_map(mx, q.xs, p.cp, q.n, p.cp, p.pieces);
+    int rc = p.direct_x ? label_map(mx, q.x, q.c, q.n, q.ldx, 1, p.kc) : label_map(mx, q.xs, p.cp, q.n, p.cp, p.pieces, p.kc);
     if (rc) return rc;
-    return p.direct_w ? label_map(mw, q.w, q.c, q.v, q.ldw, 1) : label_map(mw, q.ws, p.cp, q.v, p.cp, p.pieces);
+    return p.direct_w ? label_map(mw, q.w, q.c, q.v, q.ldw, 1, p.kc) : label_map(mw, q.ws, p.cp, q.v, p.cp, p.pieces, p.kc);
 }
 
 static void label_prep(const LabelPlan& p, const LabelPrep& q, cudaStream_t stream) {
@@ -952,16 +1105,16 @@ int rgs_cuda_label_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     if (rc) return rc;
     label_prep(p, q, st);
     RGS_CUDA_CHECK(cudaGetLastError());
-    a.items_x = (int64_t)a.nmx * a.nsx;
+    a.items_x = (unsigned)a.nmx * a.nsx;
     a.b2 = q.b2;
     a.labels = labels; a.label_bytes = (int)label_bytes;
     a.flags = count;
     a.pm = reinterpret_cast<float*>(s + p.o_pm);
     a.ps = reinterpret_cast<float*>(s + p.o_ps);
     a.at = reinterpret_cast<float*>(s + p.o_at);
-    rc = p.pieces == 1 ? label_run<1, false>(mx, mw, a, st) : label_run<3, false>(mx, mw, a, st);
+    rc = label_run<false>(p, mx, mw, st);
     if (rc) return rc;
-    rgs_label_join_kernel<<<label_grid(n, LJOIN), 256, 0, st>>>(a.pm, a.ps, a.at, labels, (int)label_bytes, n, vocab, 2 * a.nsx, (int)mean, lse, losses,
+    rgs_label_join_kernel<<<label_grid(n, LJOIN), 256, 0, st>>>(a.pm, a.ps, a.at, labels, (int)label_bytes, n, vocab, 4 * a.nsx, (int)mean, lse, losses,
                                                                 result, count, reinterpret_cast<double*>(s + p.o_bsum),
                                                                 reinterpret_cast<unsigned long long*>(s + p.o_bcount), q.ticket);
     return (int)cudaGetLastError();
@@ -984,8 +1137,8 @@ int rgs_cuda_label_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     if (rc) return rc;
     label_prep(p, q, st);
     RGS_CUDA_CHECK(cudaGetLastError());
-    a.items_x = dx ? (int64_t)a.nmx * a.nrange * a.nsx : 0;
-    a.items_w = dw || db ? (int64_t)a.nmw * a.nrange * a.nsw : 0;
+    a.items_x = dx ? (unsigned)a.nmx * a.nrange * a.nsx : 0;
+    a.items_w = dw || db ? (unsigned)a.nmw * a.nrange * a.nsw : 0;
     a.b2 = q.b2; a.kn = q.kn; a.lse = lse;
     a.labels = labels; a.label_bytes = (int)label_bytes;
     a.flags = count;
@@ -993,7 +1146,7 @@ int rgs_cuda_label_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     a.part_w = dw && a.nsw > 1 ? reinterpret_cast<float*>(s + p.o_pw) : nullptr;
     a.part_b = db ? reinterpret_cast<float*>(s + p.o_pb) : nullptr;
     a.dx = dx; a.dw = dw;
-    rc = p.pieces == 1 ? label_run<1, true>(mx, mw, a, st) : label_run<3, true>(mx, mw, a, st);
+    rc = label_run<true>(p, mx, mw, st);
     if (rc) return rc;
     if (a.part_x || a.part_w || db) {
         const int64_t work = (a.part_x ? n * (a.cq / 4) : 0) + (a.part_w ? vocab * (a.cq / 4) : 0) + (db ? vocab : 0);
