@@ -44,8 +44,8 @@ struct LabelArgs {
     int c, nk;                       // channels, chunks of 64 (32) channels
     int noc, nrange;                 // chunks of output channels per item, ranges of them
     int a_slots;                     // blocks of A that stay in shared memory (0: A goes through the ring)
-    int whole, gs, stages;           // a stage holds a whole block of B, kept for both products; tiles of a stage; stages
-    int nob;                         // output buffers in TMEM
+    int whole, stages;               // stages of B are kept for both products; stages of the ring
+    int nbuf, nob;                   // score and output buffers in TMEM
     int nmx, nmw;                    // tiles of 128 pixels, of 128 labels
     int nsx, nsw;                    // pieces of the walk over labels (forward, dX) and over pixels (dW)
     int perx, restx, perw, restw;    // tiles of a piece: per, one more in the first rest pieces
@@ -83,8 +83,12 @@ __device__ __forceinline__ bool lb_wait(unsigned long long* bar, uint32_t parity
 __device__ __forceinline__ bool lb_wait_warp(unsigned long long* bar, uint32_t parity, volatile int* fail) {
     return __all_sync(0xffffffffu, lb_wait(bar, parity, fail));
 }
+__device__ __noinline__ void lb_wait_slow(unsigned long long* bar, uint32_t parity, volatile int* fail) { lb_wait(bar, parity, fail); }
 __device__ __forceinline__ void lb_wait_quiet(unsigned long long* bar, uint32_t parity, volatile int* fail) {
-    lb_wait(bar, parity, fail);
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(rgs_smem_addr(bar)), "r"(parity) : "memory");
+    if (!ok) lb_wait_slow(bar, parity, fail);
     __syncwarp();
 }
 // One lane of a converged warp.  The producer and MMA warps run their loops with all lanes and let this one issue: the
@@ -102,20 +106,21 @@ __device__ __forceinline__ void lb_tma(void* dst, const CUtensorMap* map, int x,
 __device__ __forceinline__ void lb_commit(unsigned long long* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(rgs_smem_addr(bar)) : "memory");
 }
-// shared-memory descriptor of a tile at address 0: rows of KC channels under the swizzle of their length (128 or 64 bytes),
-// eight rows to a pattern; both strides are that of the pattern, so it reads rows as K-major or as steps of K
+// Shared-memory descriptors: rows of KC channels under the swizzle of their length (128 or 64 bytes), eight rows to a
+// pattern; both strides are that of the pattern, so a tile reads as K-major rows or as steps of K.  The low word holds the
+// address (in 16 bytes), the high word never changes: the products below take the low words alone.
+template <int KC> constexpr uint32_t lb_desc_lo = (uint32_t)KC << 16;
+template <int KC> constexpr uint32_t lb_desc_hi = (uint32_t)KC | (1u << 14) | ((KC == 64 ? 2u : 4u) << 29);
+
 template <int KC>
-__device__ __forceinline__ uint64_t lb_desc() {
-    constexpr uint64_t pattern = (KC * 16) >> 4;
-    return (pattern << 16) | (pattern << 32) | ((uint64_t)1 << 46) | ((uint64_t)(KC == 64 ? 2 : 4) << 61);
+__device__ __forceinline__ void lb_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "n"(lb_desc_hi<KC>) : "memory");
 }
-__device__ __forceinline__ void lb_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::
-                 "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
-}
-__device__ __forceinline__ void lb_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::
-                 "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+template <int KC>
+__device__ __forceinline__ void lb_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 y, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "n"(lb_desc_hi<KC>) : "memory");
 }
 #define LB_R16(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7]), \
     "+r"(r[o + 8]), "+r"(r[o + 9]), "+r"(r[o + 10]), "+r"(r[o + 11]), "+r"(r[o + 12]), "+r"(r[o + 13]), "+r"(r[o + 14]), "+r"(r[o + 15])
@@ -222,18 +227,21 @@ __device__ __forceinline__ void lb_store16(void* out, int64_t r, int c, int chan
 
 struct LabelShared {
     unsigned long long full[LSTAGES], empty[LSTAGES], a_full[2], a_empty[2], k_full[LKSLOTS], k_empty[LKSLOTS];
-    unsigned long long s_full[2], s_done[2], o_full[2], o_free[2], drain;
+    unsigned long long s_full[4], s_done[4], o_full[2], o_free[2], drain;
     uint32_t tmem;
     int fail;
 };
 #define LSMEM (1024 + LROOM + LKSLOTS * LKBYTES + (int)sizeof(LabelShared))
 
-template <int P, bool GRAD, int KC>
+template <int P, bool GRAD, int KC, int CS>
 __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                                                                    const __grid_constant__ LabelArgs a) {
-    constexpr int SB = P == 1 ? 128 : 192;        // TMEM columns of a score buffer (scores; over them G, its third piece behind)
-    constexpr int OUT = 2 * SB;                   // first column of the outputs
-    constexpr int OB = P == 1 ? 128 : 64;         // columns of an output buffer when there are two
+    constexpr int SB = GRAD && P == 3 ? 192 : 128;  // TMEM columns of a score buffer (scores; over them G, its third piece behind)
+    // 32-bit outputs are summed in two buffers: the leading products, eight steps to a tile, and the small ones.  The tensor
+    // core truncates where it adds (2^-27 of the sum a step, measured), which the 40 other steps would do to the large sum.
+    constexpr int LO = KC;                        // columns between the two
+    const int OUT = a.nbuf * SB;                  // first column of the outputs
+    constexpr int OB = 64;                        // columns of an output buffer when there are two
     constexpr int COMBOS = P == 1 ? 1 : 6;
     constexpr int CA[6] = {P == 1 ? 0 : 2, 0, 1, 1, 0, 0}, CB[6] = {0, 2, 1, 0, 1, 0};  // smallest products first
     constexpr int TB = KC * 2 * LT;               // bytes of a staged tile
@@ -245,16 +253,17 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t na = P * a.nk;                 // tiles of one block of 128 rows, chunk by chunk, its pieces together
     unsigned char* ring = tiles + a.a_slots * na * TB;
-    const uint32_t stage = a.gs * TB;             // bytes of a stage of the ring: a whole block of B, or one chunk of A or B
+    constexpr uint32_t stage = CS * P * TB;       // bytes of a stage of the ring: CS chunks of A or B, their pieces
+    const int nst = a.nk / CS;                    // stages of a block of 128 rows
 
     if (warp == 0) {
         if (lane == 0) {
             for (int i = 0; i < LSTAGES; ++i) { rgs_mbar_init(&sh->full[i], 1); rgs_mbar_init(&sh->empty[i], 1); }
             for (int i = 0; i < 2; ++i) {
                 rgs_mbar_init(&sh->a_full[i], 1); rgs_mbar_init(&sh->a_empty[i], 1);
-                rgs_mbar_init(&sh->s_full[i], 1); rgs_mbar_init(&sh->s_done[i], 256);
                 rgs_mbar_init(&sh->o_full[i], 1); rgs_mbar_init(&sh->o_free[i], 512);
             }
+            for (int i = 0; i < 4; ++i) { rgs_mbar_init(&sh->s_full[i], 1); rgs_mbar_init(&sh->s_done[i], 256); }
             for (int i = 0; i < LKSLOTS; ++i) { rgs_mbar_init(&sh->k_full[i], 1); rgs_mbar_init(&sh->k_empty[i], 256); }
             rgs_mbar_init(&sh->drain, 1);
             sh->fail = 0;
@@ -276,16 +285,14 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         LabelCursor rc, ac, kc;
         uint32_t loads = 0;
         bool ok = true;
-        // one stage: gs tiles from chunk k on, all pieces of a chunk before the next
         auto load = [&](const CUtensorMap* map, int k, int row) {
             ok = ok && lb_wait_warp(&sh->empty[rc.slot], rc.phase ^ 1, fail);
             if (!ok) return;
             if (lead) {
                 unsigned char* dst = ring + rc.slot * stage;
                 rgs_mbar_expect_tx(&sh->full[rc.slot], stage);
-                for (int u = 0; u < a.gs; u += P, ++k)
 #pragma unroll
-                    for (int p = 0; p < P; ++p) lb_tma(dst + (u + p) * TB, map, k * KC, row * LT, p, &sh->full[rc.slot]);
+                for (int u = 0; u < CS * P; ++u) lb_tma(dst + u * TB, map, (k * CS + u / P) * KC, row * LT, u % P, &sh->full[rc.slot]);
             }
             rc.next(a.stages);
             ++loads;
@@ -296,7 +303,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         int prev_j = 0, prev_oc0 = 0, prev_noc = 0, prev_dw = 0;
         auto out_tiles = [&]() {
             if (!GRAD || a.whole || !have_prev) return;
-            for (int oc = 0; oc < prev_noc && ok; ++oc) load(prev_dw ? &map_x : &map_w, prev_oc0 + oc, prev_j);
+            for (int oc = 0; oc < prev_noc && ok; oc += CS) load(prev_dw ? &map_x : &map_w, (prev_oc0 + oc) / CS, prev_j);
         };
         for (unsigned i = blockIdx.x; i < items && ok; i += gridDim.x) {
             const LabelItem it = lb_item(a, i);
@@ -322,16 +329,12 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                     rgs_bulk_g2s(kbuf + kc.slot * (LKBYTES / 4), it.dw ? a.kn + (size_t)j * (LT * 4) : a.b2 + (size_t)j * LT, bytes, &sh->k_full[kc.slot]);
                 }
                 kc.next(LKSLOTS);
-                if (a.whole) {
-                    load(mb, 0, j);
-                } else {
-                    for (int k = 0; k < a.nk && ok; ++k) {
-                        if (!a.a_slots) load(ma, k, it.m);
-                        load(mb, k, j);
-                    }
-                    out_tiles();
-                    have_prev = true; prev_j = j; prev_oc0 = it.oc0; prev_noc = it.noc; prev_dw = it.dw;
+                for (int k = 0; k < nst && ok; ++k) {
+                    if (!a.a_slots) load(ma, k, it.m);
+                    load(mb, k, j);
                 }
+                out_tiles();
+                have_prev = true; prev_j = j; prev_oc0 = it.oc0; prev_noc = it.noc; prev_dw = it.dw;
             }
         }
         if (ok) out_tiles();
@@ -359,110 +362,120 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         // shared memory and TMEM, and the warpgroups write NaN
         const bool lead = lb_elect();
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(LT >> 4) << 24);
-        LabelCursor rc, ac, oc_, gc;                         // ring, A, outputs; oldest stage not given back
-        const uint64_t dbase = lb_desc<KC>(), ring16 = rgs_smem_addr(ring) >> 4, tiles16 = rgs_smem_addr(tiles) >> 4;
-        constexpr uint32_t T16 = TB >> 4;
-        const uint32_t stage16 = stage >> 4;
-        const uint32_t last_steps = (uint32_t)(a.c - (a.nk - 1) * KC + 15) >> 4;  // of 16 channels, in the last chunk
+        LabelCursor rc, ac, oc_, gc, sc, pc;                 // ring, A, outputs; oldest stage not given back; S, its G
+        const uint32_t dlo = lb_desc_lo<KC>, ring16 = dlo + (rgs_smem_addr(ring) >> 4), tiles16 = dlo + (rgs_smem_addr(tiles) >> 4);
+        constexpr uint32_t T16 = TB >> 4, stage16 = stage >> 4;
         auto take = [&]() {
             lb_wait_quiet(&sh->full[rc.slot], rc.phase, fail);
-            const uint64_t d = dbase + ring16 + rc.slot * stage16;
+            const uint32_t d = ring16 + rc.slot * stage16;
             rc.next(a.stages);
             return d;
         };
-        auto give = [&]() {
-            if (lead) lb_commit(&sh->empty[gc.slot]);
-            gc.next(a.stages);
-        };
-        // one chunk of S: the six products of pieces, up to KC / 16 steps each
-        auto chunk_s = [&](uint32_t d, uint64_t at, uint64_t bt, int k) {
-            const uint32_t steps = k == a.nk - 1 ? last_steps : KC / 16;
+        // the chunks of a stage; channels behind the last one are zeros in shared memory
+        auto stage_s = [&](uint32_t d, uint32_t at, uint32_t bt, bool more) {
 #pragma unroll
-            for (int q = 0; q < COMBOS; ++q)
+            for (int k = 0; k < CS; ++k)
 #pragma unroll
-                for (uint32_t ks = 0; ks < KC / 16; ++ks)
-                    if (ks < steps) lb_mma_ss(d, at + CA[q] * T16 + ks * 2, bt + CB[q] * T16 + ks * 2, idesc | ((LT >> 3) << 17), !(k == 0 && q == 0 && ks == 0));
+                for (int q = 0; q < COMBOS; ++q)
+#pragma unroll
+                    for (int ks = 0; ks < KC / 16; ++ks)
+                        lb_mma_ss<KC>(d, at + (k * P + CA[q]) * T16 + ks * 2, bt + (k * P + CB[q]) * T16 + ks * 2, idesc | ((LT >> 3) << 17), k || q || ks ? true : more);
         };
-        auto issue_s = [&](const LabelItem& it, int j, uint32_t t) {
-            const uint32_t d = tmem + (t & 1) * SB;
+        auto issue_s = [&](const LabelItem& it, int j) {
+            const uint32_t d = tmem + sc.slot * SB;
+            // forward: the scores there before have been read; backward: the product with their G was issued before, and runs before
+            if (!GRAD) lb_wait_quiet(&sh->s_done[sc.slot], sc.phase ^ 1, fail);
             if (a.a_slots && j == it.j0) lb_wait_quiet(&sh->a_full[ac.slot], ac.phase, fail);
-            const uint64_t abase = dbase + tiles16 + ac.slot * (na * T16);
-            if (a.whole) {
-                const uint64_t bt = take();
+            const uint32_t abase = tiles16 + ac.slot * (na * T16);
+            const bool last = j == it.j1 - 1 && a.a_slots;
+            for (int k = 0; k < nst; ++k) {
+                const uint32_t at = a.a_slots ? abase + k * stage16 : take();
+                const uint32_t bt = take();
+                const uint32_t g0 = gc.slot;
+                if (!GRAD || !a.whole) {
+                    gc.next(a.stages);
+                    if (!a.a_slots) gc.next(a.stages);
+                }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (lead)
-                    for (int k = 0; k < a.nk; ++k) chunk_s(d, abase + k * (P * T16), bt + k * (P * T16), k);
-                if (!GRAD) give();
-            } else {
-                for (int k = 0; k < a.nk; ++k) {
-                    const uint64_t at = a.a_slots ? abase + k * (P * T16) : take();
-                    const uint64_t bt = take();
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (lead) chunk_s(d, at, bt, k);
-                    if (!a.a_slots) give();
-                    give();
+                if (lead) {
+                    stage_s(d, at, bt, k != 0);
+                    if (!GRAD || !a.whole) {
+                        lb_commit(&sh->empty[g0]);
+                        if (!a.a_slots) lb_commit(&sh->empty[g0 + 1 == (uint32_t)a.stages ? 0 : g0 + 1]);
+                    }
+                    if (k == nst - 1) {
+                        lb_commit(&sh->s_full[sc.slot]);
+                        if (last) lb_commit(&sh->a_empty[ac.slot]);
+                    }
                 }
+                __syncwarp();
             }
-            if (lead) lb_commit(&sh->s_full[t & 1]);
-            if (j == it.j1 - 1 && a.a_slots) {
-                if (lead) lb_commit(&sh->a_empty[ac.slot]);
-                ac.next(a.a_slots);
-            }
+            sc.next(a.nbuf);
+            if (last) ac.next(a.a_slots);
         };
-        // G B of score buffer t; B as the K x N operand with its channels as N, 16 rows a step
-        auto chunk_o = [&](uint32_t s, uint32_t o, uint64_t bt, int chunk, bool fresh) {
-            const uint32_t cols = min(KC, (a.c - chunk * KC + 15) & ~15);
-            const uint32_t id = idesc | (1u << 16) | ((cols >> 3) << 17);
+        // G B; B as the K x N operand with its channels as N, 16 rows a step
+        auto stage_o = [&](uint32_t s, uint32_t o, uint32_t bt, bool more) {
+            constexpr uint32_t id = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(KC >> 3) << 17) | ((uint32_t)(LT >> 4) << 24);
 #pragma unroll
-            for (int q = 0; q < COMBOS; ++q)
+            for (int k = 0; k < CS; ++k)
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    // 16 columns of G are 8 words: the first two pieces lie over the 16 scores, the third behind all
-                    const uint32_t g = CA[q] == 2 ? s + 128 + ks * 8 : s + ks * 16 + CA[q] * 8;
-                    lb_mma_ts(o, g, bt + CB[q] * T16 + ks * (KC * 2), id, !(fresh && q == 0 && ks == 0));
-                }
+                for (int q = 0; q < COMBOS; ++q)
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) {
+                        // 16 columns of G are 8 words: the first two pieces lie over the 16 scores, the third behind all
+                        const uint32_t g = CA[q] == 2 ? s + 128 + ks * 8 : s + ks * 16 + CA[q] * 8;
+                        const bool first = ks == 0 && (q == 0 || q == COMBOS - 1);
+                        lb_mma_ts<KC>(o + k * KC + (q < COMBOS - 1 ? LO : 0), g, bt + (k * P + CB[q]) * T16 + ks * (KC * 2), id, first ? more : true);
+                    }
         };
-        auto issue_o = [&](const LabelItem& it, int j, uint32_t t) {
-            lb_wait_quiet(&sh->s_done[t & 1], (t >> 1) & 1, fail);
+        auto issue_o = [&](const LabelItem& it, int j) {
+            lb_wait_quiet(&sh->s_done[pc.slot], pc.phase, fail);
             if (j == it.j0) lb_wait_quiet(&sh->o_free[oc_.slot], oc_.phase ^ 1, fail);
-            const uint32_t s = tmem + (t & 1) * SB, o = tmem + OUT + oc_.slot * OB;
-            if (a.whole) {  // the stage that S(t) took is the oldest one still held
+            const uint32_t s = tmem + pc.slot * SB, o = tmem + OUT + oc_.slot * OB;
+            pc.next(a.nbuf);
+            const bool last = j == it.j1 - 1;
+            for (int oc = 0; oc < it.noc; oc += CS) {
+                // kept stages: those that S took are the oldest ones still held (all chunks are output channels then)
+                const uint32_t bt = a.whole ? ring16 + gc.slot * stage16 : take();
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t bt = dbase + ring16 + gc.slot * stage16;
-                if (lead)
-                    for (int oc = 0; oc < it.noc; ++oc) chunk_o(s, o + oc * KC, bt + (it.oc0 + oc) * (P * T16), it.oc0 + oc, j == it.j0);
-                give();
-            } else {
-                for (int oc = 0; oc < it.noc; ++oc) {
-                    const uint64_t bt = take();
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (lead) chunk_o(s, o + oc * KC, bt, it.oc0 + oc, j == it.j0);
-                    give();
+                if (lead) {
+                    stage_o(s, o + oc * KC, bt, j != it.j0);
+                    lb_commit(&sh->empty[gc.slot]);
+                    if (last && oc + CS == it.noc) lb_commit(&sh->o_full[oc_.slot]);
                 }
+                __syncwarp();
+                gc.next(a.stages);
             }
-            if (j == it.j1 - 1) {
-                if (lead) lb_commit(&sh->o_full[oc_.slot]);
-                oc_.next(a.nob);
+            if (last) oc_.next(a.nob);
+        };
+        // walks over the score tiles: S runs nbuf - 1 tiles ahead of G B, so that a warpgroup finds its next scores ready
+        unsigned si = blockIdx.x, oi = blockIdx.x;
+        LabelItem is, io;
+        int sj = 0, oj = 0;
+        if (si < items) { is = io = lb_item(a, si); sj = oj = is.j0; }
+        auto step_s = [&]() {
+            issue_s(is, sj);
+            if (++sj == is.j1) {
+                si += gridDim.x;
+                if (si < items) { is = lb_item(a, si); sj = is.j0; }
             }
         };
-        uint32_t t = 0;
-        LabelItem prev;
-        int prev_j = 0;
-        bool have_prev = false;
-        for (unsigned i = blockIdx.x; i < items; i += gridDim.x) {
-            const LabelItem it = lb_item(a, i);
-            for (int j = it.j0; j < it.j1; ++j, ++t) {
-                // forward: the scores of t-2 have been read; backward: G(t-2) B was issued before, and runs before
-                if (!GRAD && t >= 2) lb_wait_quiet(&sh->s_done[t & 1], ((t >> 1) & 1) ^ 1, fail);
-                issue_s(it, j, t);
-                if (GRAD) {
-                    if (have_prev) issue_o(prev, prev_j, t - 1);
-                    prev = it; prev_j = j; have_prev = true;
+        if (GRAD) {
+            for (int l = 1; l < a.nbuf; ++l)
+                if (si < items) step_s();
+            while (oi < items) {
+                if (si < items) step_s();
+                issue_o(io, oj);
+                if (++oj == io.j1) {
+                    oi += gridDim.x;
+                    if (oi < items) { io = lb_item(a, oi); oj = io.j0; }
                 }
             }
+        } else {
+            while (si < items) step_s();
         }
-        if (GRAD && have_prev) issue_o(prev, prev_j, t - 1);
         if (lead) lb_commit(&sh->drain);
+        __syncwarp();
         rgs_mbar_wait(&sh->drain, 0, LWAIT);
     } else {
         // ------------------------------------------------------------------------------------------------ scores
@@ -472,8 +485,8 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         const uint32_t lanes = (uint32_t)wrow << 16;
         const float nan = __int_as_float(0x7fc00000);
         const f2 log2e = mk2(LOG2E, LOG2E);
-        uint32_t t = 0, kept = 0;                            // score tiles seen; ring stage of the B block of tile t
-        LabelCursor oc_;
+        uint32_t t = 0, kept = 0;                            // score tiles seen; ring stage where the B block of tile t begins
+        LabelCursor oc_, sc;
         bool dead = false;
         unsigned out_i = blockIdx.x;                         // next item whose output this warpgroup writes
         auto write_out = [&](unsigned i) {
@@ -493,13 +506,17 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             for (int c0 = wg * 16; c0 < it.noc * KC; c0 += 64) {
                 const int c = it.oc0 * KC + c0;
                 if (c >= a.c) break;
-                uint32_t u[16];
+                uint32_t u[16], lo[16];
                 tm_ld16(o + c0, u);
+                if (P == 3) {
+                    tm_ld16(o + LO + c0, lo);
+                    tm_wait_ld16(lo);
+                }
                 tm_wait_ld16(u);
                 if (r < rows && (!it.dw || a.dw)) {
                     float f[16];
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) f[q] = dead ? nan : __uint_as_float(u[q]);
+                    for (int q = 0; q < 16; ++q) f[q] = dead ? nan : P == 3 ? __uint_as_float(u[q]) + __uint_as_float(lo[q]) : __uint_as_float(u[q]);
                     if (ns > 1) {
                         float* p = (it.dw ? a.part_w : a.part_x) + ((int64_t)it.split * (it.dw ? a.nmw : a.nmx) * LT + r) * a.cq + c;
 #pragma unroll
@@ -535,13 +552,14 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 b2row = a.b2[r];
             }
             for (int j = it.j0; j < it.j1; ++j, ++t) {
-                const uint32_t bstage = kept;
-                if (GRAD && P == 1 && ++kept == (uint32_t)a.stages) kept = 0;
+                const uint32_t bstage = kept, buf = sc.slot, parity = sc.phase;
+                if (GRAD && P == 1 && (kept += nst) >= (uint32_t)a.stages) kept -= a.stages;
+                sc.next(a.nbuf);
                 if ((int)(t & 1) != (wg & 1)) continue;
-                const uint32_t s = tmem + lanes + (t & 1) * SB + half;
+                const uint32_t s = tmem + lanes + buf * SB + half;
                 const uint32_t ks = t & (LKSLOTS - 1);
                 if (!dead) {  // the whole warp goes on or none of it: TMEM accesses are warp-wide
-                    dead = !lb_wait(&sh->k_full[ks], (t / LKSLOTS) & 1, fail) || !lb_wait(&sh->s_full[t & 1], (t >> 1) & 1, fail);
+                    dead = !lb_wait(&sh->k_full[ks], (t / LKSLOTS) & 1, fail) || !lb_wait(&sh->s_full[buf], parity, fail);
                     dead = __any_sync(0xffffffffu, dead);
                 }
                 if (dead) continue;
@@ -557,7 +575,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                     tm_wait_ld32(u[1]);
                     // all scores are in registers: the buffer is free for the product after the next
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    rgs_mbar_arrive(&sh->s_done[t & 1]);
+                    rgs_mbar_arrive(&sh->s_done[buf]);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         f2 v[16];
@@ -695,7 +713,9 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                     // staged block are cleared (row n of every chunk, whole, whatever the swizzle)
                     if (__float_as_int(kb[3 * LT + row - half]) < 0) {
                         for (int k = 0; k < a.nk; ++k) {
-                            uint4* p = reinterpret_cast<uint4*>(ring + bstage * stage + k * TB + row * (KC * 2));
+                            uint32_t slot = bstage + k / CS;
+                            if (slot >= (uint32_t)a.stages) slot -= a.stages;
+                            uint4* p = reinterpret_cast<uint4*>(ring + slot * stage + (k % CS) * TB + row * (KC * 2));
 #pragma unroll
                             for (int q = 0; q < KC / 8; ++q) p[q] = make_uint4(0, 0, 0, 0);
                         }
@@ -705,7 +725,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 rgs_mbar_arrive(&sh->k_empty[ks]);
-                rgs_mbar_arrive(&sh->s_done[t & 1]);
+                rgs_mbar_arrive(&sh->s_done[buf]);
                 for (; out_i < i; out_i += gridDim.x) write_out(out_i);  // outputs of earlier items, behind the first scores of this one
             }
             if (!GRAD) {
@@ -969,7 +989,7 @@ static int label_pieces(int64_t tiles, int64_t nj, int64_t sms, int64_t run, int
 
 struct LabelPlan {
     LabelArgs a;
-    int pieces, kc, direct_x, direct_w, cp;
+    int pieces, kc, cs, direct_x, direct_w, cp;
     int64_t o_xs, o_ws, o_b2, o_kn, o_pm, o_ps, o_at, o_px, o_pw, o_pb, o_bsum, o_bcount, o_ticket, bytes;
 };
 
@@ -985,24 +1005,29 @@ static void label_plan(LabelPlan& p, int64_t n, int64_t c, int64_t v, int dtype,
     a.nmx = (int)((n + LT - 1) / LT); a.nmw = (int)((v + LT - 1) / LT);
     a.dtype = dtype;
     const int na = p.pieces * a.nk, room = LROOM / (256 * p.kc);
-    // whole blocks of B where a block of A (better two) leaves room for two (three) of them; else chunk by chunk, A staying
-    // where half of the room holds it
-    a.whole = 1; a.gs = na;
-    if (room >= 5 * na) a.a_slots = 2;
-    else if (room >= 3 * na) a.a_slots = 1;
-    else { a.whole = 0; a.gs = p.pieces; a.a_slots = na <= 8 ? 1 : 0; }
-    a.stages = (room - a.a_slots * na) / a.gs;
-    if (a.stages > LSTAGES) a.stages = LSTAGES;
-    const int cols = (p.pieces == 1 ? 256 : 128) / p.kc;  // chunks of output channels that TMEM holds beside the scores
+    // TMEM: 512 columns.  Up to 128 output channels leave room for three score buffers in 16 bits, more for two; the two sums
+    // of 32-bit outputs and the third piece of G leave room for two and one chunk of channels.  The forward pass takes four.
+    const int cols = p.pieces == 1 ? 256 / p.kc : 1;
     a.noc = a.nk < cols ? a.nk : cols;
     a.nrange = backward ? (a.nk + a.noc - 1) / a.noc : 1;
-    a.nob = 2 * a.noc <= cols ? 2 : 1;
+    a.nbuf = !backward ? 4 : (p.pieces == 1 && a.nk * p.kc <= 128 ? 3 : 2);
+    a.nob = (p.pieces == 1 ? a.nk * p.kc : 2 * p.kc) <= 64 ? 2 : 1;
+    // Stages of B are kept for both products where the ring holds one block to a score buffer beside the block (better two)
+    // of A and one range covers the channels; else they are fetched for each product, and A stays where half the room holds it.
+    a.a_slots = na <= 8 ? 1 : 0;
+    a.whole = backward && a.nrange == 1 && room >= na * (a.nbuf + 1);
+    if (room >= na * ((backward ? a.nbuf : 2) + 3)) a.a_slots = 2;
+    // chunks of a stage: few barriers to a block where the ring is deep enough
+    p.cs = 1;
+    if (p.pieces == 1 && p.kc == 64 && a.a_slots && a.nrange == 1) p.cs = a.nk == 2 || a.nk == 4 ? 2 : (a.nk == 3 ? 3 : 1);
+    a.stages = (room - a.a_slots * na) / (p.pieces * p.cs);
+    if (a.stages > LSTAGES) a.stages = LSTAGES;
     a.cq = (int)up(c, 16);
     // where B is fetched anew for the second product its rows cannot be cleared in place: X goes through the copy
     p.direct_x = p.pieces == 1 && (direct & 1) && (!backward || a.whole);
     p.direct_w = p.pieces == 1 && (direct & 2);
     p.cp = (int)up(c, 8);
-    const int64_t run = p.pieces == 1 ? 512 : 32;
+    const int64_t run = p.pieces == 1 ? 512 : 16;
     const int64_t rows_x = (int64_t)a.nmx * LT, rows_w = (int64_t)a.nmw * LT;
     if (backward) {
         const int64_t room = (int64_t)1 << 31;  // bytes of partial sums
@@ -1040,24 +1065,26 @@ static int label_direct(const void* x, int64_t ldx, const void* w, int64_t ldw) 
     return dx | (dw << 1);
 }
 
-template <int P, bool GRAD, int KC>
+template <int P, bool GRAD, int KC, int CS>
 static int label_launch(const CUtensorMap& mx, const CUtensorMap& mw, const LabelArgs& a, cudaStream_t stream) {
     static std::atomic<uint64_t> ready{0};  // devices whose limit on dynamic shared memory was raised
     int dev = 0;
     RGS_CUDA_CHECK(cudaGetDevice(&dev));
     if (dev > 63 || !((ready.load() >> dev) & 1)) {
-        RGS_CUDA_CHECK(cudaFuncSetAttribute(rgs_label_tc_kernel<P, GRAD, KC>, cudaFuncAttributeMaxDynamicSharedMemorySize, LSMEM));
+        RGS_CUDA_CHECK(cudaFuncSetAttribute(rgs_label_tc_kernel<P, GRAD, KC, CS>, cudaFuncAttributeMaxDynamicSharedMemorySize, LSMEM));
         if (dev <= 63) ready.fetch_or((uint64_t)1 << dev);
     }
     const int64_t items = (int64_t)a.items_x + a.items_w, sms = RGS_SMS;
-    rgs_label_tc_kernel<P, GRAD, KC><<<(unsigned)(items < sms ? items : sms), LTHREADS, LSMEM, stream>>>(mx, mw, a);
+    rgs_label_tc_kernel<P, GRAD, KC, CS><<<(unsigned)(items < sms ? items : sms), LTHREADS, LSMEM, stream>>>(mx, mw, a);
     return (int)cudaGetLastError();
 }
 
 template <bool GRAD>
 static int label_run(const LabelPlan& p, const CUtensorMap& mx, const CUtensorMap& mw, cudaStream_t stream) {
-    if (p.pieces == 1) return p.kc == 64 ? label_launch<1, GRAD, 64>(mx, mw, p.a, stream) : label_launch<1, GRAD, 32>(mx, mw, p.a, stream);
-    return p.kc == 64 ? label_launch<3, GRAD, 64>(mx, mw, p.a, stream) : label_launch<3, GRAD, 32>(mx, mw, p.a, stream);
+    if (p.pieces == 3) return p.kc == 64 ? label_launch<3, GRAD, 64, 1>(mx, mw, p.a, stream) : label_launch<3, GRAD, 32, 1>(mx, mw, p.a, stream);
+    if (p.kc == 32) return label_launch<1, GRAD, 32, 1>(mx, mw, p.a, stream);
+    if (p.cs == 3) return label_launch<1, GRAD, 64, 3>(mx, mw, p.a, stream);
+    return p.cs == 2 ? label_launch<1, GRAD, 64, 2>(mx, mw, p.a, stream) : label_launch<1, GRAD, 64, 1>(mx, mw, p.a, stream);
 }
 
 static inline unsigned label_grid(int64_t work, int64_t most) {
