@@ -4,155 +4,739 @@
 //   xhat = (x - mean) rstd,  y = xhat w + b;   a = dy w,  dx = rstd (a - mean(a) - xhat mean(a xhat)),
 //   dw = sum_n dy xhat,  db = sum_n dy
 // With codes in place of x the backward pass is that of the norm at the values the codes stand for.
-// First form: a warp per row, elements re-read for every sum.
+//
+// All of it is bound by memory, so every tensor is read and written once: a group of 1 to 32 lanes holds a row in registers,
+// the two sums of each pass are shuffles, and in the backward pass the mean and rstd are computed anew from the row (four
+// shuffles) instead of being kept.  Lanes keep the sums of their own channels for dw and db over all the rows they meet;
+// blocks write them once and a second kernel adds the blocks in order, so results do not depend on timing.
+// Rows of 4 n channels on aligned boundaries are read in vectors of four, others element by element.  Channel planes (the
+// renderer's images) pass through shared memory 32 pixels at a time.  Beyond 1024 channels a warp re-reads its row.
+#include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include "rgs_cuda_common.cuh"
 #include "rgs_field_math.h"
 
-#define NR_WARPS 8
+#define NT 256            // threads of a block
+#define NR_MAX 1024       // channels that a group holds in registers
+#define PT 32             // pixels of a tile of planes
+
+enum { SRC_F32 = 0, SRC_BF16 = 1, SRC_CODES = 2 };
 
 struct NormArgs {
-    const void* x; int dtype; int64_t ld; int planes;
-    const int8_t* codes; const uint8_t* expo;
-    int64_t n, c;
+    const void* x; int src, planes; int64_t ld;
+    const int8_t* codes; const uint8_t* expo;      // kept input (backward)
+    const void* w; const void* b; int p_dtype;
+    int64_t n; int c, blocks;                      // rows, channels, 32-channel blocks of a row
+    float eps, inv_c;
+    void* y; int y_dtype;
+    int8_t* codes_out; uint8_t* expo_out;          // forward with an 8-bit copy
+    const void* dy; int dy_dtype; int64_t ldy;
+    void* dx; int dx_dtype;
+    float* part;                                   // (blocks of the grid, 2, c)
 };
 
-__device__ __forceinline__ float norm_warp_sum(float v) {
+template <int VEC> struct Vec { float v[VEC]; };
+
+template <int VEC>
+__device__ __forceinline__ void load_vec(const void* p, int64_t i, int dtype, float (&f)[VEC]) {
+    if constexpr (VEC == 4) {
+        if (dtype == RGS_BF16) {
+            const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+            f[0] = __uint_as_float(u.x << 16); f[1] = __uint_as_float(u.x & 0xffff0000u);
+            f[2] = __uint_as_float(u.y << 16); f[3] = __uint_as_float(u.y & 0xffff0000u);
+        } else {
+            const float4 u = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+            f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
+        }
+    } else {
+        f[0] = rgs_load_as_float(p, i, dtype);
+    }
+}
+__device__ __forceinline__ uint32_t pair_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <int VEC>
+__device__ __forceinline__ void store_vec(void* p, int64_t i, int dtype, const float (&f)[VEC]) {
+    if constexpr (VEC == 4) {
+        if (dtype == RGS_BF16) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = make_uint2(pair_bf16(f[0], f[1]), pair_bf16(f[2], f[3]));
+        else *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(f[0], f[1], f[2], f[3]);
+    } else {
+        if (dtype == RGS_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(f[0]);
+        else static_cast<float*>(p)[i] = f[0];
+    }
+}
+// codes of four channels (one word) or of one, from values scaled by the inverse step of their block
+template <int VEC>
+__device__ __forceinline__ void store_codes(int8_t* p, int64_t i, const float (&f)[VEC], uint32_t e) {
+    const float inv = rgs_pack_inverse(e);
+    if constexpr (VEC == 4) {
+        uint32_t u = 0;
+        if (e != RGS_PACK_NAN)
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+            for (int k = 0; k < 4; ++k) u |= (uint32_t)(rgs_pack_code(f[k], inv) & 0xff) << (8 * k);
+        *reinterpret_cast<uint32_t*>(p + i) = u;
+    } else {
+        p[i] = (int8_t)(e == RGS_PACK_NAN ? 0 : rgs_pack_code(f[0], inv));
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void load_codes(const int8_t* p, int64_t i, float step, float (&f)[VEC]) {
+    if constexpr (VEC == 4) {
+        const uint32_t u = *reinterpret_cast<const uint32_t*>(p + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k] = (float)(int8_t)(u >> (8 * k)) * step;
+    } else {
+        f[0] = (float)p[i] * step;
+    }
+}
+
+// sum over the `lanes` lanes (a power of two) that share a row
+__device__ __forceinline__ float group_sum(float v, int lanes) {
+    for (int d = lanes >> 1; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
+__device__ __forceinline__ uint32_t group_max(uint32_t v, int lanes) {
+    for (int d = lanes >> 1; d > 0; d >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
     return v;
 }
 
-__device__ __forceinline__ float norm_value(const NormArgs& a, int64_t i, int64_t j) {
-    if (!a.codes) return rgs_load_as_float(a.x, a.planes ? j * a.ld + i : i * a.ld + j, a.dtype);
-    const int64_t blocks = (a.c + RGS_PACK_BLOCK - 1) / RGS_PACK_BLOCK, b = j / RGS_PACK_BLOCK;
-    return (float)a.codes[a.planes ? j * a.n + i : i * a.c + j] * rgs_pack_step(a.expo[a.planes ? b * a.n + i : i * blocks + b]);
-}
-
-__device__ __forceinline__ void norm_stats(const NormArgs& a, int64_t i, float eps, int lane, float& mu, float& rstd) {
+// mean and 1 / sqrt(var + eps) of a row; vector k of a lane starts at channel (k lanes + lane) VEC
+template <int VEC, int NV>
+__device__ __forceinline__ void row_stats(const float (&x)[NV][VEC], int l, int lanes, int c, float inv_c, float eps, float& mu, float& rstd) {
     float s = 0.f;
-    for (int64_t j = lane; j < a.c; j += 32) s += norm_value(a, i, j);
-    mu = norm_warp_sum(s) / (float)a.c;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) s += x[k][q];   // zero behind the last channel
+    mu = group_sum(s, lanes) * inv_c;
     s = 0.f;
-    for (int64_t j = lane; j < a.c; j += 32) { const float d = norm_value(a, i, j) - mu; s = fmaf(d, d, s); }
-    rstd = 1.0f / sqrtf(norm_warp_sum(s) / (float)a.c + eps);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+        if ((k * lanes + l) * VEC < c)
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) s = fmaf(x[k][q] - mu, x[k][q] - mu, s);
+    rstd = 1.0f / sqrtf(group_sum(s, lanes) * inv_c + eps);
 }
 
-__global__ void __launch_bounds__(NR_WARPS * 32) rgs_norm_fwd_kernel(NormArgs a, const void* w, const void* b, int p_dtype, float eps, void* y,
-                                                                     int y_dtype) {
-    const int lane = threadIdx.x & 31;
-    for (int64_t i = (int64_t)blockIdx.x * NR_WARPS + (threadIdx.x >> 5); i < a.n; i += (int64_t)gridDim.x * NR_WARPS) {
-        float mu, rstd;
-        norm_stats(a, i, eps, lane, mu, rstd);
-        for (int64_t j = lane; j < a.c; j += 32)
-            rgs_store_float(y, i * a.c + j, y_dtype,
-                            fmaf((norm_value(a, i, j) - mu) * rstd, w ? rgs_load_as_float(w, j, p_dtype) : 1.f,
-                                 b ? rgs_load_as_float(b, j, p_dtype) : 0.f));
+// the part of the backward pass that rows and planes share: a row's x, dy -> dx (over x), sums of dw and db
+template <int VEC, int NV>
+__device__ __forceinline__ void row_bwd(float (&x)[NV][VEC], float (&g)[NV][VEC], const float (&w)[NV][VEC], float (&sw)[NV][VEC], float (&sb)[NV][VEC],
+                                        int l, int lanes, int c, float inv_c, float eps) {
+    float mu, rstd, sa = 0.f, sax = 0.f;
+    row_stats<VEC, NV>(x, l, lanes, c, inv_c, eps, mu, rstd);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) {
+            const bool in = (k * lanes + l) * VEC < c;
+            x[k][q] = in ? (x[k][q] - mu) * rstd : 0.f;
+            sw[k][q] = fmaf(g[k][q], x[k][q], sw[k][q]);
+            sb[k][q] += g[k][q];
+            g[k][q] *= w[k][q];
+            sa += g[k][q];
+            sax = fmaf(g[k][q], x[k][q], sax);
+        }
+    sa = group_sum(sa, lanes) * inv_c;
+    sax = group_sum(sax, lanes) * inv_c;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) x[k][q] = rstd * (g[k][q] - sa - x[k][q] * sax);
+}
+
+template <int VEC, int NV>
+__device__ __forceinline__ void load_params(const NormArgs& a, int l, int lanes, const void* p, float none, float (&w)[NV][VEC]) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c = (k * lanes + l) * VEC;
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) w[k][q] = p && c + q < a.c ? rgs_load_as_float(p, c + q, a.p_dtype) : none;
     }
 }
 
-__global__ void __launch_bounds__(NR_WARPS * 32) rgs_norm_bwd_kernel(NormArgs a, const void* dy, int dy_dtype, int64_t ldy, const void* w,
-                                                                     int p_dtype, float eps, float2* stats, void* dx, int x_dtype) {
+// sums of a block's groups, in the order of the groups, to the block's row of the partial sums
+template <int VEC, int NV>
+__device__ __forceinline__ void block_sums(const NormArgs& a, int l, int lanes, const float (&sw)[NV][VEC], const float (&sb)[NV][VEC], float* sh) {
+    // sh: (groups of the block, channels) of one of the two sums at a time, 64 channels a turn
+    const int group = threadIdx.x / lanes, groups = NT / lanes;
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            if (k * lanes * VEC >= a.c) break;
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) sh[group * (lanes * VEC) + l * VEC + q] = which ? sb[k][q] : sw[k][q];
+            __syncthreads();
+            for (int j = threadIdx.x; j < lanes * VEC; j += NT) {
+                float t = 0.f;
+                for (int r = 0; r < groups; ++r) t += sh[r * (lanes * VEC) + j];
+                const int c = k * lanes * VEC + j;
+                if (c < a.c) a.part[((int64_t)blockIdx.x * 2 + which) * a.c + c] = t;
+            }
+        }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// rows
+// ---------------------------------------------------------------------------------------------------------------------
+template <int VEC, int NV>
+__device__ __forceinline__ void load_row(const NormArgs& a, int64_t i, int l, int lanes, float (&x)[NV][VEC]) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c = (k * lanes + l) * VEC;
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) x[k][q] = 0.f;
+        if (c < a.c) {
+            if (a.src == SRC_CODES) load_codes<VEC>(a.codes, i * a.c + c, rgs_pack_step(a.expo[i * a.blocks + c / RGS_PACK_BLOCK]), x[k]);
+            else load_vec<VEC>(a.x, i * a.ld + c, a.src, x[k]);
+        }
+    }
+}
+
+template <int VEC, int NV, int R, bool PACK>
+__global__ void __launch_bounds__(NT) rgs_norm_rows_fwd_kernel(const __grid_constant__ NormArgs a, int lanes) {
+    const int l = threadIdx.x & (lanes - 1), groups = NT / lanes;
+    const int64_t stride = (int64_t)gridDim.x * groups;
+    float w[NV][VEC], b[NV][VEC];
+    load_params<VEC, NV>(a, l, lanes, a.w, 1.f, w);
+    load_params<VEC, NV>(a, l, lanes, a.b, 0.f, b);
+    // all lanes of a warp take the same number of turns: shuffles need them
+    for (int64_t i0 = (int64_t)blockIdx.x * groups; i0 < a.n; i0 += R * stride) {
+        const int64_t i = i0 + threadIdx.x / lanes;
+        float x[R][NV][VEC];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            load_row<VEC, NV>(a, min(i + r * stride, a.n - 1), l, lanes, x[r]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = i + r * stride;
+            float mu, rstd;
+            row_stats<VEC, NV>(x[r], l, lanes, a.c, a.inv_c, a.eps, mu, rstd);
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int c = (k * lanes + l) * VEC;
+                if (PACK) {
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) top = max(top, __float_as_uint(x[r][k][q]) & 0x7fffffffu);
+                    const uint32_t e = rgs_pack_exponent(__uint_as_float(group_max(top, min(lanes, RGS_PACK_BLOCK / VEC))));
+                    if (row < a.n && c < a.c) {
+                        if (c % RGS_PACK_BLOCK == 0) a.expo_out[row * a.blocks + c / RGS_PACK_BLOCK] = (uint8_t)e;
+                        store_codes<VEC>(a.codes_out, row * a.c + c, x[r][k], e);
+                    }
+                }
+                if (a.y && row < a.n && c < a.c) {
+                    float f[VEC];
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) f[q] = fmaf((x[r][k][q] - mu) * rstd, w[k][q], b[k][q]);
+                    store_vec<VEC>(a.y, row * a.c + c, a.y_dtype, f);
+                }
+            }
+        }
+    }
+}
+
+template <int VEC, int NV, int R>
+__global__ void __launch_bounds__(NT) rgs_norm_rows_bwd_kernel(const __grid_constant__ NormArgs a, int lanes) {
+    __shared__ float sh[NT * VEC];
+    const int l = threadIdx.x & (lanes - 1), groups = NT / lanes;
+    const int64_t stride = (int64_t)gridDim.x * groups;
+    float w[NV][VEC], sw[NV][VEC], sb[NV][VEC];
+    load_params<VEC, NV>(a, l, lanes, a.w, 1.f, w);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) sw[k][q] = sb[k][q] = 0.f;
+    for (int64_t i0 = (int64_t)blockIdx.x * groups; i0 < a.n; i0 += R * stride) {
+        const int64_t i = i0 + threadIdx.x / lanes;
+        float x[R][NV][VEC], g[R][NV][VEC];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = min(i + r * stride, a.n - 1);
+            load_row<VEC, NV>(a, row, l, lanes, x[r]);
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int c = (k * lanes + l) * VEC;
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) g[r][k][q] = 0.f;
+                if (c < a.c && i + r * stride < a.n) load_vec<VEC>(a.dy, row * a.ldy + c, a.dy_dtype, g[r][k]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = i + r * stride;
+            if (row >= a.n) {  // the last row again, in place of one behind the end: nothing of it counts, whatever it holds
+#pragma unroll
+                for (int k = 0; k < NV; ++k)
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) x[r][k][q] = 0.f;
+            }
+            row_bwd<VEC, NV>(x[r], g[r], w, sw, sb, l, lanes, a.c, a.inv_c, a.eps > 0.f ? a.eps : (row >= a.n ? 1.f : 0.f));
+            if (a.dx && row < a.n)
+#pragma unroll
+                for (int k = 0; k < NV; ++k) {
+                    const int c = (k * lanes + l) * VEC;
+                    if (c < a.c) store_vec<VEC>(a.dx, row * a.c + c, a.dx_dtype, x[r][k]);
+                }
+        }
+    }
+    if (a.part) block_sums<VEC, NV>(a, l, lanes, sw, sb, sh);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// channel planes: 32 pixels at a time through shared memory, (channel, pixel) with rows of 33
+// ---------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float plane_value(const NormArgs& a, int64_t i, int c) {
+    if (a.src == SRC_CODES)
+        return (float)a.codes[(int64_t)c * a.n + i] * rgs_pack_step(a.expo[(int64_t)(c / RGS_PACK_BLOCK) * a.n + i]);
+    return rgs_load_as_float(a.x, (int64_t)c * a.ld + i, a.src);
+}
+
+template <int NV, bool BWD>
+__global__ void __launch_bounds__(NT) rgs_norm_planes_kernel(const __grid_constant__ NormArgs a, int lanes) {
+    extern __shared__ float sm[];                // (c, 33); behind it room for the sums of a block
+    const int l = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = NT / lanes;
+    const int p = threadIdx.x & 31, c0 = threadIdx.x >> 5;
+    float w[NV][1], b[NV][1], sw[NV][1], sb[NV][1];
+    load_params<1, NV>(a, l, lanes, a.w, 1.f, w);
+    if (!BWD) load_params<1, NV>(a, l, lanes, a.b, 0.f, b);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) sw[k][0] = sb[k][0] = 0.f;
+    const int64_t tiles = (a.n + PT - 1) / PT;
+    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const int64_t base = t * PT;
+        __syncthreads();
+        if (base + p < a.n) {
+#pragma unroll 8
+            for (int c = c0; c < a.c; c += NT / 32) sm[c * 33 + p] = plane_value(a, base + p, c);
+        } else {
+            for (int c = c0; c < a.c; c += NT / 32) sm[c * 33 + p] = 0.f;
+        }
+        __syncthreads();
+        if (!BWD && a.codes_out && base + p < a.n) {
+            for (int k = c0; k < a.blocks; k += NT / 32) {
+                const int end = min(a.c, (k + 1) * RGS_PACK_BLOCK);
+                uint32_t top = 0;
+                for (int c = k * RGS_PACK_BLOCK; c < end; ++c) top = max(top, __float_as_uint(sm[c * 33 + p]) & 0x7fffffffu);
+                const uint32_t e = rgs_pack_exponent(__uint_as_float(top));
+                a.expo_out[(int64_t)k * a.n + base + p] = (uint8_t)e;
+                for (int c = k * RGS_PACK_BLOCK; c < end; ++c) {
+                    const float f[1] = {sm[c * 33 + p]};
+                    store_codes<1>(a.codes_out, (int64_t)c * a.n + base + p, f, e);
+                }
+            }
+        }
+        // PT is a multiple of the groups of a block or the other way round: whole warps leave together
+        for (int r = group; r < PT; r += groups) {
+            const int64_t row = base + r;
+            float x[NV][1];
+#pragma unroll
+            for (int k = 0; k < NV; ++k) x[k][0] = k * lanes + l < a.c ? sm[(k * lanes + l) * 33 + r] : 0.f;
+            if (!BWD) {
+                float mu, rstd;
+                row_stats<1, NV>(x, l, lanes, a.c, a.inv_c, a.eps, mu, rstd);
+                if (row < a.n)
+#pragma unroll
+                    for (int k = 0; k < NV; ++k) {
+                        const int c = k * lanes + l;
+                        const float f[1] = {fmaf((x[k][0] - mu) * rstd, w[k][0], b[k][0])};
+                        if (c < a.c) store_vec<1>(a.y, row * a.c + c, a.y_dtype, f);
+                    }
+            } else {
+                float g[NV][1];
+#pragma unroll
+                for (int k = 0; k < NV; ++k)
+                    g[k][0] = k * lanes + l < a.c && row < a.n ? rgs_load_as_float(a.dy, row * a.ldy + k * lanes + l, a.dy_dtype) : 0.f;
+                row_bwd<1, NV>(x, g, w, sw, sb, l, lanes, a.c, a.inv_c, row < a.n ? a.eps : 1.f);
+#pragma unroll
+                for (int k = 0; k < NV; ++k)
+                    if (k * lanes + l < a.c) sm[(k * lanes + l) * 33 + r] = x[k][0];
+            }
+        }
+        if (BWD && a.dx) {
+            __syncthreads();
+            if (base + p < a.n)
+                for (int c = c0; c < a.c; c += NT / 32) {
+                    const float f[1] = {sm[c * 33 + p]};
+                    store_vec<1>(a.dx, (int64_t)c * a.n + base + p, a.dx_dtype, f);
+                }
+        }
+    }
+    if (BWD && a.part) {
+        __syncthreads();
+        block_sums<1, NV>(a, l, lanes, sw, sb, sm);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// more channels than a group holds: a warp re-reads its row; a block of threads per 32 channels sums dw and db
+// ---------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float wide_value(const NormArgs& a, int64_t i, int c) {
+    if (a.planes) return plane_value(a, i, c);
+    if (a.src == SRC_CODES) return (float)a.codes[i * a.c + c] * rgs_pack_step(a.expo[i * a.blocks + c / RGS_PACK_BLOCK]);
+    return rgs_load_as_float(a.x, i * a.ld + c, a.src);
+}
+
+__global__ void __launch_bounds__(NT) rgs_norm_wide_kernel(const __grid_constant__ NormArgs a, int backward, float2* stats) {
     const int lane = threadIdx.x & 31;
-    for (int64_t i = (int64_t)blockIdx.x * NR_WARPS + (threadIdx.x >> 5); i < a.n; i += (int64_t)gridDim.x * NR_WARPS) {
-        float mu, rstd, sa = 0.f, sax = 0.f;
-        norm_stats(a, i, eps, lane, mu, rstd);
+    for (int64_t i = (int64_t)blockIdx.x * (NT / 32) + (threadIdx.x >> 5); i < a.n; i += (int64_t)gridDim.x * (NT / 32)) {
+        float s = 0.f;
+        for (int j = lane; j < a.c; j += 32) s += wide_value(a, i, j);
+        const float mu = group_sum(s, 32) * a.inv_c;
+        s = 0.f;
+        for (int j = lane; j < a.c; j += 32) { const float d = wide_value(a, i, j) - mu; s = fmaf(d, d, s); }
+        const float rstd = 1.0f / sqrtf(group_sum(s, 32) * a.inv_c + a.eps);
+        if (!backward) {
+            for (int j = lane; j < a.c; j += 32)
+                rgs_store_float(a.y, i * a.c + j, a.y_dtype,
+                                fmaf((wide_value(a, i, j) - mu) * rstd, a.w ? rgs_load_as_float(a.w, j, a.p_dtype) : 1.f,
+                                     a.b ? rgs_load_as_float(a.b, j, a.p_dtype) : 0.f));
+            continue;
+        }
         if (lane == 0) stats[i] = make_float2(mu, rstd);
-        if (!dx) continue;
-        for (int64_t j = lane; j < a.c; j += 32) {
-            const float g = rgs_load_as_float(dy, i * ldy + j, dy_dtype) * (w ? rgs_load_as_float(w, j, p_dtype) : 1.f);
+        if (!a.dx) continue;
+        float sa = 0.f, sax = 0.f;
+        for (int j = lane; j < a.c; j += 32) {
+            const float g = rgs_load_as_float(a.dy, i * a.ldy + j, a.dy_dtype) * (a.w ? rgs_load_as_float(a.w, j, a.p_dtype) : 1.f);
             sa += g;
-            sax = fmaf(g, (norm_value(a, i, j) - mu) * rstd, sax);
+            sax = fmaf(g, (wide_value(a, i, j) - mu) * rstd, sax);
         }
-        sa = norm_warp_sum(sa) / (float)a.c;
-        sax = norm_warp_sum(sax) / (float)a.c;
-        for (int64_t j = lane; j < a.c; j += 32) {
-            const float g = rgs_load_as_float(dy, i * ldy + j, dy_dtype) * (w ? rgs_load_as_float(w, j, p_dtype) : 1.f);
-            rgs_store_float(dx, a.planes ? j * a.n + i : i * a.c + j, x_dtype, rstd * (g - sa - (norm_value(a, i, j) - mu) * rstd * sax));
+        sa = group_sum(sa, 32) * a.inv_c;
+        sax = group_sum(sax, 32) * a.inv_c;
+        for (int j = lane; j < a.c; j += 32) {
+            const float g = rgs_load_as_float(a.dy, i * a.ldy + j, a.dy_dtype) * (a.w ? rgs_load_as_float(a.w, j, a.p_dtype) : 1.f);
+            rgs_store_float(a.dx, a.planes ? j * a.n + i : i * a.c + j, a.dx_dtype, rstd * (g - sa - (wide_value(a, i, j) - mu) * rstd * sax));
         }
     }
 }
 
-__global__ void __launch_bounds__(256) rgs_norm_dw_kernel(NormArgs a, const void* dy, int dy_dtype, int64_t ldy, const float2* stats,
-                                                          int p_dtype, void* dw, void* db) {
-    __shared__ double sw[256], sb[256];
-    const int64_t j = blockIdx.x;
-    double tw = 0, tb = 0;
-    for (int64_t i = threadIdx.x; i < a.n; i += 256) {
-        const float g = rgs_load_as_float(dy, i * ldy + j, dy_dtype);
-        const float2 s = stats[i];
-        tw += (double)(g * (norm_value(a, i, j) - s.x) * s.y);
-        tb += (double)g;
-    }
-    sw[threadIdx.x] = tw;
-    sb[threadIdx.x] = tb;
+__global__ void __launch_bounds__(NT) rgs_norm_wide_sums_kernel(const __grid_constant__ NormArgs a, const float2* stats) {
+    const int j = blockIdx.x * 32 + (threadIdx.x & 31), rows = gridDim.y * (NT / 32);
+    float sw = 0.f, sb = 0.f;
+    if (j < a.c)
+        for (int64_t i = (int64_t)blockIdx.y * (NT / 32) + (threadIdx.x >> 5); i < a.n; i += rows) {
+            const float g = rgs_load_as_float(a.dy, i * a.ldy + j, a.dy_dtype);
+            const float2 s = stats[i];
+            sw = fmaf(g, (wide_value(a, i, j) - s.x) * s.y, sw);
+            sb += g;
+        }
+    __shared__ float sh[2][NT / 32][32];
+    sh[0][threadIdx.x >> 5][threadIdx.x & 31] = sw;
+    sh[1][threadIdx.x >> 5][threadIdx.x & 31] = sb;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int k = 1; k < 256; ++k) { tw += sw[k]; tb += sb[k]; }
-        if (dw) rgs_store_float(dw, j, p_dtype, (float)tw);
-        if (db) rgs_store_float(db, j, p_dtype, (float)tb);
+    if (threadIdx.x < 64) {
+        const int which = threadIdx.x >> 5, c = blockIdx.x * 32 + (threadIdx.x & 31);
+        float t = 0.f;
+        for (int r = 0; r < NT / 32; ++r) t += sh[which][r][threadIdx.x & 31];
+        if (c < a.c) a.part[((int64_t)blockIdx.y * 2 + which) * a.c + c] = t;
     }
 }
 
-__global__ void __launch_bounds__(256) rgs_pack8_kernel(NormArgs a, int8_t* codes, uint8_t* expo) {
-    const int64_t blocks = (a.c + RGS_PACK_BLOCK - 1) / RGS_PACK_BLOCK, total = a.n * blocks;
-    const int lane = threadIdx.x & 31;
-    for (int64_t t = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5; t < total; t += (int64_t)gridDim.x * 8) {
-        const int64_t i = t / blocks, b = t % blocks, j = b * RGS_PACK_BLOCK + lane;
-        const float v = j < a.c ? norm_value(a, i, j) : 0.f;
-        const uint32_t top = __reduce_max_sync(0xffffffffu, rgs_f2u(v) & 0x7fffffffu);
-        const uint32_t e = rgs_pack_exponent(rgs_u2f(top));
-        if (lane == 0) expo[a.planes ? b * a.n + i : t] = (uint8_t)e;
-        if (j < a.c) codes[a.planes ? j * a.n + i : i * a.c + j] = (int8_t)(e == RGS_PACK_NAN ? 0 : rgs_pack_code(v, rgs_pack_inverse(e)));
+// adds the blocks' sums in order: 32 channels to a block, 32 interleaved chains each
+__global__ void __launch_bounds__(1024) rgs_norm_reduce_kernel(const float* __restrict__ part, int parts, int c, void* dw, void* db, int p_dtype) {
+    __shared__ float sh[32][33];
+    const int lane = threadIdx.x & 31, chain = threadIdx.x >> 5, j = blockIdx.x * 32 + lane, which = blockIdx.y;
+    float t = 0.f;
+    if (j < c)
+#pragma unroll 4
+        for (int k = chain; k < parts; k += 32) t += part[((int64_t)k * 2 + which) * c + j];
+    sh[chain][lane] = t;
+    __syncthreads();
+    if (chain == 0 && j < c) {
+        t = 0.f;
+        for (int k = 0; k < 32; ++k) t += sh[k][lane];
+        void* out = which ? db : dw;
+        if (out) rgs_store_float(out, j, p_dtype, t);
     }
 }
 
-__global__ void __launch_bounds__(256) rgs_unpack8_kernel(NormArgs a, void* out, int dtype) {
-    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < a.n * a.c; t += (int64_t)gridDim.x * 256) {
-        const int64_t i = a.planes ? t % a.n : t / a.c, j = a.planes ? t / a.n : t % a.c;
-        rgs_store_float(out, t, dtype, norm_value(a, i, j));
+// ---------------------------------------------------------------------------------------------------------------------
+// the 8-bit form by itself
+// ---------------------------------------------------------------------------------------------------------------------
+// Rows: 32 / VEC lanes to a 32-channel block, so that a warp reads and writes what lies together; four blocks in flight.
+// `flat`: whole blocks that follow one another without a gap, no division.
+template <int VEC>
+__global__ void __launch_bounds__(NT) rgs_pack8_rows_kernel(const __grid_constant__ NormArgs a, int flat) {
+    constexpr int LB = RGS_PACK_BLOCK / VEC, U = 4;
+    const int l = threadIdx.x % LB;
+    const int64_t total = a.n * a.blocks, per = NT / LB;
+    for (int64_t t0 = (int64_t)blockIdx.x * (per * U); t0 < total; t0 += (int64_t)gridDim.x * (per * U)) {
+        float x[U][VEC];
+        int64_t row[U];
+        int c[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t t = t0 + u * per + threadIdx.x / LB;
+            if (flat) { row[u] = t; c[u] = l * VEC; }
+            else {
+                row[u] = total < ((int64_t)1 << 31) ? (int64_t)((uint32_t)t / (uint32_t)a.blocks) : t / a.blocks;
+                c[u] = (int)(t - row[u] * a.blocks) * RGS_PACK_BLOCK + l * VEC;
+            }
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) x[u][q] = 0.f;
+            if (t < total && (flat || c[u] < a.c)) load_vec<VEC>(a.x, flat ? t * RGS_PACK_BLOCK + c[u] : row[u] * a.ld + c[u], a.src, x[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t t = t0 + u * per + threadIdx.x / LB;
+            uint32_t top = 0;
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) top = max(top, __float_as_uint(x[u][q]) & 0x7fffffffu);
+            const uint32_t e = rgs_pack_exponent(__uint_as_float(group_max(top, LB)));
+            if (t >= total) continue;
+            if (l == 0) a.expo_out[t] = (uint8_t)e;
+            if (flat) store_codes<VEC>(a.codes_out, t * RGS_PACK_BLOCK + c[u], x[u], e);
+            else if (c[u] < a.c) store_codes<VEC>(a.codes_out, row[u] * a.c + c[u], x[u], e);
+        }
+        __syncwarp();
     }
 }
 
-static inline unsigned norm_grid(int64_t n, int per_block) {
-    const int64_t want = (n + per_block - 1) / per_block, most = RGS_SMS * 16;
-    return (unsigned)(want < 1 ? 1 : (want > most ? most : want));
+// planes: a thread per pixel and block
+__global__ void __launch_bounds__(NT) rgs_pack8_planes_kernel(const __grid_constant__ NormArgs a) {
+    const int64_t tiles = (a.n + NT - 1) / NT;
+    for (int64_t t = blockIdx.x; t < tiles * a.blocks; t += gridDim.x) {
+        const int64_t k = t / tiles, i = (t - k * tiles) * NT + threadIdx.x;
+        if (i >= a.n) continue;
+        const int c = (int)k * RGS_PACK_BLOCK;
+        float x[RGS_PACK_BLOCK];
+        uint32_t top = 0;
+#pragma unroll
+        for (int q = 0; q < RGS_PACK_BLOCK; ++q) {
+            x[q] = c + q < a.c ? rgs_load_as_float(a.x, (int64_t)(c + q) * a.ld + i, a.src) : 0.f;
+            top = max(top, __float_as_uint(x[q]) & 0x7fffffffu);
+        }
+        const uint32_t e = rgs_pack_exponent(__uint_as_float(top));
+        a.expo_out[k * a.n + i] = (uint8_t)e;
+#pragma unroll
+        for (int q = 0; q < RGS_PACK_BLOCK; ++q)
+            if (c + q < a.c) {
+                const float f[1] = {x[q]};
+                store_codes<1>(a.codes_out, (int64_t)(c + q) * a.n + i, f, e);
+            }
+    }
+}
+
+// VEC codes to a thread, four such in flight; rows (VEC divides a row) or planes (VEC divides a plane)
+template <int VEC>
+__global__ void __launch_bounds__(NT) rgs_unpack8_kernel(const __grid_constant__ NormArgs a, int flat, void* out, int dtype) {
+    constexpr int U = 4;
+    const int64_t total = a.n * a.c / VEC;
+    const uint32_t per = (uint32_t)((a.planes ? a.n : a.c) / VEC);  // (below 2^31: rows and channels are)
+    for (int64_t t0 = (int64_t)blockIdx.x * (NT * U) + threadIdx.x; t0 < total; t0 += (int64_t)gridDim.x * (NT * U)) {
+        float f[U][VEC];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t t = t0 + u * NT;
+            if (t >= total) break;
+            if (a.planes) {
+                const int64_t c = total < ((int64_t)1 << 31) ? (int64_t)((uint32_t)t / per) : t / per, i = (t - c * per) * VEC;
+                float e[VEC];
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) e[q] = rgs_pack_step(a.expo[c / RGS_PACK_BLOCK * a.n + i + q]);
+                load_codes<VEC>(a.codes, t * VEC, 1.f, f[u]);
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) f[u][q] *= e[q];
+            } else {
+                int64_t k;
+                if (flat) k = t / (RGS_PACK_BLOCK / VEC);
+                else {
+                    const int64_t i = total < ((int64_t)1 << 31) ? (int64_t)((uint32_t)t / per) : t / per;
+                    k = i * a.blocks + (t - i * per) * VEC / RGS_PACK_BLOCK;
+                }
+                load_codes<VEC>(a.codes, t * VEC, rgs_pack_step(a.expo[k]), f[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (t0 + u * NT < total) store_vec<VEC>(out, (t0 + u * NT) * VEC, dtype, f[u]);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------------
+static inline int64_t norm_grid(int64_t want, int64_t per_sm) {
+    const int64_t most = RGS_SMS * per_sm;
+    return want < 1 ? 1 : (want > most ? most : want);
+}
+static inline bool aligned_to(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes) == 0; }
+static inline int64_t four(int dtype) { return dtype == RGS_BF16 ? 8 : 16; }  // bytes of four elements
+
+// smallest power of two of lanes that covers `vectors`, at most a warp
+static int norm_lanes(int64_t vectors) {
+    int lanes = 1;
+    while (lanes < 32 && lanes < vectors) lanes *= 2;
+    return lanes;
+}
+#define NORM_PARTS 1184   // most blocks that leave partial sums
+
+template <bool PACK>
+static void norm_rows_fwd(const NormArgs& a, bool vec, cudaStream_t st) {
+    const int lanes = norm_lanes(vec ? a.c / 4 : a.c), groups = NT / lanes, per = vec ? lanes * 4 : lanes;
+    const int nv = (a.c + per - 1) / per;
+#define NORM_FWD(V, K, R) rgs_norm_rows_fwd_kernel<V, K, R, PACK><<<(unsigned)norm_grid((a.n + groups * R - 1) / (groups * R), 32), NT, 0, st>>>(a, lanes)
+    if (vec) {
+        if (nv == 1) NORM_FWD(4, 1, 4);
+        else if (nv == 2) NORM_FWD(4, 2, 2);
+        else if (nv <= 4) NORM_FWD(4, 4, 1);
+        else NORM_FWD(4, 8, 1);
+    } else {
+        if (nv == 1) NORM_FWD(1, 1, 4);
+        else if (nv == 2) NORM_FWD(1, 2, 4);
+        else if (nv <= 4) NORM_FWD(1, 4, 2);
+        else if (nv <= 8) NORM_FWD(1, 8, 1);
+        else if (nv <= 16) NORM_FWD(1, 16, 1);
+        else if (nv <= 20) NORM_FWD(1, 20, 1);
+        else if (nv <= 24) NORM_FWD(1, 24, 1);
+        else if (nv <= 28) NORM_FWD(1, 28, 1);
+        else NORM_FWD(1, 32, 1);
+    }
+#undef NORM_FWD
+}
+
+static int norm_rows_bwd(const NormArgs& a, bool vec, cudaStream_t st) {
+    const int lanes = norm_lanes(vec ? a.c / 4 : a.c), groups = NT / lanes, per = vec ? lanes * 4 : lanes;
+    const int nv = (a.c + per - 1) / per;
+    int parts = 0;
+#define NORM_BWD(V, K, R, B)                                                                     \
+    {                                                                                            \
+        parts = (int)norm_grid((a.n + groups * R - 1) / (groups * R), B);                        \
+        if (parts > NORM_PARTS) parts = NORM_PARTS;                                              \
+        rgs_norm_rows_bwd_kernel<V, K, R><<<(unsigned)parts, NT, 0, st>>>(a, lanes);             \
+    }
+    if (vec) {
+        if (nv == 1) NORM_BWD(4, 1, 2, 8)
+        else if (nv == 2) NORM_BWD(4, 2, 1, 6)
+        else if (nv <= 4) NORM_BWD(4, 4, 1, 4)
+        else NORM_BWD(4, 8, 1, 2)
+    } else {
+        if (nv == 1) NORM_BWD(1, 1, 4, 8)
+        else if (nv == 2) NORM_BWD(1, 2, 2, 8)
+        else if (nv <= 4) NORM_BWD(1, 4, 2, 6)
+        else if (nv <= 8) NORM_BWD(1, 8, 1, 6)
+        else if (nv <= 16) NORM_BWD(1, 16, 1, 4)
+        else if (nv <= 20) NORM_BWD(1, 20, 1, 3)
+        else if (nv <= 24) NORM_BWD(1, 24, 1, 3)
+        else if (nv <= 28) NORM_BWD(1, 28, 1, 2)
+        else NORM_BWD(1, 32, 1, 2)
+    }
+#undef NORM_BWD
+    return parts;
+}
+
+template <int NV, bool BWD>
+static int norm_planes_launch(const NormArgs& a, int lanes, unsigned grid, cudaStream_t st) {
+    const int sums = NT;  // floats of block_sums
+    const int smem = (a.c * 33 > sums ? a.c * 33 : sums) * 4;
+    if (smem > 48 * 1024) RGS_CUDA_CHECK(cudaFuncSetAttribute(rgs_norm_planes_kernel<NV, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    rgs_norm_planes_kernel<NV, BWD><<<grid, NT, smem, st>>>(a, lanes);
+    return (int)cudaGetLastError();
+}
+
+template <bool BWD>
+static int norm_planes(const NormArgs& a, int* parts, cudaStream_t st) {
+    const int lanes = norm_lanes(a.c), nv = (a.c + lanes - 1) / lanes;
+    int64_t per_sm = (200 * 1024) / (a.c * 33 * 4 + 1024);
+    per_sm = per_sm > 8 ? 8 : (per_sm < 1 ? 1 : per_sm);
+    const int64_t grid = norm_grid((a.n + PT - 1) / PT, per_sm);
+    *parts = (int)grid;
+    if (nv == 1) return norm_planes_launch<1, BWD>(a, lanes, (unsigned)grid, st);
+    if (nv == 2) return norm_planes_launch<2, BWD>(a, lanes, (unsigned)grid, st);
+    if (nv <= 4) return norm_planes_launch<4, BWD>(a, lanes, (unsigned)grid, st);
+    if (nv <= 8) return norm_planes_launch<8, BWD>(a, lanes, (unsigned)grid, st);
+    if (nv <= 16) return norm_planes_launch<16, BWD>(a, lanes, (unsigned)grid, st);
+    return norm_planes_launch<32, BWD>(a, lanes, (unsigned)grid, st);
 }
 
 extern "C" {
 
-int64_t rgs_cuda_norm_scratch_bytes(int64_t n, int64_t) { return n * 8 + 16; }
+int64_t rgs_cuda_norm_scratch_bytes(int64_t n, int64_t c) { return (int64_t)NORM_PARTS * 2 * c * 4 + (c > NR_MAX ? n * 8 : 0) + 16; }
 
 int rgs_cuda_pack8(const void* x, int64_t dtype, int64_t ld, int64_t planes, int64_t n, int64_t c, int8_t* codes, uint8_t* expo, void* stream) {
-    const NormArgs a{x, (int)dtype, ld, (int)planes, nullptr, nullptr, n, c};
-    rgs_pack8_kernel<<<norm_grid(n * ((c + 31) / 32), 8), 256, 0, (cudaStream_t)stream>>>(a, codes, expo);
+    cudaStream_t st = (cudaStream_t)stream;
+    NormArgs a{};
+    a.x = x; a.src = (int)dtype; a.ld = ld; a.planes = (int)planes; a.n = n; a.c = (int)c; a.blocks = (int)((c + 31) / 32);
+    a.codes_out = codes; a.expo_out = expo;
+    if (planes) {
+        rgs_pack8_planes_kernel<<<(unsigned)norm_grid((n + NT - 1) / NT * a.blocks, 16), NT, 0, st>>>(a);
+    } else if (c % 4 == 0 && ld % 4 == 0 && aligned_to(x, four(a.src))) {
+        rgs_pack8_rows_kernel<4><<<(unsigned)norm_grid((n * a.blocks * 8 + NT * 4 - 1) / (NT * 4), 32), NT, 0, st>>>(a, c % 32 == 0 && ld == c);
+    } else {
+        rgs_pack8_rows_kernel<1><<<(unsigned)norm_grid((n * a.blocks * 32 + NT * 4 - 1) / (NT * 4), 32), NT, 0, st>>>(a, 0);
+    }
     return (int)cudaGetLastError();
 }
 
 int rgs_cuda_unpack8(const int8_t* codes, const uint8_t* expo, int64_t planes, int64_t n, int64_t c, void* out, int64_t dtype, void* stream) {
-    const NormArgs a{nullptr, 0, 0, (int)planes, codes, expo, n, c};
-    rgs_unpack8_kernel<<<norm_grid(n * c, 256), 256, 0, (cudaStream_t)stream>>>(a, out, (int)dtype);
+    cudaStream_t st = (cudaStream_t)stream;
+    NormArgs a{};
+    a.codes = codes; a.expo = expo; a.planes = (int)planes; a.n = n; a.c = (int)c; a.blocks = (int)((c + 31) / 32);
+    if ((planes ? n : c) % 4 == 0)
+        rgs_unpack8_kernel<4><<<(unsigned)norm_grid((n * c / 4 + NT * 4 - 1) / (NT * 4), 32), NT, 0, st>>>(a, !planes && c % 32 == 0, out, (int)dtype);
+    else
+        rgs_unpack8_kernel<1><<<(unsigned)norm_grid((n * c + NT * 4 - 1) / (NT * 4), 32), NT, 0, st>>>(a, 0, out, (int)dtype);
     return (int)cudaGetLastError();
 }
 
 int rgs_cuda_norm_fwd(const void* x, int64_t dtype, int64_t ld, int64_t planes, const void* w, const void* b, int64_t p_dtype, int64_t n,
                       int64_t c, double eps, void* y, int64_t y_dtype, int8_t* codes, uint8_t* expo, void* stream) {
-    const NormArgs a{x, (int)dtype, ld, (int)planes, nullptr, nullptr, n, c};
-    rgs_norm_fwd_kernel<<<norm_grid(n, NR_WARPS), NR_WARPS * 32, 0, (cudaStream_t)stream>>>(a, w, b, (int)p_dtype, (float)eps, y, (int)y_dtype);
-    RGS_CUDA_CHECK(cudaGetLastError());
-    return codes ? rgs_cuda_pack8(x, dtype, ld, planes, n, c, codes, expo, stream) : 0;
+    cudaStream_t st = (cudaStream_t)stream;
+    NormArgs a{};
+    a.x = x; a.src = (int)dtype; a.ld = ld; a.planes = (int)planes;
+    a.w = w; a.b = b; a.p_dtype = (int)p_dtype;
+    a.n = n; a.c = (int)c; a.blocks = (int)((c + 31) / 32); a.eps = (float)eps; a.inv_c = 1.f / (float)c;
+    a.y = y; a.y_dtype = (int)y_dtype;
+    a.codes_out = codes; a.expo_out = expo;
+    if (c > NR_MAX) {
+        rgs_norm_wide_kernel<<<(unsigned)norm_grid((n + 7) / 8, 16), NT, 0, st>>>(a, 0, nullptr);
+        RGS_CUDA_CHECK(cudaGetLastError());
+        return codes ? rgs_cuda_pack8(x, dtype, ld, planes, n, c, codes, expo, stream) : 0;
+    }
+    if (planes) {
+        int parts;
+        return norm_planes<false>(a, &parts, st);
+    }
+    const bool vec = c % 4 == 0 && ld % 4 == 0 && aligned_to(x, four(a.src));
+    if (codes) norm_rows_fwd<true>(a, vec, st);
+    else norm_rows_fwd<false>(a, vec, st);
+    return (int)cudaGetLastError();
 }
 
 int rgs_cuda_norm_bwd(const void* x, int64_t dtype, int64_t ld, int64_t planes, const int8_t* codes, const uint8_t* expo, const void* dy,
                       int64_t dy_dtype, int64_t ldy, const void* w, int64_t p_dtype, int64_t n, int64_t c, double eps, void* scratch,
                       void* dx, void* dw, void* db, void* stream) {
-    const NormArgs a{x, (int)dtype, ld, (int)planes, codes, expo, n, c};
-    float2* stats = static_cast<float2*>(scratch);
-    rgs_norm_bwd_kernel<<<norm_grid(n, NR_WARPS), NR_WARPS * 32, 0, (cudaStream_t)stream>>>(a, dy, (int)dy_dtype, ldy, w, (int)p_dtype,
-                                                                                            (float)eps, stats, dx, (int)dtype);
-    if (dw || db)
-        rgs_norm_dw_kernel<<<(unsigned)c, 256, 0, (cudaStream_t)stream>>>(a, dy, (int)dy_dtype, ldy, stats, (int)p_dtype, dw, db);
+    cudaStream_t st = (cudaStream_t)stream;
+    NormArgs a{};
+    a.x = x; a.src = codes ? SRC_CODES : (int)dtype; a.ld = ld; a.planes = (int)planes;
+    a.codes = codes; a.expo = expo;
+    a.w = w; a.p_dtype = (int)p_dtype;
+    a.n = n; a.c = (int)c; a.blocks = (int)((c + 31) / 32); a.eps = (float)eps; a.inv_c = 1.f / (float)c;
+    a.dy = dy; a.dy_dtype = (int)dy_dtype; a.ldy = ldy;
+    a.dx = dx; a.dx_dtype = (int)dtype;
+    a.part = dw || db ? static_cast<float*>(scratch) : nullptr;
+    int parts = 0;
+    if (c > NR_MAX) {
+        float2* stats = reinterpret_cast<float2*>(static_cast<float*>(scratch) + (int64_t)NORM_PARTS * 2 * c);
+        rgs_norm_wide_kernel<<<(unsigned)norm_grid((n + 7) / 8, 16), NT, 0, st>>>(a, 1, stats);
+        if (a.part) {
+            parts = (int)norm_grid((n + 63) / 64, 1);
+            rgs_norm_wide_sums_kernel<<<dim3((unsigned)((c + 31) / 32), (unsigned)parts), NT, 0, st>>>(a, stats);
+        }
+    } else if (planes) {
+        const int rc = norm_planes<true>(a, &parts, st);
+        if (rc) return rc;
+    } else {
+        const bool vec = c % 4 == 0 && ldy % 4 == 0 && aligned_to(dy, four(a.dy_dtype)) &&
+                         (codes || (ld % 4 == 0 && aligned_to(x, four((int)dtype))));
+        parts = norm_rows_bwd(a, vec, st);
+    }
+    RGS_CUDA_CHECK(cudaGetLastError());
+    if (a.part)
+        rgs_norm_reduce_kernel<<<dim3((unsigned)((c + 31) / 32), 2), 1024, 0, st>>>(a.part, parts, (int)c, dw, db, (int)p_dtype);
     return (int)cudaGetLastError();
 }
 

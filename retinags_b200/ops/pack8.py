@@ -35,6 +35,8 @@ def as_rows(x: torch.Tensor, what: str, planes_ok: bool = True):
         raise ValueError(f"{what}: shape (..., C) with at least one channel expected, got {tuple(x.shape)}")
     c = x.shape[-1]
     n = x.numel() // c
+    if n > 2 ** 31 - 1:
+        raise ValueError(f"{what}: at most 2^31 - 1 rows, got {n}")
     if n == 0:
         return x.reshape(0, c), c, 0
     if x.is_contiguous():
