@@ -14,6 +14,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <atomic>
 #include "rgs_cuda_common.cuh"
 #include "rgs_field_math.h"
 
@@ -36,22 +37,39 @@ struct NormArgs {
     float* part;                                   // (blocks of the grid, 2, c)
 };
 
-template <int VEC> struct Vec { float v[VEC]; };
-
-template <int VEC>
-__device__ __forceinline__ void load_vec(const void* p, int64_t i, int dtype, float (&f)[VEC]) {
-    if constexpr (VEC == 4) {
-        if (dtype == RGS_BF16) {
-            const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
-            f[0] = __uint_as_float(u.x << 16); f[1] = __uint_as_float(u.x & 0xffff0000u);
-            f[2] = __uint_as_float(u.y << 16); f[3] = __uint_as_float(u.y & 0xffff0000u);
-        } else {
-            const float4 u = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-            f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
-        }
+// The switch on a type stands outside the loops over a row's vectors, so that all loads of a row are in flight together
+// (inside, every load waited for the one before: 3 to 4 times slower on wide or odd rows).
+template <int VEC, int DT>
+__device__ __forceinline__ void load_vec(const void* p, int64_t i, float (&f)[VEC]) {
+    if constexpr (VEC == 4 && DT == RGS_BF16) {
+        const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+        f[0] = __uint_as_float(u.x << 16); f[1] = __uint_as_float(u.x & 0xffff0000u);
+        f[2] = __uint_as_float(u.y << 16); f[3] = __uint_as_float(u.y & 0xffff0000u);
+    } else if constexpr (VEC == 4) {
+        const float4 u = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+        f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
+    } else if constexpr (DT == RGS_BF16) {
+        f[0] = __uint_as_float((uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
     } else {
-        f[0] = rgs_load_as_float(p, i, dtype);
+        f[0] = static_cast<const float*>(p)[i];
     }
+}
+// vectors k of a lane, (k lanes + l) VEC, of the row that starts at element i; zero behind the last channel
+template <int VEC, int NV, int LANES, int DT>
+__device__ __forceinline__ void load_all(const void* p, int64_t i, int l, int c, float (&x)[NV][VEC]) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int at = (k * LANES + l) * VEC;
+        if (at < c) load_vec<VEC, DT>(p, i + at, x[k]);
+        else
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) x[k][q] = 0.f;
+    }
+}
+template <int VEC, int NV, int LANES>
+__device__ __forceinline__ void load_typed(const void* p, int dtype, int64_t i, int l, int c, float (&x)[NV][VEC]) {
+    if (dtype == RGS_BF16) load_all<VEC, NV, LANES, RGS_BF16>(p, i, l, c, x);
+    else load_all<VEC, NV, LANES, RGS_F32>(p, i, l, c, x);
 }
 __device__ __forceinline__ uint32_t pair_bf16(float lo, float hi) {
     uint32_t r;
@@ -93,45 +111,49 @@ __device__ __forceinline__ void load_codes(const int8_t* p, int64_t i, float ste
     }
 }
 
-// sum over the `lanes` lanes (a power of two) that share a row
-__device__ __forceinline__ float group_sum(float v, int lanes) {
-    for (int d = lanes >> 1; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+// sum, or maximum, over the LANES lanes (a power of two) that share a row
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+    for (int d = LANES >> 1; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     return v;
 }
-__device__ __forceinline__ uint32_t group_max(uint32_t v, int lanes) {
-    for (int d = lanes >> 1; d > 0; d >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
+template <int LANES>
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+#pragma unroll
+    for (int d = LANES >> 1; d > 0; d >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
     return v;
 }
 
 // mean and 1 / sqrt(var + eps) of a row; vector k of a lane starts at channel (k lanes + lane) VEC
-template <int VEC, int NV>
-__device__ __forceinline__ void row_stats(const float (&x)[NV][VEC], int l, int lanes, int c, float inv_c, float eps, float& mu, float& rstd) {
+template <int VEC, int NV, int LANES>
+__device__ __forceinline__ void row_stats(const float (&x)[NV][VEC], int l, int c, float inv_c, float eps, float& mu, float& rstd) {
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int q = 0; q < VEC; ++q) s += x[k][q];   // zero behind the last channel
-    mu = group_sum(s, lanes) * inv_c;
+    mu = group_sum<LANES>(s) * inv_c;
     s = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-        if ((k * lanes + l) * VEC < c)
+        if ((k * LANES + l) * VEC < c)
 #pragma unroll
             for (int q = 0; q < VEC; ++q) s = fmaf(x[k][q] - mu, x[k][q] - mu, s);
-    rstd = 1.0f / sqrtf(group_sum(s, lanes) * inv_c + eps);
+    rstd = 1.0f / sqrtf(group_sum<LANES>(s) * inv_c + eps);
 }
 
 // the part of the backward pass that rows and planes share: a row's x, dy -> dx (over x), sums of dw and db
-template <int VEC, int NV>
+template <int VEC, int NV, int LANES>
 __device__ __forceinline__ void row_bwd(float (&x)[NV][VEC], float (&g)[NV][VEC], const float (&w)[NV][VEC], float (&sw)[NV][VEC], float (&sb)[NV][VEC],
-                                        int l, int lanes, int c, float inv_c, float eps) {
+                                        int l, int c, float inv_c, float eps) {
     float mu, rstd, sa = 0.f, sax = 0.f;
-    row_stats<VEC, NV>(x, l, lanes, c, inv_c, eps, mu, rstd);
+    row_stats<VEC, NV, LANES>(x, l, c, inv_c, eps, mu, rstd);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int q = 0; q < VEC; ++q) {
-            const bool in = (k * lanes + l) * VEC < c;
+            const bool in = (k * LANES + l) * VEC < c;
             x[k][q] = in ? (x[k][q] - mu) * rstd : 0.f;
             sw[k][q] = fmaf(g[k][q], x[k][q], sw[k][q]);
             sb[k][q] += g[k][q];
@@ -139,41 +161,43 @@ __device__ __forceinline__ void row_bwd(float (&x)[NV][VEC], float (&g)[NV][VEC]
             sa += g[k][q];
             sax = fmaf(g[k][q], x[k][q], sax);
         }
-    sa = group_sum(sa, lanes) * inv_c;
-    sax = group_sum(sax, lanes) * inv_c;
+    sa = group_sum<LANES>(sa) * inv_c;
+    sax = group_sum<LANES>(sax) * inv_c;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int q = 0; q < VEC; ++q) x[k][q] = rstd * (g[k][q] - sa - x[k][q] * sax);
 }
 
-template <int VEC, int NV>
-__device__ __forceinline__ void load_params(const NormArgs& a, int l, int lanes, const void* p, float none, float (&w)[NV][VEC]) {
+template <int VEC, int NV, int LANES>
+__device__ __forceinline__ void load_params(const NormArgs& a, int l, const void* p, float none, float (&w)[NV][VEC]) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int c = (k * lanes + l) * VEC;
+    for (int k = 0; k < NV; ++k)
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) w[k][q] = p && c + q < a.c ? rgs_load_as_float(p, c + q, a.p_dtype) : none;
-    }
+        for (int q = 0; q < VEC; ++q) {
+            const int c = (k * LANES + l) * VEC + q;
+            w[k][q] = none;
+            if (p && c < a.c) w[k][q] = a.p_dtype == RGS_BF16 ? rgs_bf16_value(static_cast<const uint16_t*>(p)[c]) : static_cast<const float*>(p)[c];
+        }
 }
 
 // sums of a block's groups, in the order of the groups, to the block's row of the partial sums
-template <int VEC, int NV>
-__device__ __forceinline__ void block_sums(const NormArgs& a, int l, int lanes, const float (&sw)[NV][VEC], const float (&sb)[NV][VEC], float* sh) {
+template <int VEC, int NV, int LANES>
+__device__ __forceinline__ void block_sums(const NormArgs& a, int l, const float (&sw)[NV][VEC], const float (&sb)[NV][VEC], float* sh) {
     // sh: (groups of the block, channels) of one of the two sums at a time, 64 channels a turn
-    const int group = threadIdx.x / lanes, groups = NT / lanes;
+    const int group = threadIdx.x / LANES, groups = NT / LANES;
     for (int which = 0; which < 2; ++which)
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            if (k * lanes * VEC >= a.c) break;
+            if (k * LANES * VEC >= a.c) break;
             __syncthreads();
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) sh[group * (lanes * VEC) + l * VEC + q] = which ? sb[k][q] : sw[k][q];
+            for (int q = 0; q < VEC; ++q) sh[group * (LANES * VEC) + l * VEC + q] = which ? sb[k][q] : sw[k][q];
             __syncthreads();
-            for (int j = threadIdx.x; j < lanes * VEC; j += NT) {
+            for (int j = threadIdx.x; j < LANES * VEC; j += NT) {
                 float t = 0.f;
-                for (int r = 0; r < groups; ++r) t += sh[r * (lanes * VEC) + j];
-                const int c = k * lanes * VEC + j;
+                for (int r = 0; r < groups; ++r) t += sh[r * (LANES * VEC) + j];
+                const int c = k * LANES * VEC + j;
                 if (c < a.c) a.part[((int64_t)blockIdx.x * 2 + which) * a.c + c] = t;
             }
         }
@@ -182,51 +206,69 @@ __device__ __forceinline__ void block_sums(const NormArgs& a, int l, int lanes, 
 // ---------------------------------------------------------------------------------------------------------------------
 // rows
 // ---------------------------------------------------------------------------------------------------------------------
-template <int VEC, int NV>
-__device__ __forceinline__ void load_row(const NormArgs& a, int64_t i, int l, int lanes, float (&x)[NV][VEC]) {
+template <int VEC, int NV, int LANES>
+__device__ __forceinline__ void load_row(const NormArgs& a, int64_t i, int l, float (&x)[NV][VEC]) {
+    if (a.src == SRC_CODES) {
+        float step[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int c = (k * lanes + l) * VEC;
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) x[k][q] = 0.f;
-        if (c < a.c) {
-            if (a.src == SRC_CODES) load_codes<VEC>(a.codes, i * a.c + c, rgs_pack_step(a.expo[i * a.blocks + c / RGS_PACK_BLOCK]), x[k]);
-            else load_vec<VEC>(a.x, i * a.ld + c, a.src, x[k]);
+        for (int k = 0; k < NV; ++k) {
+            const int at = (k * LANES + l) * VEC;
+            step[k] = at < a.c ? rgs_pack_step(a.expo[i * a.blocks + at / RGS_PACK_BLOCK]) : 0.f;
         }
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int at = (k * LANES + l) * VEC;
+            if (at < a.c) load_codes<VEC>(a.codes, i * a.c + at, step[k], x[k]);
+            else
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) x[k][q] = 0.f;
+        }
+    } else {
+        load_typed<VEC, NV, LANES>(a.x, a.src, i * a.ld, l, a.c, x);
     }
 }
 
-template <int VEC, int NV, int R, bool PACK>
-__global__ void __launch_bounds__(NT) rgs_norm_rows_fwd_kernel(const __grid_constant__ NormArgs a, int lanes) {
-    const int l = threadIdx.x & (lanes - 1), groups = NT / lanes;
+template <int VEC, int NV, int LANES, int R, bool PACK>
+__global__ void __launch_bounds__(NT) rgs_norm_rows_fwd_kernel(const __grid_constant__ NormArgs a) {
+    const int l = threadIdx.x % LANES, groups = NT / LANES;
     const int64_t stride = (int64_t)gridDim.x * groups;
     float w[NV][VEC], b[NV][VEC];
-    load_params<VEC, NV>(a, l, lanes, a.w, 1.f, w);
-    load_params<VEC, NV>(a, l, lanes, a.b, 0.f, b);
+    load_params<VEC, NV, LANES>(a, l, a.w, 1.f, w);
+    load_params<VEC, NV, LANES>(a, l, a.b, 0.f, b);
     // all lanes of a warp take the same number of turns: shuffles need them
     for (int64_t i0 = (int64_t)blockIdx.x * groups; i0 < a.n; i0 += R * stride) {
-        const int64_t i = i0 + threadIdx.x / lanes;
+        const int64_t i = i0 + threadIdx.x / LANES;
         float x[R][NV][VEC];
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            load_row<VEC, NV>(a, min(i + r * stride, a.n - 1), l, lanes, x[r]);
+            load_row<VEC, NV, LANES>(a, min(i + r * stride, a.n - 1), l, x[r]);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int64_t row = i + r * stride;
             float mu, rstd;
-            row_stats<VEC, NV>(x[r], l, lanes, a.c, a.inv_c, a.eps, mu, rstd);
+            row_stats<VEC, NV, LANES>(x[r], l, a.c, a.inv_c, a.eps, mu, rstd);
+            uint32_t top[NV];
+            if (PACK) {
+                // a block of 32 channels is 32 / VEC vectors: KB of every lane of the row, or one of some of its lanes
+                constexpr int LB = RGS_PACK_BLOCK / VEC, KB = LANES < LB ? LB / LANES : 1;
+#pragma unroll
+                for (int k = 0; k < NV; k += KB) {
+                    uint32_t m = 0;
+#pragma unroll
+                    for (int e = k; e < k + KB && e < NV; ++e)
+#pragma unroll
+                        for (int q = 0; q < VEC; ++q) m = max(m, __float_as_uint(x[r][e][q]) & 0x7fffffffu);
+                    m = rgs_pack_exponent(__uint_as_float(group_max<(LANES < LB ? LANES : LB)>(m)));
+#pragma unroll
+                    for (int e = k; e < k + KB && e < NV; ++e) top[e] = m;
+                }
+            }
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const int c = (k * lanes + l) * VEC;
-                if (PACK) {
-                    uint32_t top = 0;
-#pragma unroll
-                    for (int q = 0; q < VEC; ++q) top = max(top, __float_as_uint(x[r][k][q]) & 0x7fffffffu);
-                    const uint32_t e = rgs_pack_exponent(__uint_as_float(group_max(top, min(lanes, RGS_PACK_BLOCK / VEC))));
-                    if (row < a.n && c < a.c) {
-                        if (c % RGS_PACK_BLOCK == 0) a.expo_out[row * a.blocks + c / RGS_PACK_BLOCK] = (uint8_t)e;
-                        store_codes<VEC>(a.codes_out, row * a.c + c, x[r][k], e);
-                    }
+                const int c = (k * LANES + l) * VEC;
+                if (PACK && row < a.n && c < a.c) {
+                    if (c % RGS_PACK_BLOCK == 0) a.expo_out[row * a.blocks + c / RGS_PACK_BLOCK] = (uint8_t)top[k];
+                    store_codes<VEC>(a.codes_out, row * a.c + c, x[r][k], top[k]);
                 }
                 if (a.y && row < a.n && c < a.c) {
                     float f[VEC];
@@ -239,31 +281,25 @@ __global__ void __launch_bounds__(NT) rgs_norm_rows_fwd_kernel(const __grid_cons
     }
 }
 
-template <int VEC, int NV, int R>
-__global__ void __launch_bounds__(NT) rgs_norm_rows_bwd_kernel(const __grid_constant__ NormArgs a, int lanes) {
+template <int VEC, int NV, int LANES, int R>
+__global__ void __launch_bounds__(NT) rgs_norm_rows_bwd_kernel(const __grid_constant__ NormArgs a) {
     __shared__ float sh[NT * VEC];
-    const int l = threadIdx.x & (lanes - 1), groups = NT / lanes;
+    const int l = threadIdx.x % LANES, groups = NT / LANES;
     const int64_t stride = (int64_t)gridDim.x * groups;
     float w[NV][VEC], sw[NV][VEC], sb[NV][VEC];
-    load_params<VEC, NV>(a, l, lanes, a.w, 1.f, w);
+    load_params<VEC, NV, LANES>(a, l, a.w, 1.f, w);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int q = 0; q < VEC; ++q) sw[k][q] = sb[k][q] = 0.f;
     for (int64_t i0 = (int64_t)blockIdx.x * groups; i0 < a.n; i0 += R * stride) {
-        const int64_t i = i0 + threadIdx.x / lanes;
+        const int64_t i = i0 + threadIdx.x / LANES;
         float x[R][NV][VEC], g[R][NV][VEC];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int64_t row = min(i + r * stride, a.n - 1);
-            load_row<VEC, NV>(a, row, l, lanes, x[r]);
-#pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const int c = (k * lanes + l) * VEC;
-#pragma unroll
-                for (int q = 0; q < VEC; ++q) g[r][k][q] = 0.f;
-                if (c < a.c && i + r * stride < a.n) load_vec<VEC>(a.dy, row * a.ldy + c, a.dy_dtype, g[r][k]);
-            }
+            load_row<VEC, NV, LANES>(a, row, l, x[r]);
+            load_typed<VEC, NV, LANES>(a.dy, a.dy_dtype, row * a.ldy, l, i + r * stride < a.n ? a.c : 0, g[r]);
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -274,16 +310,16 @@ __global__ void __launch_bounds__(NT) rgs_norm_rows_bwd_kernel(const __grid_cons
 #pragma unroll
                     for (int q = 0; q < VEC; ++q) x[r][k][q] = 0.f;
             }
-            row_bwd<VEC, NV>(x[r], g[r], w, sw, sb, l, lanes, a.c, a.inv_c, a.eps > 0.f ? a.eps : (row >= a.n ? 1.f : 0.f));
+            row_bwd<VEC, NV, LANES>(x[r], g[r], w, sw, sb, l, a.c, a.inv_c, a.eps > 0.f ? a.eps : (row >= a.n ? 1.f : 0.f));
             if (a.dx && row < a.n)
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
-                    const int c = (k * lanes + l) * VEC;
+                    const int c = (k * LANES + l) * VEC;
                     if (c < a.c) store_vec<VEC>(a.dx, row * a.c + c, a.dx_dtype, x[r][k]);
                 }
         }
     }
-    if (a.part) block_sums<VEC, NV>(a, l, lanes, sw, sb, sh);
+    if (a.part) block_sums<VEC, NV, LANES>(a, l, sw, sb, sh);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -294,15 +330,27 @@ __device__ __forceinline__ float plane_value(const NormArgs& a, int64_t i, int c
         return (float)a.codes[(int64_t)c * a.n + i] * rgs_pack_step(a.expo[(int64_t)(c / RGS_PACK_BLOCK) * a.n + i]);
     return rgs_load_as_float(a.x, (int64_t)c * a.ld + i, a.src);
 }
+// channels c0, c0 + 8, ... of pixel i to shared memory
+template <int SRC>
+__device__ __forceinline__ void load_plane(const NormArgs& a, int64_t i, int c0, int p, float* sm) {
+#pragma unroll 8
+    for (int c = c0; c < a.c; c += NT / 32) {
+        float f[1];
+        if constexpr (SRC == SRC_CODES) load_codes<1>(a.codes, (int64_t)c * a.n + i, rgs_pack_step(a.expo[(int64_t)(c / RGS_PACK_BLOCK) * a.n + i]), f);
+        else load_vec<1, SRC>(a.x, (int64_t)c * a.ld + i, f);
+        sm[c * 33 + p] = f[0];
+    }
+}
 
-template <int NV, bool BWD>
-__global__ void __launch_bounds__(NT) rgs_norm_planes_kernel(const __grid_constant__ NormArgs a, int lanes) {
+template <int NV, int LANES, bool BWD>
+__global__ void __launch_bounds__(NT) rgs_norm_planes_kernel(const __grid_constant__ NormArgs a) {
     extern __shared__ float sm[];                // (c, 33); behind it room for the sums of a block
-    const int l = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = NT / lanes;
+    constexpr int WR = 32 / LANES;               // rows of a warp, LANES apart: their words lie in different banks
+    const int l = threadIdx.x % LANES;
     const int p = threadIdx.x & 31, c0 = threadIdx.x >> 5;
     float w[NV][1], b[NV][1], sw[NV][1], sb[NV][1];
-    load_params<1, NV>(a, l, lanes, a.w, 1.f, w);
-    if (!BWD) load_params<1, NV>(a, l, lanes, a.b, 0.f, b);
+    load_params<1, NV, LANES>(a, l, a.w, 1.f, w);
+    if (!BWD) load_params<1, NV, LANES>(a, l, a.b, 0.f, b);
 #pragma unroll
     for (int k = 0; k < NV; ++k) sw[k][0] = sb[k][0] = 0.f;
     const int64_t tiles = (a.n + PT - 1) / PT;
@@ -310,8 +358,9 @@ __global__ void __launch_bounds__(NT) rgs_norm_planes_kernel(const __grid_consta
         const int64_t base = t * PT;
         __syncthreads();
         if (base + p < a.n) {
-#pragma unroll 8
-            for (int c = c0; c < a.c; c += NT / 32) sm[c * 33 + p] = plane_value(a, base + p, c);
+            if (a.src == SRC_CODES) load_plane<SRC_CODES>(a, base + p, c0, p, sm);
+            else if (a.src == SRC_BF16) load_plane<SRC_BF16>(a, base + p, c0, p, sm);
+            else load_plane<SRC_F32>(a, base + p, c0, p, sm);
         } else {
             for (int c = c0; c < a.c; c += NT / 32) sm[c * 33 + p] = 0.f;
         }
@@ -329,31 +378,29 @@ __global__ void __launch_bounds__(NT) rgs_norm_planes_kernel(const __grid_consta
                 }
             }
         }
-        // PT is a multiple of the groups of a block or the other way round: whole warps leave together
-        for (int r = group; r < PT; r += groups) {
+        for (int r0 = threadIdx.x >> 5; r0 < PT / WR; r0 += NT / 32) {
+            const int r = r0 + (threadIdx.x & 31) / LANES * (PT / WR);
             const int64_t row = base + r;
             float x[NV][1];
 #pragma unroll
-            for (int k = 0; k < NV; ++k) x[k][0] = k * lanes + l < a.c ? sm[(k * lanes + l) * 33 + r] : 0.f;
+            for (int k = 0; k < NV; ++k) x[k][0] = k * LANES + l < a.c ? sm[(k * LANES + l) * 33 + r] : 0.f;
             if (!BWD) {
                 float mu, rstd;
-                row_stats<1, NV>(x, l, lanes, a.c, a.inv_c, a.eps, mu, rstd);
+                row_stats<1, NV, LANES>(x, l, a.c, a.inv_c, a.eps, mu, rstd);
                 if (row < a.n)
 #pragma unroll
                     for (int k = 0; k < NV; ++k) {
-                        const int c = k * lanes + l;
+                        const int c = k * LANES + l;
                         const float f[1] = {fmaf((x[k][0] - mu) * rstd, w[k][0], b[k][0])};
                         if (c < a.c) store_vec<1>(a.y, row * a.c + c, a.y_dtype, f);
                     }
             } else {
                 float g[NV][1];
+                load_typed<1, NV, LANES>(a.dy, a.dy_dtype, row * a.ldy, l, row < a.n ? a.c : 0, g);
+                row_bwd<1, NV, LANES>(x, g, w, sw, sb, l, a.c, a.inv_c, row < a.n ? a.eps : 1.f);
 #pragma unroll
                 for (int k = 0; k < NV; ++k)
-                    g[k][0] = k * lanes + l < a.c && row < a.n ? rgs_load_as_float(a.dy, row * a.ldy + k * lanes + l, a.dy_dtype) : 0.f;
-                row_bwd<1, NV>(x, g, w, sw, sb, l, lanes, a.c, a.inv_c, row < a.n ? a.eps : 1.f);
-#pragma unroll
-                for (int k = 0; k < NV; ++k)
-                    if (k * lanes + l < a.c) sm[(k * lanes + l) * 33 + r] = x[k][0];
+                    if (k * LANES + l < a.c) sm[(k * LANES + l) * 33 + r] = x[k][0];
             }
         }
         if (BWD && a.dx) {
@@ -367,7 +414,7 @@ __global__ void __launch_bounds__(NT) rgs_norm_planes_kernel(const __grid_consta
     }
     if (BWD && a.part) {
         __syncthreads();
-        block_sums<1, NV>(a, l, lanes, sw, sb, sm);
+        block_sums<1, NV, LANES>(a, l, sw, sb, sm);
     }
 }
 
@@ -385,10 +432,10 @@ __global__ void __launch_bounds__(NT) rgs_norm_wide_kernel(const __grid_constant
     for (int64_t i = (int64_t)blockIdx.x * (NT / 32) + (threadIdx.x >> 5); i < a.n; i += (int64_t)gridDim.x * (NT / 32)) {
         float s = 0.f;
         for (int j = lane; j < a.c; j += 32) s += wide_value(a, i, j);
-        const float mu = group_sum(s, 32) * a.inv_c;
+        const float mu = group_sum<32>(s) * a.inv_c;
         s = 0.f;
         for (int j = lane; j < a.c; j += 32) { const float d = wide_value(a, i, j) - mu; s = fmaf(d, d, s); }
-        const float rstd = 1.0f / sqrtf(group_sum(s, 32) * a.inv_c + a.eps);
+        const float rstd = 1.0f / sqrtf(group_sum<32>(s) * a.inv_c + a.eps);
         if (!backward) {
             for (int j = lane; j < a.c; j += 32)
                 rgs_store_float(a.y, i * a.c + j, a.y_dtype,
@@ -404,8 +451,8 @@ __global__ void __launch_bounds__(NT) rgs_norm_wide_kernel(const __grid_constant
             sa += g;
             sax = fmaf(g, (wide_value(a, i, j) - mu) * rstd, sax);
         }
-        sa = group_sum(sa, 32) * a.inv_c;
-        sax = group_sum(sax, 32) * a.inv_c;
+        sa = group_sum<32>(sa) * a.inv_c;
+        sax = group_sum<32>(sax) * a.inv_c;
         for (int j = lane; j < a.c; j += 32) {
             const float g = rgs_load_as_float(a.dy, i * a.ldy + j, a.dy_dtype) * (a.w ? rgs_load_as_float(a.w, j, a.p_dtype) : 1.f);
             rgs_store_float(a.dx, a.planes ? j * a.n + i : i * a.c + j, a.dx_dtype, rstd * (g - sa - (wide_value(a, i, j) - mu) * rstd * sax));
@@ -458,7 +505,7 @@ __global__ void __launch_bounds__(1024) rgs_norm_reduce_kernel(const float* __re
 // ---------------------------------------------------------------------------------------------------------------------
 // Rows: 32 / VEC lanes to a 32-channel block, so that a warp reads and writes what lies together; four blocks in flight.
 // `flat`: whole blocks that follow one another without a gap, no division.
-template <int VEC>
+template <int VEC, int DT>
 __global__ void __launch_bounds__(NT) rgs_pack8_rows_kernel(const __grid_constant__ NormArgs a, int flat) {
     constexpr int LB = RGS_PACK_BLOCK / VEC, U = 4;
     const int l = threadIdx.x % LB;
@@ -477,7 +524,7 @@ __global__ void __launch_bounds__(NT) rgs_pack8_rows_kernel(const __grid_constan
             }
 #pragma unroll
             for (int q = 0; q < VEC; ++q) x[u][q] = 0.f;
-            if (t < total && (flat || c[u] < a.c)) load_vec<VEC>(a.x, flat ? t * RGS_PACK_BLOCK + c[u] : row[u] * a.ld + c[u], a.src, x[u]);
+            if (t < total && (flat || c[u] < a.c)) load_vec<VEC, DT>(a.x, flat ? t * RGS_PACK_BLOCK + c[u] : row[u] * a.ld + c[u], x[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -485,7 +532,7 @@ __global__ void __launch_bounds__(NT) rgs_pack8_rows_kernel(const __grid_constan
             uint32_t top = 0;
 #pragma unroll
             for (int q = 0; q < VEC; ++q) top = max(top, __float_as_uint(x[u][q]) & 0x7fffffffu);
-            const uint32_t e = rgs_pack_exponent(__uint_as_float(group_max(top, LB)));
+            const uint32_t e = rgs_pack_exponent(__uint_as_float(group_max<LB>(top)));
             if (t >= total) continue;
             if (l == 0) a.expo_out[t] = (uint8_t)e;
             if (flat) store_codes<VEC>(a.codes_out, t * RGS_PACK_BLOCK + c[u], x[u], e);
@@ -496,6 +543,7 @@ __global__ void __launch_bounds__(NT) rgs_pack8_rows_kernel(const __grid_constan
 }
 
 // planes: a thread per pixel and block
+template <int DT>
 __global__ void __launch_bounds__(NT) rgs_pack8_planes_kernel(const __grid_constant__ NormArgs a) {
     const int64_t tiles = (a.n + NT - 1) / NT;
     for (int64_t t = blockIdx.x; t < tiles * a.blocks; t += gridDim.x) {
@@ -506,7 +554,9 @@ __global__ void __launch_bounds__(NT) rgs_pack8_planes_kernel(const __grid_const
         uint32_t top = 0;
 #pragma unroll
         for (int q = 0; q < RGS_PACK_BLOCK; ++q) {
-            x[q] = c + q < a.c ? rgs_load_as_float(a.x, (int64_t)(c + q) * a.ld + i, a.src) : 0.f;
+            float f[1] = {0.f};
+            if (c + q < a.c) load_vec<1, DT>(a.x, (int64_t)(c + q) * a.ld + i, f);
+            x[q] = f[0];
             top = max(top, __float_as_uint(x[q]) & 0x7fffffffu);
         }
         const uint32_t e = rgs_pack_exponent(__uint_as_float(top));
@@ -566,90 +616,83 @@ static inline int64_t norm_grid(int64_t want, int64_t per_sm) {
 static inline bool aligned_to(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes) == 0; }
 static inline int64_t four(int dtype) { return dtype == RGS_BF16 ? 8 : 16; }  // bytes of four elements
 
-// smallest power of two of lanes that covers `vectors`, at most a warp
-static int norm_lanes(int64_t vectors) {
-    int lanes = 1;
-    while (lanes < 32 && lanes < vectors) lanes *= 2;
-    return lanes;
-}
 #define NORM_PARTS 1184   // most blocks that leave partial sums
 
-template <bool PACK>
-static void norm_rows_fwd(const NormArgs& a, bool vec, cudaStream_t st) {
-    const int lanes = norm_lanes(vec ? a.c / 4 : a.c), groups = NT / lanes, per = vec ? lanes * 4 : lanes;
-    const int nv = (a.c + per - 1) / per;
-#define NORM_FWD(V, K, R) rgs_norm_rows_fwd_kernel<V, K, R, PACK><<<(unsigned)norm_grid((a.n + groups * R - 1) / (groups * R), 32), NT, 0, st>>>(a, lanes)
-    if (vec) {
-        if (nv == 1) NORM_FWD(4, 1, 4);
-        else if (nv == 2) NORM_FWD(4, 2, 2);
-        else if (nv <= 4) NORM_FWD(4, 4, 1);
-        else NORM_FWD(4, 8, 1);
-    } else {
-        if (nv == 1) NORM_FWD(1, 1, 4);
-        else if (nv == 2) NORM_FWD(1, 2, 4);
-        else if (nv <= 4) NORM_FWD(1, 4, 2);
-        else if (nv <= 8) NORM_FWD(1, 8, 1);
-        else if (nv <= 16) NORM_FWD(1, 16, 1);
-        else if (nv <= 20) NORM_FWD(1, 20, 1);
-        else if (nv <= 24) NORM_FWD(1, 24, 1);
-        else if (nv <= 28) NORM_FWD(1, 28, 1);
-        else NORM_FWD(1, 32, 1);
+// blocks of a kernel that fit on the device together: persistent grids, so that a block reads the parameters once
+template <typename K>
+static int64_t norm_resident(K kernel, int smem) {
+    int per_sm = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, NT, (size_t)smem) != cudaSuccess || per_sm < 1) per_sm = 1;
+    return RGS_SMS * per_sm;
+}
+static inline int64_t at_most(int64_t want, int64_t most) { return want < 1 ? 1 : (want > most ? most : want); }
+
+template <int VEC, int NV, int LANES, int R>
+static int norm_rows_launch(const NormArgs& a, bool backward, cudaStream_t st) {
+    const int64_t want = (a.n + (NT / LANES) * R - 1) / ((NT / LANES) * R);
+    if (backward) {
+        static std::atomic<int64_t> most{0};
+        if (!most) most = norm_resident(rgs_norm_rows_bwd_kernel<VEC, NV, LANES, R>, 0);
+        const int64_t grid = at_most(at_most(want, most), NORM_PARTS);
+        rgs_norm_rows_bwd_kernel<VEC, NV, LANES, R><<<(unsigned)grid, NT, 0, st>>>(a);
+        return (int)grid;
     }
-#undef NORM_FWD
+    static std::atomic<int64_t> most[2];
+    const int pack = a.codes_out != nullptr;
+    if (!most[pack]) most[pack] = pack ? norm_resident(rgs_norm_rows_fwd_kernel<VEC, NV, LANES, R, true>, 0) : norm_resident(rgs_norm_rows_fwd_kernel<VEC, NV, LANES, R, false>, 0);
+    const unsigned grid = (unsigned)at_most(want, most[pack]);
+    if (pack) rgs_norm_rows_fwd_kernel<VEC, NV, LANES, R, true><<<grid, NT, 0, st>>>(a);
+    else rgs_norm_rows_fwd_kernel<VEC, NV, LANES, R, false><<<grid, NT, 0, st>>>(a);
+    return 0;
 }
 
-static int norm_rows_bwd(const NormArgs& a, bool vec, cudaStream_t st) {
-    const int lanes = norm_lanes(vec ? a.c / 4 : a.c), groups = NT / lanes, per = vec ? lanes * 4 : lanes;
-    const int nv = (a.c + per - 1) / per;
-    int parts = 0;
-#define NORM_BWD(V, K, R, B)                                                                     \
-    {                                                                                            \
-        parts = (int)norm_grid((a.n + groups * R - 1) / (groups * R), B);                        \
-        if (parts > NORM_PARTS) parts = NORM_PARTS;                                              \
-        rgs_norm_rows_bwd_kernel<V, K, R><<<(unsigned)parts, NT, 0, st>>>(a, lanes);             \
-    }
+// Few lanes to a row and several vectors to a lane: the shuffles of a row's sums are what narrow rows cost most (one lane
+// to a vector: 1.4 TB/s at 33 channels, 3.4 at 64 backward).
+static int norm_rows(const NormArgs& a, bool vec, bool backward, cudaStream_t st) {
+    const int u = vec ? a.c / 4 : a.c;
     if (vec) {
-        if (nv == 1) NORM_BWD(4, 1, 2, 8)
-        else if (nv == 2) NORM_BWD(4, 2, 1, 6)
-        else if (nv <= 4) NORM_BWD(4, 4, 1, 4)
-        else NORM_BWD(4, 8, 1, 2)
-    } else {
-        if (nv == 1) NORM_BWD(1, 1, 4, 8)
-        else if (nv == 2) NORM_BWD(1, 2, 2, 8)
-        else if (nv <= 4) NORM_BWD(1, 4, 2, 6)
-        else if (nv <= 8) NORM_BWD(1, 8, 1, 6)
-        else if (nv <= 16) NORM_BWD(1, 16, 1, 4)
-        else if (nv <= 20) NORM_BWD(1, 20, 1, 3)
-        else if (nv <= 24) NORM_BWD(1, 24, 1, 3)
-        else if (nv <= 28) NORM_BWD(1, 28, 1, 2)
-        else NORM_BWD(1, 32, 1, 2)
+        if (u <= 2) return norm_rows_launch<4, 2, 1, 2>(a, backward, st);
+        if (u <= 4) return norm_rows_launch<4, 2, 2, 2>(a, backward, st);
+        if (u <= 8) return norm_rows_launch<4, 2, 4, 2>(a, backward, st);
+        if (u <= 16) return norm_rows_launch<4, 2, 8, 2>(a, backward, st);
+        if (u <= 32) return norm_rows_launch<4, 2, 16, 2>(a, backward, st);
+        if (u <= 64) return norm_rows_launch<4, 2, 32, 2>(a, backward, st);
+        if (u <= 128) return norm_rows_launch<4, 4, 32, 1>(a, backward, st);
+        return norm_rows_launch<4, 8, 32, 1>(a, backward, st);
     }
-#undef NORM_BWD
-    return parts;
+    if (u <= 4) return norm_rows_launch<1, 4, 1, 2>(a, backward, st);
+    if (u <= 8) return norm_rows_launch<1, 4, 2, 2>(a, backward, st);
+    if (u <= 16) return norm_rows_launch<1, 4, 4, 2>(a, backward, st);
+    if (u <= 32) return norm_rows_launch<1, 4, 8, 2>(a, backward, st);
+    if (u <= 64) return norm_rows_launch<1, 4, 16, 2>(a, backward, st);
+    if (u <= 128) return norm_rows_launch<1, 4, 32, 2>(a, backward, st);
+    if (u <= 256) return norm_rows_launch<1, 8, 32, 1>(a, backward, st);
+    if (u <= 512) return norm_rows_launch<1, 16, 32, 1>(a, backward, st);
+    if (u <= 640) return norm_rows_launch<1, 20, 32, 1>(a, backward, st);
+    if (u <= 768) return norm_rows_launch<1, 24, 32, 1>(a, backward, st);
+    if (u <= 896) return norm_rows_launch<1, 28, 32, 1>(a, backward, st);
+    return norm_rows_launch<1, 32, 32, 1>(a, backward, st);
 }
 
-template <int NV, bool BWD>
-static int norm_planes_launch(const NormArgs& a, int lanes, unsigned grid, cudaStream_t st) {
-    const int sums = NT;  // floats of block_sums
-    const int smem = (a.c * 33 > sums ? a.c * 33 : sums) * 4;
-    if (smem > 48 * 1024) RGS_CUDA_CHECK(cudaFuncSetAttribute(rgs_norm_planes_kernel<NV, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    rgs_norm_planes_kernel<NV, BWD><<<grid, NT, smem, st>>>(a, lanes);
+template <int NV, int LANES, bool BWD>
+static int norm_planes_launch(const NormArgs& a, int* parts, cudaStream_t st) {
+    const int smem = (a.c * 33 > NT ? a.c * 33 : NT) * 4;  // (block_sums takes NT floats of it)
+    if (smem > 48 * 1024) RGS_CUDA_CHECK(cudaFuncSetAttribute(rgs_norm_planes_kernel<NV, LANES, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    *parts = (int)at_most(at_most((a.n + PT - 1) / PT, norm_resident(rgs_norm_planes_kernel<NV, LANES, BWD>, smem)), NORM_PARTS);
+    rgs_norm_planes_kernel<NV, LANES, BWD><<<(unsigned)*parts, NT, smem, st>>>(a);
     return (int)cudaGetLastError();
 }
 
 template <bool BWD>
 static int norm_planes(const NormArgs& a, int* parts, cudaStream_t st) {
-    const int lanes = norm_lanes(a.c), nv = (a.c + lanes - 1) / lanes;
-    int64_t per_sm = (200 * 1024) / (a.c * 33 * 4 + 1024);
-    per_sm = per_sm > 8 ? 8 : (per_sm < 1 ? 1 : per_sm);
-    const int64_t grid = norm_grid((a.n + PT - 1) / PT, per_sm);
-    *parts = (int)grid;
-    if (nv == 1) return norm_planes_launch<1, BWD>(a, lanes, (unsigned)grid, st);
-    if (nv == 2) return norm_planes_launch<2, BWD>(a, lanes, (unsigned)grid, st);
-    if (nv <= 4) return norm_planes_launch<4, BWD>(a, lanes, (unsigned)grid, st);
-    if (nv <= 8) return norm_planes_launch<8, BWD>(a, lanes, (unsigned)grid, st);
-    if (nv <= 16) return norm_planes_launch<16, BWD>(a, lanes, (unsigned)grid, st);
-    return norm_planes_launch<32, BWD>(a, lanes, (unsigned)grid, st);
+    if (a.c <= 8) return norm_planes_launch<8, 1, BWD>(a, parts, st);
+    if (a.c <= 16) return norm_planes_launch<8, 2, BWD>(a, parts, st);
+    if (a.c <= 32) return norm_planes_launch<8, 4, BWD>(a, parts, st);
+    if (a.c <= 64) return norm_planes_launch<8, 8, BWD>(a, parts, st);
+    if (a.c <= 128) return norm_planes_launch<8, 16, BWD>(a, parts, st);
+    if (a.c <= 256) return norm_planes_launch<8, 32, BWD>(a, parts, st);
+    if (a.c <= 512) return norm_planes_launch<16, 32, BWD>(a, parts, st);
+    return norm_planes_launch<32, 32, BWD>(a, parts, st);
 }
 
 extern "C" {
@@ -662,11 +705,18 @@ int rgs_cuda_pack8(const void* x, int64_t dtype, int64_t ld, int64_t planes, int
     a.x = x; a.src = (int)dtype; a.ld = ld; a.planes = (int)planes; a.n = n; a.c = (int)c; a.blocks = (int)((c + 31) / 32);
     a.codes_out = codes; a.expo_out = expo;
     if (planes) {
-        rgs_pack8_planes_kernel<<<(unsigned)norm_grid((n + NT - 1) / NT * a.blocks, 16), NT, 0, st>>>(a);
+        const unsigned grid = (unsigned)norm_grid((n + NT - 1) / NT * a.blocks, 16);
+        if (a.src == SRC_BF16) rgs_pack8_planes_kernel<RGS_BF16><<<grid, NT, 0, st>>>(a);
+        else rgs_pack8_planes_kernel<RGS_F32><<<grid, NT, 0, st>>>(a);
     } else if (c % 4 == 0 && ld % 4 == 0 && aligned_to(x, four(a.src))) {
-        rgs_pack8_rows_kernel<4><<<(unsigned)norm_grid((n * a.blocks * 8 + NT * 4 - 1) / (NT * 4), 32), NT, 0, st>>>(a, c % 32 == 0 && ld == c);
+        const unsigned grid = (unsigned)norm_grid((n * a.blocks * 8 + NT * 4 - 1) / (NT * 4), 32);
+        const int flat = c % 32 == 0 && ld == c;
+        if (a.src == SRC_BF16) rgs_pack8_rows_kernel<4, RGS_BF16><<<grid, NT, 0, st>>>(a, flat);
+        else rgs_pack8_rows_kernel<4, RGS_F32><<<grid, NT, 0, st>>>(a, flat);
     } else {
-        rgs_pack8_rows_kernel<1><<<(unsigned)norm_grid((n * a.blocks * 32 + NT * 4 - 1) / (NT * 4), 32), NT, 0, st>>>(a, 0);
+        const unsigned grid = (unsigned)norm_grid((n * a.blocks * 32 + NT * 4 - 1) / (NT * 4), 32);
+        if (a.src == SRC_BF16) rgs_pack8_rows_kernel<1, RGS_BF16><<<grid, NT, 0, st>>>(a, 0);
+        else rgs_pack8_rows_kernel<1, RGS_F32><<<grid, NT, 0, st>>>(a, 0);
     }
     return (int)cudaGetLastError();
 }
@@ -701,8 +751,7 @@ int rgs_cuda_norm_fwd(const void* x, int64_t dtype, int64_t ld, int64_t planes, 
         return norm_planes<false>(a, &parts, st);
     }
     const bool vec = c % 4 == 0 && ld % 4 == 0 && aligned_to(x, four(a.src));
-    if (codes) norm_rows_fwd<true>(a, vec, st);
-    else norm_rows_fwd<false>(a, vec, st);
+    norm_rows(a, vec, false, st);
     return (int)cudaGetLastError();
 }
 
@@ -732,7 +781,7 @@ int rgs_cuda_norm_bwd(const void* x, int64_t dtype, int64_t ld, int64_t planes, 
     } else {
         const bool vec = c % 4 == 0 && ldy % 4 == 0 && aligned_to(dy, four(a.dy_dtype)) &&
                          (codes || (ld % 4 == 0 && aligned_to(x, four((int)dtype))));
-        parts = norm_rows_bwd(a, vec, st);
+        parts = norm_rows(a, vec, true, st);
     }
     RGS_CUDA_CHECK(cudaGetLastError());
     if (a.part)
