@@ -9,8 +9,11 @@
 // the two sums of each pass are shuffles, and in the backward pass the mean and rstd are computed anew from the row (four
 // shuffles) instead of being kept.  Lanes keep the sums of their own channels for dw and db over all the rows they meet;
 // blocks write them once and a second kernel adds the blocks in order, so results do not depend on timing.
-// Rows of 4 n channels on aligned boundaries are read in vectors of four, others element by element.  Channel planes (the
-// renderer's images) pass through shared memory 32 pixels at a time.  Beyond 1024 channels a warp re-reads its row.
+// Rows are read in aligned vectors of four.  Where a row does not begin on such a boundary (a width that four does not
+// divide) its vectors begin up to three elements before it: a group takes rows a multiple of four apart, so that this shift
+// and with it the channels of a lane stay the same; the first and last vector of a row are then read element by element.
+// Codes of such rows are read element by element throughout.  Channel planes (the renderer's images) pass through shared
+// memory 32 pixels at a time.  Beyond 1024 channels a warp re-reads its row.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -20,7 +23,7 @@
 
 #define NT 256            // threads of a block
 #define NR_MAX 1024       // channels that a group holds in registers
-#define PT 32             // pixels of a tile of planes
+#define NP_MAX 512        // channels of planes that a block holds
 
 enum { SRC_F32 = 0, SRC_BF16 = 1, SRC_CODES = 2 };
 
@@ -35,6 +38,7 @@ struct NormArgs {
     const void* dy; int dy_dtype; int64_t ldy;
     void* dx; int dx_dtype;
     float* part;                                   // (blocks of the grid, 2, c)
+    void* dw; void* db;                            // written at once when the grid is one block
 };
 
 // The switch on a type stands outside the loops over a row's vectors, so that all loads of a row are in flight together
@@ -54,58 +58,108 @@ __device__ __forceinline__ void load_vec(const void* p, int64_t i, float (&f)[VE
         f[0] = static_cast<const float*>(p)[i];
     }
 }
-// vectors k of a lane, (k lanes + l) VEC, of the row that starts at element i; zero behind the last channel
-template <int VEC, int NV, int LANES, int DT>
-__device__ __forceinline__ void load_all(const void* p, int64_t i, int l, int c, float (&x)[NV][VEC]) {
+// vectors k of a lane, from channel (k lanes + l) VEC - s on, of the row that starts at element i; zero outside the row
+// (edge: the last row, whose last vector may reach behind the tensor)
+template <int VEC, int NV, int LANES, int DT, bool SHIFT>
+__device__ __forceinline__ void load_all(const void* p, int64_t i, int l, int s, int c, bool edge, float (&x)[NV][VEC]) {
+    if (SHIFT && edge) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) {
+                const int at = (k * LANES + l) * VEC - s + q;
+                float f[1] = {0.f};
+                if (at >= 0 && at < c) load_vec<1, DT>(p, i + at, f);
+                x[k][q] = f[0];
+            }
+        return;
+    }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int at = (k * LANES + l) * VEC;
+        const int at = (k * LANES + l) * VEC - (SHIFT ? s : 0);
         if (at < c) load_vec<VEC, DT>(p, i + at, x[k]);
         else
 #pragma unroll
             for (int q = 0; q < VEC; ++q) x[k][q] = 0.f;
     }
+    if (SHIFT) {  // the first and the last vector of the row hold elements of its neighbours
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+            if (k == 0 || (k + 1) * LANES * VEC > c)
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) {
+                    const int at = (k * LANES + l) * VEC - s + q;
+                    x[k][q] = at >= 0 && at < c ? x[k][q] : 0.f;
+                }
+    }
 }
-template <int VEC, int NV, int LANES>
-__device__ __forceinline__ void load_typed(const void* p, int dtype, int64_t i, int l, int c, float (&x)[NV][VEC]) {
-    if (dtype == RGS_BF16) load_all<VEC, NV, LANES, RGS_BF16>(p, i, l, c, x);
-    else load_all<VEC, NV, LANES, RGS_F32>(p, i, l, c, x);
+template <int VEC, int NV, int LANES, bool SHIFT>
+__device__ __forceinline__ void load_typed(const void* p, int dtype, int64_t i, int l, int s, int c, bool edge, float (&x)[NV][VEC]) {
+    if (dtype == RGS_BF16) load_all<VEC, NV, LANES, RGS_BF16, SHIFT>(p, i, l, s, c, edge, x);
+    else load_all<VEC, NV, LANES, RGS_F32, SHIFT>(p, i, l, s, c, edge, x);
 }
 __device__ __forceinline__ uint32_t pair_bf16(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-template <int VEC>
-__device__ __forceinline__ void store_vec(void* p, int64_t i, int dtype, const float (&f)[VEC]) {
-    if constexpr (VEC == 4) {
-        if (dtype == RGS_BF16) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = make_uint2(pair_bf16(f[0], f[1]), pair_bf16(f[2], f[3]));
-        else *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(f[0], f[1], f[2], f[3]);
-    } else {
-        if (dtype == RGS_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(f[0]);
-        else static_cast<float*>(p)[i] = f[0];
+template <int VEC, int DT>
+__device__ __forceinline__ void store_vec(void* p, int64_t i, const float (&f)[VEC]) {
+    if constexpr (VEC == 4 && DT == RGS_BF16) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = make_uint2(pair_bf16(f[0], f[1]), pair_bf16(f[2], f[3]));
+    else if constexpr (VEC == 4) *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(f[0], f[1], f[2], f[3]);
+    else if constexpr (DT == RGS_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(f[0]);
+    else static_cast<float*>(p)[i] = f[0];
+}
+template <int VEC, int NV, int LANES, int DT, bool SHIFT>
+__device__ __forceinline__ void store_all(void* p, int64_t i, int l, int s, int c, const float (&x)[NV][VEC]) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int at = (k * LANES + l) * VEC - (SHIFT ? s : 0);
+        if (SHIFT ? at >= 0 && at + VEC <= c : at < c) store_vec<VEC, DT>(p, i + at, x[k]);
+    }
+    if (SHIFT) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+            if (k == 0 || ((k + 1) * LANES * VEC > c && k * LANES * VEC < c + 3)) {
+                const int at = (k * LANES + l) * VEC - s;
+                if (at < 0 || (at + VEC > c && at < c))
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) {
+                        const float f[1] = {x[k][q]};
+                        if (at + q >= 0 && at + q < c) store_vec<1, DT>(p, i + at + q, f);
+                    }
+            }
     }
 }
-// codes of four channels (one word) or of one, from values scaled by the inverse step of their block
+template <int VEC, int NV, int LANES, bool SHIFT>
+__device__ __forceinline__ void store_typed(void* p, int dtype, int64_t i, int l, int s, int c, const float (&x)[NV][VEC]) {
+    if (dtype == RGS_BF16) store_all<VEC, NV, LANES, RGS_BF16, SHIFT>(p, i, l, s, c, x);
+    else store_all<VEC, NV, LANES, RGS_F32, SHIFT>(p, i, l, s, c, x);
+}
+// Codes of four channels (one word) or of one.  v * inv + 1.5 * 2^23 leaves the code in the low byte (two's complement); only
+// the topmost exponent needs the bound of rgs_pack_code.
 template <int VEC>
 __device__ __forceinline__ void store_codes(int8_t* p, int64_t i, const float (&f)[VEC], uint32_t e) {
     const float inv = rgs_pack_inverse(e);
-    if constexpr (VEC == 4) {
-        uint32_t u = 0;
-        if (e != RGS_PACK_NAN)
+    uint32_t u[VEC];
+    if (e < 249u) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) u |= (uint32_t)(rgs_pack_code(f[k], inv) & 0xff) << (8 * k);
-        *reinterpret_cast<uint32_t*>(p + i) = u;
+        for (int k = 0; k < VEC; ++k) u[k] = __float_as_uint(fmaf(f[k], inv, 12582912.f));
     } else {
-        p[i] = (int8_t)(e == RGS_PACK_NAN ? 0 : rgs_pack_code(f[0], inv));
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) u[k] = e == RGS_PACK_NAN ? 0u : (uint32_t)rgs_pack_code(f[k], inv);
     }
+    if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(p + i) = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+    else p[i] = (int8_t)u[0];
 }
+// The value of byte k: 2^23 + (code + 128) is the float with that byte in its mantissa; the offset comes off and the step on,
+// both exactly (a conversion instruction runs at a quarter of the rate; the offset times the largest steps would overflow).
 template <int VEC>
 __device__ __forceinline__ void load_codes(const int8_t* p, int64_t i, float step, float (&f)[VEC]) {
     if constexpr (VEC == 4) {
-        const uint32_t u = *reinterpret_cast<const uint32_t*>(p + i);
+        const uint32_t u = *reinterpret_cast<const uint32_t*>(p + i) ^ 0x80808080u;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) f[k] = (float)(int8_t)(u >> (8 * k)) * step;
+        for (int k = 0; k < 4; ++k) f[k] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + k)) - 8388736.f) * step;
     } else {
         f[0] = (float)p[i] * step;
     }
@@ -125,42 +179,65 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {
     return v;
 }
 
-// mean and 1 / sqrt(var + eps) of a row; vector k of a lane starts at channel (k lanes + lane) VEC
-template <int VEC, int NV, int LANES>
-__device__ __forceinline__ void row_stats(const float (&x)[NV][VEC], int l, int c, float inv_c, float eps, float& mu, float& rstd) {
+// whether element q of vector k of a lane is a channel
+template <int VEC, int LANES, bool SHIFT>
+__device__ __forceinline__ bool in_row(int k, int q, int l, int s, int c) {
+    const int at = (k * LANES + l) * VEC;
+    return SHIFT ? at + q >= s && at + q < c + s : at < c;
+}
+
+// mean and 1 / sqrt(var + eps) of a row
+template <int VEC, int NV, int LANES, bool SHIFT>
+__device__ __forceinline__ void row_stats(const float (&x)[NV][VEC], int l, int s0, int c, float inv_c, float eps, float& mu, float& rstd) {
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) s += x[k][q];   // zero behind the last channel
+        for (int q = 0; q < VEC; ++q) s += x[k][q];   // zero outside the row
     mu = group_sum<LANES>(s) * inv_c;
     s = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-        if ((k * LANES + l) * VEC < c)
-#pragma unroll
-            for (int q = 0; q < VEC; ++q) s = fmaf(x[k][q] - mu, x[k][q] - mu, s);
-    rstd = 1.0f / sqrtf(group_sum<LANES>(s) * inv_c + eps);
-}
-
-// the part of the backward pass that rows and planes share: a row's x, dy -> dx (over x), sums of dw and db
-template <int VEC, int NV, int LANES>
-__device__ __forceinline__ void row_bwd(float (&x)[NV][VEC], float (&g)[NV][VEC], const float (&w)[NV][VEC], float (&sw)[NV][VEC], float (&sb)[NV][VEC],
-                                        int l, int c, float inv_c, float eps) {
-    float mu, rstd, sa = 0.f, sax = 0.f;
-    row_stats<VEC, NV, LANES>(x, l, c, inv_c, eps, mu, rstd);
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int q = 0; q < VEC; ++q) {
-            const bool in = (k * LANES + l) * VEC < c;
-            x[k][q] = in ? (x[k][q] - mu) * rstd : 0.f;
+            const bool whole = (k + 1) * LANES * VEC <= c && (!SHIFT || k > 0);  // (the same for all lanes)
+            const float d = whole || in_row<VEC, LANES, SHIFT>(k, q, l, s0, c) ? x[k][q] - mu : 0.f;
+            s = fmaf(d, d, s);
+        }
+    rstd = rsqrtf(group_sum<LANES>(s) * inv_c + eps);  // within two units in the last place
+}
+
+template <int VEC>
+__device__ __forceinline__ void load_param(const float* sh, int at, float (&w)[VEC]) {
+    if constexpr (VEC == 4) {
+        const float4 u = *reinterpret_cast<const float4*>(sh + at);
+        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    } else {
+        w[0] = sh[at];
+    }
+}
+
+// the backward pass of a row: x, dy -> dx (over x), sums of dw and db
+template <int VEC, int NV, int LANES, bool SHIFT>
+__device__ __forceinline__ void row_bwd(float (&x)[NV][VEC], float (&g)[NV][VEC], const float* w, float (&sw)[NV][VEC], float (&sb)[NV][VEC],
+                                        int l, int s0, int c, float inv_c, float eps) {
+    float mu, rstd, sa = 0.f, sax = 0.f;
+    row_stats<VEC, NV, LANES, SHIFT>(x, l, s0, c, inv_c, eps, mu, rstd);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        float wk[VEC];
+        load_param<VEC>(w, (k * LANES + l) * VEC, wk);
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) {
+            // (outside the row dy is zero, and so is what x adds to the sums)
+            x[k][q] = (x[k][q] - mu) * rstd;
             sw[k][q] = fmaf(g[k][q], x[k][q], sw[k][q]);
             sb[k][q] += g[k][q];
-            g[k][q] *= w[k][q];
+            g[k][q] *= wk[q];
             sa += g[k][q];
             sax = fmaf(g[k][q], x[k][q], sax);
         }
+    }
     sa = group_sum<LANES>(sa) * inv_c;
     sax = group_sum<LANES>(sax) * inv_c;
 #pragma unroll
@@ -169,46 +246,56 @@ __device__ __forceinline__ void row_bwd(float (&x)[NV][VEC], float (&g)[NV][VEC]
         for (int q = 0; q < VEC; ++q) x[k][q] = rstd * (g[k][q] - sa - x[k][q] * sax);
 }
 
-template <int VEC, int NV, int LANES>
-__device__ __forceinline__ void load_params(const NormArgs& a, int l, const void* p, float none, float (&w)[NV][VEC]) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) {
-            const int c = (k * LANES + l) * VEC + q;
-            w[k][q] = none;
-            if (p && c < a.c) w[k][q] = a.p_dtype == RGS_BF16 ? rgs_bf16_value(static_cast<const uint16_t*>(p)[c]) : static_cast<const float*>(p)[c];
-        }
+// A parameter in shared memory as the vectors of a row see it: one copy for each shift, channel c of copy s at c + s.
+template <int VEC, int NV, int LANES, bool SHIFT>
+__device__ __forceinline__ void stage_param(const NormArgs& a, const void* p, float none, float* sh) {
+    constexpr int ROW = NV * LANES * VEC;
+    for (int j = threadIdx.x; j < (SHIFT ? 4 : 1) * ROW; j += NT) {
+        const int c = SHIFT ? j % ROW - j / ROW : j;
+        sh[j] = p && c >= 0 && c < a.c ? rgs_load_as_float(p, c, a.p_dtype) : none;
+    }
 }
-
-// sums of a block's groups, in the order of the groups, to the block's row of the partial sums
-template <int VEC, int NV, int LANES>
-__device__ __forceinline__ void block_sums(const NormArgs& a, int l, const float (&sw)[NV][VEC], const float (&sb)[NV][VEC], float* sh) {
-    // sh: (groups of the block, channels) of one of the two sums at a time, 64 channels a turn
-    const int group = threadIdx.x / LANES, groups = NT / LANES;
-    for (int which = 0; which < 2; ++which)
+// Sums of a block's groups, in the order of the groups, to the block's row of the partial sums; a vector of every lane at a
+// time, and with shifted rows the three elements that its groups' vectors reach into the one before.
+template <int VEC, int NV, int LANES, bool SHIFT>
+__device__ __forceinline__ void block_sums(const NormArgs& a, int l, int s, const float (&sw)[NV][VEC], const float (&sb)[NV][VEC], float* sh) {
+    constexpr int GROUPS = NT / LANES, W = LANES * VEC, ROW = SHIFT ? W + 3 : W;
+    const int group = threadIdx.x / LANES;
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+        if (SHIFT && l == 0)
+            for (int q = 0; q < 3; ++q) sh[group * ROW + q] = 0.f;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            if (k * LANES * VEC >= a.c) break;
+            if (k * W >= a.c + (SHIFT ? 3 : 0)) break;
             __syncthreads();
+            // position 3 + channel - k W: channels of this turn, and behind a shift the last ones of the turn before
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) sh[group * (LANES * VEC) + l * VEC + q] = which ? sb[k][q] : sw[k][q];
+            for (int q = 0; q < VEC; ++q) sh[group * ROW + l * VEC + q + (SHIFT ? 3 - s : 0)] = which ? sb[k][q] : sw[k][q];
             __syncthreads();
-            for (int j = threadIdx.x; j < LANES * VEC; j += NT) {
+            const bool end = k + 1 == NV || (k + 1) * W >= a.c + (SHIFT ? 3 : 0);
+            for (int j = threadIdx.x; j < (SHIFT && !end ? W : ROW); j += NT) {
+                const int c = k * W + j - (SHIFT ? 3 : 0);
+                if (c < 0 || c >= a.c) continue;
                 float t = 0.f;
-                for (int r = 0; r < groups; ++r) t += sh[r * (LANES * VEC) + j];
-                const int c = k * LANES * VEC + j;
-                if (c < a.c) a.part[((int64_t)blockIdx.x * 2 + which) * a.c + c] = t;
+                for (int r = 0; r < GROUPS; ++r) t += sh[r * ROW + j];
+                if (gridDim.x > 1) a.part[((int64_t)blockIdx.x * 2 + which) * a.c + c] = t;
+                else if (which ? a.db : a.dw) rgs_store_float(which ? a.db : a.dw, c, a.p_dtype, t);
+            }
+            if (SHIFT) {  // what reaches into the next turn's first three places (a group overwrites those it does not reach into)
+                __syncthreads();
+                for (int q = l; q < 3; q += LANES) sh[group * ROW + q] = sh[group * ROW + W + q];
             }
         }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // rows
 // ---------------------------------------------------------------------------------------------------------------------
-template <int VEC, int NV, int LANES>
-__device__ __forceinline__ void load_row(const NormArgs& a, int64_t i, int l, float (&x)[NV][VEC]) {
-    if (a.src == SRC_CODES) {
+template <int VEC, int NV, int LANES, bool SHIFT>
+__device__ __forceinline__ void load_row(const NormArgs& a, int64_t i, int l, int s, float (&x)[NV][VEC]) {
+    if (!SHIFT && a.src == SRC_CODES) {
         float step[NV];
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -224,30 +311,43 @@ __device__ __forceinline__ void load_row(const NormArgs& a, int64_t i, int l, fl
                 for (int q = 0; q < VEC; ++q) x[k][q] = 0.f;
         }
     } else {
-        load_typed<VEC, NV, LANES>(a.x, a.src, i * a.ld, l, a.c, x);
+        load_typed<VEC, NV, LANES, SHIFT>(a.x, a.src, i * a.ld, l, s, a.c, i == a.n - 1, x);
     }
 }
 
-template <int VEC, int NV, int LANES, int R, bool PACK>
-__global__ void __launch_bounds__(NT) rgs_norm_rows_fwd_kernel(const __grid_constant__ NormArgs a) {
-    const int l = threadIdx.x % LANES, groups = NT / LANES;
-    const int64_t stride = (int64_t)gridDim.x * groups;
-    float w[NV][VEC], b[NV][VEC];
-    load_params<VEC, NV, LANES>(a, l, a.w, 1.f, w);
-    load_params<VEC, NV, LANES>(a, l, a.b, 0.f, b);
-    // all lanes of a warp take the same number of turns: shuffles need them
-    for (int64_t i0 = (int64_t)blockIdx.x * groups; i0 < a.n; i0 += R * stride) {
+template <int VEC, int NV, int LANES, int R, bool SHIFT, bool PACK>
+__global__ void __launch_bounds__(NT, NV * VEC <= 16 ? 4 : NV * VEC <= 24 ? 3 : 2) rgs_norm_rows_fwd_kernel(const __grid_constant__ NormArgs a) {
+    constexpr int GROUPS = NT / LANES;
+    const int l = threadIdx.x % LANES;
+    const int64_t stride = (int64_t)gridDim.x * GROUPS;  // a multiple of four rows: the shift stays
+    const int s = SHIFT ? (int)(((int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES) * a.c & 3) : 0;
+    constexpr int ROW = NV * LANES * VEC, COPIES = SHIFT ? 4 : 1;
+    __shared__ __align__(16) float params[2 * COPIES * ROW];
+    stage_param<VEC, NV, LANES, SHIFT>(a, a.w, 1.f, params);
+    stage_param<VEC, NV, LANES, SHIFT>(a, a.b, 0.f, params + COPIES * ROW);
+    __syncthreads();
+    const float *w = params + s * ROW, *b = params + (COPIES + s) * ROW;
+    // all lanes of a warp take the same number of turns: shuffles need them.  A row behind the end is read as zeros.
+    for (int64_t i0 = (int64_t)blockIdx.x * GROUPS; i0 < a.n; i0 += R * stride) {
         const int64_t i = i0 + threadIdx.x / LANES;
         float x[R][NV][VEC];
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-            load_row<VEC, NV, LANES>(a, min(i + r * stride, a.n - 1), l, x[r]);
+        for (int r = 0; r < R; ++r) {
+            if (i + r * stride < a.n) {
+                load_row<VEC, NV, LANES, SHIFT>(a, i + r * stride, l, s, x[r]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < NV; ++k)
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) x[r][k][q] = 0.f;
+            }
+        }
+        __syncwarp();
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int64_t row = i + r * stride;
             float mu, rstd;
-            row_stats<VEC, NV, LANES>(x[r], l, a.c, a.inv_c, a.eps, mu, rstd);
-            uint32_t top[NV];
+            row_stats<VEC, NV, LANES, SHIFT>(x[r], l, s, a.c, a.inv_c, a.eps, mu, rstd);
             if (PACK) {
                 // a block of 32 channels is 32 / VEC vectors: KB of every lane of the row, or one of some of its lanes
                 constexpr int LB = RGS_PACK_BLOCK / VEC, KB = LANES < LB ? LB / LANES : 1;
@@ -259,170 +359,324 @@ __global__ void __launch_bounds__(NT) rgs_norm_rows_fwd_kernel(const __grid_cons
 #pragma unroll
                         for (int q = 0; q < VEC; ++q) m = max(m, __float_as_uint(x[r][e][q]) & 0x7fffffffu);
                     m = rgs_pack_exponent(__uint_as_float(group_max<(LANES < LB ? LANES : LB)>(m)));
+                    if (row < a.n)
 #pragma unroll
-                    for (int e = k; e < k + KB && e < NV; ++e) top[e] = m;
+                        for (int e = k; e < k + KB && e < NV; ++e) {
+                            const int c = (e * LANES + l) * VEC;
+                            if (c >= a.c) break;
+                            if (c % RGS_PACK_BLOCK == 0) a.expo_out[row * a.blocks + c / RGS_PACK_BLOCK] = (uint8_t)m;
+                            store_codes<VEC>(a.codes_out, row * a.c + c, x[r][e], m);
+                        }
+                    __syncwarp();
                 }
             }
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const int c = (k * LANES + l) * VEC;
-                if (PACK && row < a.n && c < a.c) {
-                    if (c % RGS_PACK_BLOCK == 0) a.expo_out[row * a.blocks + c / RGS_PACK_BLOCK] = (uint8_t)top[k];
-                    store_codes<VEC>(a.codes_out, row * a.c + c, x[r][k], top[k]);
-                }
-                if (a.y && row < a.n && c < a.c) {
-                    float f[VEC];
+                float wk[VEC], bk[VEC];
+                load_param<VEC>(w, (k * LANES + l) * VEC, wk);
+                load_param<VEC>(b, (k * LANES + l) * VEC, bk);
 #pragma unroll
-                    for (int q = 0; q < VEC; ++q) f[q] = fmaf((x[r][k][q] - mu) * rstd, w[k][q], b[k][q]);
-                    store_vec<VEC>(a.y, row * a.c + c, a.y_dtype, f);
-                }
+                for (int q = 0; q < VEC; ++q) x[r][k][q] = fmaf((x[r][k][q] - mu) * rstd, wk[q], bk[q]);
             }
+            if (row < a.n) store_typed<VEC, NV, LANES, SHIFT>(a.y, a.y_dtype, row * a.c, l, s, a.c, x[r]);
+            __syncwarp();
         }
     }
 }
 
-template <int VEC, int NV, int LANES, int R>
-__global__ void __launch_bounds__(NT) rgs_norm_rows_bwd_kernel(const __grid_constant__ NormArgs a) {
-    __shared__ float sh[NT * VEC];
-    const int l = threadIdx.x % LANES, groups = NT / LANES;
-    const int64_t stride = (int64_t)gridDim.x * groups;
-    float w[NV][VEC], sw[NV][VEC], sb[NV][VEC];
-    load_params<VEC, NV, LANES>(a, l, a.w, 1.f, w);
+template <int VEC, int NV, int LANES, int R, bool SHIFT>
+__global__ void __launch_bounds__(NT, NV * VEC <= 12 ? 3 : NV * VEC <= 16 ? 2 : 1) rgs_norm_rows_bwd_kernel(const __grid_constant__ NormArgs a) {
+    constexpr int GROUPS = NT / LANES;
+    constexpr int ROW = NV * LANES * VEC, COPIES = SHIFT ? 4 : 1, SUMS = NT * VEC + (SHIFT ? 3 * GROUPS : 0);
+    __shared__ __align__(16) float sh[COPIES * ROW > SUMS ? COPIES * ROW : SUMS];
+    const int l = threadIdx.x % LANES;
+    const int64_t stride = (int64_t)gridDim.x * GROUPS;
+    const int s = SHIFT ? (int)(((int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES) * a.c & 3) : 0;
+    float sw[NV][VEC], sb[NV][VEC];
+    stage_param<VEC, NV, LANES, SHIFT>(a, a.w, 1.f, sh);
+    __syncthreads();
+    const float* w = sh + s * ROW;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int q = 0; q < VEC; ++q) sw[k][q] = sb[k][q] = 0.f;
-    for (int64_t i0 = (int64_t)blockIdx.x * groups; i0 < a.n; i0 += R * stride) {
+    for (int64_t i0 = (int64_t)blockIdx.x * GROUPS; i0 < a.n; i0 += R * stride) {
         const int64_t i = i0 + threadIdx.x / LANES;
         float x[R][NV][VEC], g[R][NV][VEC];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int64_t row = min(i + r * stride, a.n - 1);
-            load_row<VEC, NV, LANES>(a, row, l, x[r]);
-            load_typed<VEC, NV, LANES>(a.dy, a.dy_dtype, row * a.ldy, l, i + r * stride < a.n ? a.c : 0, g[r]);
+            if (i + r * stride < a.n) {
+                load_row<VEC, NV, LANES, SHIFT>(a, i + r * stride, l, s, x[r]);
+                load_typed<VEC, NV, LANES, SHIFT>(a.dy, a.dy_dtype, (i + r * stride) * a.ldy, l, s, a.c, i + r * stride == a.n - 1, g[r]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < NV; ++k)
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) x[r][k][q] = g[r][k][q] = 0.f;
+            }
         }
+        __syncwarp();
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int64_t row = i + r * stride;
-            if (row >= a.n) {  // the last row again, in place of one behind the end: nothing of it counts, whatever it holds
-#pragma unroll
-                for (int k = 0; k < NV; ++k)
-#pragma unroll
-                    for (int q = 0; q < VEC; ++q) x[r][k][q] = 0.f;
-            }
-            row_bwd<VEC, NV, LANES>(x[r], g[r], w, sw, sb, l, a.c, a.inv_c, a.eps > 0.f ? a.eps : (row >= a.n ? 1.f : 0.f));
-            if (a.dx && row < a.n)
-#pragma unroll
-                for (int k = 0; k < NV; ++k) {
-                    const int c = (k * LANES + l) * VEC;
-                    if (c < a.c) store_vec<VEC>(a.dx, row * a.c + c, a.dx_dtype, x[r][k]);
-                }
+            // (a row behind the end is zeros, and adds none to the sums: with eps = 0 its rstd would be infinite)
+            row_bwd<VEC, NV, LANES, SHIFT>(x[r], g[r], w, sw, sb, l, s, a.c, a.inv_c, row < a.n ? a.eps : 1.f);
+            if (a.dx && row < a.n) store_typed<VEC, NV, LANES, SHIFT>(a.dx, a.dx_dtype, row * a.c, l, s, a.c, x[r]);
+            __syncwarp();
         }
     }
-    if (a.part) block_sums<VEC, NV, LANES>(a, l, sw, sb, sh);
+    if (a.part) block_sums<VEC, NV, LANES, SHIFT>(a, l, s, sw, sb, sh);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// channel planes: 32 pixels at a time through shared memory, (channel, pixel) with rows of 33
+// channel planes: 32 or 64 pixels at a time, a lane to one or two; warp v of V holds channels v, v + V, ... of them, so planes are read
+// and written where they lie, sums run over the warps, and only rows (y, dy) are turned around in shared memory
 // ---------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float plane_value(const NormArgs& a, int64_t i, int c) {
-    if (a.src == SRC_CODES)
-        return (float)a.codes[(int64_t)c * a.n + i] * rgs_pack_step(a.expo[(int64_t)(c / RGS_PACK_BLOCK) * a.n + i]);
-    return rgs_load_as_float(a.x, (int64_t)c * a.ld + i, a.src);
+template <int NV, int V, int Q, int SRC>
+__device__ __forceinline__ void load_plane(const NormArgs& a, int64_t i, int v, float (&x)[Q][NV]) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c = v + k * V;
+        const int64_t at = (int64_t)c * (SRC == SRC_CODES ? a.n : a.ld) + i;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            float f[1] = {0.f};
+            if (c < a.c && i + q * 32 < a.n) {
+                if constexpr (SRC == SRC_CODES) load_codes<1>(a.codes, at + q * 32, rgs_pack_step(a.expo[(int64_t)(c / RGS_PACK_BLOCK) * a.n + i + q * 32]), f);
+                else load_vec<1, SRC>(a.x, at + q * 32, f);
+            }
+            x[q][k] = f[0];
+        }
+    }
 }
-// channels c0, c0 + 8, ... of pixel i to shared memory
-template <int SRC>
-__device__ __forceinline__ void load_plane(const NormArgs& a, int64_t i, int c0, int p, float* sm) {
-#pragma unroll 8
-    for (int c = c0; c < a.c; c += NT / 32) {
-        float f[1];
-        if constexpr (SRC == SRC_CODES) load_codes<1>(a.codes, (int64_t)c * a.n + i, rgs_pack_step(a.expo[(int64_t)(c / RGS_PACK_BLOCK) * a.n + i]), f);
-        else load_vec<1, SRC>(a.x, (int64_t)c * a.ld + i, f);
-        sm[c * 33 + p] = f[0];
+template <int NV, int V, int Q, typename T>
+__device__ __forceinline__ void store_plane(const NormArgs& a, int64_t i, int v, const float (&x)[Q][NV]) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c = v + k * V;
+        T* out = static_cast<T*>(a.dx) + (int64_t)c * a.n + i;
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+            if (c < a.c && i + q * 32 < a.n) {
+                if constexpr (sizeof(T) == 2) out[q * 32] = __float2bfloat16_rn(x[q][k]);
+                else out[q * 32] = x[q][k];
+            }
     }
 }
 
-template <int NV, int LANES, bool BWD>
-__global__ void __launch_bounds__(NT) rgs_norm_planes_kernel(const __grid_constant__ NormArgs a) {
-    extern __shared__ float sm[];                // (c, 33); behind it room for the sums of a block
-    constexpr int WR = 32 / LANES;               // rows of a warp, LANES apart: their words lie in different banks
-    const int l = threadIdx.x % LANES;
-    const int p = threadIdx.x & 31, c0 = threadIdx.x >> 5;
-    float w[NV][1], b[NV][1], sw[NV][1], sb[NV][1];
-    load_params<1, NV, LANES>(a, l, a.w, 1.f, w);
-    if (!BWD) load_params<1, NV, LANES>(a, l, a.b, 0.f, b);
+// sums over the V warps of what each holds for its Q pixels; red: (V, 32 Q)
+template <int V, int Q>
+__device__ __forceinline__ void warps_sum(float (&t)[Q], float* red, int v, int p) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) sw[k][0] = sb[k][0] = 0.f;
-    const int64_t tiles = (a.n + PT - 1) / PT;
-    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-        const int64_t base = t * PT;
-        __syncthreads();
-        if (base + p < a.n) {
-            if (a.src == SRC_CODES) load_plane<SRC_CODES>(a, base + p, c0, p, sm);
-            else if (a.src == SRC_BF16) load_plane<SRC_BF16>(a, base + p, c0, p, sm);
-            else load_plane<SRC_F32>(a, base + p, c0, p, sm);
+    for (int q = 0; q < Q; ++q) red[(v * Q + q) * 32 + p] = t[q];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        t[q] = 0.f;
+#pragma unroll
+        for (int k = 0; k < V; ++k) t[q] += red[(k * Q + q) * 32 + p];
+    }
+}
+
+// (32 Q, pitch) of T in shared memory <-> rows of c elements, ld apart; T2: two of them
+template <int V, bool STORE, typename T, typename T2>
+__device__ __forceinline__ void tile_rows(T* tile, int pitch, T* rows, int64_t ld, int count, int c, bool pairs) {
+    const int units = pairs ? c / 2 : c, lane = threadIdx.x & 31;
+    const int wide = units > 16 ? 32 : units > 8 ? 16 : units > 4 ? 8 : units > 2 ? 4 : 2;  // lanes to a row
+    const int per = 32 / wide, l = lane & (wide - 1);
+    for (int r = (threadIdx.x >> 5) * per + lane / wide; r < count; r += V * per) {
+        T* s = tile + r * pitch;
+        T* g = rows + r * ld;
+        if (pairs) {
+#pragma unroll 2
+            for (int u = l; u < units; u += wide) {
+                if (STORE) reinterpret_cast<T2*>(g)[u] = reinterpret_cast<T2*>(s)[u];
+                else reinterpret_cast<T2*>(s)[u] = reinterpret_cast<T2*>(g)[u];
+            }
         } else {
-            for (int c = c0; c < a.c; c += NT / 32) sm[c * 33 + p] = 0.f;
-        }
-        __syncthreads();
-        if (!BWD && a.codes_out && base + p < a.n) {
-            for (int k = c0; k < a.blocks; k += NT / 32) {
-                const int end = min(a.c, (k + 1) * RGS_PACK_BLOCK);
-                uint32_t top = 0;
-                for (int c = k * RGS_PACK_BLOCK; c < end; ++c) top = max(top, __float_as_uint(sm[c * 33 + p]) & 0x7fffffffu);
-                const uint32_t e = rgs_pack_exponent(__uint_as_float(top));
-                a.expo_out[(int64_t)k * a.n + base + p] = (uint8_t)e;
-                for (int c = k * RGS_PACK_BLOCK; c < end; ++c) {
-                    const float f[1] = {sm[c * 33 + p]};
-                    store_codes<1>(a.codes_out, (int64_t)c * a.n + base + p, f, e);
-                }
+#pragma unroll 2
+            for (int u = l; u < units; u += wide) {
+                if (STORE) g[u] = s[u];
+                else s[u] = g[u];
             }
         }
-        for (int r0 = threadIdx.x >> 5; r0 < PT / WR; r0 += NT / 32) {
-            const int r = r0 + (threadIdx.x & 31) / LANES * (PT / WR);
-            const int64_t row = base + r;
-            float x[NV][1];
+    }
+}
+
+template <int NV, int V, int Q, bool BWD>
+__global__ void __launch_bounds__(V * 32) rgs_norm_planes_kernel(const __grid_constant__ NormArgs a) {
+    extern __shared__ float sm[];
+    constexpr int T = 32 * Q;                           // pixels of a tile
+    float* red = sm;                                    // three sums of V x T, then the tile of y or dy
+    void* tile = sm + 3 * V * T;
+    const int p = threadIdx.x & 31, v = threadIdx.x >> 5;
+    const int dt = BWD ? a.dy_dtype : a.y_dtype;
+    // words between pixels: odd, or half a word off, so that 32 pixels of a channel lie in different banks
+    const int pitch = dt == RGS_BF16 ? (a.c % 4 == 0 ? a.c + 2 : a.c) : (a.c % 2 == 0 ? a.c + 1 : a.c);
+    const int64_t ld = BWD ? a.ldy : a.c;
+    const bool pairs = dt == RGS_BF16 && a.c % 2 == 0 && ld % 2 == 0 && (!BWD || (reinterpret_cast<uintptr_t>(a.dy) & 3) == 0);
+    float w[NV], b[NV], sw[NV], sb[NV];
 #pragma unroll
-            for (int k = 0; k < NV; ++k) x[k][0] = k * LANES + l < a.c ? sm[(k * LANES + l) * 33 + r] : 0.f;
-            if (!BWD) {
-                float mu, rstd;
-                row_stats<1, NV, LANES>(x, l, a.c, a.inv_c, a.eps, mu, rstd);
-                if (row < a.n)
+    for (int k = 0; k < NV; ++k) {
+        const int c = v + k * V;
+        w[k] = a.w && c < a.c ? rgs_load_as_float(a.w, c, a.p_dtype) : 1.f;
+        b[k] = !BWD && a.b && c < a.c ? rgs_load_as_float(a.b, c, a.p_dtype) : 0.f;
+        sw[k] = sb[k] = 0.f;
+    }
+    const int64_t tiles = (a.n + T - 1) / T;
+    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const int64_t base = t * T, i = base + p;
+        const int count = (int)(a.n - base < T ? a.n - base : T);
+        float x[Q][NV], s[Q], mu[Q], rstd[Q];
+        if (a.src == SRC_CODES) load_plane<NV, V, Q, SRC_CODES>(a, i, v, x);
+        else if (a.src == SRC_BF16) load_plane<NV, V, Q, SRC_BF16>(a, i, v, x);
+        else load_plane<NV, V, Q, SRC_F32>(a, i, v, x);
+        if (BWD) {
+            if (dt == RGS_BF16) tile_rows<V, false, uint16_t, uint32_t>(static_cast<uint16_t*>(tile), pitch, const_cast<uint16_t*>(static_cast<const uint16_t*>(a.dy)) + base * ld, ld, count, a.c, pairs);
+            else tile_rows<V, false, float, float2>(static_cast<float*>(tile), pitch, const_cast<float*>(static_cast<const float*>(a.dy)) + base * ld, ld, count, a.c, false);
+        }
 #pragma unroll
-                    for (int k = 0; k < NV; ++k) {
-                        const int c = k * LANES + l;
-                        const float f[1] = {fmaf((x[k][0] - mu) * rstd, w[k][0], b[k][0])};
-                        if (c < a.c) store_vec<1>(a.y, row * a.c + c, a.y_dtype, f);
+        for (int q = 0; q < Q; ++q) {
+            s[q] = 0.f;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) s[q] += x[q][k];
+        }
+        warps_sum<V, Q>(s, red, v, p);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            mu[q] = s[q] * a.inv_c;
+            s[q] = 0.f;
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+                if (v + k * V < a.c) s[q] = fmaf(x[q][k] - mu[q], x[q][k] - mu[q], s[q]);
+        }
+        warps_sum<V, Q>(s, red + V * T, v, p);
+        // (a pixel behind the end is zeros; its rstd takes 1 for a variance, so that with eps = 0 it stays finite)
+#pragma unroll
+        for (int q = 0; q < Q; ++q) rstd[q] = rsqrtf(i + q * 32 < a.n ? s[q] * a.inv_c + a.eps : 1.f);
+        if (!BWD) {
+            if (a.codes_out) {
+                // largest magnitude of a block of 32 channels: those of every warp lie in 32 / V of its steps
+                constexpr int KB = V < RGS_PACK_BLOCK ? RGS_PACK_BLOCK / V : 1;
+                uint32_t* top = reinterpret_cast<uint32_t*>(red + 2 * V * T);
+#pragma unroll
+                for (int k = 0; k < NV; k += KB) {
+                    if (k * V >= a.c) break;
+                    __syncthreads();
+#pragma unroll
+                    for (int q = 0; q < Q; ++q) {
+                        uint32_t m = 0;
+#pragma unroll
+                        for (int e = k; e < k + KB && e < NV; ++e) m = max(m, __float_as_uint(x[q][e]) & 0x7fffffffu);
+                        top[(v * Q + q) * 32 + p] = m;
                     }
-            } else {
-                float g[NV][1];
-                load_typed<1, NV, LANES>(a.dy, a.dy_dtype, row * a.ldy, l, row < a.n ? a.c : 0, g);
-                row_bwd<1, NV, LANES>(x, g, w, sw, sb, l, a.c, a.inv_c, row < a.n ? a.eps : 1.f);
+                    __syncthreads();
 #pragma unroll
-                for (int k = 0; k < NV; ++k)
-                    if (k * LANES + l < a.c) sm[(k * LANES + l) * 33 + r] = x[k][0];
+                    for (int q = 0; q < Q; ++q) {
+                        uint32_t m = 0;
+#pragma unroll
+                        for (int e = 0; e < V; ++e) m = max(m, top[(e * Q + q) * 32 + p]);
+                        m = rgs_pack_exponent(__uint_as_float(m));
+                        const int64_t iq = i + q * 32;
+                        if (iq < a.n) {
+                            if (v == 0) a.expo_out[(int64_t)(k * V / RGS_PACK_BLOCK) * a.n + iq] = (uint8_t)m;
+#pragma unroll
+                            for (int e = k; e < k + KB && e < NV; ++e) {
+                                const float f[1] = {x[q][e]};
+                                if (v + e * V < a.c) store_codes<1>(a.codes_out, (int64_t)(v + e * V) * a.n + iq, f, m);
+                            }
+                        }
+                    }
+                }
+            }
+            // (the last tile's rows were read before the barriers of these sums)
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+#pragma unroll
+                for (int k = 0; k < NV; ++k) x[q][k] = fmaf((x[q][k] - mu[q]) * rstd[q], w[k], b[k]);
+            if (dt == RGS_BF16) {
+                __nv_bfloat16* o = static_cast<__nv_bfloat16*>(tile) + p * pitch + v;
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+#pragma unroll
+                    for (int k = 0; k < NV; ++k)
+                        if (v + k * V < a.c) o[q * 32 * pitch + k * V] = __float2bfloat16_rn(x[q][k]);
+            } else {
+                float* o = static_cast<float*>(tile) + p * pitch + v;
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+#pragma unroll
+                    for (int k = 0; k < NV; ++k)
+                        if (v + k * V < a.c) o[q * 32 * pitch + k * V] = x[q][k];
+            }
+            __syncthreads();
+            if (dt == RGS_BF16) tile_rows<V, true, uint16_t, uint32_t>(static_cast<uint16_t*>(tile), pitch, static_cast<uint16_t*>(a.y) + base * ld, ld, count, a.c, pairs);
+            else tile_rows<V, true, float, float2>(static_cast<float*>(tile), pitch, static_cast<float*>(a.y) + base * ld, ld, count, a.c, false);
+        } else {
+            float g[Q][NV], sa[Q], sax[Q];
+            if (dt == RGS_BF16) {
+                const uint16_t* o = static_cast<const uint16_t*>(tile) + p * pitch + v;
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+#pragma unroll
+                    for (int k = 0; k < NV; ++k) g[q][k] = v + k * V < a.c && i + q * 32 < a.n ? rgs_bf16_value(o[q * 32 * pitch + k * V]) : 0.f;
+            } else {
+                const float* o = static_cast<const float*>(tile) + p * pitch + v;
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+#pragma unroll
+                    for (int k = 0; k < NV; ++k) g[q][k] = v + k * V < a.c && i + q * 32 < a.n ? o[q * 32 * pitch + k * V] : 0.f;
+            }
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                sa[q] = sax[q] = 0.f;
+#pragma unroll
+                for (int k = 0; k < NV; ++k) {  // (outside dy is zero, and so is what x adds to the sums)
+                    x[q][k] = (x[q][k] - mu[q]) * rstd[q];
+                    sw[k] = fmaf(g[q][k], x[q][k], sw[k]);
+                    sb[k] += g[q][k];
+                    g[q][k] *= w[k];
+                    sa[q] += g[q][k];
+                    sax[q] = fmaf(g[q][k], x[q][k], sax[q]);
+                }
+            }
+            warps_sum<V, Q>(sax, red + 2 * V * T, v, p);
+            warps_sum<V, Q>(sa, red, v, p);  // (every warp has read the first sum before the barrier of the second)
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                sa[q] *= a.inv_c;
+                sax[q] *= a.inv_c;
+#pragma unroll
+                for (int k = 0; k < NV; ++k) x[q][k] = rstd[q] * (g[q][k] - sa[q] - x[q][k] * sax[q]);
+            }
+            if (a.dx) {
+                if (a.dx_dtype == RGS_BF16) store_plane<NV, V, Q, __nv_bfloat16>(a, i, v, x);
+                else store_plane<NV, V, Q, float>(a, i, v, x);
+            }
+            __syncthreads();  // the sums' words have been read before the next tile's are written
+        }
+    }
+    if (BWD && a.part)
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = v + k * V;
+            const float tw = group_sum<32>(sw[k]), tb = group_sum<32>(sb[k]);
+            if (p == 0 && c < a.c) {
+                if (gridDim.x > 1) {
+                    a.part[((int64_t)blockIdx.x * 2) * a.c + c] = tw;
+                    a.part[((int64_t)blockIdx.x * 2 + 1) * a.c + c] = tb;
+                } else {
+                    if (a.dw) rgs_store_float(a.dw, c, a.p_dtype, tw);
+                    if (a.db) rgs_store_float(a.db, c, a.p_dtype, tb);
+                }
             }
         }
-        if (BWD && a.dx) {
-            __syncthreads();
-            if (base + p < a.n)
-                for (int c = c0; c < a.c; c += NT / 32) {
-                    const float f[1] = {sm[c * 33 + p]};
-                    store_vec<1>(a.dx, (int64_t)c * a.n + base + p, a.dx_dtype, f);
-                }
-        }
-    }
-    if (BWD && a.part) {
-        __syncthreads();
-        block_sums<1, NV, LANES>(a, l, sw, sb, sm);
-    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // more channels than a group holds: a warp re-reads its row; a block of threads per 32 channels sums dw and db
 // ---------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float wide_value(const NormArgs& a, int64_t i, int c) {
-    if (a.planes) return plane_value(a, i, c);
     if (a.src == SRC_CODES) return (float)a.codes[i * a.c + c] * rgs_pack_step(a.expo[i * a.blocks + c / RGS_PACK_BLOCK]);
     return rgs_load_as_float(a.x, i * a.ld + c, a.src);
 }
@@ -455,7 +709,7 @@ __global__ void __launch_bounds__(NT) rgs_norm_wide_kernel(const __grid_constant
         sax = group_sum<32>(sax) * a.inv_c;
         for (int j = lane; j < a.c; j += 32) {
             const float g = rgs_load_as_float(a.dy, i * a.ldy + j, a.dy_dtype) * (a.w ? rgs_load_as_float(a.w, j, a.p_dtype) : 1.f);
-            rgs_store_float(a.dx, a.planes ? j * a.n + i : i * a.c + j, a.dx_dtype, rstd * (g - sa - (wide_value(a, i, j) - mu) * rstd * sax));
+            rgs_store_float(a.dx, i * a.c + j, a.dx_dtype, rstd * (g - sa - (wide_value(a, i, j) - mu) * rstd * sax));
         }
     }
 }
@@ -503,42 +757,64 @@ __global__ void __launch_bounds__(1024) rgs_norm_reduce_kernel(const float* __re
 // ---------------------------------------------------------------------------------------------------------------------
 // the 8-bit form by itself
 // ---------------------------------------------------------------------------------------------------------------------
-// Rows: 32 / VEC lanes to a 32-channel block, so that a warp reads and writes what lies together; four blocks in flight.
-// `flat`: whole blocks that follow one another without a gap, no division.
+// Rows: eight lanes to a 32-channel block, four channels each (together, or eight apart where rows are not aligned), so that a
+// warp reads and writes what lies together; four blocks in flight.  `flat`: whole blocks that follow one another without a
+// gap, no division.
 template <int VEC, int DT>
 __global__ void __launch_bounds__(NT) rgs_pack8_rows_kernel(const __grid_constant__ NormArgs a, int flat) {
-    constexpr int LB = RGS_PACK_BLOCK / VEC, U = 4;
+    constexpr int LB = 8, U = 4;
     const int l = threadIdx.x % LB;
     const int64_t total = a.n * a.blocks, per = NT / LB;
     for (int64_t t0 = (int64_t)blockIdx.x * (per * U); t0 < total; t0 += (int64_t)gridDim.x * (per * U)) {
-        float x[U][VEC];
+        float x[U][4];
         int64_t row[U];
         int c[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t t = t0 + u * per + threadIdx.x / LB;
-            if (flat) { row[u] = t; c[u] = l * VEC; }
+            if (flat) { row[u] = t; c[u] = 0; }
             else {
                 row[u] = total < ((int64_t)1 << 31) ? (int64_t)((uint32_t)t / (uint32_t)a.blocks) : t / a.blocks;
-                c[u] = (int)(t - row[u] * a.blocks) * RGS_PACK_BLOCK + l * VEC;
+                c[u] = (int)(t - row[u] * a.blocks) * RGS_PACK_BLOCK;
             }
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) x[u][q] = 0.f;
-            if (t < total && (flat || c[u] < a.c)) load_vec<VEC, DT>(a.x, flat ? t * RGS_PACK_BLOCK + c[u] : row[u] * a.ld + c[u], x[u]);
+            for (int q = 0; q < 4; ++q) x[u][q] = 0.f;
+            if (t >= total) continue;
+            const int64_t at = flat ? t * RGS_PACK_BLOCK : row[u] * a.ld + c[u];
+            if constexpr (VEC == 4) {
+                if (flat || c[u] + l * 4 < a.c) load_vec<4, DT>(a.x, at + l * 4, x[u]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float f[1] = {0.f};
+                    if (c[u] + q * 8 + l < a.c) load_vec<1, DT>(a.x, at + q * 8 + l, f);
+                    x[u][q] = f[0];
+                }
+            }
         }
+        __syncwarp();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t t = t0 + u * per + threadIdx.x / LB;
             uint32_t top = 0;
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) top = max(top, __float_as_uint(x[u][q]) & 0x7fffffffu);
+            for (int q = 0; q < 4; ++q) top = max(top, __float_as_uint(x[u][q]) & 0x7fffffffu);
             const uint32_t e = rgs_pack_exponent(__uint_as_float(group_max<LB>(top)));
-            if (t >= total) continue;
-            if (l == 0) a.expo_out[t] = (uint8_t)e;
-            if (flat) store_codes<VEC>(a.codes_out, t * RGS_PACK_BLOCK + c[u], x[u], e);
-            else if (c[u] < a.c) store_codes<VEC>(a.codes_out, row[u] * a.c + c[u], x[u], e);
+            if (t < total) {
+                if (l == 0) a.expo_out[t] = (uint8_t)e;
+                const int64_t at = flat ? t * RGS_PACK_BLOCK : row[u] * a.c + c[u];
+                if constexpr (VEC == 4) {
+                    if (flat || c[u] + l * 4 < a.c) store_codes<4>(a.codes_out, at + l * 4, x[u], e);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float f[1] = {x[u][q]};
+                        if (c[u] + q * 8 + l < a.c) store_codes<1>(a.codes_out, at + q * 8 + l, f, e);
+                    }
+                }
+            }
+            __syncwarp();
         }
-        __syncwarp();
     }
 }
 
@@ -602,7 +878,10 @@ __global__ void __launch_bounds__(NT) rgs_unpack8_kernel(const __grid_constant__
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (t0 + u * NT < total) store_vec<VEC>(out, (t0 + u * NT) * VEC, dtype, f[u]);
+            if (t0 + u * NT < total) {
+                if (dtype == RGS_BF16) store_vec<VEC, RGS_BF16>(out, (t0 + u * NT) * VEC, f[u]);
+                else store_vec<VEC, RGS_F32>(out, (t0 + u * NT) * VEC, f[u]);
+            }
     }
 }
 
@@ -627,72 +906,81 @@ static int64_t norm_resident(K kernel, int smem) {
 }
 static inline int64_t at_most(int64_t want, int64_t most) { return want < 1 ? 1 : (want > most ? most : want); }
 
-template <int VEC, int NV, int LANES, int R>
+template <int VEC, int NV, int LANES, int R, bool SHIFT>
 static int norm_rows_launch(const NormArgs& a, bool backward, cudaStream_t st) {
     const int64_t want = (a.n + (NT / LANES) * R - 1) / ((NT / LANES) * R);
     if (backward) {
         static std::atomic<int64_t> most{0};
-        if (!most) most = norm_resident(rgs_norm_rows_bwd_kernel<VEC, NV, LANES, R>, 0);
-        const int64_t grid = at_most(at_most(want, most), NORM_PARTS);
-        rgs_norm_rows_bwd_kernel<VEC, NV, LANES, R><<<(unsigned)grid, NT, 0, st>>>(a);
+        if (!most) most = norm_resident(rgs_norm_rows_bwd_kernel<VEC, NV, LANES, R, SHIFT>, 0);
+        // a few rows: one block, no partial sums, one launch
+        const int64_t grid = want <= 4 ? 1 : at_most(at_most(want, most), NORM_PARTS);
+        rgs_norm_rows_bwd_kernel<VEC, NV, LANES, R, SHIFT><<<(unsigned)grid, NT, 0, st>>>(a);
         return (int)grid;
     }
     static std::atomic<int64_t> most[2];
-    const int pack = a.codes_out != nullptr;
-    if (!most[pack]) most[pack] = pack ? norm_resident(rgs_norm_rows_fwd_kernel<VEC, NV, LANES, R, true>, 0) : norm_resident(rgs_norm_rows_fwd_kernel<VEC, NV, LANES, R, false>, 0);
+    const int pack = !SHIFT && a.codes_out != nullptr;
+    if (!most[pack])
+        most[pack] = pack ? norm_resident(rgs_norm_rows_fwd_kernel<VEC, NV, LANES, R, SHIFT, !SHIFT>, 0) : norm_resident(rgs_norm_rows_fwd_kernel<VEC, NV, LANES, R, SHIFT, false>, 0);
     const unsigned grid = (unsigned)at_most(want, most[pack]);
-    if (pack) rgs_norm_rows_fwd_kernel<VEC, NV, LANES, R, true><<<grid, NT, 0, st>>>(a);
-    else rgs_norm_rows_fwd_kernel<VEC, NV, LANES, R, false><<<grid, NT, 0, st>>>(a);
+    if (pack) rgs_norm_rows_fwd_kernel<VEC, NV, LANES, R, SHIFT, !SHIFT><<<grid, NT, 0, st>>>(a);
+    else rgs_norm_rows_fwd_kernel<VEC, NV, LANES, R, SHIFT, false><<<grid, NT, 0, st>>>(a);
     return 0;
 }
 
 // Few lanes to a row and several vectors to a lane: the shuffles of a row's sums are what narrow rows cost most (one lane
 // to a vector: 1.4 TB/s at 33 channels, 3.4 at 64 backward).
-static int norm_rows(const NormArgs& a, bool vec, bool backward, cudaStream_t st) {
-    const int u = vec ? a.c / 4 : a.c;
-    if (vec) {
-        if (u <= 2) return norm_rows_launch<4, 2, 1, 2>(a, backward, st);
-        if (u <= 4) return norm_rows_launch<4, 2, 2, 2>(a, backward, st);
-        if (u <= 8) return norm_rows_launch<4, 2, 4, 2>(a, backward, st);
-        if (u <= 16) return norm_rows_launch<4, 2, 8, 2>(a, backward, st);
-        if (u <= 32) return norm_rows_launch<4, 2, 16, 2>(a, backward, st);
-        if (u <= 64) return norm_rows_launch<4, 2, 32, 2>(a, backward, st);
-        if (u <= 128) return norm_rows_launch<4, 4, 32, 1>(a, backward, st);
-        return norm_rows_launch<4, 8, 32, 1>(a, backward, st);
-    }
-    if (u <= 4) return norm_rows_launch<1, 4, 1, 2>(a, backward, st);
-    if (u <= 8) return norm_rows_launch<1, 4, 2, 2>(a, backward, st);
-    if (u <= 16) return norm_rows_launch<1, 4, 4, 2>(a, backward, st);
-    if (u <= 32) return norm_rows_launch<1, 4, 8, 2>(a, backward, st);
-    if (u <= 64) return norm_rows_launch<1, 4, 16, 2>(a, backward, st);
-    if (u <= 128) return norm_rows_launch<1, 4, 32, 2>(a, backward, st);
-    if (u <= 256) return norm_rows_launch<1, 8, 32, 1>(a, backward, st);
-    if (u <= 512) return norm_rows_launch<1, 16, 32, 1>(a, backward, st);
-    if (u <= 640) return norm_rows_launch<1, 20, 32, 1>(a, backward, st);
-    if (u <= 768) return norm_rows_launch<1, 24, 32, 1>(a, backward, st);
-    if (u <= 896) return norm_rows_launch<1, 28, 32, 1>(a, backward, st);
-    return norm_rows_launch<1, 32, 32, 1>(a, backward, st);
+template <bool SHIFT>
+static int norm_rows_vec(const NormArgs& a, bool backward, cudaStream_t st) {
+    const int u = (a.c + (SHIFT ? 6 : 0)) / 4;  // vectors of a row
+    if (u <= 3) return norm_rows_launch<4, 3, 1, 1, SHIFT>(a, backward, st);
+    if (u <= 4) return norm_rows_launch<4, 4, 1, 1, SHIFT>(a, backward, st);
+    if (u <= 6) return norm_rows_launch<4, 3, 2, 1, SHIFT>(a, backward, st);
+    if (u <= 8) return norm_rows_launch<4, 4, 2, 1, SHIFT>(a, backward, st);
+    if (u <= 12) return norm_rows_launch<4, 3, 4, 1, SHIFT>(a, backward, st);
+    if (u <= 16) return norm_rows_launch<4, 4, 4, 1, SHIFT>(a, backward, st);
+    if (u <= 24) return norm_rows_launch<4, 3, 8, 1, SHIFT>(a, backward, st);
+    if (u <= 32) return norm_rows_launch<4, 4, 8, 1, SHIFT>(a, backward, st);
+    if (u <= 48) return norm_rows_launch<4, 3, 16, 1, SHIFT>(a, backward, st);
+    if (u <= 64) return norm_rows_launch<4, 4, 16, 1, SHIFT>(a, backward, st);
+    if (u <= 96) return norm_rows_launch<4, 3, 32, 1, SHIFT>(a, backward, st);
+    if (u <= 128) return norm_rows_launch<4, 4, 32, 1, SHIFT>(a, backward, st);
+    if (u <= 192) return norm_rows_launch<4, 6, 32, 1, SHIFT>(a, backward, st);
+    return norm_rows_launch<4, 8, 32, 1, SHIFT>(a, backward, st);
+}
+// element by element: rows apart by a stride that four does not divide, codes of an odd width
+static int norm_rows_single(const NormArgs& a, bool backward, cudaStream_t st) {
+    const int u = a.c;
+    if (u <= 8) return norm_rows_launch<1, 8, 1, 1, false>(a, backward, st);
+    if (u <= 16) return norm_rows_launch<1, 8, 2, 1, false>(a, backward, st);
+    if (u <= 32) return norm_rows_launch<1, 8, 4, 1, false>(a, backward, st);
+    if (u <= 64) return norm_rows_launch<1, 8, 8, 1, false>(a, backward, st);
+    if (u <= 128) return norm_rows_launch<1, 8, 16, 1, false>(a, backward, st);
+    if (u <= 256) return norm_rows_launch<1, 8, 32, 1, false>(a, backward, st);
+    if (u <= 512) return norm_rows_launch<1, 16, 32, 1, false>(a, backward, st);
+    if (u <= 768) return norm_rows_launch<1, 24, 32, 1, false>(a, backward, st);
+    return norm_rows_launch<1, 32, 32, 1, false>(a, backward, st);
 }
 
-template <int NV, int LANES, bool BWD>
+template <int NV, int V, int Q, bool BWD>
 static int norm_planes_launch(const NormArgs& a, int* parts, cudaStream_t st) {
-    const int smem = (a.c * 33 > NT ? a.c * 33 : NT) * 4;  // (block_sums takes NT floats of it)
-    if (smem > 48 * 1024) RGS_CUDA_CHECK(cudaFuncSetAttribute(rgs_norm_planes_kernel<NV, LANES, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    *parts = (int)at_most(at_most((a.n + PT - 1) / PT, norm_resident(rgs_norm_planes_kernel<NV, LANES, BWD>, smem)), NORM_PARTS);
-    rgs_norm_planes_kernel<NV, LANES, BWD><<<(unsigned)*parts, NT, smem, st>>>(a);
+    const int smem = 3 * V * 32 * Q * 4 + 32 * Q * (a.c + 2) * 4;
+    if (smem > 48 * 1024) RGS_CUDA_CHECK(cudaFuncSetAttribute(rgs_norm_planes_kernel<NV, V, Q, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    int per_sm = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, rgs_norm_planes_kernel<NV, V, Q, BWD>, V * 32, (size_t)smem) != cudaSuccess || per_sm < 1) per_sm = 1;
+    *parts = (int)at_most(at_most((a.n + 32 * Q - 1) / (32 * Q), RGS_SMS * per_sm), NORM_PARTS);
+    rgs_norm_planes_kernel<NV, V, Q, BWD><<<(unsigned)*parts, V * 32, smem, st>>>(a);
     return (int)cudaGetLastError();
 }
 
 template <bool BWD>
 static int norm_planes(const NormArgs& a, int* parts, cudaStream_t st) {
-    if (a.c <= 8) return norm_planes_launch<8, 1, BWD>(a, parts, st);
-    if (a.c <= 16) return norm_planes_launch<8, 2, BWD>(a, parts, st);
-    if (a.c <= 32) return norm_planes_launch<8, 4, BWD>(a, parts, st);
-    if (a.c <= 64) return norm_planes_launch<8, 8, BWD>(a, parts, st);
-    if (a.c <= 128) return norm_planes_launch<8, 16, BWD>(a, parts, st);
-    if (a.c <= 256) return norm_planes_launch<8, 32, BWD>(a, parts, st);
-    if (a.c <= 512) return norm_planes_launch<16, 32, BWD>(a, parts, st);
-    return norm_planes_launch<32, 32, BWD>(a, parts, st);
+    if (a.c <= 8) return norm_planes_launch<1, 8, 2, BWD>(a, parts, st);
+    if (a.c <= 16) return norm_planes_launch<2, 8, 2, BWD>(a, parts, st);
+    if (a.c <= 32) return norm_planes_launch<4, 8, 2, BWD>(a, parts, st);
+    if (a.c <= 64) return norm_planes_launch<8, 8, 2, BWD>(a, parts, st);
+    if (a.c <= 128) return norm_planes_launch<8, 16, 1, BWD>(a, parts, st);
+    if (a.c <= 256) return norm_planes_launch<16, 16, 1, BWD>(a, parts, st);
+    return norm_planes_launch<16, 32, 1, BWD>(a, parts, st);
 }
 
 extern "C" {
@@ -741,6 +1029,7 @@ int rgs_cuda_norm_fwd(const void* x, int64_t dtype, int64_t ld, int64_t planes, 
     a.n = n; a.c = (int)c; a.blocks = (int)((c + 31) / 32); a.eps = (float)eps; a.inv_c = 1.f / (float)c;
     a.y = y; a.y_dtype = (int)y_dtype;
     a.codes_out = codes; a.expo_out = expo;
+    if (planes && c > NP_MAX) return 23;
     if (c > NR_MAX) {
         rgs_norm_wide_kernel<<<(unsigned)norm_grid((n + 7) / 8, 16), NT, 0, st>>>(a, 0, nullptr);
         RGS_CUDA_CHECK(cudaGetLastError());
@@ -750,8 +1039,13 @@ int rgs_cuda_norm_fwd(const void* x, int64_t dtype, int64_t ld, int64_t planes, 
         int parts;
         return norm_planes<false>(a, &parts, st);
     }
-    const bool vec = c % 4 == 0 && ld % 4 == 0 && aligned_to(x, four(a.src));
-    norm_rows(a, vec, false, st);
+    const bool start = aligned_to(x, four(a.src));
+    if (start && c % 4 == 0 && ld % 4 == 0) norm_rows_vec<false>(a, false, st);
+    else if (start && (ld - c) % 4 == 0 && c <= NR_MAX - 6) {
+        norm_rows_vec<true>(a, false, st);  // its blocks of 32 channels begin anywhere in a vector: packed by themselves
+        RGS_CUDA_CHECK(cudaGetLastError());
+        if (codes) return rgs_cuda_pack8(x, dtype, ld, planes, n, c, codes, expo, stream);
+    } else norm_rows_single(a, false, st);
     return (int)cudaGetLastError();
 }
 
@@ -767,7 +1061,9 @@ int rgs_cuda_norm_bwd(const void* x, int64_t dtype, int64_t ld, int64_t planes, 
     a.dy = dy; a.dy_dtype = (int)dy_dtype; a.ldy = ldy;
     a.dx = dx; a.dx_dtype = (int)dtype;
     a.part = dw || db ? static_cast<float*>(scratch) : nullptr;
+    a.dw = dw; a.db = db;
     int parts = 0;
+    if (planes && c > NP_MAX) return 23;
     if (c > NR_MAX) {
         float2* stats = reinterpret_cast<float2*>(static_cast<float*>(scratch) + (int64_t)NORM_PARTS * 2 * c);
         rgs_norm_wide_kernel<<<(unsigned)norm_grid((n + 7) / 8, 16), NT, 0, st>>>(a, 1, stats);
@@ -779,12 +1075,13 @@ int rgs_cuda_norm_bwd(const void* x, int64_t dtype, int64_t ld, int64_t planes, 
         const int rc = norm_planes<true>(a, &parts, st);
         if (rc) return rc;
     } else {
-        const bool vec = c % 4 == 0 && ldy % 4 == 0 && aligned_to(dy, four(a.dy_dtype)) &&
-                         (codes || (ld % 4 == 0 && aligned_to(x, four((int)dtype))));
-        parts = norm_rows(a, vec, true, st);
+        const bool start = aligned_to(dy, four(a.dy_dtype)) && (codes || aligned_to(x, four((int)dtype)));
+        if (start && c % 4 == 0 && ldy % 4 == 0 && (codes || ld % 4 == 0)) parts = norm_rows_vec<false>(a, true, st);
+        else if (start && !codes && (ld - c) % 4 == 0 && (ldy - c) % 4 == 0 && c <= NR_MAX - 6) parts = norm_rows_vec<true>(a, true, st);
+        else parts = norm_rows_single(a, true, st);
     }
     RGS_CUDA_CHECK(cudaGetLastError());
-    if (a.part)
+    if (a.part && (parts > 1 || c > NR_MAX))
         rgs_norm_reduce_kernel<<<dim3((unsigned)((c + 31) / 32), 2), 1024, 0, st>>>(a.part, parts, (int)c, dw, db, (int)p_dtype);
     return (int)cudaGetLastError();
 }

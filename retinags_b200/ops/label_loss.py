@@ -8,8 +8,6 @@ the kernels (``csrc/rgs_label.cu``) walk the vocabulary in pieces, keep two numb
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import native
@@ -23,12 +21,9 @@ _LIMIT = 2 ** 31 - 1
 def _scratch(x: torch.Tensor, ldx: int, w: torch.Tensor, ldw: int, backward: int) -> torch.Tensor:
     """Workspace of one pass; it depends on whether the kernels can read the rows as they lie (16-byte boundaries)."""
     device = x.device
-    direct = sum((ld % 8 == 0 and t.data_ptr() % 16 == 0) << k for k, (t, ld) in enumerate(((x, ldx), (w, ldw))))
-    kind = "cuda" if device.type == "cuda" else "cpu"
-    fn = getattr(native.lib(kind), f"rgs_{kind}_label_scratch_bytes")
-    fn.argtypes, fn.restype = [ctypes.c_int64] * 6, ctypes.c_int64
-    with torch.cuda.device(device) if kind == "cuda" else torch.no_grad():
-        return torch.empty(int(fn(*x.shape, w.shape[0], DTYPES[x.dtype], direct, backward)), dtype=torch.uint8, device=device)
+    direct = (ldx % 8 == 0 and x.data_ptr() % 16 == 0) + 2 * (ldw % 8 == 0 and w.data_ptr() % 16 == 0)
+    size = native.size_of("label_scratch_bytes", device, x.shape[0], x.shape[1], w.shape[0], DTYPES[x.dtype], direct, backward)
+    return torch.empty(size, dtype=torch.uint8, device=device)
 
 
 class _LabelLoss(torch.autograd.Function):

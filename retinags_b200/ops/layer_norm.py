@@ -7,25 +7,27 @@ rows in ``out_dtype``.  Sums are held in 32 bits whatever the types.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import native
 from .pack8 import DTYPES, alloc_codes, as_rows, dtype_code, empty_like_layout
 
 
+MAX_PLANES = 512  # channels up to which planes are read and written where they lie; more are copied into rows and back
+
+
 def _scratch(device: torch.device, n: int, c: int) -> torch.Tensor:
-    kind = "cuda" if device.type == "cuda" else "cpu"
-    fn = getattr(native.lib(kind), f"rgs_{kind}_norm_scratch_bytes")
-    fn.argtypes, fn.restype = [ctypes.c_int64, ctypes.c_int64], ctypes.c_int64
-    return torch.empty(int(fn(n, c)), dtype=torch.uint8, device=device)
+    return torch.empty(native.size_of("norm_scratch_bytes", device, n, c), dtype=torch.uint8, device=device)
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, out_dtype, keep):
         flat, ld, planes = as_rows(x, "layer_norm")
+        out_planes = planes
+        if planes and flat.shape[1] > MAX_PLANES:
+            flat = flat.contiguous()
+            ld, planes = flat.shape[1], 0
         n, c = flat.shape
         y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
         p_code = DTYPES[weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32]
@@ -37,7 +39,7 @@ class _LayerNorm(torch.autograd.Function):
             native.call("norm_fwd", x.device, flat, DTYPES[x.dtype], ld, planes, weight, bias, p_code, n, c, eps, y, DTYPES[out_dtype],
                         codes, exponents)
         ctx.save_for_backward(flat if codes is None else None, codes, exponents, weight)
-        ctx.layout = (tuple(x.shape), x.dtype, ld, planes, n, c, p_code, eps)
+        ctx.layout = (tuple(x.shape), x.dtype, ld, planes, out_planes, n, c, p_code, eps)
         ctx.param_dtypes = (weight.dtype if weight is not None else None, bias.dtype if bias is not None else None)
         return y
 
@@ -45,7 +47,7 @@ class _LayerNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         flat, codes, exponents, weight = ctx.saved_tensors
-        shape, x_dtype, ld, planes, n, c, p_code, eps = ctx.layout
+        shape, x_dtype, ld, planes, out_planes, n, c, p_code, eps = ctx.layout
         dev = dy.device
         dyf, ldy, _ = as_rows(dy, "layer_norm", planes_ok=False)
         dx = empty_like_layout(shape, planes, x_dtype, dev) if ctx.needs_input_grad[0] else None
@@ -55,6 +57,8 @@ class _LayerNorm(torch.autograd.Function):
         if n:
             native.call("norm_bwd", dev, flat, DTYPES[x_dtype], ld, planes, codes, exponents, dyf, DTYPES[dyf.dtype], ldy, weight, p_code,
                         n, c, eps, _scratch(dev, n, c), dx, dw, db)
+        if dx is not None and out_planes != planes:
+            dx = empty_like_layout(shape, out_planes, x_dtype, dev).copy_(dx)
         return dx, dw, db, None, None, None
 
 

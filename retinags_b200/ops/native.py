@@ -154,15 +154,21 @@ def ptr(x):
     raise TypeError(type(x))
 
 
+_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr(device: torch.device):
     if device.type != "cuda":
         return None
+    if _RAW_STREAM is not None and device.index is not None:  # the same number without a Stream object around it
+        return _RAW_STREAM(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
 # kernels launched by one call of an entry point (the radix sort's count depends on the tile count)
 _KERNELS = {"project_slots": 1, "project_slots2": 2, "project_slots2_geom": 2, "colour_slab": 1, "tile_maps_or": 1, "tile_map_push": 1, "project_emit": 1, "blend_fwd": 1, "blend_bwd": 1, "geom_bwd": 1, "scatter_radii": 1, "adam": 1, "adam_rows": 2,
-            "composite_fwd": 1, "composite_bwd": 1, "ssim_fwd": 1, "ssim_bwd": 1, "densify_classify": 2, "blend_fwd_slab": 1, "blend_bwd_slab": 1}
+            "composite_fwd": 1, "composite_bwd": 1, "ssim_fwd": 1, "ssim_bwd": 1, "densify_classify": 2, "blend_fwd_slab": 1, "blend_bwd_slab": 1,
+            "label_fwd": 3, "label_bwd": 3, "norm_fwd": 1, "norm_bwd": 2, "pack8": 1, "unpack8": 1}
 _LAUNCHES = [0]
 _SORT_SWEEP = [os.environ.get("RGS_SORT", "") != "3k"]
 
@@ -212,25 +218,48 @@ def _count_launches(name: str, args) -> int:
     return _KERNELS.get(name, 1)
 
 
+def _raw(a):
+    """Argument of an entry point: numbers as they are, buffers by their address."""
+    t = type(a)
+    return a if t is int or t is float or a is None else a.data_ptr() if t is torch.Tensor else ptr(a) if isinstance(
+        a, (torch.Tensor, ctypes.Structure, ctypes.Array)) else a
+
+
+_FNS: dict = {}
+
+
 def call(name: str, device: torch.device, *args, sig: str | None = None) -> None:
     """Invoke ``rgs_<cpu|cuda>_<name>(*args, stream)`` and raise on a non-zero status."""
     kind = "cuda" if device.type == "cuda" else "cpu"
+    fn = _FNS.get((kind, name))
+    if fn is None or kind not in _LIBS:
+        fn = _FNS[(kind, name)] = _fn(kind, name, sig)
+    conv = [_raw(a) for a in args]
     if kind == "cuda":
         _LAUNCHES[0] += _count_launches(name, args)
-    fn = _fn(kind, name, sig)
-    conv = []
-    for a in args:
-        if isinstance(a, (torch.Tensor, ctypes.Structure, ctypes.Array)) or a is None:
-            conv.append(ptr(a))
-        else:
-            conv.append(a)
-    if kind == "cuda":
-        with torch.cuda.device(device):
+        if device.index is None or device.index == torch.cuda.current_device():
             rc = fn(*conv, stream_ptr(device))
+        else:
+            with torch.cuda.device(device):
+                rc = fn(*conv, stream_ptr(device))
     else:
         rc = fn(*conv, None)
     if rc != 0:
         raise RuntimeError(f"rgs_{kind}_{name} failed with status {rc}")
+
+
+def size_of(name: str, device: torch.device, *args: int) -> int:
+    """Value of a size query ``rgs_<cpu|cuda>_<name>(*args)`` (integers in and out), asked on ``device``."""
+    kind = "cuda" if device.type == "cuda" else "cpu"
+    fn = _FNS.get((kind, name))
+    if fn is None or kind not in _LIBS:
+        fn = getattr(lib(kind), f"rgs_{kind}_{name}")
+        fn.argtypes, fn.restype = [ctypes.c_int64] * len(args), ctypes.c_int64
+        _FNS[(kind, name)] = fn
+    if kind == "cpu" or device.index is None or device.index == torch.cuda.current_device():
+        return int(fn(*args))
+    with torch.cuda.device(device):
+        return int(fn(*args))
 
 
 def pointer_array(tensors) -> ctypes.Array:
