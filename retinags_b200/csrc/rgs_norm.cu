@@ -432,35 +432,46 @@ __global__ void __launch_bounds__(NT, NV * VEC <= 12 ? 3 : NV * VEC <= 16 ? 2 : 
 // channel planes: 32 or 64 pixels at a time, a lane to one or two; warp v of V holds channels v, v + V, ... of them, so planes are read
 // and written where they lie, sums run over the warps, and only rows (y, dy) are turned around in shared memory
 // ---------------------------------------------------------------------------------------------------------------------
+// off: the lane's pixels relative to the tile (behind the last pixel: the last pixel again, which then counts nowhere)
 template <int NV, int V, int Q, int SRC>
-__device__ __forceinline__ void load_plane(const NormArgs& a, int64_t i, int v, float (&x)[Q][NV]) {
+__device__ __forceinline__ void load_plane(const NormArgs& a, int64_t base, const int (&off)[Q], int v, float (&x)[Q][NV]) {
+    constexpr int SIZE = SRC == SRC_CODES ? 1 : SRC == SRC_BF16 ? 2 : 4;
+    const int64_t ld = SRC == SRC_CODES ? a.n : a.ld;
+    const char* p = static_cast<const char*>(SRC == SRC_CODES ? static_cast<const void*>(a.codes) : a.x) + (v * ld + base) * SIZE;
+    const uint8_t* expo = a.expo + base;
+    float step[Q];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int c = v + k * V;
-        const int64_t at = (int64_t)c * (SRC == SRC_CODES ? a.n : a.ld) + i;
+        if (SRC == SRC_CODES && k * V % RGS_PACK_BLOCK == 0) {  // (V divides 32: the warps' channels of a step lie in one block)
+#pragma unroll
+            for (int q = 0; q < Q; ++q) step[q] = k * V < a.c ? rgs_pack_step(expo[off[q]]) : 0.f;
+            expo += a.n;
+        }
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
             float f[1] = {0.f};
-            if (c < a.c && i + q * 32 < a.n) {
-                if constexpr (SRC == SRC_CODES) load_codes<1>(a.codes, at + q * 32, rgs_pack_step(a.expo[(int64_t)(c / RGS_PACK_BLOCK) * a.n + i + q * 32]), f);
-                else load_vec<1, SRC>(a.x, at + q * 32, f);
+            if (v + k * V < a.c) {
+                if constexpr (SRC == SRC_CODES) load_codes<1>(reinterpret_cast<const int8_t*>(p), off[q], step[q], f);
+                else load_vec<1, SRC>(p, off[q], f);
             }
             x[q][k] = f[0];
         }
+        p += V * ld * SIZE;
     }
 }
 template <int NV, int V, int Q, typename T>
-__device__ __forceinline__ void store_plane(const NormArgs& a, int64_t i, int v, const float (&x)[Q][NV]) {
+__device__ __forceinline__ void store_plane(const NormArgs& a, int64_t i, int v, const bool (&in)[Q], const float (&x)[Q][NV]) {
+    T* out = static_cast<T*>(a.dx) + v * a.n + i;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int c = v + k * V;
-        T* out = static_cast<T*>(a.dx) + (int64_t)c * a.n + i;
+        if (v + k * V < a.c)
 #pragma unroll
-        for (int q = 0; q < Q; ++q)
-            if (c < a.c && i + q * 32 < a.n) {
-                if constexpr (sizeof(T) == 2) out[q * 32] = __float2bfloat16_rn(x[q][k]);
-                else out[q * 32] = x[q][k];
-            }
+            for (int q = 0; q < Q; ++q)
+                if (in[q]) {
+                    if constexpr (sizeof(T) == 2) out[q * 32] = __float2bfloat16_rn(x[q][k]);
+                    else out[q * 32] = x[q][k];
+                }
+        out += V * a.n;
     }
 }
 
@@ -478,59 +489,79 @@ __device__ __forceinline__ void warps_sum(float (&t)[Q], float* red, int v, int 
     }
 }
 
+// eight rows at a time, all read before the first is written: one row after the other would wait for memory once a row
+template <int V, typename T>
+__device__ __forceinline__ void read_rows(T* tile, int pitch, const T* rows, int64_t ld, int r0, int step, int l, int wide, int count, int units) {
+    for (int u = l; u < units; u += wide)
+        for (int r = r0; r < count; r += step * 8) {
+            T t[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (r + k * step < count) t[k] = rows[(r + k * step) * ld + u];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (r + k * step < count) tile[(r + k * step) * pitch + u] = t[k];
+        }
+}
+
 // (32 Q, pitch) of T in shared memory <-> rows of c elements, ld apart; T2: two of them
 template <int V, bool STORE, typename T, typename T2>
 __device__ __forceinline__ void tile_rows(T* tile, int pitch, T* rows, int64_t ld, int count, int c, bool pairs) {
     const int units = pairs ? c / 2 : c, lane = threadIdx.x & 31;
     const int wide = units > 16 ? 32 : units > 8 ? 16 : units > 4 ? 8 : units > 2 ? 4 : 2;  // lanes to a row
     const int per = 32 / wide, l = lane & (wide - 1);
-    for (int r = (threadIdx.x >> 5) * per + lane / wide; r < count; r += V * per) {
-        T* s = tile + r * pitch;
-        T* g = rows + r * ld;
-        if (pairs) {
-#pragma unroll 2
-            for (int u = l; u < units; u += wide) {
-                if (STORE) reinterpret_cast<T2*>(g)[u] = reinterpret_cast<T2*>(s)[u];
-                else reinterpret_cast<T2*>(s)[u] = reinterpret_cast<T2*>(g)[u];
-            }
-        } else {
-#pragma unroll 2
-            for (int u = l; u < units; u += wide) {
-                if (STORE) g[u] = s[u];
-                else s[u] = g[u];
-            }
+    const int r0 = (threadIdx.x >> 5) * per + lane / wide;
+    if constexpr (STORE) {
+        for (int r = r0; r < count; r += V * per) {
+            if (pairs)
+                for (int u = l; u < units; u += wide) reinterpret_cast<T2*>(rows + r * ld)[u] = reinterpret_cast<const T2*>(tile + r * pitch)[u];
+            else
+                for (int u = l; u < units; u += wide) rows[r * ld + u] = tile[r * pitch + u];
         }
+    } else if (pairs) {
+        read_rows<V, T2>(reinterpret_cast<T2*>(tile), pitch / 2, reinterpret_cast<const T2*>(rows), ld / 2, r0, V * per, l, wide, count, units);
+    } else {
+        read_rows<V, T>(tile, pitch, rows, ld, r0, V * per, l, wide, count, units);
     }
 }
 
 template <int NV, int V, int Q, bool BWD>
-__global__ void __launch_bounds__(V * 32) rgs_norm_planes_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(V * 32, V == 4 ? (BWD ? 5 : 8) : V == 8 ? (BWD ? 3 : 4) : V == 16 ? (BWD ? 1 : 2) : 1) rgs_norm_planes_kernel(const __grid_constant__ NormArgs a) {
     extern __shared__ float sm[];
     constexpr int T = 32 * Q;                           // pixels of a tile
-    float* red = sm;                                    // three sums of V x T, then the tile of y or dy
-    void* tile = sm + 3 * V * T;
+    float* red = sm;                                    // three sums of V x T, w and b, then the tile of y or dy
+    float *w = sm + 3 * V * T, *b = w + NV * V;
+    void* tile = b + NV * V;
     const int p = threadIdx.x & 31, v = threadIdx.x >> 5;
     const int dt = BWD ? a.dy_dtype : a.y_dtype;
     // words between pixels: odd, or half a word off, so that 32 pixels of a channel lie in different banks
     const int pitch = dt == RGS_BF16 ? (a.c % 4 == 0 ? a.c + 2 : a.c) : (a.c % 2 == 0 ? a.c + 1 : a.c);
     const int64_t ld = BWD ? a.ldy : a.c;
     const bool pairs = dt == RGS_BF16 && a.c % 2 == 0 && ld % 2 == 0 && (!BWD || (reinterpret_cast<uintptr_t>(a.dy) & 3) == 0);
-    float w[NV], b[NV], sw[NV], sb[NV];
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int c = v + k * V;
-        w[k] = a.w && c < a.c ? rgs_load_as_float(a.w, c, a.p_dtype) : 1.f;
-        b[k] = !BWD && a.b && c < a.c ? rgs_load_as_float(a.b, c, a.p_dtype) : 0.f;
-        sw[k] = sb[k] = 0.f;
+    for (int c = threadIdx.x; c < NV * V; c += V * 32) {
+        w[c] = a.w && c < a.c ? rgs_load_as_float(a.w, c, a.p_dtype) : 1.f;
+        b[c] = a.b && c < a.c ? rgs_load_as_float(a.b, c, a.p_dtype) : 0.f;
     }
+    w += v;
+    b += v;
+    float sw[NV], sb[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) sw[k] = sb[k] = 0.f;
     const int64_t tiles = (a.n + T - 1) / T;
     for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
         const int64_t base = t * T, i = base + p;
         const int count = (int)(a.n - base < T ? a.n - base : T);
         float x[Q][NV], s[Q], mu[Q], rstd[Q];
-        if (a.src == SRC_CODES) load_plane<NV, V, Q, SRC_CODES>(a, i, v, x);
-        else if (a.src == SRC_BF16) load_plane<NV, V, Q, SRC_BF16>(a, i, v, x);
-        else load_plane<NV, V, Q, SRC_F32>(a, i, v, x);
+        int off[Q];
+        bool in[Q];
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            in[q] = p + q * 32 < count;
+            off[q] = min(p + q * 32, count - 1);
+        }
+        if (a.src == SRC_CODES) load_plane<NV, V, Q, SRC_CODES>(a, base, off, v, x);
+        else if (a.src == SRC_BF16) load_plane<NV, V, Q, SRC_BF16>(a, base, off, v, x);
+        else load_plane<NV, V, Q, SRC_F32>(a, base, off, v, x);
         if (BWD) {
             if (dt == RGS_BF16) tile_rows<V, false, uint16_t, uint32_t>(static_cast<uint16_t*>(tile), pitch, const_cast<uint16_t*>(static_cast<const uint16_t*>(a.dy)) + base * ld, ld, count, a.c, pairs);
             else tile_rows<V, false, float, float2>(static_cast<float*>(tile), pitch, const_cast<float*>(static_cast<const float*>(a.dy)) + base * ld, ld, count, a.c, false);
@@ -551,9 +582,8 @@ __global__ void __launch_bounds__(V * 32) rgs_norm_planes_kernel(const __grid_co
                 if (v + k * V < a.c) s[q] = fmaf(x[q][k] - mu[q], x[q][k] - mu[q], s[q]);
         }
         warps_sum<V, Q>(s, red + V * T, v, p);
-        // (a pixel behind the end is zeros; its rstd takes 1 for a variance, so that with eps = 0 it stays finite)
 #pragma unroll
-        for (int q = 0; q < Q; ++q) rstd[q] = rsqrtf(i + q * 32 < a.n ? s[q] * a.inv_c + a.eps : 1.f);
+        for (int q = 0; q < Q; ++q) rstd[q] = rsqrtf(s[q] * a.inv_c + a.eps);
         if (!BWD) {
             if (a.codes_out) {
                 // largest magnitude of a block of 32 channels: those of every warp lie in 32 / V of its steps
@@ -578,7 +608,7 @@ __global__ void __launch_bounds__(V * 32) rgs_norm_planes_kernel(const __grid_co
                         for (int e = 0; e < V; ++e) m = max(m, top[(e * Q + q) * 32 + p]);
                         m = rgs_pack_exponent(__uint_as_float(m));
                         const int64_t iq = i + q * 32;
-                        if (iq < a.n) {
+                        if (in[q]) {
                             if (v == 0) a.expo_out[(int64_t)(k * V / RGS_PACK_BLOCK) * a.n + iq] = (uint8_t)m;
 #pragma unroll
                             for (int e = k; e < k + KB && e < NV; ++e) {
@@ -591,9 +621,11 @@ __global__ void __launch_bounds__(V * 32) rgs_norm_planes_kernel(const __grid_co
             }
             // (the last tile's rows were read before the barriers of these sums)
 #pragma unroll
-            for (int q = 0; q < Q; ++q)
+            for (int k = 0; k < NV; ++k) {
+                const float wk = w[k * V], bk = b[k * V];
 #pragma unroll
-                for (int k = 0; k < NV; ++k) x[q][k] = fmaf((x[q][k] - mu[q]) * rstd[q], w[k], b[k]);
+                for (int q = 0; q < Q; ++q) x[q][k] = fmaf((x[q][k] - mu[q]) * rstd[q], wk, bk);
+            }
             if (dt == RGS_BF16) {
                 __nv_bfloat16* o = static_cast<__nv_bfloat16*>(tile) + p * pitch + v;
 #pragma unroll
@@ -619,23 +651,28 @@ __global__ void __launch_bounds__(V * 32) rgs_norm_planes_kernel(const __grid_co
 #pragma unroll
                 for (int q = 0; q < Q; ++q)
 #pragma unroll
-                    for (int k = 0; k < NV; ++k) g[q][k] = v + k * V < a.c && i + q * 32 < a.n ? rgs_bf16_value(o[q * 32 * pitch + k * V]) : 0.f;
+                    for (int k = 0; k < NV; ++k) g[q][k] = v + k * V < a.c ? rgs_bf16_value(o[q * 32 * pitch + k * V]) : 0.f;
             } else {
                 const float* o = static_cast<const float*>(tile) + p * pitch + v;
 #pragma unroll
                 for (int q = 0; q < Q; ++q)
 #pragma unroll
-                    for (int k = 0; k < NV; ++k) g[q][k] = v + k * V < a.c && i + q * 32 < a.n ? o[q * 32 * pitch + k * V] : 0.f;
+                    for (int k = 0; k < NV; ++k) g[q][k] = v + k * V < a.c ? o[q * 32 * pitch + k * V] : 0.f;
             }
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
                 sa[q] = sax[q] = 0.f;
+                if (count < T && !in[q]) {  // the last pixel again: none of it counts, whatever it holds
+                    mu[q] = rstd[q] = 0.f;
+#pragma unroll
+                    for (int k = 0; k < NV; ++k) x[q][k] = g[q][k] = 0.f;
+                }
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {  // (outside dy is zero, and so is what x adds to the sums)
                     x[q][k] = (x[q][k] - mu[q]) * rstd[q];
                     sw[k] = fmaf(g[q][k], x[q][k], sw[k]);
                     sb[k] += g[q][k];
-                    g[q][k] *= w[k];
+                    g[q][k] *= w[k * V];
                     sa[q] += g[q][k];
                     sax[q] = fmaf(g[q][k], x[q][k], sax[q]);
                 }
@@ -650,8 +687,8 @@ __global__ void __launch_bounds__(V * 32) rgs_norm_planes_kernel(const __grid_co
                 for (int k = 0; k < NV; ++k) x[q][k] = rstd[q] * (g[q][k] - sa[q] - x[q][k] * sax[q]);
             }
             if (a.dx) {
-                if (a.dx_dtype == RGS_BF16) store_plane<NV, V, Q, __nv_bfloat16>(a, i, v, x);
-                else store_plane<NV, V, Q, float>(a, i, v, x);
+                if (a.dx_dtype == RGS_BF16) store_plane<NV, V, Q, __nv_bfloat16>(a, i, v, in, x);
+                else store_plane<NV, V, Q, float>(a, i, v, in, x);
             }
             __syncthreads();  // the sums' words have been read before the next tile's are written
         }
@@ -963,7 +1000,7 @@ static int norm_rows_single(const NormArgs& a, bool backward, cudaStream_t st) {
 
 template <int NV, int V, int Q, bool BWD>
 static int norm_planes_launch(const NormArgs& a, int* parts, cudaStream_t st) {
-    const int smem = 3 * V * 32 * Q * 4 + 32 * Q * (a.c + 2) * 4;
+    const int smem = (3 * V * 32 * Q + 2 * NV * V + 32 * Q * (a.c + 2)) * 4;
     if (smem > 48 * 1024) RGS_CUDA_CHECK(cudaFuncSetAttribute(rgs_norm_planes_kernel<NV, V, Q, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     int per_sm = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, rgs_norm_planes_kernel<NV, V, Q, BWD>, V * 32, (size_t)smem) != cudaSuccess || per_sm < 1) per_sm = 1;
@@ -974,11 +1011,12 @@ static int norm_planes_launch(const NormArgs& a, int* parts, cudaStream_t st) {
 
 template <bool BWD>
 static int norm_planes(const NormArgs& a, int* parts, cudaStream_t st) {
-    if (a.c <= 8) return norm_planes_launch<1, 8, 2, BWD>(a, parts, st);
-    if (a.c <= 16) return norm_planes_launch<2, 8, 2, BWD>(a, parts, st);
-    if (a.c <= 32) return norm_planes_launch<4, 8, 2, BWD>(a, parts, st);
+    // few warps to a pixel: what the sums over the warps cost is what narrow planes cost most
+    if (a.c <= 8) return norm_planes_launch<4, 2, 4, BWD>(a, parts, st);
+    if (a.c <= 16) return norm_planes_launch<8, 2, 2, BWD>(a, parts, st);
+    if (a.c <= 32) return norm_planes_launch<8, 4, 2, BWD>(a, parts, st);
     if (a.c <= 64) return norm_planes_launch<8, 8, 2, BWD>(a, parts, st);
-    if (a.c <= 128) return norm_planes_launch<8, 16, 1, BWD>(a, parts, st);
+    if (a.c <= 128) return norm_planes_launch<16, 8, 1, BWD>(a, parts, st);
     if (a.c <= 256) return norm_planes_launch<16, 16, 1, BWD>(a, parts, st);
     return norm_planes_launch<16, 32, 1, BWD>(a, parts, st);
 }
