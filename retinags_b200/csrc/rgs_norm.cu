@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <atomic>
+#include <type_traits>
 #include "rgs_cuda_common.cuh"
 #include "rgs_field_math.h"
 
@@ -59,28 +60,25 @@ __device__ __forceinline__ void load_vec(const void* p, int64_t i, float (&f)[VE
     }
 }
 // vectors k of a lane, from channel (k lanes + l) VEC - s on, of the row that starts at element i; zero outside the row
-// (edge: the last row, whose last vector may reach behind the tensor)
-template <int VEC, int NV, int LANES, int DT, bool SHIFT>
-__device__ __forceinline__ void load_all(const void* p, int64_t i, int l, int s, int c, bool edge, float (&x)[NV][VEC]) {
-    if (SHIFT && edge) {
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int q = 0; q < VEC; ++q) {
-                const int at = (k * LANES + l) * VEC - s + q;
-                float f[1] = {0.f};
-                if (at >= 0 && at < c) load_vec<1, DT>(p, i + at, f);
-                x[k][q] = f[0];
-            }
-        return;
-    }
+// (EDGE: the last row, whose last vector may reach behind the tensor)
+template <int VEC, int NV, int LANES, int DT, bool SHIFT, bool EDGE>
+__device__ __forceinline__ void load_all(const void* p, int64_t i, int l, int s, int c, float (&x)[NV][VEC]) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int at = (k * LANES + l) * VEC - (SHIFT ? s : 0);
-        if (at < c) load_vec<VEC, DT>(p, i + at, x[k]);
-        else
+        if (EDGE && at < c && at + VEC > c) {
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) {
+                float f[1] = {0.f};
+                if (at + q >= 0 && at + q < c) load_vec<1, DT>(p, i + at + q, f);
+                x[k][q] = f[0];
+            }
+        } else if (at < c) {
+            load_vec<VEC, DT>(p, i + at, x[k]);
+        } else {
 #pragma unroll
             for (int q = 0; q < VEC; ++q) x[k][q] = 0.f;
+        }
     }
     if (SHIFT) {  // the first and the last vector of the row hold elements of its neighbours
 #pragma unroll
@@ -93,10 +91,10 @@ __device__ __forceinline__ void load_all(const void* p, int64_t i, int l, int s,
                 }
     }
 }
-template <int VEC, int NV, int LANES, bool SHIFT>
-__device__ __forceinline__ void load_typed(const void* p, int dtype, int64_t i, int l, int s, int c, bool edge, float (&x)[NV][VEC]) {
-    if (dtype == RGS_BF16) load_all<VEC, NV, LANES, RGS_BF16, SHIFT>(p, i, l, s, c, edge, x);
-    else load_all<VEC, NV, LANES, RGS_F32, SHIFT>(p, i, l, s, c, edge, x);
+template <int VEC, int NV, int LANES, bool SHIFT, bool EDGE>
+__device__ __forceinline__ void load_typed(const void* p, int dtype, int64_t i, int l, int s, int c, float (&x)[NV][VEC]) {
+    if (dtype == RGS_BF16) load_all<VEC, NV, LANES, RGS_BF16, SHIFT, EDGE>(p, i, l, s, c, x);
+    else load_all<VEC, NV, LANES, RGS_F32, SHIFT, EDGE>(p, i, l, s, c, x);
 }
 __device__ __forceinline__ uint32_t pair_bf16(float lo, float hi) {
     uint32_t r;
@@ -293,7 +291,7 @@ __device__ __forceinline__ void block_sums(const NormArgs& a, int l, int s, cons
 // ---------------------------------------------------------------------------------------------------------------------
 // rows
 // ---------------------------------------------------------------------------------------------------------------------
-template <int VEC, int NV, int LANES, bool SHIFT>
+template <int VEC, int NV, int LANES, bool SHIFT, bool EDGE>
 __device__ __forceinline__ void load_row(const NormArgs& a, int64_t i, int l, int s, float (&x)[NV][VEC]) {
     if (!SHIFT && a.src == SRC_CODES) {
         float step[NV];
@@ -311,11 +309,11 @@ __device__ __forceinline__ void load_row(const NormArgs& a, int64_t i, int l, in
                 for (int q = 0; q < VEC; ++q) x[k][q] = 0.f;
         }
     } else {
-        load_typed<VEC, NV, LANES, SHIFT>(a.x, a.src, i * a.ld, l, s, a.c, i == a.n - 1, x);
+        load_typed<VEC, NV, LANES, SHIFT, EDGE>(a.x, a.src, i * a.ld, l, s, a.c, x);
     }
 }
 
-template <int VEC, int NV, int LANES, int R, bool SHIFT, bool PACK>
+template <int VEC, int NV, int LANES, bool SHIFT, bool PACK>
 __global__ void __launch_bounds__(NT, NV * VEC <= 16 ? 4 : NV * VEC <= 24 ? 3 : 2) rgs_norm_rows_fwd_kernel(const __grid_constant__ NormArgs a) {
     constexpr int GROUPS = NT / LANES;
     const int l = threadIdx.x % LANES;
@@ -327,65 +325,61 @@ __global__ void __launch_bounds__(NT, NV * VEC <= 16 ? 4 : NV * VEC <= 24 ? 3 : 
     stage_param<VEC, NV, LANES, SHIFT>(a, a.b, 0.f, params + COPIES * ROW);
     __syncthreads();
     const float *w = params + s * ROW, *b = params + (COPIES + s) * ROW;
-    // all lanes of a warp take the same number of turns: shuffles need them.  A row behind the end is read as zeros.
-    for (int64_t i0 = (int64_t)blockIdx.x * GROUPS; i0 < a.n; i0 += R * stride) {
-        const int64_t i = i0 + threadIdx.x / LANES;
-        float x[R][NV][VEC];
+    // all lanes of a warp take the same number of turns: shuffles need them.  A row that is not there is zeros.
+    auto turn = [&](int64_t row, bool there, auto edge) {
+        float x[NV][VEC];
+        if (there) {
+            load_row<VEC, NV, LANES, SHIFT, decltype(edge)::value>(a, row, l, s, x);
+        } else {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            if (i + r * stride < a.n) {
-                load_row<VEC, NV, LANES, SHIFT>(a, i + r * stride, l, s, x[r]);
-            } else {
+            for (int k = 0; k < NV; ++k)
 #pragma unroll
-                for (int k = 0; k < NV; ++k)
-#pragma unroll
-                    for (int q = 0; q < VEC; ++q) x[r][k][q] = 0.f;
-            }
+                for (int q = 0; q < VEC; ++q) x[k][q] = 0.f;
         }
         __syncwarp();
+        float mu, rstd;
+        row_stats<VEC, NV, LANES, SHIFT>(x, l, s, a.c, a.inv_c, a.eps, mu, rstd);
+        if (PACK) {
+            // a block of 32 channels is 32 / VEC vectors: KB of every lane of the row, or one of some of its lanes
+            constexpr int LB = RGS_PACK_BLOCK / VEC, KB = LANES < LB ? LB / LANES : 1;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int64_t row = i + r * stride;
-            float mu, rstd;
-            row_stats<VEC, NV, LANES, SHIFT>(x[r], l, s, a.c, a.inv_c, a.eps, mu, rstd);
-            if (PACK) {
-                // a block of 32 channels is 32 / VEC vectors: KB of every lane of the row, or one of some of its lanes
-                constexpr int LB = RGS_PACK_BLOCK / VEC, KB = LANES < LB ? LB / LANES : 1;
+            for (int k = 0; k < NV; k += KB) {
+                uint32_t m = 0;
 #pragma unroll
-                for (int k = 0; k < NV; k += KB) {
-                    uint32_t m = 0;
+                for (int e = k; e < k + KB && e < NV; ++e)
 #pragma unroll
-                    for (int e = k; e < k + KB && e < NV; ++e)
+                    for (int q = 0; q < VEC; ++q) m = max(m, __float_as_uint(x[e][q]) & 0x7fffffffu);
+                m = rgs_pack_exponent(__uint_as_float(group_max<(LANES < LB ? LANES : LB)>(m)));
+                if (there)
 #pragma unroll
-                        for (int q = 0; q < VEC; ++q) m = max(m, __float_as_uint(x[r][e][q]) & 0x7fffffffu);
-                    m = rgs_pack_exponent(__uint_as_float(group_max<(LANES < LB ? LANES : LB)>(m)));
-                    if (row < a.n)
-#pragma unroll
-                        for (int e = k; e < k + KB && e < NV; ++e) {
-                            const int c = (e * LANES + l) * VEC;
-                            if (c >= a.c) break;
-                            if (c % RGS_PACK_BLOCK == 0) a.expo_out[row * a.blocks + c / RGS_PACK_BLOCK] = (uint8_t)m;
-                            store_codes<VEC>(a.codes_out, row * a.c + c, x[r][e], m);
-                        }
-                    __syncwarp();
-                }
+                    for (int e = k; e < k + KB && e < NV; ++e) {
+                        const int c = (e * LANES + l) * VEC;
+                        if (c >= a.c) break;
+                        if (c % RGS_PACK_BLOCK == 0) a.expo_out[row * a.blocks + c / RGS_PACK_BLOCK] = (uint8_t)m;
+                        store_codes<VEC>(a.codes_out, row * a.c + c, x[e], m);
+                    }
+                __syncwarp();
             }
-#pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                float wk[VEC], bk[VEC];
-                load_param<VEC>(w, (k * LANES + l) * VEC, wk);
-                load_param<VEC>(b, (k * LANES + l) * VEC, bk);
-#pragma unroll
-                for (int q = 0; q < VEC; ++q) x[r][k][q] = fmaf((x[r][k][q] - mu) * rstd, wk[q], bk[q]);
-            }
-            if (row < a.n) store_typed<VEC, NV, LANES, SHIFT>(a.y, a.y_dtype, row * a.c, l, s, a.c, x[r]);
-            __syncwarp();
         }
-    }
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            float wk[VEC], bk[VEC];
+            load_param<VEC>(w, (k * LANES + l) * VEC, wk);
+            load_param<VEC>(b, (k * LANES + l) * VEC, bk);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) x[k][q] = fmaf((x[k][q] - mu) * rstd, wk[q], bk[q]);
+        }
+        if (there) store_typed<VEC, NV, LANES, SHIFT>(a.y, a.y_dtype, row * a.c, l, s, a.c, x);
+        __syncwarp();
+    };
+    const int64_t rows = SHIFT ? a.n - 1 : a.n;
+    for (int64_t i = (int64_t)blockIdx.x * GROUPS; i < rows; i += stride) turn(i + threadIdx.x / LANES, i + threadIdx.x / LANES < rows, std::false_type());
+    // the last row by itself: its last vector may reach behind the tensor (a group of the first block with its shift)
+    if (SHIFT && blockIdx.x == 0) turn(rows, threadIdx.x / LANES == (rows & 3), std::true_type());
 }
 
-template <int VEC, int NV, int LANES, int R, bool SHIFT>
-__global__ void __launch_bounds__(NT, NV * VEC <= 12 ? 3 : NV * VEC <= 16 ? 2 : 1) rgs_norm_rows_bwd_kernel(const __grid_constant__ NormArgs a) {
+template <int VEC, int NV, int LANES, bool SHIFT>
+__global__ void __launch_bounds__(NT, NV * VEC <= 12 ? 3 : NV * VEC <= 24 ? 2 : 1) rgs_norm_rows_bwd_kernel(const __grid_constant__ NormArgs a) {
     constexpr int GROUPS = NT / LANES;
     constexpr int ROW = NV * LANES * VEC, COPIES = SHIFT ? 4 : 1, SUMS = NT * VEC + (SHIFT ? 3 * GROUPS : 0);
     __shared__ __align__(16) float sh[COPIES * ROW > SUMS ? COPIES * ROW : SUMS];
@@ -400,31 +394,26 @@ __global__ void __launch_bounds__(NT, NV * VEC <= 12 ? 3 : NV * VEC <= 16 ? 2 : 
     for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int q = 0; q < VEC; ++q) sw[k][q] = sb[k][q] = 0.f;
-    for (int64_t i0 = (int64_t)blockIdx.x * GROUPS; i0 < a.n; i0 += R * stride) {
-        const int64_t i = i0 + threadIdx.x / LANES;
-        float x[R][NV][VEC], g[R][NV][VEC];
+    auto turn = [&](int64_t row, bool there, auto edge) {
+        float x[NV][VEC], g[NV][VEC];
+        if (there) {
+            load_row<VEC, NV, LANES, SHIFT, decltype(edge)::value>(a, row, l, s, x);
+            load_typed<VEC, NV, LANES, SHIFT, decltype(edge)::value>(a.dy, a.dy_dtype, row * a.ldy, l, s, a.c, g);
+        } else {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            if (i + r * stride < a.n) {
-                load_row<VEC, NV, LANES, SHIFT>(a, i + r * stride, l, s, x[r]);
-                load_typed<VEC, NV, LANES, SHIFT>(a.dy, a.dy_dtype, (i + r * stride) * a.ldy, l, s, a.c, i + r * stride == a.n - 1, g[r]);
-            } else {
+            for (int k = 0; k < NV; ++k)
 #pragma unroll
-                for (int k = 0; k < NV; ++k)
-#pragma unroll
-                    for (int q = 0; q < VEC; ++q) x[r][k][q] = g[r][k][q] = 0.f;
-            }
+                for (int q = 0; q < VEC; ++q) x[k][q] = g[k][q] = 0.f;
         }
         __syncwarp();
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int64_t row = i + r * stride;
-            // (a row behind the end is zeros, and adds none to the sums: with eps = 0 its rstd would be infinite)
-            row_bwd<VEC, NV, LANES, SHIFT>(x[r], g[r], w, sw, sb, l, s, a.c, a.inv_c, row < a.n ? a.eps : 1.f);
-            if (a.dx && row < a.n) store_typed<VEC, NV, LANES, SHIFT>(a.dx, a.dx_dtype, row * a.c, l, s, a.c, x[r]);
-            __syncwarp();
-        }
-    }
+        // (a row that is not there adds none to the sums: with eps = 0 its rstd would be infinite)
+        row_bwd<VEC, NV, LANES, SHIFT>(x, g, w, sw, sb, l, s, a.c, a.inv_c, there ? a.eps : 1.f);
+        if (a.dx && there) store_typed<VEC, NV, LANES, SHIFT>(a.dx, a.dx_dtype, row * a.c, l, s, a.c, x);
+        __syncwarp();
+    };
+    const int64_t rows = SHIFT ? a.n - 1 : a.n;
+    for (int64_t i = (int64_t)blockIdx.x * GROUPS; i < rows; i += stride) turn(i + threadIdx.x / LANES, i + threadIdx.x / LANES < rows, std::false_type());
+    if (SHIFT && blockIdx.x == 0) turn(rows, threadIdx.x / LANES == (rows & 3), std::true_type());
     if (a.part) block_sums<VEC, NV, LANES, SHIFT>(a, l, s, sw, sb, sh);
 }
 
@@ -943,24 +932,24 @@ static int64_t norm_resident(K kernel, int smem) {
 }
 static inline int64_t at_most(int64_t want, int64_t most) { return want < 1 ? 1 : (want > most ? most : want); }
 
-template <int VEC, int NV, int LANES, int R, bool SHIFT>
+template <int VEC, int NV, int LANES, bool SHIFT>
 static int norm_rows_launch(const NormArgs& a, bool backward, cudaStream_t st) {
-    const int64_t want = (a.n + (NT / LANES) * R - 1) / ((NT / LANES) * R);
+    const int64_t want = (a.n + NT / LANES - 1) / (NT / LANES);
     if (backward) {
         static std::atomic<int64_t> most{0};
-        if (!most) most = norm_resident(rgs_norm_rows_bwd_kernel<VEC, NV, LANES, R, SHIFT>, 0);
+        if (!most) most = norm_resident(rgs_norm_rows_bwd_kernel<VEC, NV, LANES, SHIFT>, 0);
         // a few rows: one block, no partial sums, one launch
         const int64_t grid = want <= 4 ? 1 : at_most(at_most(want, most), NORM_PARTS);
-        rgs_norm_rows_bwd_kernel<VEC, NV, LANES, R, SHIFT><<<(unsigned)grid, NT, 0, st>>>(a);
+        rgs_norm_rows_bwd_kernel<VEC, NV, LANES, SHIFT><<<(unsigned)grid, NT, 0, st>>>(a);
         return (int)grid;
     }
     static std::atomic<int64_t> most[2];
     const int pack = !SHIFT && a.codes_out != nullptr;
     if (!most[pack])
-        most[pack] = pack ? norm_resident(rgs_norm_rows_fwd_kernel<VEC, NV, LANES, R, SHIFT, !SHIFT>, 0) : norm_resident(rgs_norm_rows_fwd_kernel<VEC, NV, LANES, R, SHIFT, false>, 0);
+        most[pack] = pack ? norm_resident(rgs_norm_rows_fwd_kernel<VEC, NV, LANES, SHIFT, !SHIFT>, 0) : norm_resident(rgs_norm_rows_fwd_kernel<VEC, NV, LANES, SHIFT, false>, 0);
     const unsigned grid = (unsigned)at_most(want, most[pack]);
-    if (pack) rgs_norm_rows_fwd_kernel<VEC, NV, LANES, R, SHIFT, !SHIFT><<<grid, NT, 0, st>>>(a);
-    else rgs_norm_rows_fwd_kernel<VEC, NV, LANES, R, SHIFT, false><<<grid, NT, 0, st>>>(a);
+    if (pack) rgs_norm_rows_fwd_kernel<VEC, NV, LANES, SHIFT, !SHIFT><<<grid, NT, 0, st>>>(a);
+    else rgs_norm_rows_fwd_kernel<VEC, NV, LANES, SHIFT, false><<<grid, NT, 0, st>>>(a);
     return 0;
 }
 
@@ -969,33 +958,35 @@ static int norm_rows_launch(const NormArgs& a, bool backward, cudaStream_t st) {
 template <bool SHIFT>
 static int norm_rows_vec(const NormArgs& a, bool backward, cudaStream_t st) {
     const int u = (a.c + (SHIFT ? 6 : 0)) / 4;  // vectors of a row
-    if (u <= 3) return norm_rows_launch<4, 3, 1, 1, SHIFT>(a, backward, st);
-    if (u <= 4) return norm_rows_launch<4, 4, 1, 1, SHIFT>(a, backward, st);
-    if (u <= 6) return norm_rows_launch<4, 3, 2, 1, SHIFT>(a, backward, st);
-    if (u <= 8) return norm_rows_launch<4, 4, 2, 1, SHIFT>(a, backward, st);
-    if (u <= 12) return norm_rows_launch<4, 3, 4, 1, SHIFT>(a, backward, st);
-    if (u <= 16) return norm_rows_launch<4, 4, 4, 1, SHIFT>(a, backward, st);
-    if (u <= 24) return norm_rows_launch<4, 3, 8, 1, SHIFT>(a, backward, st);
-    if (u <= 32) return norm_rows_launch<4, 4, 8, 1, SHIFT>(a, backward, st);
-    if (u <= 48) return norm_rows_launch<4, 3, 16, 1, SHIFT>(a, backward, st);
-    if (u <= 64) return norm_rows_launch<4, 4, 16, 1, SHIFT>(a, backward, st);
-    if (u <= 96) return norm_rows_launch<4, 3, 32, 1, SHIFT>(a, backward, st);
-    if (u <= 128) return norm_rows_launch<4, 4, 32, 1, SHIFT>(a, backward, st);
-    if (u <= 192) return norm_rows_launch<4, 6, 32, 1, SHIFT>(a, backward, st);
-    return norm_rows_launch<4, 8, 32, 1, SHIFT>(a, backward, st);
+    if (u <= 3) return norm_rows_launch<4, 3, 1, SHIFT>(a, backward, st);
+    if (u <= 4) return norm_rows_launch<4, 4, 1, SHIFT>(a, backward, st);
+    if (u <= 6) return norm_rows_launch<4, 3, 2, SHIFT>(a, backward, st);
+    if (u <= 8) return norm_rows_launch<4, 4, 2, SHIFT>(a, backward, st);
+    if (u <= 12) return norm_rows_launch<4, 3, 4, SHIFT>(a, backward, st);
+    if (u <= 16) return norm_rows_launch<4, 4, 4, SHIFT>(a, backward, st);
+    if (u <= 24) return norm_rows_launch<4, 3, 8, SHIFT>(a, backward, st);
+    if (u <= 32) return norm_rows_launch<4, 4, 8, SHIFT>(a, backward, st);
+    if (u <= 48) return norm_rows_launch<4, 3, 16, SHIFT>(a, backward, st);
+    if (u <= 64) return norm_rows_launch<4, 4, 16, SHIFT>(a, backward, st);
+    if (u <= 96) return norm_rows_launch<4, 3, 32, SHIFT>(a, backward, st);
+    if (u <= 128) return norm_rows_launch<4, 4, 32, SHIFT>(a, backward, st);
+    if (u <= 160) return norm_rows_launch<4, 5, 32, SHIFT>(a, backward, st);
+    if (u <= 192) return norm_rows_launch<4, 6, 32, SHIFT>(a, backward, st);
+    if (u <= 224) return norm_rows_launch<4, 7, 32, SHIFT>(a, backward, st);
+    return norm_rows_launch<4, 8, 32, SHIFT>(a, backward, st);
 }
 // element by element: rows apart by a stride that four does not divide, codes of an odd width
 static int norm_rows_single(const NormArgs& a, bool backward, cudaStream_t st) {
     const int u = a.c;
-    if (u <= 8) return norm_rows_launch<1, 8, 1, 1, false>(a, backward, st);
-    if (u <= 16) return norm_rows_launch<1, 8, 2, 1, false>(a, backward, st);
-    if (u <= 32) return norm_rows_launch<1, 8, 4, 1, false>(a, backward, st);
-    if (u <= 64) return norm_rows_launch<1, 8, 8, 1, false>(a, backward, st);
-    if (u <= 128) return norm_rows_launch<1, 8, 16, 1, false>(a, backward, st);
-    if (u <= 256) return norm_rows_launch<1, 8, 32, 1, false>(a, backward, st);
-    if (u <= 512) return norm_rows_launch<1, 16, 32, 1, false>(a, backward, st);
-    if (u <= 768) return norm_rows_launch<1, 24, 32, 1, false>(a, backward, st);
-    return norm_rows_launch<1, 32, 32, 1, false>(a, backward, st);
+    if (u <= 8) return norm_rows_launch<1, 8, 1, false>(a, backward, st);
+    if (u <= 16) return norm_rows_launch<1, 8, 2, false>(a, backward, st);
+    if (u <= 32) return norm_rows_launch<1, 8, 4, false>(a, backward, st);
+    if (u <= 64) return norm_rows_launch<1, 8, 8, false>(a, backward, st);
+    if (u <= 128) return norm_rows_launch<1, 8, 16, false>(a, backward, st);
+    if (u <= 256) return norm_rows_launch<1, 8, 32, false>(a, backward, st);
+    if (u <= 512) return norm_rows_launch<1, 16, 32, false>(a, backward, st);
+    if (u <= 768) return norm_rows_launch<1, 24, 32, false>(a, backward, st);
+    return norm_rows_launch<1, 32, 32, false>(a, backward, st);
 }
 
 template <int NV, int V, int Q, bool BWD>

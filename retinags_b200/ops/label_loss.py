@@ -32,7 +32,7 @@ class _LabelLoss(torch.autograd.Function):
         dev = features.device
         x, ldx, _ = as_rows(features, "label_loss", planes_ok=False)
         w, ldw, _ = as_rows(weight, "label_loss", planes_ok=False)
-        y = labels.reshape(-1).contiguous()
+        y = labels if labels.dim() == 1 and labels.is_contiguous() else labels.reshape(-1).contiguous()
         n, c = x.shape
         v = w.shape[0]
         per_row = reduction == "none"
@@ -46,27 +46,34 @@ class _LabelLoss(torch.autograd.Function):
             native.call("label_fwd", dev, x, ldx, w, ldw, bias, y, y.element_size(), n, c, v, DTYPES[x.dtype], b_code,
                         int(reduction == "mean"), _scratch(x, ldx, w, ldw, 0), lse, losses, result, count)
         ctx.save_for_backward(x, w, bias, y, lse, count)
-        ctx.args = (tuple(features.shape), tuple(weight.shape), ldx, ldw, b_code, reduction)
+        ctx.args = (features.shape, weight.shape, ldx, ldw, b_code, reduction)
         return losses.view(features.shape[:-1]) if per_row else result
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gout):
-        x, w, bias, y, lse, count = ctx.saved_tensors
-        x_shape, w_shape, ldx, ldw, b_code, reduction = ctx.args
-        dev = x.device
-        n, c = x.shape
-        v = w.shape[0]
-        g = gout.reshape(-1).contiguous()
-        new = torch.empty if n else torch.zeros
-        dx = torch.empty(x_shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
-        dw = new(w_shape, dtype=w.dtype, device=dev) if ctx.needs_input_grad[1] else None
-        db = new(v, dtype=bias.dtype, device=dev) if ctx.needs_input_grad[2] else None
-        if n and (dx is not None or dw is not None or db is not None):
-            native.call("label_bwd", dev, x, ldx, w, ldw, bias, y, y.element_size(), n, c, v, DTYPES[x.dtype], b_code, lse, g,
-                        int(reduction == "none"), int(reduction == "mean"), count,
-                        _scratch(x, ldx, w, ldw, 1), dx, dw, db)
-        return dx, dw, db, None, None
+        # (the wrapper that refuses a second derivative costs as much as a launch: only where one is being recorded)
+        return _label_backward_once(ctx, gout) if torch.is_grad_enabled() else _label_backward(ctx, gout)
+
+
+def _label_backward(ctx, gout):
+    x, w, bias, y, lse, count = ctx.saved_tensors
+    x_shape, w_shape, ldx, ldw, b_code, reduction = ctx.args
+    dev = x.device
+    n, c = x.shape
+    v = w.shape[0]
+    g = gout if gout.dim() < 2 and gout.is_contiguous() else gout.reshape(-1).contiguous()
+    new = torch.empty if n else torch.zeros
+    dx = torch.empty(x_shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
+    dw = new(w_shape, dtype=w.dtype, device=dev) if ctx.needs_input_grad[1] else None
+    db = new(v, dtype=bias.dtype, device=dev) if ctx.needs_input_grad[2] else None
+    if n and (dx is not None or dw is not None or db is not None):
+        native.call("label_bwd", dev, x, ldx, w, ldw, bias, y, y.element_size(), n, c, v, DTYPES[x.dtype], b_code, lse, g,
+                    int(reduction == "none"), int(reduction == "mean"), count,
+                    _scratch(x, ldx, w, ldw, 1), dx, dw, db)
+    return dx, dw, db, None, None
+
+
+_label_backward_once = torch.autograd.function.once_differentiable(_label_backward)
 
 
 def label_loss(features: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, bias: torch.Tensor | None = None,
@@ -106,7 +113,8 @@ def label_loss(features: torch.Tensor, weight: torch.Tensor, labels: torch.Tenso
             raise ValueError(f"label_loss: bias of shape ({v},) expected, got {tuple(bias.shape)}")
         if DTYPES.get(bias.dtype, -1) not in (0, code):
             raise TypeError(f"label_loss: bias of type {features.dtype} or float32 expected, got {bias.dtype}")
+    device = features.device
     for name, t in (("weight", weight), ("labels", labels), ("bias", bias)):
-        if t is not None and t.device != features.device:
+        if t is not None and t.device != device:
             raise ValueError(f"label_loss: {name} on {features.device} expected, got {t.device}")
     return _LabelLoss.apply(features, weight, bias.contiguous() if bias is not None else None, labels, reduction)

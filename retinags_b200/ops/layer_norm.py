@@ -24,42 +24,51 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, out_dtype, keep):
         flat, ld, planes = as_rows(x, "layer_norm")
-        out_planes = planes
-        if planes and flat.shape[1] > MAX_PLANES:
-            flat = flat.contiguous()
-            ld, planes = flat.shape[1], 0
         n, c = flat.shape
-        y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+        out_planes = planes
+        if planes and c > MAX_PLANES:
+            flat = flat.contiguous()
+            ld, planes = c, 0
+        dev = x.device
+        y = torch.empty(x.shape, dtype=out_dtype, device=dev)
         p_code = DTYPES[weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32]
         codes = exponents = None
         # bias alone needs no input in the backward pass
         if keep == "int8" and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]):
-            codes, exponents = alloc_codes(x.shape, planes, x.device)
+            codes, exponents = alloc_codes(x.shape, planes, dev)
         if n:
-            native.call("norm_fwd", x.device, flat, DTYPES[x.dtype], ld, planes, weight, bias, p_code, n, c, eps, y, DTYPES[out_dtype],
+            native.call("norm_fwd", dev, flat, DTYPES[x.dtype], ld, planes, weight, bias, p_code, n, c, eps, y, DTYPES[out_dtype],
                         codes, exponents)
         ctx.save_for_backward(flat if codes is None else None, codes, exponents, weight)
-        ctx.layout = (tuple(x.shape), x.dtype, ld, planes, out_planes, n, c, p_code, eps)
-        ctx.param_dtypes = (weight.dtype if weight is not None else None, bias.dtype if bias is not None else None)
+        ctx.layout = (x.shape, x.dtype, ld, planes, out_planes, n, c, p_code, eps, weight.dtype if weight is not None else None,
+                      bias.dtype if bias is not None else None)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        flat, codes, exponents, weight = ctx.saved_tensors
-        shape, x_dtype, ld, planes, out_planes, n, c, p_code, eps = ctx.layout
-        dev = dy.device
-        dyf, ldy, _ = as_rows(dy, "layer_norm", planes_ok=False)
-        dx = empty_like_layout(shape, planes, x_dtype, dev) if ctx.needs_input_grad[0] else None
-        new = torch.empty if n else torch.zeros
-        dw = new(c, dtype=ctx.param_dtypes[0], device=dev) if ctx.needs_input_grad[1] else None
-        db = new(c, dtype=ctx.param_dtypes[1], device=dev) if ctx.needs_input_grad[2] else None
-        if n:
-            native.call("norm_bwd", dev, flat, DTYPES[x_dtype], ld, planes, codes, exponents, dyf, DTYPES[dyf.dtype], ldy, weight, p_code,
-                        n, c, eps, _scratch(dev, n, c), dx, dw, db)
-        if dx is not None and out_planes != planes:
-            dx = empty_like_layout(shape, out_planes, x_dtype, dev).copy_(dx)
-        return dx, dw, db, None, None, None
+        # (the wrapper that refuses a second derivative costs as much as a launch: only where one is being recorded)
+        return _norm_backward_once(ctx, dy) if torch.is_grad_enabled() else _norm_backward(ctx, dy)
+
+
+def _norm_backward(ctx, dy):
+    flat, codes, exponents, weight = ctx.saved_tensors
+    shape, x_dtype, ld, planes, out_planes, n, c, p_code, eps, w_dtype, b_dtype = ctx.layout
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    dev = dy.device
+    dyf, ldy, _ = as_rows(dy, "layer_norm", planes_ok=False)
+    dx = empty_like_layout(shape, planes, x_dtype, dev) if need_x else None
+    new = torch.empty if n else torch.zeros
+    dw = new(c, dtype=w_dtype, device=dev) if need_w else None
+    db = new(c, dtype=b_dtype, device=dev) if need_b else None
+    if n:
+        native.call("norm_bwd", dev, flat, DTYPES[x_dtype], ld, planes, codes, exponents, dyf, DTYPES[dyf.dtype], ldy, weight, p_code,
+                    n, c, eps, _scratch(dev, n, c), dx, dw, db)
+    if dx is not None and out_planes != planes:
+        dx = empty_like_layout(shape, out_planes, x_dtype, dev).copy_(dx)
+    return dx, dw, db, None, None, None
+
+
+_norm_backward_once = torch.autograd.function.once_differentiable(_norm_backward)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
@@ -75,22 +84,27 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype not in DTYPES:
         raise TypeError(f"layer_norm: out_dtype float32 or bfloat16 expected, got {out_dtype}")
-    if keep not in ("input", "int8"):
+    if keep != "input" and keep != "int8":
         raise ValueError(f"layer_norm: keep is 'input' or 'int8', got {keep!r}")
     if not eps >= 0.0:
         raise ValueError(f"layer_norm: eps >= 0 expected, got {eps}")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"layer_norm: shape (..., C) with at least one channel expected, got {tuple(x.shape)}")
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            continue
-        dtype_code(p, f"layer_norm {name}")
-        if p.shape != (x.shape[-1],):
-            raise ValueError(f"layer_norm: {name} of shape ({x.shape[-1]},) expected, got {tuple(p.shape)}")
-        if p.device != x.device:
-            raise ValueError(f"layer_norm: {name} on {x.device} expected, got {p.device}")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError(f"layer_norm: weight and bias of one type expected, got {weight.dtype} and {bias.dtype}")
-    weight = weight.contiguous() if weight is not None else None
-    bias = bias.contiguous() if bias is not None else None
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"layer_norm: shape (..., C) with at least one channel expected, got {tuple(shape)}")
+    if weight is not None:
+        weight = _param(x, weight, shape[-1], "weight")
+    if bias is not None:
+        bias = _param(x, bias, shape[-1], "bias")
+        if weight is not None and weight.dtype != bias.dtype:
+            raise TypeError(f"layer_norm: weight and bias of one type expected, got {weight.dtype} and {bias.dtype}")
     return _LayerNorm.apply(x, weight, bias, float(eps), out_dtype, keep)
+
+
+def _param(x: torch.Tensor, p: torch.Tensor, c: int, name: str) -> torch.Tensor:
+    if p.dtype not in DTYPES:
+        raise TypeError(f"layer_norm {name}: float32 or bfloat16 expected, got {p.dtype}")
+    if p.dim() != 1 or p.shape[0] != c:
+        raise ValueError(f"layer_norm: {name} of shape ({c},) expected, got {tuple(p.shape)}")
+    if p.device != x.device:
+        raise ValueError(f"layer_norm: {name} on {x.device} expected, got {p.device}")
+    return p if p.is_contiguous() else p.contiguous()
