@@ -14,6 +14,13 @@
 // dX and dW in one launch.  For dW the roles are swapped (rows of A are labels, columns are pixels); the scores are
 // computed anew there: five products of 2NVC operations in all against four with scores kept, and no N x V traffic.
 //
+// What depends on a row alone rides along in the product: sixteen extra channels hold (b in three bf16 pieces, 1, 1, 1) of a
+// label and (1, 1, 1, -lse in three pieces) of a pixel, so S is the score with its bias and, backward, minus lse: the
+// warpgroups need nothing per column but the labels of dW (constants per column read from shared memory cost as much of its
+// bandwidth as half of the products' operands).  Columns behind the last label and pixels without one have -inf there.
+// Where scores are so large that log z would vanish beside m (a mask of the type's lowest value over all labels), -m alone
+// rides along and 1/z is multiplied; the same factor serves gradients that differ from pixel to pixel.
+//
 // 32-bit inputs: every operand is split into three bf16 pieces (8 + 8 + 8 bits of mantissa) and six of the nine piece
 // products are kept; what is dropped is below 2^-24 of a product.  G is split the same way in registers.
 //
@@ -30,14 +37,18 @@
 #include "rgs_field_math.h"
 
 #define LT 128                      // rows of a tile of either matrix
-#define LROOM (13 * 16384)          // bytes of staged tiles: 128 rows x 64 (or 32) channels bf16 each
+#define LROOM (25 * 8192)           // bytes of staged tiles: 128 rows x 64 (or 32) channels bf16 each
 #define LSTAGES 13                  // most stages of the ring
-#define LKSLOTS 4                   // staged blocks of column constants
-#define LKBYTES 2048
+#define LE 4096                     // bytes of a tile of the extra channels, 128 x 16 bf16
+#define LESLOTS 3                   // such tiles of B (of A there are two)
+#define LKSLOTS 3                   // staged blocks of what dW needs of 128 pixels: label, g, factor
+#define LKBYTES (3 * LT * 4)
 #define LTHREADS 576                // warp 0 TMA, warp 1 MMA, warps 2-17 four warpgroups on the scores
 #define LWAIT (1u << 20)
 #define LOG2E 1.4426950408889634f
-#define LN2 0.6931471805599453f
+
+enum { LF_DIRTY = 1,   // a pixel without a label holds something that is not finite
+       LF_LARGE = 2 }; // a largest score above 2^10: m and log z are not added up
 
 struct LabelArgs {
     int64_t n, v;
@@ -50,11 +61,12 @@ struct LabelArgs {
     int nsx, nsw;                    // pieces of the walk over labels (forward, dX) and over pixels (dW)
     int perx, restx, perw, restw;    // tiles of a piece: per, one more in the first rest pieces
     unsigned items_x, items_w;
-    const float* b2;                 // (nmw * 128) bias * log2 e; -inf behind the last label
-    const float* kn;                 // (nmx, 4, 128) per pixel: -m * log2 e, g / z, g, label (bits); backward only
-    const float* lse;                // (2, n) m and log z, both in units of log 2
+    const float* kn;                 // (nmx, 3, 128) per pixel: label (bits; -1: none), g, factor; backward only
+    const float* lse;                // (2, n) m and log z
+    const float* gs;                 // g of all pixels where they share it
+    int per_row;                     // a gradient to a pixel
     const void* labels; int label_bytes;
-    const float* flags;              // [1] != 0: a pixel without a label holds something that is not finite
+    const float* flags;              // [1]: LF_ bits
     float* pm; float* ps; float* at; // forward: (4 nsx, n) partial maximum and sum, (n) score of the label
     float* part_x; float* part_w;    // (nsx, nmx*128, cq), (nsw, nmw*128, cq) when split
     float* part_b;                   // (4 nsw, nmw*128)
@@ -106,11 +118,11 @@ __device__ __forceinline__ void lb_tma(void* dst, const CUtensorMap* map, int x,
 __device__ __forceinline__ void lb_commit(unsigned long long* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(rgs_smem_addr(bar)) : "memory");
 }
-// Shared-memory descriptors: rows of KC channels under the swizzle of their length (128 or 64 bytes), eight rows to a
+// Shared-memory descriptors: rows of KC channels under the swizzle of their length (128, 64 or 32 bytes), eight rows to a
 // pattern; both strides are that of the pattern, so a tile reads as K-major rows or as steps of K.  The low word holds the
 // address (in 16 bytes), the high word never changes: the products below take the low words alone.
 template <int KC> constexpr uint32_t lb_desc_lo = (uint32_t)KC << 16;
-template <int KC> constexpr uint32_t lb_desc_hi = (uint32_t)KC | (1u << 14) | ((KC == 64 ? 2u : 4u) << 29);
+template <int KC> constexpr uint32_t lb_desc_hi = (uint32_t)KC | (1u << 14) | ((KC == 64 ? 2u : KC == 32 ? 4u : 6u) << 29);
 
 template <int KC>
 __device__ __forceinline__ void lb_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
@@ -227,14 +239,17 @@ __device__ __forceinline__ void lb_store16(void* out, int64_t r, int c, int chan
 
 struct LabelShared {
     unsigned long long full[LSTAGES], empty[LSTAGES], a_full[2], a_empty[2], k_full[LKSLOTS], k_empty[LKSLOTS];
+    unsigned long long ea_full[2], ea_empty[2], e_full[LESLOTS], e_empty[LESLOTS];
     unsigned long long s_full[4], s_done[4], o_full[2], o_free[2], drain;
     uint32_t tmem;
     int fail;
 };
-#define LSMEM (1024 + LROOM + LKSLOTS * LKBYTES + (int)sizeof(LabelShared))
+#define LSMEM (1024 + LROOM + (2 + LESLOTS) * LE + LKSLOTS * LKBYTES + (int)sizeof(LabelShared))
+static_assert(LSMEM <= 232448, "shared memory of an SM");
 
 template <int P, bool GRAD, int KC, int CS>
 __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                                                                   const __grid_constant__ CUtensorMap map_ex, const __grid_constant__ CUtensorMap map_ew,
                                                                    const __grid_constant__ LabelArgs a) {
     constexpr int SB = GRAD && P == 3 ? 192 : 128;  // TMEM columns of a score buffer (scores; over them G, its third piece behind)
     // 32-bit outputs are summed in two buffers: the leading products, eight steps to a tile, and the small ones.  The tensor
@@ -247,8 +262,9 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
     constexpr int TB = KC * 2 * LT;               // bytes of a staged tile
     extern __shared__ unsigned char raw[];
     unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    float* kbuf = reinterpret_cast<float*>(tiles + LROOM);
-    LabelShared* sh = reinterpret_cast<LabelShared*>(tiles + LROOM + LKSLOTS * LKBYTES);
+    unsigned char *ea_tiles = tiles + LROOM, *e_tiles = ea_tiles + 2 * LE;
+    float* kbuf = reinterpret_cast<float*>(e_tiles + LESLOTS * LE);
+    LabelShared* sh = reinterpret_cast<LabelShared*>(e_tiles + LESLOTS * LE + LKSLOTS * LKBYTES);
     volatile int* fail = &sh->fail;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t na = P * a.nk;                 // tiles of one block of 128 rows, chunk by chunk, its pieces together
@@ -261,10 +277,12 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             for (int i = 0; i < LSTAGES; ++i) { rgs_mbar_init(&sh->full[i], 1); rgs_mbar_init(&sh->empty[i], 1); }
             for (int i = 0; i < 2; ++i) {
                 rgs_mbar_init(&sh->a_full[i], 1); rgs_mbar_init(&sh->a_empty[i], 1);
+                rgs_mbar_init(&sh->ea_full[i], 1); rgs_mbar_init(&sh->ea_empty[i], 1);
                 rgs_mbar_init(&sh->o_full[i], 1); rgs_mbar_init(&sh->o_free[i], 512);
             }
             for (int i = 0; i < 4; ++i) { rgs_mbar_init(&sh->s_full[i], 1); rgs_mbar_init(&sh->s_done[i], 256); }
             for (int i = 0; i < LKSLOTS; ++i) { rgs_mbar_init(&sh->k_full[i], 1); rgs_mbar_init(&sh->k_empty[i], 256); }
+            for (int i = 0; i < LESLOTS; ++i) { rgs_mbar_init(&sh->e_full[i], 1); rgs_mbar_init(&sh->e_empty[i], 1); }
             rgs_mbar_init(&sh->drain, 1);
             sh->fail = 0;
             rgs_fence_mbar_init();
@@ -282,8 +300,8 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
     if (warp == 0) {
         // ------------------------------------------------------------------------------------------------ TMA
         const bool lead = lb_elect();
-        LabelCursor rc, ac, kc;
-        uint32_t loads = 0;
+        LabelCursor rc, ac, kc, eac, ec;
+        uint32_t loads = 0, labels = 0;
         bool ok = true;
         auto load = [&](const CUtensorMap* map, int k, int row) {
             ok = ok && lb_wait_warp(&sh->empty[rc.slot], rc.phase ^ 1, fail);
@@ -308,6 +326,14 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         for (unsigned i = blockIdx.x; i < items && ok; i += gridDim.x) {
             const LabelItem it = lb_item(a, i);
             const CUtensorMap *ma = it.dw ? &map_w : &map_x, *mb = it.dw ? &map_x : &map_w;
+            // (forward: the pixels' extra channels are the same for all, one tile of them)
+            ok = lb_wait_warp(&sh->ea_empty[eac.slot], eac.phase ^ 1, fail);
+            if (!ok) break;
+            if (lead) {
+                rgs_mbar_expect_tx(&sh->ea_full[eac.slot], LE);
+                lb_tma(ea_tiles + eac.slot * LE, it.dw ? &map_ew : &map_ex, 0, GRAD ? it.m * LT : 0, 0, &sh->ea_full[eac.slot]);
+            }
+            eac.next(2);
             if (a.a_slots) {
                 ok = lb_wait_warp(&sh->a_empty[ac.slot], ac.phase ^ 1, fail);
                 if (!ok) break;
@@ -321,14 +347,23 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 ac.next(a.a_slots);
             }
             for (int j = it.j0; j < it.j1 && ok; ++j) {
-                ok = lb_wait_warp(&sh->k_empty[kc.slot], kc.phase ^ 1, fail);
+                ok = lb_wait_warp(&sh->e_empty[ec.slot], ec.phase ^ 1, fail);
                 if (!ok) break;
                 if (lead) {
-                    const uint32_t bytes = it.dw ? LT * 16 : LT * 4;
-                    rgs_mbar_expect_tx(&sh->k_full[kc.slot], bytes);
-                    rgs_bulk_g2s(kbuf + kc.slot * (LKBYTES / 4), it.dw ? a.kn + (size_t)j * (LT * 4) : a.b2 + (size_t)j * LT, bytes, &sh->k_full[kc.slot]);
+                    rgs_mbar_expect_tx(&sh->e_full[ec.slot], LE);
+                    lb_tma(e_tiles + ec.slot * LE, it.dw ? &map_ex : &map_ew, 0, j * LT, 0, &sh->e_full[ec.slot]);
                 }
-                kc.next(LKSLOTS);
+                ec.next(LESLOTS);
+                if (GRAD && it.dw) {
+                    ok = lb_wait_warp(&sh->k_empty[kc.slot], kc.phase ^ 1, fail);
+                    if (!ok) break;
+                    if (lead) {
+                        rgs_mbar_expect_tx(&sh->k_full[kc.slot], LKBYTES);
+                        rgs_bulk_g2s(kbuf + kc.slot * (LKBYTES / 4), a.kn + (size_t)j * (3 * LT), LKBYTES, &sh->k_full[kc.slot]);
+                    }
+                    kc.next(LKSLOTS);
+                    ++labels;
+                }
                 for (int k = 0; k < nst && ok; ++k) {
                     if (!a.a_slots) load(ma, k, it.m);
                     load(mb, k, j);
@@ -345,10 +380,20 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 --rc.slot;
                 rgs_mbar_wait(&sh->full[rc.slot], rc.phase, 1u << 12);
             }
-            for (int k = 0; k < LKSLOTS; ++k) {
+            for (uint32_t k = 0; k < LKSLOTS && k < labels; ++k) {
                 if (kc.slot == 0) { kc.slot = LKSLOTS; kc.phase ^= 1; }
                 --kc.slot;
                 rgs_mbar_wait(&sh->k_full[kc.slot], kc.phase, 1u << 12);
+            }
+            for (uint32_t k = 0; k < LESLOTS; ++k) {
+                if (ec.slot == 0) { ec.slot = LESLOTS; ec.phase ^= 1; }
+                --ec.slot;
+                rgs_mbar_wait(&sh->e_full[ec.slot], ec.phase, 1u << 12);
+            }
+            for (int k = 0; k < 2; ++k) {
+                if (eac.slot == 0) { eac.slot = 2; eac.phase ^= 1; }
+                --eac.slot;
+                rgs_mbar_wait(&sh->ea_full[eac.slot], eac.phase, 1u << 12);
             }
             for (int k = 0; k < a.a_slots; ++k) {
                 if (ac.slot == 0) { ac.slot = a.a_slots; ac.phase ^= 1; }
@@ -362,7 +407,8 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         // shared memory and TMEM, and the warpgroups write NaN
         const bool lead = lb_elect();
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(LT >> 4) << 24);
-        LabelCursor rc, ac, oc_, gc, sc, pc;                 // ring, A, outputs; oldest stage not given back; S, its G
+        LabelCursor rc, ac, oc_, gc, sc, pc, eac, ec;        // ring, A, outputs; oldest stage not given back; S, its G; extra channels
+        const uint32_t ea16 = lb_desc_lo<16> + (rgs_smem_addr(ea_tiles) >> 4), e16 = lb_desc_lo<16> + (rgs_smem_addr(e_tiles) >> 4);
         const uint32_t dlo = lb_desc_lo<KC>, ring16 = dlo + (rgs_smem_addr(ring) >> 4), tiles16 = dlo + (rgs_smem_addr(tiles) >> 4);
         constexpr uint32_t T16 = TB >> 4, stage16 = stage >> 4;
         auto take = [&]() {
@@ -385,9 +431,13 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             const uint32_t d = tmem + sc.slot * SB;
             // forward: the scores there before have been read; backward: the product with their G was issued before, and runs before
             if (!GRAD) lb_wait_quiet(&sh->s_done[sc.slot], sc.phase ^ 1, fail);
-            if (a.a_slots && j == it.j0) lb_wait_quiet(&sh->a_full[ac.slot], ac.phase, fail);
+            if (j == it.j0) {
+                lb_wait_quiet(&sh->ea_full[eac.slot], eac.phase, fail);
+                if (a.a_slots) lb_wait_quiet(&sh->a_full[ac.slot], ac.phase, fail);
+            }
+            lb_wait_quiet(&sh->e_full[ec.slot], ec.phase, fail);
             const uint32_t abase = tiles16 + ac.slot * (na * T16);
-            const bool last = j == it.j1 - 1 && a.a_slots;
+            const bool last = j == it.j1 - 1;
             for (int k = 0; k < nst; ++k) {
                 const uint32_t at = a.a_slots ? abase + k * stage16 : take();
                 const uint32_t bt = take();
@@ -404,14 +454,24 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                         if (!a.a_slots) lb_commit(&sh->empty[g0 + 1 == (uint32_t)a.stages ? 0 : g0 + 1]);
                     }
                     if (k == nst - 1) {
+                        // last: where b and m are huge and cancel, what is small beside them is gone, as it is from the scores
+                        lb_mma_ss<16>(d, ea16 + eac.slot * (LE >> 4), e16 + ec.slot * (LE >> 4), idesc | ((LT >> 3) << 17), true);
                         lb_commit(&sh->s_full[sc.slot]);
-                        if (last) lb_commit(&sh->a_empty[ac.slot]);
+                        lb_commit(&sh->e_empty[ec.slot]);
+                        if (last) {
+                            lb_commit(&sh->ea_empty[eac.slot]);
+                            if (a.a_slots) lb_commit(&sh->a_empty[ac.slot]);
+                        }
                     }
                 }
                 __syncwarp();
             }
             sc.next(a.nbuf);
-            if (last) ac.next(a.a_slots);
+            ec.next(LESLOTS);
+            if (last) {
+                eac.next(2);
+                if (a.a_slots) ac.next(a.a_slots);
+            }
         };
         // G B; B as the K x N operand with its channels as N, 16 rows a step
         auto stage_o = [&](uint32_t s, uint32_t o, uint32_t bt, bool more) {
@@ -486,8 +546,11 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         const float nan = __int_as_float(0x7fc00000);
         const f2 log2e = mk2(LOG2E, LOG2E);
         uint32_t t = 0, kept = 0;                            // score tiles seen; ring stage where the B block of tile t begins
-        LabelCursor oc_, sc;
+        LabelCursor oc_, sc, kc;
         bool dead = false;
+        const int flags = GRAD ? (int)a.flags[1] : 0;
+        const bool large = flags & LF_LARGE, scaled = GRAD && (large || a.per_row);  // factors to dW's columns
+        const float gshare = GRAD && !scaled ? *a.gs : 1.f;
         unsigned out_i = blockIdx.x;                         // next item whose output this warpgroup writes
         auto write_out = [&](unsigned i) {
             const LabelItem it = lb_item(a, i);
@@ -496,12 +559,12 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             const uint32_t o = tmem + lanes + OUT + oc_.slot * OB;
             const int64_t r = (int64_t)it.m * LT + row, rows = it.dw ? a.v : a.n;
             const int ns = it.dw ? a.nsw : a.nsx;
-            float scale = 1.f;
+            float scale = gshare;
             int label = 0;
             if (!it.dw) {
-                const float* k = a.kn + (size_t)it.m * (LT * 4);
-                scale = k[2 * LT + row];
-                label = __float_as_int(k[3 * LT + row]);
+                const float* k = a.kn + (size_t)it.m * (3 * LT);
+                scale = k[LT + row];
+                label = __float_as_int(k[row]);
             }
             for (int c0 = wg * 16; c0 < it.noc * KC; c0 += 64) {
                 const int c = it.oc0 * KC + c0;
@@ -518,6 +581,9 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
 #pragma unroll
                     for (int q = 0; q < 16; ++q) f[q] = dead ? nan : P == 3 ? __uint_as_float(u[q]) + __uint_as_float(lo[q]) : __uint_as_float(u[q]);
                     if (ns > 1) {
+                        if (it.dw)
+#pragma unroll
+                            for (int q = 0; q < 16; ++q) f[q] *= scale;
                         float* p = (it.dw ? a.part_w : a.part_x) + ((int64_t)it.split * (it.dw ? a.nmw : a.nmx) * LT + r) * a.cq + c;
 #pragma unroll
                         for (int q = 0; q < 16; q += 4) *reinterpret_cast<float4*>(p + q) = make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]);
@@ -533,38 +599,36 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             rgs_mbar_arrive(&sh->o_free[oc_.slot]);
             oc_.next(a.nob);
         };
-        const bool dirty = GRAD && P == 1 && a.whole && a.flags[1] != 0.f;
+        const bool dirty = P == 1 && a.whole && (flags & LF_DIRTY);
         for (unsigned i = blockIdx.x; i < items; i += gridDim.x) {
             const LabelItem it = lb_item(a, i);
             const int64_t r = (int64_t)it.m * LT + row;
             // per-row values
             int64_t y = -1;
-            float m2 = -INFINITY, inv_z = 0.f, sum = 0.f, b2row = 0.f;
+            float m = -INFINITY, inv_z = 1.f, sum = 0.f;
             if (!it.dw) {
                 if (GRAD) {
-                    m2 = INFINITY;
-                    if (r < a.n) { m2 = a.lse[r]; inv_z = ex2(-a.lse[a.n + r]); }
-                    y = __float_as_int(a.kn[(size_t)it.m * (LT * 4) + 3 * LT + row]);
+                    if (large && r < a.n) inv_z = ex2(-a.lse[a.n + r] * LOG2E);
+                    y = __float_as_int(a.kn[(size_t)it.m * (3 * LT) + row]);
                 } else if (r < a.n) {
                     y = rgs_label(a.labels, r, a.label_bytes, a.v);
                 }
-            } else {
-                b2row = a.b2[r];
             }
             for (int j = it.j0; j < it.j1; ++j, ++t) {
                 const uint32_t bstage = kept, buf = sc.slot, parity = sc.phase;
                 if (GRAD && P == 1 && (kept += nst) >= (uint32_t)a.stages) kept -= a.stages;
+                const uint32_t kslot = kc.slot, kparity = kc.phase;
                 sc.next(a.nbuf);
+                if (GRAD && it.dw) kc.next(LKSLOTS);
                 if ((int)(t & 1) != (wg & 1)) continue;
                 const uint32_t s = tmem + lanes + buf * SB + half;
-                const uint32_t ks = t & (LKSLOTS - 1);
                 if (!dead) {  // the whole warp goes on or none of it: TMEM accesses are warp-wide
-                    dead = !lb_wait(&sh->k_full[ks], (t / LKSLOTS) & 1, fail) || !lb_wait(&sh->s_full[buf], parity, fail);
+                    dead = !lb_wait(&sh->s_full[buf], parity, fail) || (GRAD && it.dw && !lb_wait(&sh->k_full[kslot], kparity, fail));
                     dead = __any_sync(0xffffffffu, dead);
                 }
                 if (dead) continue;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const float* kb = kbuf + ks * (LKBYTES / 4) + half;
+                const float* kb = kbuf + kslot * (LKBYTES / 4) + half;
                 const int64_t yt = y - (int64_t)j * LT - half;
                 const int yl = y >= 0 && yt >= 0 && yt < 64 ? (int)yt : -1;  // the row's label among these columns
                 if (!GRAD) {
@@ -578,16 +642,9 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                     rgs_mbar_arrive(&sh->s_done[buf]);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        f2 v[16];
                         float f[32];
 #pragma unroll
-                        for (int q = 0; q < 16; q += 2) {
-                            const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(kb + h * 32 + 2 * q);
-                            v[q] = fma2(mk2u(u[h][2 * q], u[h][2 * q + 1]), log2e, b.x);
-                            v[q + 1] = fma2(mk2u(u[h][2 * q + 2], u[h][2 * q + 3]), log2e, b.y);
-                        }
-#pragma unroll
-                        for (int q = 0; q < 16; ++q) un2(v[q], f[2 * q], f[2 * q + 1]);
+                        for (int q = 0; q < 32; ++q) f[q] = __uint_as_float(u[h][q]);
                         float top[4];
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
@@ -605,22 +662,21 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                                 for (int q = 0; q < w; ++q) z[q] = yl & w ? z[q + w] : z[q];
                             a.at[r] = z[0];
                         }
-                        const float best = fmaxf(m2, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+                        const float best = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
                         const float ref = best == -INFINITY ? 0.f : best;
                         const f2 minus = mk2(-ref, -ref);
                         f2 acc[2] = {0ull, 0ull};
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) {
+                        for (int q = 0; q < 16; ++q) {  // (the difference first: scores at the type's lowest value times log2 e are none)
                             float e0, e1;
-                            un2(add2(v[q], minus), e0, e1);
+                            un2(mul2(add2(mk2(f[2 * q], f[2 * q + 1]), minus), log2e), e0, e1);
                             acc[q & 1] = add2(acc[q & 1], mk2(ex2(e0), ex2(e1)));
                         }
                         float s0, s1;
                         un2(add2(acc[0], acc[1]), s0, s1);
-                        sum = fmaf(sum, ex2(m2 - ref), s0 + s1);
-                        m2 = best;
+                        sum = fmaf(sum, ex2((m - ref) * LOG2E), s0 + s1);
+                        m = best;
                     }
-                    rgs_mbar_arrive(&sh->k_empty[ks]);
                     continue;
                 }
 #pragma unroll 1
@@ -632,42 +688,34 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
 #pragma unroll
                     for (int o = 0; o < 32; o += 16) {  // 16 columns: one step of the product's inner dimension
                         float e[16];
+#pragma unroll
+                        for (int q = 0; q < 16; q += 2) {
+                            un2(mul2(mk2u(u[o + q], u[o + q + 1]), log2e), e[q], e[q + 1]);
+                            e[q] = ex2(e[q]);
+                            e[q + 1] = ex2(e[q + 1]);
+                        }
                         if (!it.dw) {
-                            const f2 minus = mk2(-m2, -m2), factor = mk2(inv_z, inv_z);
+                            if (large) {
 #pragma unroll
-                            for (int q = 0; q < 16; q += 4) {
-                                const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(kb + h + o + q);
-                                un2(add2(fma2(mk2u(u[o + q], u[o + q + 1]), log2e, b.x), minus), e[q], e[q + 1]);
-                                un2(add2(fma2(mk2u(u[o + q + 2], u[o + q + 3]), log2e, b.y), minus), e[q + 2], e[q + 3]);
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) e[q + k] = ex2(e[q + k]);
-                                un2(mul2(mk2(e[q], e[q + 1]), factor), e[q], e[q + 1]);
-                                un2(mul2(mk2(e[q + 2], e[q + 3]), factor), e[q + 2], e[q + 3]);
+                                for (int q = 0; q < 16; ++q) e[q] *= inv_z;
                             }
                             if ((yl >> 4) == ((h + o) >> 4)) {  // before the rounding: p - 1 of a pixel that is nearly certain is small
 #pragma unroll
                                 for (int q = 0; q < 16; ++q) sub_if(e[q], 1.f, yl & 15, q);
                             }
                         } else {
-                            const f2 b2 = mk2(b2row, b2row);
+                            if (scaled) {
 #pragma unroll
-                            for (int q = 0; q < 16; q += 4) {  // the constants hold -m: one addition
-                                const ulonglong2 m = *reinterpret_cast<const ulonglong2*>(kb + h + o + q);
-                                const ulonglong2 z = *reinterpret_cast<const ulonglong2*>(kb + LT + h + o + q);
-                                un2(add2(fma2(mk2u(u[o + q], u[o + q + 1]), log2e, b2), m.x), e[q], e[q + 1]);
-                                un2(add2(fma2(mk2u(u[o + q + 2], u[o + q + 3]), log2e, b2), m.y), e[q + 2], e[q + 3]);
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) e[q + k] = ex2(e[q + k]);
-                                un2(mul2(mk2(e[q], e[q + 1]), z.x), e[q], e[q + 1]);
-                                un2(mul2(mk2(e[q + 2], e[q + 3]), z.y), e[q + 2], e[q + 3]);
+                                for (int q = 0; q < 16; ++q) e[q] *= kb[2 * LT + h + o + q];
                             }
                             // pixels of these 16 whose label is one of the warp's 32 rows
-                            const int* lab = reinterpret_cast<const int*>(kb + 3 * LT + h + o);
+                            const int* lab = reinterpret_cast<const int*>(kb + h + o);
                             if (__any_sync(0xffffffffu, (unsigned)(lab[lane & 15] - it.m * LT - wrow) < 32u)) {
 #pragma unroll
                                 for (int q = 0; q < 16; q += 4) {
                                     const int4 l = *reinterpret_cast<const int4*>(lab + q);
-                                    const float4 g = *reinterpret_cast<const float4*>(kb + 2 * LT + h + o + q);
+                                    float4 g = make_float4(1.f, 1.f, 1.f, 1.f);
+                                    if (scaled) g = *reinterpret_cast<const float4*>(kb + LT + h + o + q);
                                     sub_if(e[q], g.x, l.x, (int)r);
                                     sub_if(e[q + 1], g.y, l.y, (int)r);
                                     sub_if(e[q + 2], g.z, l.z, (int)r);
@@ -711,7 +759,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 if (P == 1 && dirty && it.dw) {
                     // pixels without a label whose features are not finite: 0 * inf must not reach dW, so their rows of the
                     // staged block are cleared (row n of every chunk, whole, whatever the swizzle)
-                    if (__float_as_int(kb[3 * LT + row - half]) < 0) {
+                    if (__float_as_int(kb[row - half]) < 0) {
                         for (int k = 0; k < a.nk; ++k) {
                             uint32_t slot = bstage + k / CS;
                             if (slot >= (uint32_t)a.stages) slot -= a.stages;
@@ -724,17 +772,17 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                rgs_mbar_arrive(&sh->k_empty[ks]);
+                if (it.dw) rgs_mbar_arrive(&sh->k_empty[kslot]);
                 rgs_mbar_arrive(&sh->s_done[buf]);
                 for (; out_i < i; out_i += gridDim.x) write_out(out_i);  // outputs of earlier items, behind the first scores of this one
             }
             if (!GRAD) {
                 if (r < a.n) {
-                    a.pm[((int64_t)it.split * 4 + wg) * a.n + r] = dead ? nan : m2;
+                    a.pm[((int64_t)it.split * 4 + wg) * a.n + r] = dead ? nan : m;
                     a.ps[((int64_t)it.split * 4 + wg) * a.n + r] = dead ? nan : sum;
                 }
             } else if (it.dw && a.part_b && it.oc0 == 0) {
-                a.part_b[((int64_t)it.split * 4 + wg) * a.nmw * LT + r] = dead ? nan : sum;
+                a.part_b[((int64_t)it.split * 4 + wg) * a.nmw * LT + r] = dead ? nan : sum * gshare;
             }
         }
         if (GRAD)
@@ -751,11 +799,12 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
 // ---------------------------------------------------------------------------------------------------------------------
 struct LabelPrep {
     const void* x; int64_t ldx; const void* w; int64_t ldw; const void* bias; const void* labels;
-    int label_bytes, dtype, b_dtype, backward, per_row, pieces;
+    int label_bytes, dtype, b_dtype, backward, per_row, mean, pieces;
     int64_t n, v;
     int c, cp, nmx, nmw;
     __nv_bfloat16* xs; __nv_bfloat16* ws;  // (pieces, rows, cp) or null where the tensor itself is read
-    float* b2; float* kn;
+    __nv_bfloat16* ew; __nv_bfloat16* ex;  // extra channels, (nmw * 128, 16) and (nmx * 128, 16); forward: ex (128, 16)
+    float* kn; float* gs;
     const float* lse; const float* gout; const float* count;
     unsigned* ticket;
 };
@@ -791,11 +840,37 @@ __device__ __forceinline__ void lb_split8(const void* src, int64_t ld, int dtype
     }
 }
 
+// a value in three bf16 pieces (an infinity, or what rounds to one, whole in the first where it cannot be split)
+__device__ __forceinline__ void lb_split3(float v, uint32_t (&p)[3]) {
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+        uint32_t u = bf16x2(v, 0.f) & 0xffffu;
+        if ((u & 0x7fffu) >= 0x7f80u) {
+            if (fabsf(v) <= 3.402823466e38f) u = __float_as_uint(v) >> 16;
+            else { p[q] = u; v = 0.f; continue; }
+        }
+        p[q] = u;
+        v -= __uint_as_float(u << 16);
+    }
+}
+// sixteen extra channels of a row: three values and three more, zeros behind
+__device__ __forceinline__ void lb_extra(__nv_bfloat16* dst, const uint32_t (&a)[3], const uint32_t (&b)[3]) {
+    uint4* d = reinterpret_cast<uint4*>(dst);
+    d[0] = make_uint4(a[0] | (a[1] << 16), a[2] | (b[0] << 16), b[1] | (b[2] << 16), 0u);
+    d[1] = make_uint4(0u, 0u, 0u, 0u);
+}
+
 __global__ void __launch_bounds__(256) rgs_label_prep_kernel(const __grid_constant__ LabelPrep a) {
     const int groups = a.cp / 8;
     const int64_t gx = a.xs ? a.n * groups : 0, gw = a.ws ? a.v * groups : 0, gb = (int64_t)a.nmw * LT;
-    const int64_t gk = a.backward ? (int64_t)a.nmx * LT : 0;
-    if (blockIdx.x == 0 && threadIdx.x == 0 && a.ticket) *a.ticket = 0u;
+    const int64_t gk = a.backward ? (int64_t)a.nmx * LT : LT;
+    const uint32_t ones[3] = {0x3f80u, 0x3f80u, 0x3f80u}, none[3] = {0xff80u, 0u, 0u};  // 1; -infinity
+    const bool large = a.backward && ((int)a.count[1] & LF_LARGE);
+    const float mean = a.mean ? 1.f / fmaxf(a.count[0], 1.f) : 1.f;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        if (a.ticket) *a.ticket = 0u;
+        if (a.gs) *a.gs = a.gout[0] * mean;
+    }
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < gx + gw + gb + gk; i += (int64_t)gridDim.x * 256) {
         int64_t k = i;
         if (k < gx) {
@@ -812,25 +887,34 @@ __global__ void __launch_bounds__(256) rgs_label_prep_kernel(const __grid_consta
         }
         k -= gw;
         if (k < gb) {
-            float b = k < a.v ? 0.f : -INFINITY;
-            if (k < a.v && a.bias) {
-                const float raw = rgs_load_as_float(a.bias, k, a.b_dtype);
-                b = raw * LOG2E;  // a finite bias stays finite: the lowest value of the type is no -inf
-                if (fabsf(raw) <= 3.402823466e38f) b = fminf(fmaxf(b, -3.402823466e38f), 3.402823466e38f);
+            uint32_t b[3] = {0u, 0u, 0u};
+            if (k < a.v) {
+                if (a.bias) lb_split3(rgs_load_as_float(a.bias, k, a.b_dtype), b);
+                lb_extra(a.ew + k * 16, b, ones);
+            } else {
+                lb_extra(a.ew + k * 16, none, ones);
             }
-            a.b2[k] = b;
             continue;
         }
         k -= gb;
-        const int64_t y = k < a.n ? rgs_label(a.labels, k, a.label_bytes, a.v) : -1;
-        float m = INFINITY, z = 0.f, g = 0.f;  // -m is what is kept: a pixel without a label has exp(-inf) = 0
-        if (y >= 0) {
-            g = a.gout[a.per_row ? k : 0] * (a.count ? 1.f / fmaxf(a.count[0], 1.f) : 1.f);
-            m = a.lse[k];
-            z = g * exp2f(-a.lse[a.n + k]);
+        uint32_t c[3] = {0u, 0u, 0u};
+        if (!a.backward) {
+            lb_extra(a.ex + k * 16, ones, c);
+            continue;
         }
-        float* o = a.kn + (k / LT) * (4 * LT) + k % LT;
-        o[0] = -m; o[LT] = z; o[2 * LT] = g; o[3 * LT] = __int_as_float((int)y);
+        const int64_t y = k < a.n ? rgs_label(a.labels, k, a.label_bytes, a.v) : -1;
+        float g = 0.f, f = 0.f;
+        if (y >= 0) {
+            g = a.gout[a.per_row ? k : 0] * mean;
+            const float m = a.lse[k], lz = a.lse[a.n + k];
+            lb_split3(large ? -m : -(m + lz), c);
+            f = large ? g * expf(-lz) : g;
+            lb_extra(a.ex + k * 16, ones, c);
+        } else {
+            lb_extra(a.ex + k * 16, ones, none);
+        }
+        float* o = a.kn + (k / LT) * (3 * LT) + k % LT;
+        o[0] = __int_as_float((int)y); o[LT] = g; o[2 * LT] = f;
     }
 }
 
@@ -854,16 +938,17 @@ __global__ void __launch_bounds__(256) rgs_label_join_kernel(const float* __rest
         for (int k = 1; k < parts; ++k) m = fmaxf(m, pm[(int64_t)k * n + i]);
         const float ref = m == -INFINITY ? 0.f : m;
         float z = 0.f;
-        for (int k = 0; k < parts; ++k) z = fmaf(ps[(int64_t)k * n + i], exp2f(pm[(int64_t)k * n + i] - ref), z);
-        const float lz = log2f(z);
+        for (int k = 0; k < parts; ++k) z = fmaf(ps[(int64_t)k * n + i], expf(pm[(int64_t)k * n + i] - ref), z);
+        const float lz = logf(z);
         lse[i] = m;
         lse[n + i] = lz;
         float loss = 0.f;
         if (y >= 0) {
-            loss = (lz + (m - at[i])) * LN2;
+            loss = lz + (m - at[i]);
             ++rows;
+            if (fabsf(m) > 1024.f) dirty |= LF_LARGE;
         } else if (!(fabsf(m) <= 3.402823466e38f) || !(fabsf(lz) <= 3.402823466e38f)) {
-            dirty = 1;
+            dirty |= LF_DIRTY;
         }
         if (losses) losses[i] = loss;
         total += (double)loss;
@@ -871,14 +956,14 @@ __global__ void __launch_bounds__(256) rgs_label_join_kernel(const float* __rest
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) { total += __shfl_xor_sync(0xffffffffu, total, d); rows += __shfl_xor_sync(0xffffffffu, rows, d); }
     __syncthreads();
-    if (dirty) sdirty = 1;
+    if (dirty) atomicOr(&sdirty, dirty);
     if ((threadIdx.x & 31) == 0) { ssum[threadIdx.x >> 5] = total; scount[threadIdx.x >> 5] = rows; }
     __syncthreads();
     if (threadIdx.x == 0) {
         total = 0; rows = 0;
         for (int k = 0; k < 8; ++k) { total += ssum[k]; rows += scount[k]; }
         bsum[blockIdx.x] = total;
-        bcount[blockIdx.x] = rows * 2 + (unsigned)sdirty;
+        bcount[blockIdx.x] = rows * 4 + (unsigned)sdirty;
         __threadfence();
         last = atomicAdd(ticket, 1u) == gridDim.x - 1;
     }
@@ -889,18 +974,21 @@ __global__ void __launch_bounds__(256) rgs_label_join_kernel(const float* __rest
     for (unsigned k = threadIdx.x; k < gridDim.x; k += 256) {
         total += __ldcg(&bsum[k]);
         const unsigned long long u = __ldcg(&bcount[k]);
-        rows += u >> 1;
-        dirty |= (int)(u & 1);
+        rows += u >> 2;
+        dirty |= (int)(u & 3);
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) { total += __shfl_xor_sync(0xffffffffu, total, d); rows += __shfl_xor_sync(0xffffffffu, rows, d); }
     if ((threadIdx.x & 31) == 0) { ssum[threadIdx.x >> 5] = total; scount[threadIdx.x >> 5] = rows; }
-    dirty = __syncthreads_or(dirty);
+    if (threadIdx.x == 0) sdirty = 0;
+    __syncthreads();
+    if (dirty) atomicOr(&sdirty, dirty);
+    __syncthreads();
     if (threadIdx.x == 0) {
         total = 0; rows = 0;
         for (int k = 0; k < 8; ++k) { total += ssum[k]; rows += scount[k]; }
         count[0] = (float)rows;
-        count[1] = dirty ? 1.f : 0.f;
+        count[1] = (float)sdirty;
         if (result) *result = (float)(mean ? total / (double)(rows > 0 ? rows : 1) : total);
     }
 }
@@ -930,9 +1018,9 @@ __global__ void __launch_bounds__(256) rgs_label_reduce_kernel(const __grid_cons
         }
         float f[4] = {s.x, s.y, s.z, s.w};
         if (!is_w) {
-            const float* k = a.kn + (r / LT) * (4 * LT) + r % LT;
-            const float scale = k[2 * LT];
-            const bool zero = __float_as_int(k[3 * LT]) < 0;
+            const float* k = a.kn + (r / LT) * (3 * LT) + r % LT;
+            const float scale = k[LT];
+            const bool zero = __float_as_int(k[0]) < 0;
 #pragma unroll
             for (int q = 0; q < 4; ++q) f[q] = zero ? 0.f : f[q] * scale;
         }
@@ -963,14 +1051,14 @@ static LabelEncode label_encode() {
 }
 
 // (channels, rows, pieces) of bf16; boxes of kc channels x 128 rows; what lies outside reads as zero
-static int label_map(CUtensorMap* map, const void* base, int64_t c, int64_t rows, int64_t ld, int64_t pieces, int kc) {
+static int label_map(CUtensorMap* map, const void* base, int64_t c, int64_t rows, int64_t ld, int64_t pieces, int kc) {  // kc: 64, 32, 16
     LabelEncode enc = label_encode();
     if (!enc) return 20;
     const cuuint64_t dims[3] = {(cuuint64_t)c, (cuuint64_t)rows, (cuuint64_t)pieces};
     const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)ld * 2 * (cuuint64_t)rows};
     const cuuint32_t box[3] = {(cuuint32_t)kc, LT, 1}, estr[3] = {1, 1, 1};
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               kc == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : 21;
+               kc == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : kc == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : 21;
 }
 
 static inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
@@ -990,7 +1078,7 @@ static int label_pieces(int64_t tiles, int64_t nj, int64_t sms, int64_t run, int
 struct LabelPlan {
     LabelArgs a;
     int pieces, kc, cs, direct_x, direct_w, cp;
-    int64_t o_xs, o_ws, o_b2, o_kn, o_pm, o_ps, o_at, o_px, o_pw, o_pb, o_bsum, o_bcount, o_ticket, bytes;
+    int64_t o_xs, o_ws, o_ew, o_ex, o_kn, o_gs, o_pm, o_ps, o_at, o_px, o_pw, o_pb, o_bsum, o_bcount, o_ticket, bytes;
 };
 
 #define LJOIN 592  // most blocks of the joining kernel
@@ -1043,9 +1131,11 @@ static void label_plan(LabelPlan& p, int64_t n, int64_t c, int64_t v, int dtype,
     auto take = [&](int64_t bytes) { const int64_t at = o; o = up(o + bytes, 1024); return at; };
     p.o_xs = p.direct_x ? -1 : take(n * p.cp * 2 * p.pieces);
     p.o_ws = p.direct_w ? -1 : take(v * p.cp * 2 * p.pieces);
-    p.o_b2 = take(rows_w * 4);
+    p.o_ew = take(rows_w * 32);
+    p.o_ex = take((backward ? rows_x : LT) * 32);
     if (backward) {
-        p.o_kn = take(rows_x * 16);
+        p.o_kn = take(rows_x * 12);
+        p.o_gs = take(4);
         p.o_px = a.nsx > 1 ? take(a.nsx * rows_x * a.cq * 4) : -1;
         p.o_pw = a.nsw > 1 ? take(a.nsw * rows_w * a.cq * 4) : -1;
         p.o_pb = take(4 * a.nsw * rows_w * 4);
@@ -1065,8 +1155,10 @@ static int label_direct(const void* x, int64_t ldx, const void* w, int64_t ldw) 
     return dx | (dw << 1);
 }
 
+struct LabelMaps { CUtensorMap x, w, ex, ew; };
+
 template <int P, bool GRAD, int KC, int CS>
-static int label_launch(const CUtensorMap& mx, const CUtensorMap& mw, const LabelArgs& a, cudaStream_t stream) {
+static int label_launch(const LabelMaps& m, const LabelArgs& a, cudaStream_t stream) {
     static std::atomic<uint64_t> ready{0};  // devices whose limit on dynamic shared memory was raised
     int dev = 0;
     RGS_CUDA_CHECK(cudaGetDevice(&dev));
@@ -1075,16 +1167,16 @@ static int label_launch(const CUtensorMap& mx, const CUtensorMap& mw, const Labe
         if (dev <= 63) ready.fetch_or((uint64_t)1 << dev);
     }
     const int64_t items = (int64_t)a.items_x + a.items_w, sms = RGS_SMS;
-    rgs_label_tc_kernel<P, GRAD, KC, CS><<<(unsigned)(items < sms ? items : sms), LTHREADS, LSMEM, stream>>>(mx, mw, a);
+    rgs_label_tc_kernel<P, GRAD, KC, CS><<<(unsigned)(items < sms ? items : sms), LTHREADS, LSMEM, stream>>>(m.x, m.w, m.ex, m.ew, a);
     return (int)cudaGetLastError();
 }
 
 template <bool GRAD>
-static int label_run(const LabelPlan& p, const CUtensorMap& mx, const CUtensorMap& mw, cudaStream_t stream) {
-    if (p.pieces == 3) return p.kc == 64 ? label_launch<3, GRAD, 64, 1>(mx, mw, p.a, stream) : label_launch<3, GRAD, 32, 1>(mx, mw, p.a, stream);
-    if (p.kc == 32) return label_launch<1, GRAD, 32, 1>(mx, mw, p.a, stream);
-    if (p.cs == 3) return label_launch<1, GRAD, 64, 3>(mx, mw, p.a, stream);
-    return p.cs == 2 ? label_launch<1, GRAD, 64, 2>(mx, mw, p.a, stream) : label_launch<1, GRAD, 64, 1>(mx, mw, p.a, stream);
+static int label_run(const LabelPlan& p, const LabelMaps& m, cudaStream_t stream) {
+    if (p.pieces == 3) return p.kc == 64 ? label_launch<3, GRAD, 64, 1>(m, p.a, stream) : label_launch<3, GRAD, 32, 1>(m, p.a, stream);
+    if (p.kc == 32) return label_launch<1, GRAD, 32, 1>(m, p.a, stream);
+    if (p.cs == 3) return label_launch<1, GRAD, 64, 3>(m, p.a, stream);
+    return p.cs == 2 ? label_launch<1, GRAD, 64, 2>(m, p.a, stream) : label_launch<1, GRAD, 64, 1>(m, p.a, stream);
 }
 
 static inline unsigned label_grid(int64_t work, int64_t most) {
@@ -1092,19 +1184,31 @@ static inline unsigned label_grid(int64_t work, int64_t most) {
     return (unsigned)(want < 1 ? 1 : (want > most ? most : want));
 }
 
-static int label_operands(const LabelPlan& p, const LabelPrep& q, CUtensorMap* mx, CUtensorMap* mw) {
+static int label_operands(const LabelPlan& p, const LabelPrep& q, LabelMaps* m) {
     // autograd runs the backward pass on a thread of its own, where the driver has no context yet: cudaSetDevice binds it
     int dev = 0;
     RGS_CUDA_CHECK(cudaGetDevice(&dev));
     RGS_CUDA_CHECK(cudaSetDevice(dev));
-    int rc = p.direct_x ? label_map(mx, q.x, q.c, q.n, q.ldx, 1, p.kc) : label_map(mx, q.xs, p.cp, q.n, p.cp, p.pieces, p.kc);
-    if (rc) return rc;
-    return p.direct_w ? label_map(mw, q.w, q.c, q.v, q.ldw, 1, p.kc) : label_map(mw, q.ws, p.cp, q.v, p.cp, p.pieces, p.kc);
+    int rc = p.direct_x ? label_map(&m->x, q.x, q.c, q.n, q.ldx, 1, p.kc) : label_map(&m->x, q.xs, p.cp, q.n, p.cp, p.pieces, p.kc);
+    if (!rc) rc = p.direct_w ? label_map(&m->w, q.w, q.c, q.v, q.ldw, 1, p.kc) : label_map(&m->w, q.ws, p.cp, q.v, p.cp, p.pieces, p.kc);
+    if (!rc) rc = label_map(&m->ex, q.ex, 16, q.backward ? (int64_t)q.nmx * LT : LT, 16, 1, 16);
+    return rc ? rc : label_map(&m->ew, q.ew, 16, (int64_t)q.nmw * LT, 16, 1, 16);
 }
 
 static void label_prep(const LabelPlan& p, const LabelPrep& q, cudaStream_t stream) {
-    const int64_t work = ((q.xs ? q.n : 0) + (q.ws ? q.v : 0)) * (q.cp / 8) + (int64_t)q.nmw * LT + (q.backward ? (int64_t)q.nmx * LT : 0);
+    const int64_t work = ((q.xs ? q.n : 0) + (q.ws ? q.v : 0)) * (q.cp / 8) + (int64_t)q.nmw * LT + (q.backward ? (int64_t)q.nmx * LT : LT);
     rgs_label_prep_kernel<<<label_grid(work, RGS_SMS * 16), 256, 0, stream>>>(q);
+}
+
+static void label_fill(LabelPrep& q, const LabelPlan& p, unsigned char* s, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                       const void* labels, int label_bytes, int dtype, int b_dtype) {
+    q.x = x; q.ldx = ldx; q.w = w; q.ldw = ldw; q.bias = bias; q.labels = labels;
+    q.label_bytes = label_bytes; q.dtype = dtype; q.b_dtype = b_dtype; q.pieces = p.pieces;
+    q.n = p.a.n; q.v = p.a.v; q.c = p.a.c; q.cp = p.cp; q.nmx = p.a.nmx; q.nmw = p.a.nmw;
+    q.xs = p.direct_x ? nullptr : reinterpret_cast<__nv_bfloat16*>(s + p.o_xs);
+    q.ws = p.direct_w ? nullptr : reinterpret_cast<__nv_bfloat16*>(s + p.o_ws);
+    q.ew = reinterpret_cast<__nv_bfloat16*>(s + p.o_ew);
+    q.ex = reinterpret_cast<__nv_bfloat16*>(s + p.o_ex);
 }
 
 extern "C" {
@@ -1124,22 +1228,21 @@ int rgs_cuda_label_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     label_plan(p, n, c, vocab, (int)dtype, label_direct(x, ldx, w, ldw), 0);
     LabelArgs& a = p.a;
     unsigned char* s = reinterpret_cast<unsigned char*>(up((int64_t)reinterpret_cast<uintptr_t>(scratch), 1024));
-    LabelPrep q{x, ldx, w, ldw, bias, labels, (int)label_bytes, (int)dtype, (int)b_dtype, 0, 0, p.pieces, n, vocab, (int)c, p.cp, a.nmx, a.nmw,
-                p.direct_x ? nullptr : reinterpret_cast<__nv_bfloat16*>(s + p.o_xs), p.direct_w ? nullptr : reinterpret_cast<__nv_bfloat16*>(s + p.o_ws),
-                reinterpret_cast<float*>(s + p.o_b2), nullptr, nullptr, nullptr, nullptr, reinterpret_cast<unsigned*>(s + p.o_ticket)};
-    CUtensorMap mx, mw;
-    int rc = label_operands(p, q, &mx, &mw);
+    LabelPrep q{};
+    label_fill(q, p, s, x, ldx, w, ldw, bias, labels, (int)label_bytes, (int)dtype, (int)b_dtype);
+    q.ticket = reinterpret_cast<unsigned*>(s + p.o_ticket);
+    LabelMaps m;
+    int rc = label_operands(p, q, &m);
     if (rc) return rc;
     label_prep(p, q, st);
     RGS_CUDA_CHECK(cudaGetLastError());
     a.items_x = (unsigned)a.nmx * a.nsx;
-    a.b2 = q.b2;
     a.labels = labels; a.label_bytes = (int)label_bytes;
     a.flags = count;
     a.pm = reinterpret_cast<float*>(s + p.o_pm);
     a.ps = reinterpret_cast<float*>(s + p.o_ps);
     a.at = reinterpret_cast<float*>(s + p.o_at);
-    rc = label_run<false>(p, mx, mw, st);
+    rc = label_run<false>(p, m, st);
     if (rc) return rc;
     rgs_label_join_kernel<<<label_grid(n, LJOIN), 256, 0, st>>>(a.pm, a.ps, a.at, labels, (int)label_bytes, n, vocab, 4 * a.nsx, (int)mean, lse, losses,
                                                                 result, count, reinterpret_cast<double*>(s + p.o_bsum),
@@ -1155,25 +1258,27 @@ int rgs_cuda_label_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     label_plan(p, n, c, vocab, (int)dtype, label_direct(x, ldx, w, ldw), 1);
     LabelArgs& a = p.a;
     unsigned char* s = reinterpret_cast<unsigned char*>(up((int64_t)reinterpret_cast<uintptr_t>(scratch), 1024));
-    LabelPrep q{x, ldx, w, ldw, bias, labels, (int)label_bytes, (int)dtype, (int)b_dtype, 1, (int)per_row, p.pieces, n, vocab, (int)c, p.cp, a.nmx,
-                a.nmw, p.direct_x ? nullptr : reinterpret_cast<__nv_bfloat16*>(s + p.o_xs),
-                p.direct_w ? nullptr : reinterpret_cast<__nv_bfloat16*>(s + p.o_ws), reinterpret_cast<float*>(s + p.o_b2),
-                reinterpret_cast<float*>(s + p.o_kn), lse, gout, mean ? count : nullptr, nullptr};
-    CUtensorMap mx, mw;
-    int rc = label_operands(p, q, &mx, &mw);
+    LabelPrep q{};
+    label_fill(q, p, s, x, ldx, w, ldw, bias, labels, (int)label_bytes, (int)dtype, (int)b_dtype);
+    q.backward = 1; q.per_row = (int)per_row; q.mean = (int)mean;
+    q.lse = lse; q.gout = gout; q.count = count;
+    q.kn = reinterpret_cast<float*>(s + p.o_kn);
+    q.gs = reinterpret_cast<float*>(s + p.o_gs);
+    LabelMaps m;
+    int rc = label_operands(p, q, &m);
     if (rc) return rc;
     label_prep(p, q, st);
     RGS_CUDA_CHECK(cudaGetLastError());
     a.items_x = dx ? (unsigned)a.nmx * a.nrange * a.nsx : 0;
     a.items_w = dw || db ? (unsigned)a.nmw * a.nrange * a.nsw : 0;
-    a.b2 = q.b2; a.kn = q.kn; a.lse = lse;
+    a.kn = q.kn; a.lse = lse; a.gs = q.gs; a.per_row = (int)per_row;
     a.labels = labels; a.label_bytes = (int)label_bytes;
     a.flags = count;
     a.part_x = dx && a.nsx > 1 ? reinterpret_cast<float*>(s + p.o_px) : nullptr;
     a.part_w = dw && a.nsw > 1 ? reinterpret_cast<float*>(s + p.o_pw) : nullptr;
     a.part_b = db ? reinterpret_cast<float*>(s + p.o_pb) : nullptr;
     a.dx = dx; a.dw = dw;
-    rc = label_run<true>(p, mx, mw, st);
+    rc = label_run<true>(p, m, st);
     if (rc) return rc;
     if (a.part_x || a.part_w || db) {
         const int64_t work = (a.part_x ? n * (a.cq / 4) : 0) + (a.part_w ? vocab * (a.cq / 4) : 0) + (db ? vocab : 0);
