@@ -115,8 +115,8 @@ __device__ __forceinline__ void lb_tma(void* dst, const CUtensorMap* map, int x,
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
                  "r"(rgs_smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(rgs_smem_addr(bar)) : "memory");
 }
-__device__ __forceinline__ void lb_commit(unsigned long long* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(rgs_smem_addr(bar)) : "memory");
+__device__ __forceinline__ void lb_commit(uint32_t lead, unsigned long long* bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(rgs_smem_addr(bar)), "r"(lead) : "memory");
 }
 // Shared-memory descriptors: rows of KC channels under the swizzle of their length (128, 64 or 32 bytes), eight rows to a
 // pattern; both strides are that of the pattern, so a tile reads as K-major rows or as steps of K.  The low word holds the
@@ -125,14 +125,14 @@ template <int KC> constexpr uint32_t lb_desc_lo = (uint32_t)KC << 16;
 template <int KC> constexpr uint32_t lb_desc_hi = (uint32_t)KC | (1u << 14) | ((KC == 64 ? 2u : KC == 32 ? 4u : 6u) << 29);
 
 template <int KC>
-__device__ __forceinline__ void lb_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
-    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "n"(lb_desc_hi<KC>) : "memory");
+__device__ __forceinline__ void lb_mma_ss(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "n"(lb_desc_hi<KC>), "r"(lead) : "memory");
 }
 template <int KC>
-__device__ __forceinline__ void lb_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
-    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 y, {%2, %5};\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "n"(lb_desc_hi<KC>) : "memory");
+__device__ __forceinline__ void lb_mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 y, {%2, %5};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "n"(lb_desc_hi<KC>), "r"(lead) : "memory");
 }
 #define LB_R16(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7]), \
     "+r"(r[o + 8]), "+r"(r[o + 9]), "+r"(r[o + 10]), "+r"(r[o + 11]), "+r"(r[o + 12]), "+r"(r[o + 13]), "+r"(r[o + 14]), "+r"(r[o + 15])
@@ -405,7 +405,10 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         // ------------------------------------------------------------------------------------------------ MMA
         // once a wait has run out the others return at once: the loop goes through its (bounded) motions on whatever lies in
         // shared memory and TMEM, and the warpgroups write NaN
-        const bool lead = lb_elect();
+        const uint32_t lead = lb_elect();
+        // one product after the other by predicate (several chunks to a stage), or a branch around all of them: each the
+        // faster one (256 channels backward 4.09 -> 3.85 ms with predicates, 32 channels in 32 bits 1.74 -> 1.86 ms)
+        const uint32_t issue = P == 3 || CS == 1 ? 1u : lead;
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(LT >> 4) << 24);
         LabelCursor rc, ac, oc_, gc, sc, pc, eac, ec;        // ring, A, outputs; oldest stage not given back; S, its G; extra channels
         const uint32_t ea16 = lb_desc_lo<16> + (rgs_smem_addr(ea_tiles) >> 4), e16 = lb_desc_lo<16> + (rgs_smem_addr(e_tiles) >> 4);
@@ -425,7 +428,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 for (int q = 0; q < COMBOS; ++q)
 #pragma unroll
                     for (int ks = 0; ks < KC / 16; ++ks)
-                        lb_mma_ss<KC>(d, at + (k * P + CA[q]) * T16 + ks * 2, bt + (k * P + CB[q]) * T16 + ks * 2, idesc | ((LT >> 3) << 17), k || q || ks ? true : more);
+                        lb_mma_ss<KC>(issue, d, at + (k * P + CA[q]) * T16 + ks * 2, bt + (k * P + CB[q]) * T16 + ks * 2, idesc | ((LT >> 3) << 17), k || q || ks ? true : more);
         };
         auto issue_s = [&](const LabelItem& it, int j) {
             const uint32_t d = tmem + sc.slot * SB;
@@ -447,20 +450,20 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                     if (!a.a_slots) gc.next(a.stages);
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (lead) {
+                if ((P == 1 && CS > 1) || lead) {
                     stage_s(d, at, bt, k != 0);
                     if (!GRAD || !a.whole) {
-                        lb_commit(&sh->empty[g0]);
-                        if (!a.a_slots) lb_commit(&sh->empty[g0 + 1 == (uint32_t)a.stages ? 0 : g0 + 1]);
+                        lb_commit(issue, &sh->empty[g0]);
+                        if (!a.a_slots) lb_commit(issue, &sh->empty[g0 + 1 == (uint32_t)a.stages ? 0 : g0 + 1]);
                     }
                     if (k == nst - 1) {
                         // last: where b and m are huge and cancel, what is small beside them is gone, as it is from the scores
-                        lb_mma_ss<16>(d, ea16 + eac.slot * (LE >> 4), e16 + ec.slot * (LE >> 4), idesc | ((LT >> 3) << 17), true);
-                        lb_commit(&sh->s_full[sc.slot]);
-                        lb_commit(&sh->e_empty[ec.slot]);
+                        lb_mma_ss<16>(issue, d, ea16 + eac.slot * (LE >> 4), e16 + ec.slot * (LE >> 4), idesc | ((LT >> 3) << 17), true);
+                        lb_commit(issue, &sh->s_full[sc.slot]);
+                        lb_commit(issue, &sh->e_empty[ec.slot]);
                         if (last) {
-                            lb_commit(&sh->ea_empty[eac.slot]);
-                            if (a.a_slots) lb_commit(&sh->a_empty[ac.slot]);
+                            lb_commit(issue, &sh->ea_empty[eac.slot]);
+                            if (a.a_slots) lb_commit(issue, &sh->a_empty[ac.slot]);
                         }
                     }
                 }
@@ -475,18 +478,19 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         };
         // G B; B as the K x N operand with its channels as N, 16 rows a step
         auto stage_o = [&](uint32_t s, uint32_t o, uint32_t bt, bool more) {
-            constexpr uint32_t id = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(KC >> 3) << 17) | ((uint32_t)(LT >> 4) << 24);
+            // 16 bits: the chunks of a stage lie a tile apart and are one operand of CS KC columns, so that G is read once for them
+            constexpr int W = P == 1 ? CS * KC : KC;
+            constexpr uint32_t id = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(W >> 3) << 17) | ((uint32_t)(LT >> 4) << 24);
+            if (P == 1) bt += (T16 - KC) << 16;
 #pragma unroll
-            for (int k = 0; k < CS; ++k)
+            for (int q = 0; q < COMBOS; ++q)
 #pragma unroll
-                for (int q = 0; q < COMBOS; ++q)
-#pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) {
-                        // 16 columns of G are 8 words: the first two pieces lie over the 16 scores, the third behind all
-                        const uint32_t g = CA[q] == 2 ? s + 128 + ks * 8 : s + ks * 16 + CA[q] * 8;
-                        const bool first = ks == 0 && (q == 0 || q == COMBOS - 1);
-                        lb_mma_ts<KC>(o + k * KC + (q < COMBOS - 1 ? LO : 0), g, bt + (k * P + CB[q]) * T16 + ks * (KC * 2), id, first ? more : true);
-                    }
+                for (int ks = 0; ks < 8; ++ks) {
+                    // 16 columns of G are 8 words: the first two pieces lie over the 16 scores, the third behind all
+                    const uint32_t g = CA[q] == 2 ? s + 128 + ks * 8 : s + ks * 16 + CA[q] * 8;
+                    const bool first = ks == 0 && (q == 0 || q == COMBOS - 1);
+                    lb_mma_ts<KC>(issue, o + (q < COMBOS - 1 ? LO : 0), g, bt + CB[q] * T16 + ks * (KC * 2), id, first ? more : true);
+                }
         };
         auto issue_o = [&](const LabelItem& it, int j) {
             lb_wait_quiet(&sh->s_done[pc.slot], pc.phase, fail);
@@ -498,10 +502,10 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 // kept stages: those that S took are the oldest ones still held (all chunks are output channels then)
                 const uint32_t bt = a.whole ? ring16 + gc.slot * stage16 : take();
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (lead) {
+                if ((P == 1 && CS > 1) || lead) {
                     stage_o(s, o + oc * KC, bt, j != it.j0);
-                    lb_commit(&sh->empty[gc.slot]);
-                    if (last && oc + CS == it.noc) lb_commit(&sh->o_full[oc_.slot]);
+                    lb_commit(issue, &sh->empty[gc.slot]);
+                    if (last && oc + CS == it.noc) lb_commit(issue, &sh->o_full[oc_.slot]);
                 }
                 __syncwarp();
                 gc.next(a.stages);
@@ -534,7 +538,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         } else {
             while (si < items) step_s();
         }
-        if (lead) lb_commit(&sh->drain);
+        lb_commit(lead, &sh->drain);
         __syncwarp();
         rgs_mbar_wait(&sh->drain, 0, LWAIT);
     } else {
@@ -552,20 +556,27 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         const bool large = flags & LF_LARGE, scaled = GRAD && (large || a.per_row);  // factors to dW's columns
         const float gshare = GRAD && !scaled ? *a.gs : 1.f;
         unsigned out_i = blockIdx.x;                         // next item whose output this warpgroup writes
-        auto write_out = [&](unsigned i) {
+        // what a row of A brings to an item, fetched an item ahead: from memory at its start it would cost as much as a score tile
+        auto row_label = [&](unsigned i) -> int {
+            if (i >= items) return -1;
+            const LabelItem it = lb_item(a, i);
+            if (it.dw) return 0;
+            if (GRAD) return __float_as_int(a.kn[(size_t)it.m * (3 * LT) + row]);
+            const int64_t r = (int64_t)it.m * LT + row;
+            return r < a.n ? (int)rgs_label(a.labels, r, a.label_bytes, a.v) : -1;
+        };
+        auto row_scale = [&](unsigned i) -> float {
+            if (!GRAD || i >= items) return 1.f;
+            const LabelItem it = lb_item(a, i);
+            return it.dw ? gshare : a.kn[(size_t)it.m * (3 * LT) + LT + row];
+        };
+        auto write_out = [&](unsigned i, float scale, int label) {
             const LabelItem it = lb_item(a, i);
             if (!dead) dead = __any_sync(0xffffffffu, !lb_wait(&sh->o_full[oc_.slot], oc_.phase, fail));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t o = tmem + lanes + OUT + oc_.slot * OB;
             const int64_t r = (int64_t)it.m * LT + row, rows = it.dw ? a.v : a.n;
             const int ns = it.dw ? a.nsw : a.nsx;
-            float scale = gshare;
-            int label = 0;
-            if (!it.dw) {
-                const float* k = a.kn + (size_t)it.m * (3 * LT);
-                scale = k[LT + row];
-                label = __float_as_int(k[row]);
-            }
             for (int c0 = wg * 16; c0 < it.noc * KC; c0 += 64) {
                 const int c = it.oc0 * KC + c0;
                 if (c >= a.c) break;
@@ -600,20 +611,19 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             oc_.next(a.nob);
         };
         const bool dirty = P == 1 && a.whole && (flags & LF_DIRTY);
+        int next_label = row_label(blockIdx.x), out_label = 0;
+        float next_scale = row_scale(blockIdx.x), out_scale = 1.f;  // out_: of the first item whose output is not written
         for (unsigned i = blockIdx.x; i < items; i += gridDim.x) {
             const LabelItem it = lb_item(a, i);
             const int64_t r = (int64_t)it.m * LT + row;
-            // per-row values
-            int64_t y = -1;
+            const int label = next_label;
+            const float scale = next_scale;
+            next_label = row_label(i + gridDim.x);
+            next_scale = row_scale(i + gridDim.x);
+            if (out_i == i) { out_label = label; out_scale = scale; }
+            const int64_t y = it.dw ? -1 : label;
             float m = -INFINITY, inv_z = 1.f, sum = 0.f;
-            if (!it.dw) {
-                if (GRAD) {
-                    if (large && r < a.n) inv_z = ex2(-a.lse[a.n + r] * LOG2E);
-                    y = __float_as_int(a.kn[(size_t)it.m * (3 * LT) + row]);
-                } else if (r < a.n) {
-                    y = rgs_label(a.labels, r, a.label_bytes, a.v);
-                }
-            }
+            if (GRAD && large && !it.dw && r < a.n) inv_z = ex2(-a.lse[a.n + r] * LOG2E);
             for (int j = it.j0; j < it.j1; ++j, ++t) {
                 const uint32_t bstage = kept, buf = sc.slot, parity = sc.phase;
                 if (GRAD && P == 1 && (kept += nst) >= (uint32_t)a.stages) kept -= a.stages;
@@ -774,7 +784,12 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 if (it.dw) rgs_mbar_arrive(&sh->k_empty[kslot]);
                 rgs_mbar_arrive(&sh->s_done[buf]);
-                for (; out_i < i; out_i += gridDim.x) write_out(out_i);  // outputs of earlier items, behind the first scores of this one
+                if (out_i < i) {  // outputs of earlier items, behind the first scores of this one
+                    write_out(out_i, out_scale, out_label);
+                    for (out_i += gridDim.x; out_i < i; out_i += gridDim.x) write_out(out_i, row_scale(out_i), row_label(out_i));
+                    out_label = label;
+                    out_scale = scale;
+                }
             }
             if (!GRAD) {
                 if (r < a.n) {
@@ -785,8 +800,10 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 a.part_b[((int64_t)it.split * 4 + wg) * a.nmw * LT + r] = dead ? nan : sum * gshare;
             }
         }
-        if (GRAD)
-            for (; out_i < items; out_i += gridDim.x) write_out(out_i);
+        if (GRAD && out_i < items) {
+            write_out(out_i, out_scale, out_label);
+            for (out_i += gridDim.x; out_i < items; out_i += gridDim.x) write_out(out_i, row_scale(out_i), row_label(out_i));
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -993,41 +1010,71 @@ __global__ void __launch_bounds__(256) rgs_label_join_kernel(const float* __rest
     }
 }
 
-// after the backward pass: adds up the pieces in order
-__global__ void __launch_bounds__(256) rgs_label_reduce_kernel(const __grid_constant__ LabelArgs a, void* db, int b_dtype) {
-    const int64_t tx = a.part_x ? a.n * (a.cq / 4) : 0, tw = a.part_w ? a.v * (a.cq / 4) : 0, tb = db ? a.v : 0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < tx + tw + tb; i += (int64_t)gridDim.x * 256) {
-        if (i >= tx + tw) {
-            const int64_t v = i - tx - tw;
-            float s = 0.f;
-            for (int k = 0; k < 4 * a.nsw; ++k) s += a.part_b[((int64_t)k * a.nmw) * LT + v];
-            rgs_store_float(db, v, b_dtype, s);
-            continue;
-        }
-        const bool is_w = i >= tx;
-        const int64_t e = is_w ? i - tx : i, r = e / (a.cq / 4);
-        const int c = (int)(e - r * (a.cq / 4)) * 4;
+// After the backward pass: adds up the pieces of dX, in order, a thread to four channels (few pieces, many rows).
+__global__ void __launch_bounds__(256) rgs_label_reduce_x_kernel(const __grid_constant__ LabelArgs a) {
+    const int per = a.cq / 4;
+    const int64_t stride = (int64_t)a.nmx * LT * a.cq;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.n * per; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per;
+        const int c = (int)(i - r * per) * 4;
         if (c >= a.c) continue;
-        const int ns = is_w ? a.nsw : a.nsx;
-        const int64_t stride = (int64_t)(is_w ? a.nmw : a.nmx) * LT * a.cq;
-        const float* p = (is_w ? a.part_w : a.part_x) + r * a.cq + c;
+        const float* p = a.part_x + r * a.cq + c;
         float4 s = *reinterpret_cast<const float4*>(p);
-        for (int k = 1; k < ns; ++k) {
+        for (int k = 1; k < a.nsx; ++k) {
             const float4 t = *reinterpret_cast<const float4*>(p + k * stride);
             s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
         }
-        float f[4] = {s.x, s.y, s.z, s.w};
-        if (!is_w) {
-            const float* k = a.kn + (r / LT) * (3 * LT) + r % LT;
-            const float scale = k[LT];
-            const bool zero = __float_as_int(k[0]) < 0;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) f[q] = zero ? 0.f : f[q] * scale;
-        }
-        void* out = is_w ? a.dw : a.dx;
+        const float f[4] = {s.x, s.y, s.z, s.w};
+        const float* k = a.kn + (r / LT) * (3 * LT) + r % LT;
+        const float scale = k[LT];
+        const bool zero = __float_as_int(k[0]) < 0;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            if (c + q < a.c) rgs_store_float(out, r * a.c + c + q, a.dtype, f[q]);
+            if (c + q < a.c) rgs_store_float(a.dx, r * a.c + c + q, a.dtype, zero ? 0.f : f[q] * scale);
+    }
+}
+
+// The pieces of dW and db are many and the sums few (810 pieces of 512 x 32 in the 32-bit view): sixteen chains of every
+// sum side by side, 32 sums of four channels (of one label for db) to a block, joined in order.  A thread to a sum: 220 us.
+__global__ void __launch_bounds__(512) rgs_label_reduce_w_kernel(const __grid_constant__ LabelArgs a, int blocks_w, void* db, int b_dtype) {
+    __shared__ float4 sh[16][32];
+    const int lane = threadIdx.x & 31, chain = threadIdx.x >> 5;
+    if ((int)blockIdx.x < blocks_w) {
+        const int64_t i = (int64_t)blockIdx.x * 32 + lane, total = a.v * (a.cq / 4), stride = (int64_t)a.nmw * LT * a.cq;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < total)
+#pragma unroll 4
+            for (int k = chain; k < a.nsw; k += 16) {
+                const float4 t = *reinterpret_cast<const float4*>(a.part_w + k * stride + i * 4);
+                s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
+            }
+        sh[chain][lane] = s;
+        __syncthreads();
+        if (chain == 0 && i < total) {
+            const int chains = a.nsw < 16 ? a.nsw : 16;
+            for (int k = 1; k < chains; ++k) {
+                const float4 t = sh[k][lane];
+                s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
+            }
+            const int64_t r = i / (a.cq / 4);
+            const int c = (int)(i - r * (a.cq / 4)) * 4;
+            const float f[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (c + q < a.c) rgs_store_float(a.dw, r * a.c + c + q, a.dtype, f[q]);
+        }
+        return;
+    }
+    const int64_t v = (int64_t)(blockIdx.x - blocks_w) * 32 + lane;
+    float s = 0.f;
+    if (v < a.v)
+#pragma unroll 8
+        for (int k = chain; k < 4 * a.nsw; k += 16) s += a.part_b[(int64_t)k * a.nmw * LT + v];
+    sh[chain][lane].x = s;
+    __syncthreads();
+    if (chain == 0 && v < a.v) {
+        for (int k = 1; k < 16; ++k) s += sh[k][lane].x;
+        rgs_store_float(db, v, b_dtype, s);
     }
 }
 
@@ -1280,10 +1327,9 @@ int rgs_cuda_label_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     a.dx = dx; a.dw = dw;
     rc = label_run<true>(p, m, st);
     if (rc) return rc;
-    if (a.part_x || a.part_w || db) {
-        const int64_t work = (a.part_x ? n * (a.cq / 4) : 0) + (a.part_w ? vocab * (a.cq / 4) : 0) + (db ? vocab : 0);
-        rgs_label_reduce_kernel<<<label_grid(work, RGS_SMS * 16), 256, 0, st>>>(a, db, (int)b_dtype);
-    }
+    if (a.part_x) rgs_label_reduce_x_kernel<<<label_grid(n * (a.cq / 4), RGS_SMS * 16), 256, 0, st>>>(a);
+    const int64_t blocks_w = a.part_w ? (vocab * (a.cq / 4) + 31) / 32 : 0, blocks_b = db ? (vocab + 31) / 32 : 0;
+    if (blocks_w + blocks_b) rgs_label_reduce_w_kernel<<<(unsigned)(blocks_w + blocks_b), 512, 0, st>>>(a, (int)blocks_w, db, (int)b_dtype);
     return (int)cudaGetLastError();
 }
 
