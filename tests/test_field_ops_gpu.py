@@ -294,3 +294,78 @@ def test_offsets_that_pass_32_bits():
     torch.testing.assert_close(gx[-100:], wx, atol=1e-6, rtol=2.0 ** -7)
     torch.testing.assert_close(gw, ww, atol=1e-4, rtol=2.0 ** -6)
     assert (gx[:-100] == 0).all()
+
+
+@pytest.mark.parametrize("op", ["label", "norm"])
+def test_a_second_derivative_is_refused(op):
+    x = torch.randn(40, 16, device="cuda", requires_grad=True)
+    w = torch.randn(5, 16, device="cuda", requires_grad=True)
+    out = R.label_loss(x, w, torch.arange(40, device="cuda") % 5) if op == "label" else R.layer_norm(x, w[0]).square().sum()
+    (g,) = torch.autograd.grad(out, x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), x)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_label_loss_scores_far_from_zero(dtype, reduction):
+    """Scores of some thousands (m and log z are then not added up) and, beside them, pixels of ordinary ones."""
+    x, w, y, b = make_label_case(300, 40, 200, F32, seed=12, device="cuda")
+    x[:100] *= 1500.0
+    _check_label(x.to(dtype), w.to(dtype), y, b.to(dtype), reduction=reduction)
+
+
+def test_label_loss_many_short_items_and_one_label_tile():
+    """One tile of labels: every item of dX is one score tile, so that outputs wait for scores of later items."""
+    for n, c, v, dtype in ((40000, 20, 7, BF16), (40000, 70, 100, BF16), (30000, 40, 128, F32), (300, 64, 60000, BF16)):
+        _check_label(*make_label_case(n, c, v, dtype, seed=v, device="cuda"))
+
+
+def test_two_streams_at_once():
+    """Two losses on two streams, no order between them: workspaces are each call's own."""
+    cases = [make_label_case(5000, 48, 400, F32, seed=k, device="cuda") for k in range(2)]
+    want = []
+    for x, w, y, b in cases:
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        want.append(torch.autograd.grad(R.label_loss(leaves[0], leaves[1], y, bias=leaves[2]), leaves))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for k, (x, w, y, b) in enumerate(cases):
+            with torch.cuda.stream(streams[k]):
+                leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+                got[k] = torch.autograd.grad(R.label_loss(leaves[0], leaves[1], y, bias=leaves[2]), leaves)
+        torch.cuda.synchronize()
+        for k in range(2):
+            assert all(torch.equal(p, q) for p, q in zip(got[k], want[k]))
+
+
+@pytest.mark.parametrize("n,c", [(5, 3), (1, 771), (3, 7), (67, 515), (200, 1019), (4099, 13), (31, 1022)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_layer_norm_reads_nothing_of_its_neighbours(n, c, dtype):
+    """Odd widths are read in vectors that begin and end inside the neighbouring rows: NaN there must not show, nor may
+    rows in front of and behind a view."""
+    g = torch.Generator().manual_seed(c)
+    base = torch.full((n + 2, c), float("nan"), dtype=dtype, device="cuda")
+    view = base[1:-1]
+    view.copy_(torch.randn(n, c, generator=g).to(dtype))
+    _check_norm(view, F32, "input")
+    if n > 2:
+        hole = view.clone()
+        hole[1] = float("nan")
+        leaf = hole.requires_grad_(True)
+        y = R.layer_norm(leaf)
+        (gx,) = torch.autograd.grad(y, leaf, torch.ones_like(y))
+        keep = torch.arange(n, device="cuda") != 1
+        assert torch.isfinite(y[keep]).all() and torch.isfinite(gx[keep]).all()
+
+
+def test_layer_norm_with_eps_zero():
+    for planes in (False, True):
+        x = torch.randn(70, 24, generator=torch.Generator().manual_seed(5)).cuda()
+        leaf = (x.t().contiguous().t() if planes else x).requires_grad_(True)
+        w = torch.ones(24, device="cuda", requires_grad=True)
+        y = R.layer_norm(leaf, w, eps=0.0)
+        gx, gw = torch.autograd.grad(y.square().sum(), [leaf, w])
+        assert torch.isfinite(y).all() and torch.isfinite(gx).all() and torch.isfinite(gw).all()
