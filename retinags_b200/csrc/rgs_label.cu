@@ -33,6 +33,7 @@
 #include <stdint.h>
 #include <string.h>
 #include <atomic>
+#include <type_traits>
 #include "rgs_cuda_common.cuh"
 #include "rgs_field_math.h"
 
@@ -239,7 +240,7 @@ __device__ __forceinline__ void lb_store16(void* out, int64_t r, int c, int chan
 
 struct LabelShared {
     unsigned long long full[LSTAGES], empty[LSTAGES], a_full[2], a_empty[2], k_full[LKSLOTS], k_empty[LKSLOTS];
-    unsigned long long ea_full[2], ea_empty[2], e_full[LESLOTS], e_empty[LESLOTS];
+    unsigned long long ea_full[2], ea_empty[2], e_empty[LESLOTS];
     unsigned long long s_full[4], s_done[4], o_full[2], o_free[2], drain;
     uint32_t tmem;
     int fail;
@@ -247,7 +248,8 @@ struct LabelShared {
 #define LSMEM (1024 + LROOM + (2 + LESLOTS) * LE + LKSLOTS * LKBYTES + (int)sizeof(LabelShared))
 static_assert(LSMEM <= 232448, "shared memory of an SM");
 
-template <int P, bool GRAD, int KC, int CS>
+// WHOLE: A stays in shared memory and, backward, so do the stages of B between the two products
+template <int P, bool GRAD, int KC, int CS, bool WHOLE>
 __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                                                                    const __grid_constant__ CUtensorMap map_ex, const __grid_constant__ CUtensorMap map_ew,
                                                                    const __grid_constant__ LabelArgs a) {
@@ -270,7 +272,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
     const uint32_t na = P * a.nk;                 // tiles of one block of 128 rows, chunk by chunk, its pieces together
     unsigned char* ring = tiles + a.a_slots * na * TB;
     constexpr uint32_t stage = CS * P * TB;       // bytes of a stage of the ring: CS chunks of A or B, their pieces
-    const int nst = a.nk / CS;                    // stages of a block of 128 rows
+    const int nst = GRAD && WHOLE && CS != 2 ? 1 : a.nk / CS;  // stages of a block of 128 rows
 
     if (warp == 0) {
         if (lane == 0) {
@@ -282,7 +284,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             }
             for (int i = 0; i < 4; ++i) { rgs_mbar_init(&sh->s_full[i], 1); rgs_mbar_init(&sh->s_done[i], 256); }
             for (int i = 0; i < LKSLOTS; ++i) { rgs_mbar_init(&sh->k_full[i], 1); rgs_mbar_init(&sh->k_empty[i], 256); }
-            for (int i = 0; i < LESLOTS; ++i) { rgs_mbar_init(&sh->e_full[i], 1); rgs_mbar_init(&sh->e_empty[i], 1); }
+            for (int i = 0; i < LESLOTS; ++i) rgs_mbar_init(&sh->e_empty[i], 1);
             rgs_mbar_init(&sh->drain, 1);
             sh->fail = 0;
             rgs_fence_mbar_init();
@@ -303,12 +305,13 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         LabelCursor rc, ac, kc, eac, ec;
         uint32_t loads = 0, labels = 0;
         bool ok = true;
-        auto load = [&](const CUtensorMap* map, int k, int row) {
+        auto load = [&](const CUtensorMap* map, int k, int row, const CUtensorMap* extra) {
             ok = ok && lb_wait_warp(&sh->empty[rc.slot], rc.phase ^ 1, fail);
             if (!ok) return;
             if (lead) {
                 unsigned char* dst = ring + rc.slot * stage;
-                rgs_mbar_expect_tx(&sh->full[rc.slot], stage);
+                rgs_mbar_expect_tx(&sh->full[rc.slot], extra ? stage + LE : stage);
+                if (extra) lb_tma(e_tiles + ec.slot * LE, extra, 0, row * LT, 0, &sh->full[rc.slot]);
 #pragma unroll
                 for (int u = 0; u < CS * P; ++u) lb_tma(dst + u * TB, map, (k * CS + u / P) * KC, row * LT, u % P, &sh->full[rc.slot]);
             }
@@ -320,8 +323,8 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         bool have_prev = false;
         int prev_j = 0, prev_oc0 = 0, prev_noc = 0, prev_dw = 0;
         auto out_tiles = [&]() {
-            if (!GRAD || a.whole || !have_prev) return;
-            for (int oc = 0; oc < prev_noc && ok; oc += CS) load(prev_dw ? &map_x : &map_w, (prev_oc0 + oc) / CS, prev_j);
+            if (!GRAD || WHOLE || !have_prev) return;
+            for (int oc = 0; oc < prev_noc && ok; oc += CS) load(prev_dw ? &map_x : &map_w, (prev_oc0 + oc) / CS, prev_j, nullptr);
         };
         for (unsigned i = blockIdx.x; i < items && ok; i += gridDim.x) {
             const LabelItem it = lb_item(a, i);
@@ -334,7 +337,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 lb_tma(ea_tiles + eac.slot * LE, it.dw ? &map_ew : &map_ex, 0, GRAD ? it.m * LT : 0, 0, &sh->ea_full[eac.slot]);
             }
             eac.next(2);
-            if (a.a_slots) {
+            if (WHOLE || a.a_slots) {
                 ok = lb_wait_warp(&sh->a_empty[ac.slot], ac.phase ^ 1, fail);
                 if (!ok) break;
                 if (lead) {
@@ -349,11 +352,6 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             for (int j = it.j0; j < it.j1 && ok; ++j) {
                 ok = lb_wait_warp(&sh->e_empty[ec.slot], ec.phase ^ 1, fail);
                 if (!ok) break;
-                if (lead) {
-                    rgs_mbar_expect_tx(&sh->e_full[ec.slot], LE);
-                    lb_tma(e_tiles + ec.slot * LE, it.dw ? &map_ex : &map_ew, 0, j * LT, 0, &sh->e_full[ec.slot]);
-                }
-                ec.next(LESLOTS);
                 if (GRAD && it.dw) {
                     ok = lb_wait_warp(&sh->k_empty[kc.slot], kc.phase ^ 1, fail);
                     if (!ok) break;
@@ -365,9 +363,10 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                     ++labels;
                 }
                 for (int k = 0; k < nst && ok; ++k) {
-                    if (!a.a_slots) load(ma, k, it.m);
-                    load(mb, k, j);
+                    if (!WHOLE && !a.a_slots) load(ma, k, it.m, nullptr);
+                    load(mb, k, j, k == 0 ? (it.dw ? &map_ex : &map_ew) : nullptr);  // the extra channels come with the first stage
                 }
+                ec.next(LESLOTS);
                 out_tiles();
                 have_prev = true; prev_j = j; prev_oc0 = it.oc0; prev_noc = it.noc; prev_dw = it.dw;
             }
@@ -384,11 +383,6 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 if (kc.slot == 0) { kc.slot = LKSLOTS; kc.phase ^= 1; }
                 --kc.slot;
                 rgs_mbar_wait(&sh->k_full[kc.slot], kc.phase, 1u << 12);
-            }
-            for (uint32_t k = 0; k < LESLOTS; ++k) {
-                if (ec.slot == 0) { ec.slot = LESLOTS; ec.phase ^= 1; }
-                --ec.slot;
-                rgs_mbar_wait(&sh->e_full[ec.slot], ec.phase, 1u << 12);
             }
             for (int k = 0; k < 2; ++k) {
                 if (eac.slot == 0) { eac.slot = 2; eac.phase ^= 1; }
@@ -436,25 +430,24 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             if (!GRAD) lb_wait_quiet(&sh->s_done[sc.slot], sc.phase ^ 1, fail);
             if (j == it.j0) {
                 lb_wait_quiet(&sh->ea_full[eac.slot], eac.phase, fail);
-                if (a.a_slots) lb_wait_quiet(&sh->a_full[ac.slot], ac.phase, fail);
+                if (WHOLE || a.a_slots) lb_wait_quiet(&sh->a_full[ac.slot], ac.phase, fail);
             }
-            lb_wait_quiet(&sh->e_full[ec.slot], ec.phase, fail);
             const uint32_t abase = tiles16 + ac.slot * (na * T16);
             const bool last = j == it.j1 - 1;
             for (int k = 0; k < nst; ++k) {
-                const uint32_t at = a.a_slots ? abase + k * stage16 : take();
+                const uint32_t at = WHOLE || a.a_slots ? abase + k * stage16 : take();
                 const uint32_t bt = take();
                 const uint32_t g0 = gc.slot;
-                if (!GRAD || !a.whole) {
+                if (!GRAD || !WHOLE) {
                     gc.next(a.stages);
-                    if (!a.a_slots) gc.next(a.stages);
+                    if (!WHOLE && !a.a_slots) gc.next(a.stages);
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if ((P == 1 && CS > 1) || lead) {
                     stage_s(d, at, bt, k != 0);
-                    if (!GRAD || !a.whole) {
+                    if (!GRAD || !WHOLE) {
                         lb_commit(issue, &sh->empty[g0]);
-                        if (!a.a_slots) lb_commit(issue, &sh->empty[g0 + 1 == (uint32_t)a.stages ? 0 : g0 + 1]);
+                        if (!WHOLE && !a.a_slots) lb_commit(issue, &sh->empty[g0 + 1 == (uint32_t)a.stages ? 0 : g0 + 1]);
                     }
                     if (k == nst - 1) {
                         // last: where b and m are huge and cancel, what is small beside them is gone, as it is from the scores
@@ -463,7 +456,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                         lb_commit(issue, &sh->e_empty[ec.slot]);
                         if (last) {
                             lb_commit(issue, &sh->ea_empty[eac.slot]);
-                            if (a.a_slots) lb_commit(issue, &sh->a_empty[ac.slot]);
+                            if (WHOLE || a.a_slots) lb_commit(issue, &sh->a_empty[ac.slot]);
                         }
                     }
                 }
@@ -473,7 +466,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             ec.next(LESLOTS);
             if (last) {
                 eac.next(2);
-                if (a.a_slots) ac.next(a.a_slots);
+                if (WHOLE || a.a_slots) ac.next(a.a_slots);
             }
         };
         // G B; B as the K x N operand with its channels as N, 16 rows a step
@@ -500,7 +493,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             const bool last = j == it.j1 - 1;
             for (int oc = 0; oc < it.noc; oc += CS) {
                 // kept stages: those that S took are the oldest ones still held (all chunks are output channels then)
-                const uint32_t bt = a.whole ? ring16 + gc.slot * stage16 : take();
+                const uint32_t bt = WHOLE ? ring16 + gc.slot * stage16 : take();
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if ((P == 1 && CS > 1) || lead) {
                     stage_o(s, o + oc * KC, bt, j != it.j0);
@@ -610,7 +603,8 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             rgs_mbar_arrive(&sh->o_free[oc_.slot]);
             oc_.next(a.nob);
         };
-        const bool dirty = P == 1 && a.whole && (flags & LF_DIRTY);
+        const bool dirty = GRAD && P == 1 && WHOLE && (flags & LF_DIRTY);
+        const bool rare = dirty || scaled;
         int next_label = row_label(blockIdx.x), out_label = 0;
         float next_scale = row_scale(blockIdx.x), out_scale = 1.f;  // out_: of the first item whose output is not written
         for (unsigned i = blockIdx.x; i < items; i += gridDim.x) {
@@ -689,6 +683,9 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                     }
                     continue;
                 }
+                // factors and pixels to be kept out are in a copy of their own: their tests alone, never met, cost a fifth
+                auto gradient = [&](auto rare_) {
+                constexpr bool RARE = decltype(rare_)::value;
 #pragma unroll 1
                 for (int h = 0; h < 64; h += 32) {
                     uint32_t u[32];
@@ -705,7 +702,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                             e[q + 1] = ex2(e[q + 1]);
                         }
                         if (!it.dw) {
-                            if (large) {
+                            if (RARE && large) {
 #pragma unroll
                                 for (int q = 0; q < 16; ++q) e[q] *= inv_z;
                             }
@@ -714,7 +711,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                                 for (int q = 0; q < 16; ++q) sub_if(e[q], 1.f, yl & 15, q);
                             }
                         } else {
-                            if (scaled) {
+                            if (RARE && scaled) {
 #pragma unroll
                                 for (int q = 0; q < 16; ++q) e[q] *= kb[2 * LT + h + o + q];
                             }
@@ -725,14 +722,14 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                                 for (int q = 0; q < 16; q += 4) {
                                     const int4 l = *reinterpret_cast<const int4*>(lab + q);
                                     float4 g = make_float4(1.f, 1.f, 1.f, 1.f);
-                                    if (scaled) g = *reinterpret_cast<const float4*>(kb + LT + h + o + q);
+                                    if (RARE && scaled) g = *reinterpret_cast<const float4*>(kb + LT + h + o + q);
                                     sub_if(e[q], g.x, l.x, (int)r);
                                     sub_if(e[q + 1], g.y, l.y, (int)r);
                                     sub_if(e[q + 2], g.z, l.z, (int)r);
                                     sub_if(e[q + 3], g.w, l.w, (int)r);
                                 }
                             }
-                            if (P == 1 && dirty) {
+                            if (RARE && dirty) {
 #pragma unroll
                                 for (int q = 0; q < 16; ++q)
                                     if (lab[q] < 0) e[q] = 0.f;
@@ -766,6 +763,9 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                         }
                     }
                 }
+                };
+                if (rare) gradient(std::true_type());
+                else gradient(std::false_type());
                 if (P == 1 && dirty && it.dw) {
                     // pixels without a label whose features are not finite: 0 * inf must not reach dW, so their rows of the
                     // staged block are cleared (row n of every chunk, whole, whatever the swizzle)
@@ -1154,7 +1154,7 @@ static void label_plan(LabelPlan& p, int64_t n, int64_t c, int64_t v, int dtype,
     if (room >= na * ((backward ? a.nbuf : 2) + 3)) a.a_slots = 2;
     // chunks of a stage: few barriers to a block where the ring is deep enough
     p.cs = 1;
-    if (p.pieces == 1 && p.kc == 64 && a.a_slots && a.nrange == 1) p.cs = a.nk == 2 || a.nk == 4 ? 2 : (a.nk == 3 ? 3 : 1);
+    if (p.pieces == 1 && p.kc == 64 && a.a_slots && a.nk <= 4) p.cs = a.nk == 2 || a.nk == 4 ? 2 : (a.nk == 3 ? 3 : 1);
     a.stages = (room - a.a_slots * na) / (p.pieces * p.cs);
     if (a.stages > LSTAGES) a.stages = LSTAGES;
     a.cq = (int)up(c, 16);
@@ -1204,26 +1204,28 @@ static int label_direct(const void* x, int64_t ldx, const void* w, int64_t ldw) 
 
 struct LabelMaps { CUtensorMap x, w, ex, ew; };
 
-template <int P, bool GRAD, int KC, int CS>
+template <int P, bool GRAD, int KC, int CS, bool WHOLE>
 static int label_launch(const LabelMaps& m, const LabelArgs& a, cudaStream_t stream) {
     static std::atomic<uint64_t> ready{0};  // devices whose limit on dynamic shared memory was raised
     int dev = 0;
     RGS_CUDA_CHECK(cudaGetDevice(&dev));
     if (dev > 63 || !((ready.load() >> dev) & 1)) {
-        RGS_CUDA_CHECK(cudaFuncSetAttribute(rgs_label_tc_kernel<P, GRAD, KC, CS>, cudaFuncAttributeMaxDynamicSharedMemorySize, LSMEM));
+        RGS_CUDA_CHECK(cudaFuncSetAttribute(rgs_label_tc_kernel<P, GRAD, KC, CS, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, LSMEM));
         if (dev <= 63) ready.fetch_or((uint64_t)1 << dev);
     }
     const int64_t items = (int64_t)a.items_x + a.items_w, sms = RGS_SMS;
-    rgs_label_tc_kernel<P, GRAD, KC, CS><<<(unsigned)(items < sms ? items : sms), LTHREADS, LSMEM, stream>>>(m.x, m.w, m.ex, m.ew, a);
+    rgs_label_tc_kernel<P, GRAD, KC, CS, WHOLE><<<(unsigned)(items < sms ? items : sms), LTHREADS, LSMEM, stream>>>(m.x, m.w, m.ex, m.ew, a);
     return (int)cudaGetLastError();
 }
 
 template <bool GRAD>
 static int label_run(const LabelPlan& p, const LabelMaps& m, cudaStream_t stream) {
-    if (p.pieces == 3) return p.kc == 64 ? label_launch<3, GRAD, 64, 1>(m, p.a, stream) : label_launch<3, GRAD, 32, 1>(m, p.a, stream);
-    if (p.kc == 32) return label_launch<1, GRAD, 32, 1>(m, p.a, stream);
-    if (p.cs == 3) return label_launch<1, GRAD, 64, 3>(m, p.a, stream);
-    return p.cs == 2 ? label_launch<1, GRAD, 64, 2>(m, p.a, stream) : label_launch<1, GRAD, 64, 1>(m, p.a, stream);
+    const bool whole = GRAD ? p.a.whole != 0 : p.a.a_slots > 0;
+    if (p.kc == 32) return p.pieces == 3 ? label_launch<3, GRAD, 32, 1, true>(m, p.a, stream) : label_launch<1, GRAD, 32, 1, true>(m, p.a, stream);
+    if (p.pieces == 3) return whole ? label_launch<3, GRAD, 64, 1, true>(m, p.a, stream) : label_launch<3, GRAD, 64, 1, false>(m, p.a, stream);
+    if (!whole) return label_launch<1, GRAD, 64, 1, false>(m, p.a, stream);
+    if (p.cs == 3) return label_launch<1, GRAD, 64, 3, true>(m, p.a, stream);
+    return p.cs == 2 ? label_launch<1, GRAD, 64, 2, true>(m, p.a, stream) : label_launch<1, GRAD, 64, 1, true>(m, p.a, stream);
 }
 
 static inline unsigned label_grid(int64_t work, int64_t most) {
