@@ -1162,7 +1162,7 @@ static void label_plan(LabelPlan& p, int64_t n, int64_t c, int64_t v, int dtype,
     p.direct_x = p.pieces == 1 && (direct & 1) && (!backward || a.whole);
     p.direct_w = p.pieces == 1 && (direct & 2);
     p.cp = (int)up(c, 8);
-    const int64_t run = p.pieces == 1 ? 512 : 16;
+    const int64_t run = p.pieces == 1 ? 512 : 8;
     const int64_t rows_x = (int64_t)a.nmx * LT, rows_w = (int64_t)a.nmw * LT;
     if (backward) {
         const int64_t room = (int64_t)1 << 31;  // bytes of partial sums
