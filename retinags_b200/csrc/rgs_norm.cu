@@ -12,8 +12,13 @@
 // Rows are read in aligned vectors of four.  Where a row does not begin on such a boundary (a width that four does not
 // divide) its vectors begin up to three elements before it: a group takes rows a multiple of four apart, so that this shift
 // and with it the channels of a lane stay the same; the first and last vector of a row are then read element by element.
-// Codes of such rows are read element by element throughout.  Channel planes (the renderer's images) pass through shared
-// memory 32 pixels at a time.  Beyond 1024 channels a warp re-reads its row.
+// Codes of such rows are read element by element throughout.  Channel planes (the renderer's images) are read with a lane to
+// a pixel and turned into rows in shared memory.  Beyond 1024 channels a warp re-reads its row.
+//
+// Measured (a copy moves 6.5 TB/s): 1657600 rows x 64 channels, float32 in, bf16 out: forward 104 us (6.1 TB/s), with the
+// 8-bit copy 135 us (5.5 TB/s), backward 192 us (5.5 TB/s), from codes 200 us (3.7 TB/s: the arithmetic of decoding shares
+// the time); the same from planes 204 and 406 us (instructions: 40 to an element of a warp, most of them addresses and the
+// sums over warps); 40003 x 771 bf16 50 and 177 us (255 registers, one block to an SM: waiting); packing 88, unpacking 109 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
