@@ -483,19 +483,36 @@ __device__ __forceinline__ void warps_sum(float (&t)[Q], float* red, int v, int 
     }
 }
 
-// eight rows at a time, all read before the first is written: one row after the other would wait for memory once a row
-template <int V, typename T>
-__device__ __forceinline__ void read_rows(T* tile, int pitch, const T* rows, int64_t ld, int r0, int step, int l, int wide, int count, int units) {
-    for (int u = l; u < units; u += wide)
-        for (int r = r0; r < count; r += step * 8) {
-            T t[8];
+// rows of `from` to rows of `to`, B at a time: all are read before the first is written (one row after the other waits once
+// a row: 76 us of 213 forward)
+template <int B, typename T>
+__device__ __forceinline__ void copy_batch(T* to, int64_t to_ld, const T* from, int64_t from_ld, int first, int step, int count) {
+    T t[B];
+    for (int r = first; r < count; r += step * B) {
+        const T* p = from + r * from_ld;
+        T* q = to + r * to_ld;
+        if (r + (B - 1) * step < count) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (r + k * step < count) t[k] = rows[(r + k * step) * ld + u];
+            for (int k = 0; k < B; ++k) t[k] = p[k * step * from_ld];
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (r + k * step < count) tile[(r + k * step) * pitch + u] = t[k];
+            for (int k = 0; k < B; ++k) q[k * step * to_ld] = t[k];
+        } else {
+            for (int k = 0; r + k * step < count; ++k) q[k * step * to_ld] = p[k * step * from_ld];
         }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void copy_rows(T* to, int64_t to_ld, const T* from, int64_t from_ld, int r0, int step, int l, int wide, int count, int units) {
+    if (count > 7 * step) {
+        for (int u = l; u < units; u += wide) copy_batch<8>(to + u, to_ld, from + u, from_ld, r0, step, count);
+    } else if (count > 3 * step) {
+        for (int u = l; u < units; u += wide) copy_batch<4>(to + u, to_ld, from + u, from_ld, r0, step, count);
+    } else {  // fewer rows to a warp: places of a row
+        for (int r = r0; r < count; r += step) {
+            if (units > 7 * wide) copy_batch<8>(to + r * to_ld, 1, from + r * from_ld, 1, l, wide, units);
+            else copy_batch<4>(to + r * to_ld, 1, from + r * from_ld, 1, l, wide, units);
+        }
+    }
 }
 
 // (32 Q, pitch) of T in shared memory <-> rows of c elements, ld apart; T2: two of them
@@ -506,21 +523,16 @@ __device__ __forceinline__ void tile_rows(T* tile, int pitch, T* rows, int64_t l
     const int per = 32 / wide, l = lane & (wide - 1);
     const int r0 = (threadIdx.x >> 5) * per + lane / wide;
     if constexpr (STORE) {
-        for (int r = r0; r < count; r += V * per) {
-            if (pairs)
-                for (int u = l; u < units; u += wide) reinterpret_cast<T2*>(rows + r * ld)[u] = reinterpret_cast<const T2*>(tile + r * pitch)[u];
-            else
-                for (int u = l; u < units; u += wide) rows[r * ld + u] = tile[r * pitch + u];
-        }
-    } else if (pairs) {
-        read_rows<V, T2>(reinterpret_cast<T2*>(tile), pitch / 2, reinterpret_cast<const T2*>(rows), ld / 2, r0, V * per, l, wide, count, units);
+        if (pairs) copy_rows<T2>(reinterpret_cast<T2*>(rows), ld / 2, reinterpret_cast<const T2*>(tile), pitch / 2, r0, V * per, l, wide, count, units);
+        else copy_rows<T>(rows, ld, tile, pitch, r0, V * per, l, wide, count, units);
     } else {
-        read_rows<V, T>(tile, pitch, rows, ld, r0, V * per, l, wide, count, units);
+        if (pairs) copy_rows<T2>(reinterpret_cast<T2*>(tile), pitch / 2, reinterpret_cast<const T2*>(rows), ld / 2, r0, V * per, l, wide, count, units);
+        else copy_rows<T>(tile, pitch, rows, ld, r0, V * per, l, wide, count, units);
     }
 }
 
 template <int NV, int V, int Q, bool BWD>
-__global__ void __launch_bounds__(V * 32, V == 4 ? (BWD ? 5 : 8) : V == 8 ? (BWD ? 3 : 4) : V == 16 ? (BWD ? 1 : 2) : 1) rgs_norm_planes_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(V * 32, V == 4 ? (BWD ? 5 : 8) : V == 8 ? (NV == 16 ? (BWD ? 2 : 3) : (BWD ? 3 : 4)) : V == 16 ? (BWD ? 1 : 2) : 1) rgs_norm_planes_kernel(const __grid_constant__ NormArgs a) {
     extern __shared__ float sm[];
     constexpr int T = 32 * Q;                           // pixels of a tile
     float* red = sm;                                    // three sums of V x T, w and b, then the tile of y or dy
