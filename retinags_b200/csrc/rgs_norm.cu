@@ -47,6 +47,12 @@ struct NormArgs {
     void* dw; void* db;                            // written at once when the grid is one block
 };
 
+// Whether vector k of a lane can reach outside the row.  The widths that a kernel of vectors of four takes fill all but its
+// last vectors (norm_rows_vec), so only these, and the first one of shifted rows, are tested and masked.
+template <int VEC, int NV, int LANES, bool SHIFT>
+__device__ __forceinline__ constexpr bool maybe_out(int k) {
+    return VEC == 1 || (LANES == 1 && NV == 3) || (SHIFT && k == 0) || k >= NV - (SHIFT ? 2 : 1);
+}
 // The switch on a type stands outside the loops over a row's vectors, so that all loads of a row are in flight together
 // (inside, every load waited for the one before: 3 to 4 times slower on wide or odd rows).
 template <int VEC, int DT>
@@ -71,7 +77,9 @@ __device__ __forceinline__ void load_all(const void* p, int64_t i, int l, int s,
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int at = (k * LANES + l) * VEC - (SHIFT ? s : 0);
-        if (EDGE && at < c && at + VEC > c) {
+        if (!maybe_out<VEC, NV, LANES, SHIFT>(k)) {
+            load_vec<VEC, DT>(p, i + at, x[k]);
+        } else if (EDGE && at < c && at + VEC > c) {
 #pragma unroll
             for (int q = 0; q < VEC; ++q) {
                 float f[1] = {0.f};
@@ -88,7 +96,7 @@ __device__ __forceinline__ void load_all(const void* p, int64_t i, int l, int s,
     if (SHIFT) {  // the first and the last vector of the row hold elements of its neighbours
 #pragma unroll
         for (int k = 0; k < NV; ++k)
-            if (k == 0 || (k + 1) * LANES * VEC > c)
+            if (maybe_out<VEC, NV, LANES, SHIFT>(k))
 #pragma unroll
                 for (int q = 0; q < VEC; ++q) {
                     const int at = (k * LANES + l) * VEC - s + q;
@@ -118,12 +126,12 @@ __device__ __forceinline__ void store_all(void* p, int64_t i, int l, int s, int 
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int at = (k * LANES + l) * VEC - (SHIFT ? s : 0);
-        if (SHIFT ? at >= 0 && at + VEC <= c : at < c) store_vec<VEC, DT>(p, i + at, x[k]);
+        if (!maybe_out<VEC, NV, LANES, SHIFT>(k) || (SHIFT ? at >= 0 && at + VEC <= c : at < c)) store_vec<VEC, DT>(p, i + at, x[k]);
     }
     if (SHIFT) {
 #pragma unroll
         for (int k = 0; k < NV; ++k)
-            if (k == 0 || ((k + 1) * LANES * VEC > c && k * LANES * VEC < c + 3)) {
+            if (maybe_out<VEC, NV, LANES, SHIFT>(k)) {
                 const int at = (k * LANES + l) * VEC - s;
                 if (at < 0 || (at + VEC > c && at < c))
 #pragma unroll
@@ -203,8 +211,7 @@ __device__ __forceinline__ void row_stats(const float (&x)[NV][VEC], int l, int 
     for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int q = 0; q < VEC; ++q) {
-            const bool whole = (k + 1) * LANES * VEC <= c && (!SHIFT || k > 0);  // (the same for all lanes)
-            const float d = whole || in_row<VEC, LANES, SHIFT>(k, q, l, s0, c) ? x[k][q] - mu : 0.f;
+            const float d = !maybe_out<VEC, NV, LANES, SHIFT>(k) || in_row<VEC, LANES, SHIFT>(k, q, l, s0, c) ? x[k][q] - mu : 0.f;
             s = fmaf(d, d, s);
         }
     rstd = rsqrtf(group_sum<LANES>(s) * inv_c + eps);  // within two units in the last place
@@ -384,7 +391,7 @@ __global__ void __launch_bounds__(NT, NV * VEC <= 16 ? 4 : NV * VEC <= 24 ? 3 : 
 }
 
 template <int VEC, int NV, int LANES, bool SHIFT>
-__global__ void __launch_bounds__(NT, NV * VEC <= 12 ? 3 : NV * VEC <= 24 ? 2 : 1) rgs_norm_rows_bwd_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(NT, NV * VEC <= 12 ? 3 : NV * VEC <= (SHIFT ? 24 : 16) ? 2 : 1) rgs_norm_rows_bwd_kernel(const __grid_constant__ NormArgs a) {
     constexpr int GROUPS = NT / LANES;
     constexpr int ROW = NV * LANES * VEC, COPIES = SHIFT ? 4 : 1, SUMS = NT * VEC + (SHIFT ? 3 * GROUPS : 0);
     __shared__ __align__(16) float sh[COPIES * ROW > SUMS ? COPIES * ROW : SUMS];
@@ -399,8 +406,7 @@ __global__ void __launch_bounds__(NT, NV * VEC <= 12 ? 3 : NV * VEC <= 24 ? 2 : 
     for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int q = 0; q < VEC; ++q) sw[k][q] = sb[k][q] = 0.f;
-    auto turn = [&](int64_t row, bool there, auto edge) {
-        float x[NV][VEC], g[NV][VEC];
+    auto fetch = [&](int64_t row, bool there, auto edge, float (&x)[NV][VEC], float (&g)[NV][VEC]) {
         if (there) {
             load_row<VEC, NV, LANES, SHIFT, decltype(edge)::value>(a, row, l, s, x);
             load_typed<VEC, NV, LANES, SHIFT, decltype(edge)::value>(a.dy, a.dy_dtype, row * a.ldy, l, s, a.c, g);
@@ -410,15 +416,40 @@ __global__ void __launch_bounds__(NT, NV * VEC <= 12 ? 3 : NV * VEC <= 24 ? 2 : 
 #pragma unroll
                 for (int q = 0; q < VEC; ++q) x[k][q] = g[k][q] = 0.f;
         }
+    };
+    auto turn = [&](int64_t row, bool there, float (&x)[NV][VEC], float (&g)[NV][VEC]) {
         __syncwarp();
         // (a row that is not there adds none to the sums: with eps = 0 its rstd would be infinite)
         row_bwd<VEC, NV, LANES, SHIFT>(x, g, w, sw, sb, l, s, a.c, a.inv_c, there ? a.eps : 1.f);
         if (a.dx && there) store_typed<VEC, NV, LANES, SHIFT>(a.dx, a.dx_dtype, row * a.c, l, s, a.c, x);
         __syncwarp();
     };
-    const int64_t rows = SHIFT ? a.n - 1 : a.n;
-    for (int64_t i = (int64_t)blockIdx.x * GROUPS; i < rows; i += stride) turn(i + threadIdx.x / LANES, i + threadIdx.x / LANES < rows, std::false_type());
-    if (SHIFT && blockIdx.x == 0) turn(rows, threadIdx.x / LANES == (rows & 3), std::true_type());
+    const int64_t rows = SHIFT ? a.n - 1 : a.n, mine = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES;
+    float x[NV][VEC], g[NV][VEC];
+    if constexpr (NV * VEC >= 20 && !SHIFT) {
+        // one block to an SM: the next row is on its way while this one is worked on (771 shifted channels have no registers
+        // left for it: 177 -> 284 us; 772 channels 114 -> 99 us)
+        fetch(mine, mine < rows, std::false_type(), x, g);
+        for (int64_t i = mine - threadIdx.x / LANES, row = mine; i < rows; i += stride, row += stride) {
+            float nx[NV][VEC], ng[NV][VEC];
+            fetch(row + stride, row + stride < rows, std::false_type(), nx, ng);
+            turn(row, row < rows, x, g);
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) { x[k][q] = nx[k][q]; g[k][q] = ng[k][q]; }
+        }
+    } else {
+        for (int64_t i = mine - threadIdx.x / LANES, row = mine; i < rows; i += stride, row += stride) {
+            fetch(row, row < rows, std::false_type(), x, g);
+            turn(row, row < rows, x, g);
+        }
+    }
+    if (SHIFT && blockIdx.x == 0) {
+        const bool there = threadIdx.x / LANES == (rows & 3);
+        fetch(rows, there, std::true_type(), x, g);
+        turn(rows, there, x, g);
+    }
     if (a.part) block_sums<VEC, NV, LANES, SHIFT>(a, l, s, sw, sb, sh);
 }
 

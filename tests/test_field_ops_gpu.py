@@ -369,3 +369,19 @@ def test_layer_norm_with_eps_zero():
         y = R.layer_norm(leaf, w, eps=0.0)
         gx, gw = torch.autograd.grad(y.square().sum(), [leaf, w])
         assert torch.isfinite(y).all() and torch.isfinite(gx).all() and torch.isfinite(gw).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_layer_norm_every_width(dtype):
+    """Every number of channels up to the widest that a group of lanes holds: the number of vectors and lanes, and which of them
+    are tested against the row's end, follow from it."""
+    g = torch.Generator().manual_seed(3)
+    x, dy = torch.randn(6, 1030, generator=g).to(dtype).cuda(), torch.randn(6, 1030, generator=g).cuda()
+    w, b = torch.rand(1030, generator=g).cuda() + 0.5, torch.randn(1030, generator=g).cuda()
+    for c in range(1, 1031):
+        args = [t[..., :c].contiguous() for t in (x, w, b, dy)]
+        ref = norm_reference(*args, 1e-5, args[0], F32, dtype, F32)
+        leaves = [t.requires_grad_(True) for t in args[:3]]
+        y = R.layer_norm(*leaves, out_dtype=F32)
+        for name, got, r in zip(("y", "dx", "dw", "db"), (y.detach(), *torch.autograd.grad(y, leaves, args[3])), ref):
+            assert_within(got, r, f"{name} of {c} channels")
