@@ -385,3 +385,14 @@ def test_layer_norm_every_width(dtype):
         y = R.layer_norm(*leaves, out_dtype=F32)
         for name, got, r in zip(("y", "dx", "dw", "db"), (y.detach(), *torch.autograd.grad(y, leaves, args[3])), ref):
             assert_within(got, r, f"{name} of {c} channels")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_label_loss_every_width_and_every_remainder(dtype):
+    """Channels 1 to 270 (chunks, stages and what stays in shared memory follow from them), then pixels and labels around the
+    tile of 128."""
+    for c in list(range(1, 271)) + [319, 320, 321, 383, 384, 385, 511, 513, 576, 640]:
+        _check_label(*make_label_case(131, c, 140, dtype, seed=c, device="cuda"))
+    for k in list(range(1, 20)) + [63, 64, 65, 127, 128, 129, 191, 192, 193, 255, 256, 257, 383, 384, 385]:
+        _check_label(*make_label_case(k, 40, 131, dtype, seed=k, device="cuda"))
+        _check_label(*make_label_case(133, 72, k, dtype, seed=k, device="cuda"))
