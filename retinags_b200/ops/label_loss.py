@@ -37,15 +37,16 @@ class _LabelLoss(torch.autograd.Function):
         v = w.shape[0]
         per_row = reduction == "none"
         new = torch.empty if n else torch.zeros
-        lse = torch.empty(2, n, dtype=torch.float32, device=dev)
+        # kept for the backward pass: m and log z of every pixel, number of pixels that count, flags
+        state = torch.empty(2 * n + 2, dtype=torch.float32, device=dev)
+        lse = state.data_ptr()
         losses = torch.empty(n, dtype=torch.float32, device=dev) if per_row else None
         result = None if per_row else new((), dtype=torch.float32, device=dev)
-        count = new(2, dtype=torch.float32, device=dev)
         b_code = DTYPES[bias.dtype] if bias is not None else 0
         if n:
             native.call("label_fwd", dev, x, ldx, w, ldw, bias, y, y.element_size(), n, c, v, DTYPES[x.dtype], b_code,
-                        int(reduction == "mean"), _scratch(x, ldx, w, ldw, 0), lse, losses, result, count)
-        ctx.save_for_backward(x, w, bias, y, lse, count)
+                        int(reduction == "mean"), _scratch(x, ldx, w, ldw, 0), lse, losses, result, lse + 8 * n)
+        ctx.save_for_backward(x, w, bias, y, state)
         ctx.args = (features.shape, weight.shape, ldx, ldw, b_code, reduction)
         return losses.view(features.shape[:-1]) if per_row else result
 
@@ -56,7 +57,7 @@ class _LabelLoss(torch.autograd.Function):
 
 
 def _label_backward(ctx, gout):
-    x, w, bias, y, lse, count = ctx.saved_tensors
+    x, w, bias, y, state = ctx.saved_tensors
     x_shape, w_shape, ldx, ldw, b_code, reduction = ctx.args
     dev = x.device
     n, c = x.shape
@@ -67,8 +68,8 @@ def _label_backward(ctx, gout):
     dw = new(w_shape, dtype=w.dtype, device=dev) if ctx.needs_input_grad[1] else None
     db = new(v, dtype=bias.dtype, device=dev) if ctx.needs_input_grad[2] else None
     if n and (dx is not None or dw is not None or db is not None):
-        native.call("label_bwd", dev, x, ldx, w, ldw, bias, y, y.element_size(), n, c, v, DTYPES[x.dtype], b_code, lse, g,
-                    int(reduction == "none"), int(reduction == "mean"), count,
+        native.call("label_bwd", dev, x, ldx, w, ldw, bias, y, y.element_size(), n, c, v, DTYPES[x.dtype], b_code, state, g,
+                    int(reduction == "none"), int(reduction == "mean"), state.data_ptr() + 8 * n,
                     _scratch(x, ldx, w, ldw, 1), dx, dw, db)
     return dx, dw, db, None, None
 

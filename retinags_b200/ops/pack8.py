@@ -40,7 +40,7 @@ def as_rows(x: torch.Tensor, what: str, planes_ok: bool = True):
     if n == 0:
         return x.reshape(0, c), c, 0
     if x.is_contiguous():
-        return x.view(n, c), c, 0
+        return x if x.dim() == 2 else x.view(n, c), c, 0
     try:
         flat = x.view(n, c)
     except RuntimeError:
