@@ -15,10 +15,11 @@
 // Codes of such rows are read element by element throughout.  Channel planes (the renderer's images) are read with a lane to
 // a pixel and turned into rows in shared memory.  Beyond 1024 channels a warp re-reads its row.
 //
-// Measured (a copy moves 6.5 TB/s): 1657600 rows x 64 channels, float32 in, bf16 out: forward 104 us (6.1 TB/s), with the
-// 8-bit copy 135 us (5.5 TB/s), backward 192 us (5.5 TB/s), from codes 200 us (3.7 TB/s: the arithmetic of decoding shares
-// the time); the same from planes 204 and 406 us (instructions: 40 to an element of a warp, most of them addresses and the
-// sums over warps); 40003 x 771 bf16 50 and 177 us (255 registers, one block to an SM: waiting); packing 88, unpacking 109 us.
+// Measured (a copy moves 6.5 TB/s): 1657600 rows x 64 channels, float32 in, bf16 out: forward 107 us (5.9 TB/s), with the
+// 8-bit copy 128 us (5.8 TB/s), backward 198 us (5.4 TB/s), from codes 211 us (3.5 TB/s: the arithmetic of decoding shares
+// the time); the same from planes 194 and 309 us (instructions: two thirds of the issue slots, most of them addresses and
+// the sums over warps); 40003 x 771 bf16 46 and 136 us (backward: 255 registers, one block to an SM, a quarter of the issue
+// slots: waiting, although the next row is on its way); packing 92, unpacking 117 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
