@@ -1091,7 +1091,7 @@ int rgs_cuda_unpack8(const int8_t* codes, const uint8_t* expo, int64_t planes, i
     cudaStream_t st = (cudaStream_t)stream;
     NormArgs a{};
     a.codes = codes; a.expo = expo; a.planes = (int)planes; a.n = n; a.c = (int)c; a.blocks = (int)((c + 31) / 32);
-    if ((planes ? n : c) % 4 == 0)
+    if ((planes ? n : c) % 4 == 0 && aligned_to(codes, 4))  // (codes may be a slice that begins at any byte)
         rgs_unpack8_kernel<4><<<(unsigned)norm_grid((n * c / 4 + NT * 4 - 1) / (NT * 4), 32), NT, 0, st>>>(a, !planes && c % 32 == 0, out, (int)dtype);
     else
         rgs_unpack8_kernel<1><<<(unsigned)norm_grid((n * c + NT * 4 - 1) / (NT * 4), 32), NT, 0, st>>>(a, 0, out, (int)dtype);

@@ -60,6 +60,11 @@ def empty_like_layout(shape, planes: int, dtype, device) -> torch.Tensor:
     return torch.empty(tuple(shape), dtype=dtype, device=device)
 
 
+def _dense(t: torch.Tensor, planes: int) -> torch.Tensor:
+    """``t`` in the order in which it is read: dense rows, or dense planes as (C, ...); a copy only if it is a slice or a view."""
+    return (t.movedim(-1, 0) if planes else t).contiguous()
+
+
 @dataclass
 class Packed8:
     """Codes (..., C) int8 and exponent bytes (..., ceil(C/32)) uint8, both stored in the layout of the packed tensor."""
@@ -82,11 +87,23 @@ class Packed8:
         dtype = self.dtype if dtype is None else dtype
         if dtype not in DTYPES:
             raise TypeError(f"unpack: float32 or bfloat16 expected, got {dtype}")
-        out = empty_like_layout(self.shape, self.planes, dtype, self.codes.device)
-        c = self.shape[-1]
-        n = self.codes.numel() // c
+        codes, exponents = self.codes, self.exponents
+        if codes.dtype != torch.int8 or exponents.dtype != torch.uint8:
+            raise TypeError(f"unpack: int8 codes and uint8 exponents expected, got {codes.dtype} and {exponents.dtype}")
+        if codes.dim() < 1 or codes.shape[-1] < 1:
+            raise ValueError(f"unpack: codes (..., C) with at least one channel expected, got {tuple(codes.shape)}")
+        c = codes.shape[-1]
+        if exponents.shape != (*codes.shape[:-1], (c + BLOCK - 1) // BLOCK):
+            raise ValueError(f"unpack: one exponent to {BLOCK} channels expected, got {tuple(exponents.shape)} for {tuple(codes.shape)}")
+        if exponents.device != codes.device:
+            raise ValueError(f"unpack: exponents on {codes.device} expected, got {exponents.device}")
+        n = codes.numel() // c
+        if n > 2 ** 31 - 1:
+            raise ValueError(f"unpack: at most 2^31 - 1 rows, got {n}")
+        out = empty_like_layout(codes.shape, self.planes, dtype, codes.device)
         if n:
-            native.call("unpack8", self.codes.device, self.codes, self.exponents, self.planes, n, c, out, DTYPES[dtype])
+            native.call("unpack8", codes.device, _dense(codes, self.planes), _dense(exponents, self.planes), int(bool(self.planes)), n, c,
+                        out, DTYPES[dtype])
         return out
 
 

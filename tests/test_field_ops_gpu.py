@@ -396,3 +396,24 @@ def test_label_loss_every_width_and_every_remainder(dtype):
     for k in list(range(1, 20)) + [63, 64, 65, 127, 128, 129, 191, 192, 193, 255, 256, 257, 383, 384, 385]:
         _check_label(*make_label_case(k, 40, 131, dtype, seed=k, device="cuda"))
         _check_label(*make_label_case(133, 72, k, dtype, seed=k, device="cuda"))
+
+
+@pytest.mark.parametrize("planes", [False, True])
+@pytest.mark.parametrize("n,c", [(24, 64), (24, 36), (23, 33)])
+def test_unpack_of_parts_and_of_codes_at_any_byte(n, c, planes):
+    x = torch.randn(n, c, generator=torch.Generator().manual_seed(2)) * torch.arange(1, n + 1)[:, None]
+    p = R.pack8((x.t().contiguous().t() if planes else x).cuda())
+    whole = p.unpack()
+    assert torch.equal(whole.cpu().double(), pack_reference(x))
+    for part in (slice(None, None, 2), slice(3, 9), slice(5, 6)):
+        assert torch.equal(R.Packed8(p.codes[part], p.exponents[part], p.planes, F32).unpack(), whole[part])
+    for at in (1, 2, 3, 4):  # dense codes that begin inside a larger buffer
+        parts = []
+        for t in (p.codes, p.exponents):
+            t = t.movedim(-1, 0) if planes else t
+            room = torch.empty(t.numel() + 8, dtype=t.dtype, device="cuda")[at:at + t.numel()].view(t.shape).copy_(t)
+            parts.append(room.movedim(0, -1) if planes else room)
+        assert parts[0].data_ptr() % 4 == at % 4
+        assert torch.equal(R.Packed8(*parts, p.planes, F32).unpack(), whole)
+    with pytest.raises(ValueError):
+        R.Packed8(p.codes, p.exponents.cpu(), p.planes, F32).unpack()

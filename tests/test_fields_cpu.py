@@ -227,6 +227,24 @@ def test_pack8_edges_and_refusals():
         p.unpack(torch.float16)
 
 
+@pytest.mark.parametrize("planes", [False, True])
+def test_unpack_of_parts_and_of_codes_that_do_not_fit(planes):
+    x = torch.randn(12, 70, generator=torch.Generator().manual_seed(2)) * torch.arange(1, 13)[:, None]
+    p = R.pack8(x.t().contiguous().t() if planes else x)
+    assert p.planes == int(planes)
+    whole = p.unpack()
+    for part in (slice(None, None, 2), slice(3, 9), slice(5, 6)):
+        assert torch.equal(R.Packed8(p.codes[part], p.exponents[part], p.planes, F32).unpack(), whole[part])
+    assert torch.equal(R.Packed8(p.codes[:, 32:], p.exponents[:, 1:], p.planes, F32).unpack(), whole[:, 32:])
+    assert torch.equal(R.Packed8(p.codes, p.exponents, 1 - p.planes, F32).unpack(), whole)  # the other order: copied
+    for err, codes, exponents in [(ValueError, p.codes, p.exponents[:, :2]), (ValueError, p.codes[:, :64], p.exponents),
+                                  (ValueError, p.codes, p.exponents[:6]), (ValueError, p.codes, p.exponents.to("meta")),
+                                  (TypeError, p.codes.int(), p.exponents), (TypeError, p.codes, p.exponents.char()),
+                                  (ValueError, p.codes[:, :0], p.exponents[:, :0]), (ValueError, p.codes[0, 0], p.exponents[0, 0])]:
+        with pytest.raises(err):
+            R.Packed8(codes, exponents, p.planes, F32).unpack()
+
+
 def test_label_field_on_rendered_features():
     """Features of splats rendered by the rasteriser, normed in 8 bits, scored against labels: gradients reach the splats."""
     from helpers import activated, small_scene
