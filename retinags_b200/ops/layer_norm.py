@@ -97,6 +97,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         bias = _param(x, bias, shape[-1], "bias")
         if weight is not None and weight.dtype != bias.dtype:
             raise TypeError(f"layer_norm: weight and bias of one type expected, got {weight.dtype} and {bias.dtype}")
+    if not torch.is_grad_enabled():
+        keep = "input"  # no backward pass will read codes
     return _LayerNorm.apply(x, weight, bias, float(eps), out_dtype, keep)
 
 

@@ -175,6 +175,17 @@ def test_layer_norm_does_not_hold_its_input_in_8_bits():
     assert sum(t.numel() * t.element_size() for t in held) == 64 * 96 + 64 * 3
 
 
+def test_layer_norm_makes_no_codes_without_gradients(monkeypatch):
+    made = []
+    from retinags_b200.ops import layer_norm as module
+    alloc = module.alloc_codes
+    monkeypatch.setattr(module, "alloc_codes", lambda *a: (made.append(1), alloc(*a))[1])
+    x, w = torch.randn(5, 40), torch.rand(40, requires_grad=True)
+    with torch.no_grad():
+        y = R.layer_norm(x, w, keep="int8")
+    assert not made and torch.equal(y, R.layer_norm(x, w, keep="int8").detach()) and made
+
+
 def test_layer_norm_refusals():
     x, w = torch.randn(4, 6), torch.ones(6)
     bad = [(TypeError, dict(x=x.half())), (TypeError, dict(out_dtype=torch.float16)), (ValueError, dict(keep="fp8")),
