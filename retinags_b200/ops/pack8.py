@@ -25,7 +25,13 @@ def dtype_code(t: torch.Tensor, what: str) -> int:
     code = DTYPES.get(t.dtype)
     if code is None:
         raise TypeError(f"{what}: float32 or bfloat16 expected, got {t.dtype}")
+    check_device(t, what)
     return code
+
+
+def check_device(t: torch.Tensor, what: str) -> None:
+    if not (t.is_cuda or t.is_cpu):
+        raise ValueError(f"{what}: a tensor on the CPU or a CUDA device expected, got {t.device}")
 
 
 def as_rows(x: torch.Tensor, what: str, planes_ok: bool = True):
@@ -88,6 +94,7 @@ class Packed8:
         if dtype not in DTYPES:
             raise TypeError(f"unpack: float32 or bfloat16 expected, got {dtype}")
         codes, exponents = self.codes, self.exponents
+        check_device(codes, "unpack")
         if codes.dtype != torch.int8 or exponents.dtype != torch.uint8:
             raise TypeError(f"unpack: int8 codes and uint8 exponents expected, got {codes.dtype} and {exponents.dtype}")
         if codes.dim() < 1 or codes.shape[-1] < 1:

@@ -256,6 +256,15 @@ def test_unpack_of_parts_and_of_codes_that_do_not_fit(planes):
             R.Packed8(codes, exponents, p.planes, F32).unpack()
 
 
+def test_tensors_without_memory_are_refused():
+    x, w = torch.zeros(3, 8, device="meta"), torch.zeros(5, 8, device="meta")
+    codes, exponents = torch.zeros(3, 8, dtype=torch.int8, device="meta"), torch.zeros(3, 1, dtype=torch.uint8, device="meta")
+    for fn in (lambda: R.layer_norm(x), lambda: R.pack8(x), lambda: R.label_loss(x, w, torch.zeros(3, dtype=torch.long, device="meta")),
+               lambda: R.Packed8(codes, exponents, 0, F32).unpack()):
+        with pytest.raises(ValueError, match="meta"):
+            fn()
+
+
 def test_label_field_on_rendered_features():
     """Features of splats rendered by the rasteriser, normed in 8 bits, scored against labels: gradients reach the splats."""
     from helpers import activated, small_scene
