@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import native
-from .pack8 import DTYPES, as_rows, dtype_code
+from .pack8 import DTYPES, as_rows, dtype_code, restored, saved_as
 
 MAX_CHANNELS = 1024
 _REDUCTIONS = ("mean", "sum", "none")
@@ -47,7 +47,7 @@ class _LabelLoss(torch.autograd.Function):
             native.call("label_fwd", dev, x, ldx, w, ldw, bias, y, y.element_size(), n, c, v, DTYPES[x.dtype], b_code,
                         int(reduction == "mean"), _scratch(x, ldx, w, ldw, 0), lse, losses, result, lse + 8 * n)
         ctx.save_for_backward(x, w, bias, y, state)
-        ctx.args = (features.shape, weight.shape, ldx, ldw, b_code, reduction)
+        ctx.args = (features.shape, weight.shape, saved_as(x, w, bias, y, state), b_code, reduction)
         return losses.view(features.shape[:-1]) if per_row else result
 
     @staticmethod
@@ -57,8 +57,11 @@ class _LabelLoss(torch.autograd.Function):
 
 
 def _label_backward(ctx, gout):
-    x, w, bias, y, state = ctx.saved_tensors
-    x_shape, w_shape, ldx, ldw, b_code, reduction = ctx.args
+    x_shape, w_shape, kinds, b_code, reduction = ctx.args
+    x, w, bias, y, state = restored(ctx.saved_tensors, kinds, "label_loss")
+    x, ldx, _ = as_rows(x, "label_loss", planes_ok=False)
+    w, ldw, _ = as_rows(w, "label_loss", planes_ok=False)
+    bias, y, state = bias.contiguous() if bias is not None else None, y.contiguous(), state.contiguous()
     dev = x.device
     n, c = x.shape
     v = w.shape[0]

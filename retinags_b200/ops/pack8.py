@@ -59,6 +59,21 @@ def as_rows(x: torch.Tensor, what: str, planes_ok: bool = True):
     return flat.contiguous(), c, 0
 
 
+def saved_as(*tensors):
+    """What ``restored`` asks of tensors kept for a backward pass."""
+    return tuple(None if t is None else (t.shape, t.dtype, t.device) for t in tensors)
+
+
+def restored(tensors, kinds, what: str):
+    """Tensors as autograd gives them back.  Saved-tensor hooks (offloading, compression) may restore them with other strides, so
+    nothing about their layout is kept across the passes; another shape, type or device is refused."""
+    for t, kind in zip(tensors, kinds):
+        if kind is not None and (t is None or (t.shape, t.dtype, t.device) != kind):
+            got = "nothing" if t is None else f"{t.dtype} of shape {tuple(t.shape)} on {t.device}"
+            raise RuntimeError(f"{what}: a saved tensor came back as {got}, {kind[1]} of shape {tuple(kind[0])} on {kind[2]} expected")
+    return tensors
+
+
 def empty_like_layout(shape, planes: int, dtype, device) -> torch.Tensor:
     """Tensor (..., C) stored as dense rows, or as dense channel planes."""
     if planes:
@@ -66,7 +81,7 @@ def empty_like_layout(shape, planes: int, dtype, device) -> torch.Tensor:
     return torch.empty(tuple(shape), dtype=dtype, device=device)
 
 
-def _dense(t: torch.Tensor, planes: int) -> torch.Tensor:
+def dense(t: torch.Tensor, planes: int) -> torch.Tensor:
     """``t`` in the order in which it is read: dense rows, or dense planes as (C, ...); a copy only if it is a slice or a view."""
     return (t.movedim(-1, 0) if planes else t).contiguous()
 
@@ -109,7 +124,7 @@ class Packed8:
             raise ValueError(f"unpack: at most 2^31 - 1 rows, got {n}")
         out = empty_like_layout(codes.shape, self.planes, dtype, codes.device)
         if n:
-            native.call("unpack8", codes.device, _dense(codes, self.planes), _dense(exponents, self.planes), int(bool(self.planes)), n, c,
+            native.call("unpack8", codes.device, dense(codes, self.planes), dense(exponents, self.planes), int(bool(self.planes)), n, c,
                         out, DTYPES[dtype])
         return out
 

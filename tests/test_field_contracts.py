@@ -1,0 +1,108 @@
+"""Label loss, layer norm and 8-bit features where callers meet them from the side: saved-tensor hooks, layouts of gradients,
+limits inside the accepted ranges.  Every case runs on the CPU backend and on the GPU."""
+import pytest
+import torch
+
+import retinags_b200 as R
+from field_reference import make_label_case
+
+F32, BF16 = torch.float32, torch.bfloat16
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _dense_copy(t):
+    """The values, densely, inside a larger buffer: other strides and another alignment."""
+    room = torch.zeros(4 * t.numel() + 9, dtype=t.dtype, device=t.device)
+    return room[5:5 + t.numel()].view(t.shape).copy_(t)
+
+
+def _wide_copy(t):
+    """The values with gaps between the rows."""
+    if t.dim() == 0:
+        return t.clone()
+    room = torch.zeros(*t.shape[:-1], 2 * t.shape[-1] + 3, dtype=t.dtype, device=t.device)
+    return room[..., 1:2 * t.shape[-1] + 1:2].copy_(t)
+
+
+def _other_order(t):
+    return t.movedim(-1, 0).contiguous().movedim(0, -1) if t.dim() > 1 else t.clone()
+
+
+COPIES = [_dense_copy, _wide_copy, _other_order]
+
+
+@pytest.mark.parametrize("copy", COPIES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("device", DEVICES)
+def test_label_loss_takes_its_saved_tensors_in_any_layout(device, dtype, copy):
+    x, w, y, b = make_label_case(60, 24, 17, dtype, seed=2, device=device)
+    wide, ww = torch.zeros(61, 40, dtype=dtype, device=device), torch.zeros(18, 41, dtype=dtype, device=device)
+    wide[:60, 8:32], ww[1:, 7:31] = x, w
+    for f, v in ((x, w), (wide[:60, 8:32], w), (x, ww[1:, 7:31]), (x.t().contiguous().t(), w), (wide[:60, 8:32].view(5, 12, 24), w)):
+        leaves = [t.detach().requires_grad_(True) for t in (f, v, b)]
+        labels = y.view(f.shape[:-1])
+        for reduction in ("mean", "none"):
+            up = torch.rand(labels.shape, generator=torch.Generator().manual_seed(1)).to(device) if reduction == "none" else None
+            out = R.label_loss(leaves[0], leaves[1], labels, bias=leaves[2], reduction=reduction)
+            want = torch.autograd.grad(out, leaves, up)
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone() if t is not None else t, copy):
+                out = R.label_loss(leaves[0], leaves[1], labels, bias=leaves[2], reduction=reduction)
+            got = torch.autograd.grad(out, leaves, up)
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("copy", COPIES)
+@pytest.mark.parametrize("keep", ["input", "int8"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("device", DEVICES)
+def test_layer_norm_takes_its_saved_tensors_in_any_layout(device, dtype, keep, copy):
+    gen = torch.Generator().manual_seed(4)
+    for n, c in ((35, 24), (1, 40), (35, 33), (6, 600)):
+        x, dy = torch.randn(n, c, generator=gen).to(dtype).to(device), torch.randn(n, c, generator=gen).to(dtype).to(device)
+        w, b = (torch.rand(c, generator=gen).to(device).requires_grad_(True) for _ in range(2))
+        wide = torch.zeros(n + 1, c + 11, dtype=dtype, device=device)
+        wide[:n, 4:c + 4] = x
+        for f in (x, x.t().contiguous().t(), wide[:n, 4:c + 4], wide[:n, 4:c + 4].t().contiguous().t()):
+            leaf = f.detach().requires_grad_(True)
+            want = torch.autograd.grad(R.layer_norm(leaf, w, b, keep=keep), [leaf, w, b], dy)
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), copy):
+                y = R.layer_norm(leaf, w, b, keep=keep)
+            got = torch.autograd.grad(y, [leaf, w, b], dy)
+            assert got[0].stride() == want[0].stride()
+            # another layout may take another kernel, which adds in another order.  Two sums of 35 rows with |dy xhat| about 22
+            # in all: 2 * 39 * 2^-24 * 22 = 1e-4; means over 600 channels: 2 * 606 * 2^-24 = 7e-5; 16-bit outputs may then
+            # round to the neighbour, 2^-7 of the value
+            for p, q in zip(got, want):
+                torch.testing.assert_close(p, q, atol=2e-4, rtol=0 if p.dtype == F32 else 2.0 ** -7)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_save_on_cpu_and_planes(device):
+    planes = torch.randn(24, 5, 7, generator=torch.Generator().manual_seed(4)).to(device)
+    w, v = (torch.randn(24, generator=torch.Generator().manual_seed(5)).to(device).requires_grad_(True),
+            torch.randn(9, 24, generator=torch.Generator().manual_seed(6)).to(device).requires_grad_(True))
+    labels = torch.arange(35, device=device).view(5, 7) % 9
+    for keep in ("input", "int8"):
+        grads = []
+        for offload in (False, True):
+            leaf = planes.clone().requires_grad_(True)
+            hook = torch.autograd.graph.save_on_cpu() if offload else torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t)
+            with hook:
+                loss = R.label_loss(R.layer_norm(leaf.permute(1, 2, 0), w, keep=keep), v, labels)
+            grads.append(torch.autograd.grad(loss, [leaf, w, v]))
+        for p, q in zip(*grads):
+            torch.testing.assert_close(p, q, atol=1e-6, rtol=0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_saved_tensors_of_another_kind_are_refused(device):
+    x, w, y, b = make_label_case(12, 8, 5, F32, seed=2, device=device)
+    bad = [lambda t: t.double() if t.is_floating_point() else t, lambda t: t[:-1] if t.dim() and t.shape[0] > 1 else t,
+           lambda t: t.bfloat16() if t.dtype == F32 else t.short() if t.dtype != torch.int8 else t, lambda t: t.to("meta")]
+    for unpack in bad:
+        for op in ("label", "input", "int8"):
+            leaf, gain = x.clone().requires_grad_(True), torch.ones(8, device=device, requires_grad=True)
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+                out = R.label_loss(leaf, w, y, bias=b) if op == "label" else R.layer_norm(leaf, gain, keep=op).sum()
+            with pytest.raises(RuntimeError, match="came back as"):
+                torch.autograd.grad(out, leaf)
