@@ -46,6 +46,13 @@ RGS_HD uint16_t rgs_bf16_bits(float f) {
 }
 RGS_HD float rgs_bf16_value(uint16_t b) { return rgs_u2f((uint32_t)b << 16); }
 
+// Whether rows of c channels, ld apart and the first of them aligned, may be read in aligned vectors of four that begin inside
+// the row in front (rgs_norm.cu; the last row is read by itself).  The shift repeats where ld = c modulo 4, and a lane holds
+// 1024 channels with it.  Of the other rows the vectors end up to three elements behind the row: with ld >= 2 that is inside the
+// tensor (row n-2 ends at (n-1) ld - ld + c; 2 and 3 channels: the multiple of four behind it is at most (n-1) ld + c), with
+// single elements it is not: row n-3 or n-2 would be read up to element n.
+RGS_HD bool rgs_rows_shifted(int64_t c, int64_t ld) { return (ld - c) % 4 == 0 && c <= 1024 - 6 && ld > 1; }
+
 RGS_HD float rgs_load_as_float(const void* p, int64_t i, int dtype) {
     return dtype == RGS_BF16 ? rgs_bf16_value(static_cast<const uint16_t*>(p)[i]) : static_cast<const float*>(p)[i];
 }

@@ -10,6 +10,7 @@ extern "C" {
 
 int64_t rgs_cpu_norm_scratch_bytes(int64_t, int64_t) { return 16; }
 int64_t rgs_cpu_label_scratch_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) { return 16; }
+int64_t rgs_cpu_rows_shifted(int64_t c, int64_t ld) { return rgs_rows_shifted(c, ld); }  // the rule of rgs_norm.cu
 
 int rgs_cpu_pack8(const void* x, int64_t dtype, int64_t ld, int64_t planes, int64_t n, int64_t c, int8_t* codes, uint8_t* expo, void*) {
     const int64_t blocks = (c + RGS_PACK_BLOCK - 1) / RGS_PACK_BLOCK;

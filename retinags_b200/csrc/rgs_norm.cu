@@ -1119,7 +1119,7 @@ int rgs_cuda_norm_fwd(const void* x, int64_t dtype, int64_t ld, int64_t planes, 
     }
     const bool start = aligned_to(x, four(a.src));
     if (start && c % 4 == 0 && ld % 4 == 0) norm_rows_vec<false>(a, false, st);
-    else if (start && (ld - c) % 4 == 0 && c <= NR_MAX - 6) {
+    else if (start && rgs_rows_shifted(c, ld)) {
         norm_rows_vec<true>(a, false, st);  // its blocks of 32 channels begin anywhere in a vector: packed by themselves
         RGS_CUDA_CHECK(cudaGetLastError());
         if (codes) return rgs_cuda_pack8(x, dtype, ld, planes, n, c, codes, expo, stream);
@@ -1155,7 +1155,7 @@ int rgs_cuda_norm_bwd(const void* x, int64_t dtype, int64_t ld, int64_t planes, 
     } else {
         const bool start = aligned_to(dy, four(a.dy_dtype)) && (codes || aligned_to(x, four((int)dtype)));
         if (start && c % 4 == 0 && ldy % 4 == 0 && (codes || ld % 4 == 0)) parts = norm_rows_vec<false>(a, true, st);
-        else if (start && !codes && (ld - c) % 4 == 0 && (ldy - c) % 4 == 0 && c <= NR_MAX - 6) parts = norm_rows_vec<true>(a, true, st);
+        else if (start && !codes && rgs_rows_shifted(c, ld) && rgs_rows_shifted(c, ldy)) parts = norm_rows_vec<true>(a, true, st);
         else parts = norm_rows_single(a, true, st);
     }
     RGS_CUDA_CHECK(cudaGetLastError());

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import retinags_b200 as R
+from retinags_b200.ops import native
 from field_reference import make_label_case
 
 F32, BF16 = torch.float32, torch.bfloat16
@@ -106,3 +107,36 @@ def test_saved_tensors_of_another_kind_are_refused(device):
                 out = R.label_loss(leaf, w, y, bias=b) if op == "label" else R.layer_norm(leaf, gain, keep=op).sum()
             with pytest.raises(RuntimeError, match="came back as"):
                 torch.autograd.grad(out, leaf)
+
+
+def test_shifted_rows_are_read_inside_the_tensor():
+    """Vectors of four that begin in the row in front: for every width and stride that the rule admits, those of all rows but the
+    last (read element by element) end inside the tensor."""
+    admitted, cpu = 0, torch.device("cpu")
+    for c in list(range(1, 24)) + [771, 1017, 1018, 1019]:
+        for ld in range(c, c + 13):
+            if not native.size_of("rows_shifted", cpu, c, ld):
+                continue
+            admitted += 1
+            for n in range(1, 12):
+                total = (n - 1) * ld + c
+                for row in range(n - 1):
+                    start = row * ld - (row * c) % 4
+                    assert start % 4 == 0 and start >= 0
+                    assert -(-(row * ld + c) // 4) * 4 <= total, (n, c, ld, row)
+    assert admitted > 60
+    assert not native.size_of("rows_shifted", cpu, 1, 1) and not native.size_of("rows_shifted", cpu, 1019, 1019)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("device", DEVICES)
+def test_layer_norm_of_one_channel(device, dtype):
+    """Nothing varies: the output is the bias, and neither the input nor the weight has a gradient."""
+    for n in range(1, 14):
+        for stride in (1, 2, 5):
+            room = torch.randn(n * stride, dtype=torch.float32, generator=torch.Generator().manual_seed(n)).to(dtype).to(device)
+            leaf = room[::stride].view(n, 1).detach().requires_grad_(True)
+            w, b = torch.full((1,), 3.0, device=device, requires_grad=True), torch.full((1,), 0.5, device=device, requires_grad=True)
+            y = R.layer_norm(leaf, w, b, out_dtype=F32)
+            gx, gw, gb = torch.autograd.grad(y, [leaf, w, b], torch.ones_like(y))
+            assert (y == 0.5).all() and (gx == 0).all() and gw.item() == 0.0 and gb.item() == n
