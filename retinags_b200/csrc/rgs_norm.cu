@@ -1153,7 +1153,8 @@ int rgs_cuda_norm_bwd(const void* x, int64_t dtype, int64_t ld, int64_t planes, 
         const int rc = norm_planes<true>(a, &parts, st);
         if (rc) return rc;
     } else {
-        const bool start = aligned_to(dy, four(a.dy_dtype)) && (codes || aligned_to(x, four((int)dtype)));
+        // (codes that were kept elsewhere in between may come back at any byte)
+        const bool start = aligned_to(dy, four(a.dy_dtype)) && (codes ? aligned_to(codes, 4) : aligned_to(x, four((int)dtype)));
         if (start && c % 4 == 0 && ldy % 4 == 0 && (codes || ld % 4 == 0)) parts = norm_rows_vec<false>(a, true, st);
         else if (start && !codes && rgs_rows_shifted(c, ld) && rgs_rows_shifted(c, ldy)) parts = norm_rows_vec<true>(a, true, st);
         else parts = norm_rows_single(a, true, st);
