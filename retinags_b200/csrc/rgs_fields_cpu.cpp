@@ -119,6 +119,16 @@ int rgs_cpu_norm_bwd(const void* x, int64_t dtype, int64_t ld, int64_t planes, c
     return 0;
 }
 
+// Score of a row and a label, rounded to 32 bits as on the GPU: the largest one is kept for the backward pass as a float, and only
+// of numbers that it holds exactly do the differences stay (a 64-bit score of 1e9 differs from its float by up to 32, and exp of
+// that is not at most one).
+static inline double label_score(const void* x, int64_t xi, const void* w, int64_t wi, const void* bias, int64_t v, int64_t c, int dtype,
+                                 int b_dtype) {
+    double l = bias ? rgs_load_as_float(bias, v, b_dtype) : 0.f;
+    for (int64_t j = 0; j < c; ++j) l += (double)rgs_load_as_float(x, xi + j, dtype) * rgs_load_as_float(w, wi + j, dtype);
+    return (double)(float)l;
+}
+
 // lse (2,n): largest score and log sum exp(score - largest) of a row, two numbers so that scores of any size (all labels at
 // the lowest value of the type, say) keep their differences; losses[i] per row, result[0] = sum / max(count, 1) or sum, count[0] = rows that count
 int rgs_cpu_label_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* labels, int64_t label_bytes,
@@ -131,9 +141,7 @@ int rgs_cpu_label_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, co
         const int64_t y = rgs_label(labels, i, (int)label_bytes, vocab);
         double m = -INFINITY, s = 0, at = 0;
         for (int64_t v = 0; v < vocab; ++v) {
-            double l = bias ? rgs_load_as_float(bias, v, (int)b_dtype) : 0.f;
-            for (int64_t j = 0; j < c; ++j)
-                l += (double)rgs_load_as_float(x, i * ldx + j, (int)dtype) * rgs_load_as_float(w, v * ldw + j, (int)dtype);
+            const double l = label_score(x, i * ldx, w, v * ldw, bias, v, c, (int)dtype, (int)b_dtype);
             if (v == y) at = l;
             if (l > m || l != l) { s *= exp(m - l); m = l; }
             s += l == -INFINITY && m == -INFINITY ? 0.0 : exp(l - m);
@@ -156,9 +164,7 @@ int rgs_cpu_label_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, co
                       int64_t per_row, int64_t mean, const float* count, void*, void* dx, void* dw, void* db, void*) {
     const double scale = mean ? 1.0 / (*count > 1.f ? *count : 1.f) : 1.0;
     auto grad = [&](int64_t i, int64_t v, int64_t y) -> double {
-        double l = bias ? rgs_load_as_float(bias, v, (int)b_dtype) : 0.f;
-        for (int64_t j = 0; j < c; ++j)
-            l += (double)rgs_load_as_float(x, i * ldx + j, (int)dtype) * rgs_load_as_float(w, v * ldw + j, (int)dtype);
+        const double l = label_score(x, i * ldx, w, v * ldw, bias, v, c, (int)dtype, (int)b_dtype);
         return (exp((l - lse[i]) - lse[n + i]) - (v == y)) * gout[per_row ? i : 0] * scale;
     };
     if (dx) {

@@ -140,3 +140,33 @@ def test_layer_norm_of_one_channel(device, dtype):
             y = R.layer_norm(leaf, w, b, out_dtype=F32)
             gx, gw, gb = torch.autograd.grad(y, [leaf, w, b], torch.ones_like(y))
             assert (y == 0.5).all() and (gx == 0).all() and gw.item() == 0.0 and gb.item() == n
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("device", DEVICES)
+def test_label_loss_scores_that_32_bits_hold_coarsely(device, dtype):
+    """Scores of 1e9 lie 64 apart in 32 bits.  Probabilities stay probabilities: gradients are differences of two rows of the
+    weight (or their averages over labels that tie), never infinite."""
+    x, w, y, b = make_label_case(40, 8, 50, F32, seed=3, device=device, unlabelled=0.0)
+    leaves = [(t * s).to(dtype).requires_grad_(True) for t, s in ((x, 3e4), (w, 3e4), (b, 1.0))]
+    losses = R.label_loss(leaves[0], leaves[1], y, bias=leaves[2], reduction="none")
+    gx, gw, gb = torch.autograd.grad(losses.sum(), leaves)
+    xd, wd = leaves[0].detach().double(), leaves[1].detach().double()
+    s = xd @ wd.t() + leaves[2].detach().double()
+    at = s.gather(1, y[:, None])[:, 0]
+    # a score: (6 C / 16 + 8) * 2 roundings of its absolute sum (three pieces on the tensor core; fewer on the CPU)
+    es = (6 * 8 / 16 + 8) * 2 * 2.0 ** -24 * (xd.abs() @ wd.abs().t()).max(1).values
+    want = torch.logsumexp(s, 1) - at
+    assert ((losses.detach().double() - want).abs() <= 2 * es + 2.0 ** -23 * want.abs() + 1e-4).all()
+    assert all(torch.isfinite(g).all() for g in (gx, gw, gb))
+    # sum_v |p_v - [v = y]| is at most 2: |dx| <= 2 max|w|, |dw_v| <= sum_n |x_n|, |db_v| <= pixels (and the outputs' rounding)
+    room = 1.0 + 2.0 ** -7
+    assert (gx.abs().double() <= 2 * wd.abs().max(0).values * room).all()
+    assert (gw.abs().double() <= xd.abs().sum(0) * room).all() and (gb.abs() <= 40 * room).all()
+    # where the largest score is far above the others, p is one label and the gradient is w_top - w_y
+    top = s.topk(2, 1).values
+    clear = top[:, 0] - top[:, 1] > 4 * es + 200.0
+    assert clear.sum() > 20
+    ref = (wd[s.argmax(1)] - wd[y])[clear]
+    half = 2.0 ** -24 if dtype == F32 else 2.0 ** -8
+    assert ((gx[clear].double() - ref).abs() <= 2 * half * ref.abs() + 2.0 ** -21 * wd.abs().max()).all()
