@@ -18,8 +18,10 @@
 // label and (1, 1, 1, -lse in three pieces) of a pixel, so S is the score with its bias and, backward, minus lse: the
 // warpgroups need nothing per column but the labels of dW (constants per column read from shared memory cost as much of its
 // bandwidth as half of the products' operands).  Columns behind the last label and pixels without one have -inf there.
-// Where scores are so large that log z would vanish beside m (a mask of the type's lowest value over all labels), -m alone
-// rides along and 1/z is multiplied; the same factor serves gradients that differ from pixel to pixel.
+// Where scores are so large that log z would vanish beside m (a mask of the type's lowest value over all labels), only the bias
+// rides along: the scores are then formed in the very steps of the forward pass, m is taken off them in registers and 1/z is
+// multiplied.  (With -m in the product x.w + b - m is rounded in other places than m was: 64 apart at scores of 1e9, and exp of
+// that is no probability.)  The same factor serves gradients that differ from pixel to pixel.
 //
 // 32-bit inputs: every operand is split into three bf16 pieces (8 + 8 + 8 bits of mantissa) and six of the nine piece
 // products are kept; what is dropped is below 2^-24 of a product.  G is split the same way in registers.
@@ -55,7 +57,7 @@
 #define LOG2E 1.4426950408889634f
 
 enum { LF_DIRTY = 1,   // a pixel without a label holds something that is not finite
-       LF_LARGE = 2 }; // a largest score above 2^10: m and log z are not added up
+       LF_LARGE = 2 }; // a largest score above 2^10: m and log z are not added up, and m stays out of the product
 
 struct LabelArgs {
     int64_t n, v;
@@ -265,7 +267,8 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
     const int OUT = a.nbuf * SB;                  // first column of the outputs
     constexpr int OB = 64;                        // columns of an output buffer when there are two
     constexpr int COMBOS = P == 1 ? 1 : 6;
-    constexpr int CA[6] = {P == 1 ? 0 : 2, 0, 1, 1, 0, 0}, CB[6] = {0, 2, 1, 0, 1, 0};  // smallest products first
+    // smallest products first; the piece of X first where S = X W^T, and the same pairs in the same order where S = W X^T
+    constexpr int CA[6] = {P == 1 ? 0 : 2, 0, 1, 1, 0, 0}, CB[6] = {0, 2, 1, 0, 1, 0};
     constexpr int TB = KC * 2 * LT;               // bytes of a staged tile
     extern __shared__ unsigned char raw[];
     unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -420,14 +423,17 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             return d;
         };
         // the chunks of a stage; channels behind the last one are zeros in shared memory
-        auto stage_s = [&](uint32_t d, uint32_t at, uint32_t bt, bool more) {
+        auto stage_s = [&](uint32_t d, uint32_t at, uint32_t bt, bool more, bool swap) {
+            // pairs (2,0) (0,2) (1,1) (1,0) (0,1) (0,0) of pieces of A and B, or with their members swapped
+            const uint32_t a2 = swap ? 0 : 2 * T16, a1 = swap ? 0 : T16;
+            const uint32_t oa[6] = {P == 1 ? 0 : a2, 2 * T16 - a2, T16, a1, T16 - a1, 0}, ob[6] = {P == 1 ? 0 : 2 * T16 - a2, a2, T16, T16 - a1, a1, 0};
 #pragma unroll
             for (int k = 0; k < CS; ++k)
 #pragma unroll
                 for (int q = 0; q < COMBOS; ++q)
 #pragma unroll
                     for (int ks = 0; ks < KC / 16; ++ks)
-                        lb_mma_ss<KC>(issue, d, at + (k * P + CA[q]) * T16 + ks * 2, bt + (k * P + CB[q]) * T16 + ks * 2, idesc | ((LT >> 3) << 17), k || q || ks ? true : more);
+                        lb_mma_ss<KC>(issue, d, at + k * P * T16 + oa[q] + ks * 2, bt + k * P * T16 + ob[q] + ks * 2, idesc | ((LT >> 3) << 17), k || q || ks ? true : more);
         };
         auto issue_s = [&](const LabelItem& it, int j) {
             const uint32_t d = tmem + sc.slot * SB;
@@ -449,13 +455,13 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if ((P == 1 && CS > 1) || lead) {
-                    stage_s(d, at, bt, k != 0);
+                    stage_s(d, at, bt, k != 0, GRAD && it.dw);
                     if (!GRAD || !WHOLE) {
                         lb_commit(issue, &sh->empty[g0]);
                         if (!WHOLE && !a.a_slots) lb_commit(issue, &sh->empty[g0 + 1 == (uint32_t)a.stages ? 0 : g0 + 1]);
                     }
                     if (k == nst - 1) {
-                        // last: where b and m are huge and cancel, what is small beside them is gone, as it is from the scores
+                        // last: where b is huge and -(m + log z) cancels it, what is small beside them is gone, as it is from the scores
                         lb_mma_ss<16>(issue, d, ea16 + eac.slot * (LE >> 4), e16 + ec.slot * (LE >> 4), idesc | ((LT >> 3) << 17), true);
                         lb_commit(issue, &sh->s_full[sc.slot]);
                         lb_commit(issue, &sh->e_empty[ec.slot]);
@@ -622,7 +628,10 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             if (out_i == i) { out_label = label; out_scale = scale; }
             const int64_t y = it.dw ? -1 : label;
             float m = -INFINITY, inv_z = 1.f, sum = 0.f;
-            if (GRAD && large && !it.dw && r < a.n) inv_z = ex2(-a.lse[a.n + r] * LOG2E);
+            if (GRAD) {
+                m = 0.f;
+                if (large && !it.dw && label >= 0) { m = a.lse[r]; inv_z = ex2(-a.lse[a.n + r] * LOG2E); }
+            }
             for (int j = it.j0; j < it.j1; ++j, ++t) {
                 const uint32_t bstage = kept, buf = sc.slot, parity = sc.phase;
                 if (GRAD && P == 1 && (kept += nst) >= (uint32_t)a.stages) kept -= a.stages;
@@ -697,6 +706,14 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                     __syncwarp();
                     tm_ld32(s + h, u);
                     tm_wait_ld32(u);
+                    if (RARE && large) {  // m of the row, or of the 32 pixels of the columns (none: -infinity stays)
+                        if (it.dw) {
+                            const int lab = reinterpret_cast<const int*>(kb)[h + lane];
+                            m = lab >= 0 ? a.lse[(int64_t)j * LT + half + h + lane] : 0.f;
+                        }
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) u[q] = __float_as_uint(__uint_as_float(u[q]) - (it.dw ? __shfl_sync(0xffffffffu, m, q) : m));
+                    }
 #pragma unroll
                     for (int o = 0; o < 32; o += 16) {  // 16 columns: one step of the product's inner dimension
                         float e[16];
@@ -929,7 +946,7 @@ __global__ void __launch_bounds__(256) rgs_label_prep_kernel(const __grid_consta
         if (y >= 0) {
             g = a.gout[a.per_row ? k : 0] * mean;
             const float m = a.lse[k], lz = a.lse[a.n + k];
-            lb_split3(large ? -m : -(m + lz), c);
+            if (!large) lb_split3(-(m + lz), c);
             f = large ? g * expf(-lz) : g;
             lb_extra(a.ex + k * 16, ones, c);
         } else {
