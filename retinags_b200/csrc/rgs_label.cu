@@ -34,7 +34,11 @@
 //     product reads 128 bytes of operands a clock, all that shared memory gives, while TMA writes the next block there
 //   1657600 x 32 x 512, 32 bits: forward 0.39 ms, gradients 1.4 ms: the split of G in three and six products for one
 //
-// All waits are bounded; when one runs out the CTA stops waiting, writes NaN into what it still owes and frees its TMEM.
+// All waits are bounded.  A warp whose wait runs out says so in shared memory (fail) before anything else it does.  From then on
+// barriers may complete for work that is not whole: the MMA warp goes through its motions to the end of its item.  So the
+// warpgroups look at fail behind the last wait that an output hangs on, and write NaN; one whose own wait ran out arrives
+// nowhere any more, so that no buffer of it is used again.  A loss or gradient is right or NaN (a forward pass that gave up makes
+// its backward pass NaN).  Copies in flight land before the CTA leaves, and its TMEM is freed.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -81,6 +85,7 @@ struct LabelArgs {
     float* part_b;                   // (4 nsw, nmw*128)
     int cq;
     void* dx; void* dw; int dtype;
+    uint32_t wait, loads;            // limits: tries of a wait; stages that the producer of a CTA fills before it gives up
 };
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -88,29 +93,39 @@ struct LabelArgs {
 // ---------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
-__device__ __forceinline__ bool lb_wait(unsigned long long* bar, uint32_t parity, volatile int* fail) {
-    const uint32_t addr = rgs_smem_addr(bar);
-    for (uint32_t it = 0; it < LWAIT; ++it) {
-        uint32_t ok;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(ok) : "r"(addr), "r"(parity) : "memory");
-        if (ok) return true;
-        if ((it & 15u) == 15u && *fail) return false;
-    }
-    *fail = 1;
-    return false;
-}
-// the same by a whole warp, with one answer for all of it
-__device__ __forceinline__ bool lb_wait_warp(unsigned long long* bar, uint32_t parity, volatile int* fail) {
-    return __all_sync(0xffffffffu, lb_wait(bar, parity, fail));
-}
-__device__ __noinline__ void lb_wait_slow(unsigned long long* bar, uint32_t parity, volatile int* fail) { lb_wait(bar, parity, fail); }
-__device__ __forceinline__ void lb_wait_quiet(unsigned long long* bar, uint32_t parity, volatile int* fail) {
+__device__ __forceinline__ bool lb_try(unsigned long long* bar, uint32_t parity) {
     uint32_t ok;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(ok) : "r"(rgs_smem_addr(bar)), "r"(parity) : "memory");
-    if (!ok) lb_wait_slow(bar, parity, fail);
+    return ok;
+}
+__device__ __forceinline__ bool lb_wait(unsigned long long* bar, uint32_t parity, volatile int* fail, uint32_t limit) {
+    for (uint32_t it = 0; it < limit; ++it) {
+        if (lb_try(bar, parity)) return true;
+        if ((it & 15u) == 15u && *fail) break;
+    }
+    *fail = 1;
+    __threadfence_block();  // seen before what this warp issues next
+    return false;
+}
+// the same by a whole warp, with one answer for all of it
+__device__ __forceinline__ bool lb_wait_warp(unsigned long long* bar, uint32_t parity, volatile int* fail, uint32_t limit) {
+    return __all_sync(0xffffffffu, lb_wait(bar, parity, fail, limit));
+}
+// The MMA warp's.  It goes on either way: every answer that its loop looks at costs (votes 3 % of a pass, a lane that gives up
+// issuing 20 to 50 %).
+__device__ __noinline__ void lb_wait_slow(unsigned long long* bar, uint32_t parity, volatile int* fail, uint32_t limit) {
+    if (*fail) __threadfence_block();
+    else lb_wait(bar, parity, fail, limit);
+}
+__device__ __forceinline__ void lb_wait_quiet(unsigned long long* bar, uint32_t parity, volatile int* fail, uint32_t limit) {
+    if (!lb_try(bar, parity)) lb_wait_slow(bar, parity, fail, limit);
     __syncwarp();
+}
+// all roles of a CTA have come to their end
+__device__ __forceinline__ void lb_end_of_role() {
+    __syncwarp();
+    asm volatile("barrier.sync 1, %0;" ::"n"(LTHREADS) : "memory");
 }
 // One lane of a converged warp.  The producer and MMA warps run their loops with all lanes and let this one issue (a single
 // thread in the loop: codebook forward 2.53 instead of 1.99 ms).  Asked once: to elect anew costs more than a product.
@@ -314,7 +329,8 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         uint32_t loads = 0, labels = 0;
         bool ok = true;
         auto load = [&](const CUtensorMap* map, int k, int row, const CUtensorMap* extra) {
-            ok = ok && lb_wait_warp(&sh->empty[rc.slot], rc.phase ^ 1, fail);
+            if (ok && loads >= a.loads) { *fail = 1; ok = false; }
+            ok = ok && lb_wait_warp(&sh->empty[rc.slot], rc.phase ^ 1, fail, a.wait);
             if (!ok) return;
             if (lead) {
                 unsigned char* dst = ring + rc.slot * stage;
@@ -338,7 +354,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             const LabelItem it = lb_item(a, i);
             const CUtensorMap *ma = it.dw ? &map_w : &map_x, *mb = it.dw ? &map_x : &map_w;
             // (forward: the pixels' extra channels are the same for all, one tile of them)
-            ok = lb_wait_warp(&sh->ea_empty[eac.slot], eac.phase ^ 1, fail);
+            ok = lb_wait_warp(&sh->ea_empty[eac.slot], eac.phase ^ 1, fail, a.wait);
             if (!ok) break;
             if (lead) {
                 rgs_mbar_expect_tx(&sh->ea_full[eac.slot], LE);
@@ -346,7 +362,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             }
             eac.next(2);
             if (WHOLE || a.a_slots) {
-                ok = lb_wait_warp(&sh->a_empty[ac.slot], ac.phase ^ 1, fail);
+                ok = lb_wait_warp(&sh->a_empty[ac.slot], ac.phase ^ 1, fail, a.wait);
                 if (!ok) break;
                 if (lead) {
                     unsigned char* dst = tiles + ac.slot * na * TB;
@@ -358,10 +374,10 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 ac.next(a.a_slots);
             }
             for (int j = it.j0; j < it.j1 && ok; ++j) {
-                ok = lb_wait_warp(&sh->e_empty[ec.slot], ec.phase ^ 1, fail);
+                ok = lb_wait_warp(&sh->e_empty[ec.slot], ec.phase ^ 1, fail, a.wait);
                 if (!ok) break;
                 if (GRAD && it.dw) {
-                    ok = lb_wait_warp(&sh->k_empty[kc.slot], kc.phase ^ 1, fail);
+                    ok = lb_wait_warp(&sh->k_empty[kc.slot], kc.phase ^ 1, fail, a.wait);
                     if (!ok) break;
                     if (lead) {
                         rgs_mbar_expect_tx(&sh->k_full[kc.slot], LKBYTES);
@@ -380,6 +396,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             }
         }
         if (ok) out_tiles();
+        lb_end_of_role();
         if (*fail) {  // copies still in flight land before the CTA leaves (all were consumed unless a wait ran out)
             const uint32_t live = loads < (uint32_t)a.stages ? loads : a.stages;
             for (uint32_t k = 0; k < live; ++k) {
@@ -405,8 +422,6 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------------------------------------------ MMA
-        // once a wait has run out the others return at once: the loop goes through its (bounded) motions on whatever lies in
-        // shared memory and TMEM, and the warpgroups write NaN
         const uint32_t lead = lb_elect();
         // one product after the other by predicate (several chunks to a stage), or a branch around all of them: each the
         // faster one (256 channels backward 4.09 -> 3.85 ms with predicates, 32 channels in 32 bits 1.74 -> 1.86 ms)
@@ -417,7 +432,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         const uint32_t dlo = lb_desc_lo<KC>, ring16 = dlo + (rgs_smem_addr(ring) >> 4), tiles16 = dlo + (rgs_smem_addr(tiles) >> 4);
         constexpr uint32_t T16 = TB >> 4, stage16 = stage >> 4;
         auto take = [&]() {
-            lb_wait_quiet(&sh->full[rc.slot], rc.phase, fail);
+            lb_wait_quiet(&sh->full[rc.slot], rc.phase, fail, a.wait);
             const uint32_t d = ring16 + rc.slot * stage16;
             rc.next(a.stages);
             return d;
@@ -438,10 +453,10 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         auto issue_s = [&](const LabelItem& it, int j) {
             const uint32_t d = tmem + sc.slot * SB;
             // forward: the scores there before have been read; backward: the product with their G was issued before, and runs before
-            if (!GRAD) lb_wait_quiet(&sh->s_done[sc.slot], sc.phase ^ 1, fail);
+            if (!GRAD) lb_wait_quiet(&sh->s_done[sc.slot], sc.phase ^ 1, fail, a.wait);
             if (j == it.j0) {
-                lb_wait_quiet(&sh->ea_full[eac.slot], eac.phase, fail);
-                if (WHOLE || a.a_slots) lb_wait_quiet(&sh->a_full[ac.slot], ac.phase, fail);
+                lb_wait_quiet(&sh->ea_full[eac.slot], eac.phase, fail, a.wait);
+                if (WHOLE || a.a_slots) lb_wait_quiet(&sh->a_full[ac.slot], ac.phase, fail, a.wait);
             }
             const uint32_t abase = tiles16 + ac.slot * (na * T16);
             const bool last = j == it.j1 - 1;
@@ -497,8 +512,8 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 }
         };
         auto issue_o = [&](const LabelItem& it, int j) {
-            lb_wait_quiet(&sh->s_done[pc.slot], pc.phase, fail);
-            if (j == it.j0) lb_wait_quiet(&sh->o_free[oc_.slot], oc_.phase ^ 1, fail);
+            lb_wait_quiet(&sh->s_done[pc.slot], pc.phase, fail, a.wait);
+            if (j == it.j0) lb_wait_quiet(&sh->o_free[oc_.slot], oc_.phase ^ 1, fail, a.wait);
             const uint32_t s = tmem + pc.slot * SB, o = tmem + OUT + oc_.slot * OB;
             pc.next(a.nbuf);
             const bool last = j == it.j1 - 1;
@@ -528,6 +543,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 if (si < items) { is = lb_item(a, si); sj = is.j0; }
             }
         };
+        auto failed = [&]() { return __any_sync(0xffffffffu, *fail); };
         if (GRAD) {
             for (int l = 1; l < a.nbuf; ++l)
                 if (si < items) step_s();
@@ -535,16 +551,22 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 if (si < items) step_s();
                 issue_o(io, oj);
                 if (++oj == io.j1) {
+                    if (failed()) break;
                     oi += gridDim.x;
                     if (oi < items) { io = lb_item(a, oi); oj = io.j0; }
                 }
             }
         } else {
-            while (si < items) step_s();
+            while (si < items) {
+                const unsigned i = si;
+                step_s();
+                if (si != i && failed()) break;
+            }
         }
-        lb_commit(lead, &sh->drain);
+        lb_commit(lead, &sh->drain);  // what was issued is done before TMEM goes
         __syncwarp();
         rgs_mbar_wait(&sh->drain, 0, LWAIT);
+        lb_end_of_role();
     } else {
         // ------------------------------------------------------------------------------------------------ scores
         const int wg = (warp - 2) >> 2;                      // warpgroup: score tiles t with t % 2 == wg % 2,
@@ -576,7 +598,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         };
         auto write_out = [&](unsigned i, float scale, int label) {
             const LabelItem it = lb_item(a, i);
-            if (!dead) dead = __any_sync(0xffffffffu, !lb_wait(&sh->o_full[oc_.slot], oc_.phase, fail));
+            if (!dead) dead = __any_sync(0xffffffffu, !lb_wait(&sh->o_full[oc_.slot], oc_.phase, fail, a.wait));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t o = tmem + lanes + OUT + oc_.slot * OB;
             const int64_t r = (int64_t)it.m * LT + row, rows = it.dw ? a.v : a.n;
@@ -591,10 +613,11 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                     tm_wait_ld16(lo);
                 }
                 tm_wait_ld16(u);
+                const bool lost = dead || *fail;  // behind the loads: a buffer is given to other work only after fail is set
                 if (r < rows && (!it.dw || a.dw)) {
                     float f[16];
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) f[q] = dead ? nan : P == 3 ? __uint_as_float(u[q]) + __uint_as_float(lo[q]) : __uint_as_float(u[q]);
+                    for (int q = 0; q < 16; ++q) f[q] = lost ? nan : P == 3 ? __uint_as_float(u[q]) + __uint_as_float(lo[q]) : __uint_as_float(u[q]);
                     if (ns > 1) {
                         if (it.dw)
 #pragma unroll
@@ -611,7 +634,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 __syncwarp();
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            rgs_mbar_arrive(&sh->o_free[oc_.slot]);
+            if (!dead) rgs_mbar_arrive(&sh->o_free[oc_.slot]);
             oc_.next(a.nob);
         };
         const bool dirty = GRAD && P == 1 && WHOLE && (flags & LF_DIRTY);
@@ -627,11 +650,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             next_scale = row_scale(i + gridDim.x);
             if (out_i == i) { out_label = label; out_scale = scale; }
             const int64_t y = it.dw ? -1 : label;
-            float m = -INFINITY, inv_z = 1.f, sum = 0.f;
-            if (GRAD) {
-                m = 0.f;
-                if (large && !it.dw && label >= 0) { m = a.lse[r]; inv_z = ex2(-a.lse[a.n + r] * LOG2E); }
-            }
+            float m = -INFINITY, sum = 0.f;
             for (int j = it.j0; j < it.j1; ++j, ++t) {
                 const uint32_t bstage = kept, buf = sc.slot, parity = sc.phase;
                 if (GRAD && P == 1 && (kept += nst) >= (uint32_t)a.stages) kept -= a.stages;
@@ -641,7 +660,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 if ((int)(t & 1) != (wg & 1)) continue;
                 const uint32_t s = tmem + lanes + buf * SB + half;
                 if (!dead) {  // the whole warp goes on or none of it: TMEM accesses are warp-wide
-                    dead = !lb_wait(&sh->s_full[buf], parity, fail) || (GRAD && it.dw && !lb_wait(&sh->k_full[kslot], kparity, fail));
+                    dead = !lb_wait(&sh->s_full[buf], parity, fail, a.wait) || (GRAD && it.dw && !lb_wait(&sh->k_full[kslot], kparity, fail, a.wait));
                     dead = __any_sync(0xffffffffu, dead);
                 }
                 if (dead) continue;
@@ -700,6 +719,8 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 // factors and pixels to be kept out are in a copy of their own: their tests alone, never met, cost a fifth
                 auto gradient = [&](auto rare_) {
                 constexpr bool RARE = decltype(rare_)::value;
+                float row_m = 0.f, inv_z = 1.f;
+                if (RARE && large && !it.dw && label >= 0) { row_m = a.lse[r]; inv_z = ex2(-a.lse[a.n + r] * LOG2E); }
 #pragma unroll 1
                 for (int h = 0; h < 64; h += 32) {
                     uint32_t u[32];
@@ -709,10 +730,10 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                     if (RARE && large) {  // m of the row, or of the 32 pixels of the columns (none: -infinity stays)
                         if (it.dw) {
                             const int lab = reinterpret_cast<const int*>(kb)[h + lane];
-                            m = lab >= 0 ? a.lse[(int64_t)j * LT + half + h + lane] : 0.f;
+                            row_m = lab >= 0 ? a.lse[(int64_t)j * LT + half + h + lane] : 0.f;
                         }
 #pragma unroll
-                        for (int q = 0; q < 32; ++q) u[q] = __float_as_uint(__uint_as_float(u[q]) - (it.dw ? __shfl_sync(0xffffffffu, m, q) : m));
+                        for (int q = 0; q < 32; ++q) u[q] = __float_as_uint(__uint_as_float(u[q]) - (it.dw ? __shfl_sync(0xffffffffu, row_m, q) : row_m));
                     }
 #pragma unroll
                     for (int o = 0; o < 32; o += 16) {  // 16 columns: one step of the product's inner dimension
@@ -814,11 +835,13 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 }
             }
             if (!GRAD) {
+                dead = __any_sync(0xffffffffu, dead || *fail);
                 if (r < a.n) {
                     a.pm[((int64_t)it.split * 4 + wg) * a.n + r] = dead ? nan : m;
                     a.ps[((int64_t)it.split * 4 + wg) * a.n + r] = dead ? nan : sum;
                 }
             } else if (it.dw && a.part_b && it.oc0 == 0) {
+                dead = __any_sync(0xffffffffu, dead || *fail);
                 a.part_b[((int64_t)it.split * 4 + wg) * a.nmw * LT + r] = dead ? nan : sum * gshare;
             }
         }
@@ -826,6 +849,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             write_out(out_i, out_scale, out_label);
             for (out_i += gridDim.x; out_i < items; out_i += gridDim.x) write_out(out_i, row_scale(out_i), row_label(out_i));
         }
+        lb_end_of_role();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -1130,6 +1154,9 @@ static int label_map(CUtensorMap* map, const void* base, int64_t c, int64_t rows
                kc == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : kc == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : 21;
 }
 
+// Limits of the waits: [0] tries, [1] stages that the producer of a CTA fills before it gives up.  Tests lower them.
+static std::atomic<int64_t> label_limits[2] = {{LWAIT}, {0xffffffffll}};
+
 static inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
 // Number of pieces of a walk over nj tiles made by `tiles` row tiles: one where there are three row tiles or more to an
@@ -1229,7 +1256,7 @@ static int label_direct(const void* x, int64_t ldx, const void* w, int64_t ldw) 
 struct LabelMaps { CUtensorMap x, w, ex, ew; };
 
 template <int P, bool GRAD, int KC, int CS, bool WHOLE>
-static int label_launch(const LabelMaps& m, const LabelArgs& a, cudaStream_t stream) {
+static int label_launch(const LabelMaps& m, LabelArgs a, cudaStream_t stream) {
     static std::atomic<uint64_t> ready{0};  // devices whose limit on dynamic shared memory was raised
     int dev = 0;
     RGS_CUDA_CHECK(cudaGetDevice(&dev));
@@ -1238,6 +1265,8 @@ static int label_launch(const LabelMaps& m, const LabelArgs& a, cudaStream_t str
         if (dev <= 63) ready.fetch_or((uint64_t)1 << dev);
     }
     const int64_t items = (int64_t)a.items_x + a.items_w, sms = RGS_SMS;
+    a.wait = (uint32_t)label_limits[0].load();
+    a.loads = (uint32_t)label_limits[1].load();
     rgs_label_tc_kernel<P, GRAD, KC, CS, WHOLE><<<(unsigned)(items < sms ? items : sms), LTHREADS, LSMEM, stream>>>(m.x, m.w, m.ex, m.ew, a);
     return (int)cudaGetLastError();
 }
@@ -1285,6 +1314,14 @@ static void label_fill(LabelPrep& q, const LabelPlan& p, unsigned char* s, const
 }
 
 extern "C" {
+
+// Sets limit `which` (0: tries of a wait, 1: stages a producer fills) to `value`, a negative one to its default, for launches from
+// now on; returns the value before, or -1 for a limit that there is not.
+int64_t rgs_cuda_label_limit(int64_t which, int64_t value) {
+    if (which < 0 || which > 1) return -1;
+    if (value < 0) value = which ? 0xffffffffll : LWAIT;
+    return label_limits[which].exchange(value);
+}
 
 // direct: bit 0 / 1: rows of x / w start on 16-byte boundaries
 int64_t rgs_cuda_label_scratch_bytes(int64_t n, int64_t c, int64_t vocab, int64_t dtype, int64_t direct, int64_t backward) {

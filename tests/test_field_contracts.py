@@ -171,3 +171,61 @@ def test_label_loss_scores_that_32_bits_hold_coarsely(device, dtype, spread, bia
     ref = (wd[s.argmax(1)] - wd[y])[clear]
     half = 2.0 ** -24 if dtype == F32 else 2.0 ** -8
     assert ((gx[clear].double() - ref).abs() <= 2 * half * ref.abs() + 2.0 ** -21 * wd.abs().max()).all()
+
+
+@pytest.fixture
+def label_limit():
+    """Sets a limit of the label kernel's waits (0: tries, 1: stages that a producer fills); defaults afterwards."""
+    dev = torch.device("cuda")
+    yield lambda which, value: native.size_of("label_limit", dev, which, value)
+    for which in (0, 1):
+        native.size_of("label_limit", dev, which, -1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,c,v,dtype", [(20000, 64, 700, BF16), (3000, 300, 900, BF16), (20000, 32, 300, F32), (2000, 200, 600, F32),
+                                         (300, 64, 9000, BF16), (20000, 40, 100, BF16)])
+def test_label_loss_is_right_or_nan_when_waits_run_out(label_limit, n, c, v, dtype):
+    """The producer of every CTA gives up after a few stages, or waits have a few tries only: the call returns, every number
+    that it gives is that of an undisturbed run or NaN, and the next call is undisturbed."""
+    x, w, y, b = make_label_case(n, c, v, dtype, seed=c, device="cuda")
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    labelled = y >= 0
+    up = torch.rand(n, generator=torch.Generator().manual_seed(1)).cuda() + 0.5
+
+    def forward(reduction):
+        return R.label_loss(x, w, y, bias=b, reduction=reduction)
+
+    def right_or_nan(got, want):
+        assert (torch.isnan(got) | (got == want)).all()
+        return bool(torch.isnan(got).any())
+
+    losses, mean = forward("none").detach(), forward("mean").detach()
+    grads = {r: torch.autograd.grad(forward(r), leaves, u) for r, u in (("none", up), ("mean", None))}
+    assert all(torch.isfinite(t).all() for t in (losses, mean, *grads["none"], *grads["mean"]))
+    for which, values in ((1, (0, 1, 2, 3, 5, 8, 13, 40)), (0, (0, 1, 2, 3, 6))):
+        for value in values:
+            label_limit(which, value)
+            got = forward("none").detach()
+            hit = right_or_nan(got, losses)
+            got_mean = forward("mean").detach()
+            right_or_nan(got_mean, mean)
+            label_limit(which, -1)
+            if value == 0:
+                assert hit and torch.isnan(got[labelled]).all() and torch.isnan(got_mean) and (got[~labelled] == 0).all()
+            for reduction, u in (("none", up), ("mean", None)):
+                out = forward(reduction)
+                label_limit(which, value)
+                part = torch.autograd.grad(out, leaves, u)
+                label_limit(which, -1)
+                hits = [right_or_nan(p, q) for p, q in zip(part, grads[reduction])]
+                if value == 0:
+                    assert all(hits) and torch.isnan(part[0][labelled]).all() and (part[0][~labelled] == 0).all()
+                    assert torch.isnan(part[1]).all() and torch.isnan(part[2]).all()
+        # a forward pass that gave up: what hangs on it is NaN in the backward pass, not a gradient of something else
+        label_limit(which, 0)
+        out = forward("mean")
+        label_limit(which, -1)
+        assert all(torch.isnan(t).any() for t in (out, *torch.autograd.grad(out, leaves)))
+    assert torch.equal(forward("none"), losses)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(forward("mean"), leaves), grads["mean"]))
