@@ -132,7 +132,7 @@ static inline double label_score(const void* x, int64_t xi, const void* w, int64
 // lse (2,n): largest score and log sum exp(score - largest) of a row, two numbers so that scores of any size (all labels at
 // the lowest value of the type, say) keep their differences; losses[i] per row, result[0] = sum / max(count, 1) or sum, count[0] = rows that count
 int rgs_cpu_label_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* labels, int64_t label_bytes,
-                      int64_t n, int64_t c, int64_t vocab, int64_t dtype, int64_t b_dtype, int64_t mean, void*, float* lse, float* losses,
+                      int64_t n, int64_t c, int64_t vocab, int64_t dtype, int64_t b_dtype, int64_t mean, void*, int64_t, float* lse, float* losses,
                       float* result, float* count, void*) {
     double total = 0;
     int64_t rows = 0;
@@ -161,7 +161,7 @@ int rgs_cpu_label_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, co
 // gout: one gradient for all rows (per_row = 0; divided by max(count, 1) for the mean) or one per row
 int rgs_cpu_label_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* labels, int64_t label_bytes,
                       int64_t n, int64_t c, int64_t vocab, int64_t dtype, int64_t b_dtype, const float* lse, const float* gout,
-                      int64_t per_row, int64_t mean, const float* count, void*, void* dx, void* dw, void* db, void*) {
+                      int64_t per_row, int64_t mean, const float* count, void*, int64_t, void* dx, void* dw, void* db, void*) {
     const double scale = mean ? 1.0 / (*count > 1.f ? *count : 1.f) : 1.0;
     auto grad = [&](int64_t i, int64_t v, int64_t y) -> double {
         const double l = label_score(x, i * ldx, w, v * ldw, bias, v, c, (int)dtype, (int)b_dtype);

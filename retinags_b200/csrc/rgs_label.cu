@@ -71,7 +71,8 @@ struct LabelArgs {
     int whole, stages;               // stages of B are kept for both products; stages of the ring
     int nbuf, nob;                   // score and output buffers in TMEM
     int nmx, nmw;                    // tiles of 128 pixels, of 128 labels
-    int nsx, nsw;                    // pieces of the walk over labels (forward, dX) and over pixels (dW)
+    int nsx, nsw;                    // partial sums of the walk over labels (forward, dX) and over pixels (dW)
+    int subx, subw, sub;             // pieces added into a partial sum, one a launch; those of this launch
     int perx, restx, perw, restw;    // tiles of a piece: per, one more in the first rest pieces
     unsigned items_x, items_w;
     const float* kn;                 // (nmx, 3, 128) per pixel: label (bits; -1: none), g, factor; backward only
@@ -219,6 +220,7 @@ __device__ __forceinline__ LabelItem lb_item(const LabelArgs& a, unsigned i) {
     it.oc0 = (int)range * a.noc;
     it.noc = min(a.noc, a.nk - it.oc0);
     it.split = (int)q;
+    q = q * (unsigned)(it.dw ? a.subw : a.subx) + (unsigned)a.sub;  // its piece
     it.j0 = (int)(q * base + min(q, rest));  // the first `rest` pieces are one tile longer
     it.j1 = it.j0 + (int)base + (q < rest);
     return it;
@@ -233,7 +235,8 @@ struct LabelCursor {
 };
 
 // sixteen channels of a row of the output, rounded to its type; vector stores where rows keep their alignment
-__device__ __forceinline__ void lb_store16(void* out, int64_t r, int c, int channels, int dtype, const float (&f)[16]) {
+// (add: on top of what is there, 32 bits only)
+__device__ __forceinline__ void lb_store16(void* out, int64_t r, int c, int channels, int dtype, bool add, float (&f)[16]) {
     if (dtype == RGS_BF16) {
         __nv_bfloat16* p = static_cast<__nv_bfloat16*>(out) + r * channels + c;
         if ((channels & 7) == 0) {
@@ -248,6 +251,9 @@ __device__ __forceinline__ void lb_store16(void* out, int64_t r, int c, int chan
         }
     } else {
         float* p = static_cast<float*>(out) + r * channels + c;
+        if (add)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) f[q] += c + q < channels ? p[q] : 0.f;
         if ((channels & 3) == 0) {
 #pragma unroll
             for (int q = 0; q < 16; q += 4)
@@ -602,7 +608,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t o = tmem + lanes + OUT + oc_.slot * OB;
             const int64_t r = (int64_t)it.m * LT + row, rows = it.dw ? a.v : a.n;
-            const int ns = it.dw ? a.nsw : a.nsx;
+            float* part = it.dw ? a.part_w : a.part_x;
             for (int c0 = wg * 16; c0 < it.noc * KC; c0 += 64) {
                 const int c = it.oc0 * KC + c0;
                 if (c >= a.c) break;
@@ -618,17 +624,20 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                     float f[16];
 #pragma unroll
                     for (int q = 0; q < 16; ++q) f[q] = lost ? nan : P == 3 ? __uint_as_float(u[q]) + __uint_as_float(lo[q]) : __uint_as_float(u[q]);
-                    if (ns > 1) {
+                    if (part) {
                         if (it.dw)
 #pragma unroll
                             for (int q = 0; q < 16; ++q) f[q] *= scale;
-                        float* p = (it.dw ? a.part_w : a.part_x) + ((int64_t)it.split * (it.dw ? a.nmw : a.nmx) * LT + r) * a.cq + c;
+                        float* p = part + ((int64_t)it.split * (it.dw ? a.nmw : a.nmx) * LT + r) * a.cq + c;
+                        if (a.sub)
+#pragma unroll
+                            for (int q = 0; q < 16; ++q) f[q] += p[q];
 #pragma unroll
                         for (int q = 0; q < 16; q += 4) *reinterpret_cast<float4*>(p + q) = make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]);
                     } else {
 #pragma unroll
                         for (int q = 0; q < 16; ++q) f[q] = label < 0 ? 0.f : f[q] * scale;
-                        lb_store16(it.dw ? a.dw : a.dx, r, c, a.c, a.dtype, f);
+                        lb_store16(it.dw ? a.dw : a.dx, r, c, a.c, a.dtype, a.sub != 0, f);
                     }
                 }
                 __syncwarp();
@@ -842,7 +851,8 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 }
             } else if (it.dw && a.part_b && it.oc0 == 0) {
                 dead = __any_sync(0xffffffffu, dead || *fail);
-                a.part_b[((int64_t)it.split * 4 + wg) * a.nmw * LT + r] = dead ? nan : sum * gshare;
+                float* p = a.part_b + ((int64_t)it.split * 4 + wg) * a.nmw * LT + r;
+                *p = (dead ? nan : sum * gshare) + (a.sub ? *p : 0.f);
             }
         }
         if (GRAD && out_i < items) {
@@ -1154,26 +1164,36 @@ static int label_map(CUtensorMap* map, const void* base, int64_t c, int64_t rows
                kc == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : kc == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : 21;
 }
 
-// Limits of the waits: [0] tries, [1] stages that the producer of a CTA fills before it gives up.  Tests lower them.
-static std::atomic<int64_t> label_limits[2] = {{LWAIT}, {0xffffffffll}};
+// Limits: [0] tries of a wait, [1] stages that the producer of a CTA fills before it gives up, [2] bytes of partial sums of dX and
+// of dW (and one sum more).  Tests lower them.
+static const int64_t label_defaults[3] = {LWAIT, 0xffffffffll, (int64_t)1 << 31};
+static std::atomic<int64_t> label_limits[3] = {{label_defaults[0]}, {label_defaults[1]}, {label_defaults[2]}};
 
 static inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
-// Number of pieces of a walk over nj tiles made by `tiles` row tiles: one where there are three row tiles or more to an
-// SM; else pieces short enough for six items to an SM.  `run` bounds the tiles that one accumulator sums, `most` the pieces.
-static int label_pieces(int64_t tiles, int64_t nj, int64_t sms, int64_t run, int64_t most) {
+// A walk over nj tiles made by `tiles` row tiles, in `slots` partial sums of `subs` pieces each.  One piece where there are three
+// row tiles or more to an SM; else pieces short enough for six items to an SM.  No piece is longer than `run` tiles, the most
+// that one accumulator may sum; there is room for `most` partial sums, and where that is too few the pieces of one follow each
+// other in launches of their own, each adding to what the ones before left (1657600 pixels x 64 channels x 32771 labels in 32 bits:
+// with pieces of 43 tiles in place of eight dX was off by 1.5e-5 of its absolute sum, with one sign throughout, instead of 1.9e-6).
+static void label_pieces(int64_t tiles, int64_t nj, int64_t sms, int64_t run, int64_t most, int* slots, int* subs) {
     int64_t per = nj;
     if (tiles < 3 * sms) per = (tiles * nj + sms * 6 - 1) / (sms * 6);
     if (per > run) per = run;
     if (per < 1) per = 1;
-    int64_t ns = (nj + per - 1) / per;
-    if (ns > most) ns = most;
-    return (int)(ns < 1 ? 1 : ns);
+    int64_t ns = (nj + per - 1) / per, k = 1;
+    if (ns > most) {
+        ns = most < 1 ? 1 : most;
+        k = ((nj + run - 1) / run + ns - 1) / ns;
+        if (ns * k > nj) ns = nj / k;  // no empty pieces
+    }
+    *slots = (int)(ns < 1 ? 1 : ns);
+    *subs = (int)k;
 }
 
 struct LabelPlan {
     LabelArgs a;
-    int pieces, kc, cs, direct_x, direct_w, cp;
+    int pieces, kc, cs, direct_x, direct_w, cp, parts_x, parts_w;
     int64_t o_xs, o_ws, o_ew, o_ex, o_kn, o_gs, o_pm, o_ps, o_at, o_px, o_pw, o_pb, o_bsum, o_bcount, o_ticket, bytes;
 };
 
@@ -1216,15 +1236,19 @@ static void label_plan(LabelPlan& p, int64_t n, int64_t c, int64_t v, int dtype,
     const int64_t run = p.pieces == 1 ? 512 : 8;
     const int64_t rows_x = (int64_t)a.nmx * LT, rows_w = (int64_t)a.nmw * LT;
     if (backward) {
-        const int64_t room = (int64_t)1 << 31;  // bytes of partial sums
-        a.nsx = label_pieces((int64_t)a.nmx * a.nrange, a.nmw, sms, run, room / (rows_x * a.cq * 4) + 1);
-        a.nsw = label_pieces((int64_t)a.nmw * a.nrange, a.nmx, sms, run, room / (rows_w * a.cq * 4) + 1);
+        const int64_t room = label_limits[2].load();
+        label_pieces((int64_t)a.nmx * a.nrange, a.nmw, sms, run, room / (rows_x * a.cq * 4) + 1, &a.nsx, &a.subx);
+        label_pieces((int64_t)a.nmw * a.nrange, a.nmx, sms, run, room / (rows_w * a.cq * 4) + 1, &a.nsw, &a.subw);
     } else {
-        a.nsx = label_pieces(a.nmx, a.nmw, sms, a.nmw, a.nmw);
-        a.nsw = 1;
+        label_pieces(a.nmx, a.nmw, sms, a.nmw, a.nmw, &a.nsx, &a.subx);
+        a.nsw = a.subw = 1;
     }
-    a.perx = a.nmw / a.nsx; a.restx = a.nmw % a.nsx;
-    a.perw = a.nmx / a.nsw; a.restw = a.nmx % a.nsw;
+    const int px = a.nsx * a.subx, pw = a.nsw * a.subw;
+    a.perx = a.nmw / px; a.restx = a.nmw % px;
+    a.perw = a.nmx / pw; a.restw = a.nmx % pw;
+    // one partial sum: 32-bit outputs are added up where they lie
+    p.parts_x = a.nsx > 1 || (a.subx > 1 && dtype == RGS_BF16);
+    p.parts_w = a.nsw > 1 || (a.subw > 1 && dtype == RGS_BF16);
     int64_t o = 0;
     auto take = [&](int64_t bytes) { const int64_t at = o; o = up(o + bytes, 1024); return at; };
     p.o_xs = p.direct_x ? -1 : take(n * p.cp * 2 * p.pieces);
@@ -1234,8 +1258,8 @@ static void label_plan(LabelPlan& p, int64_t n, int64_t c, int64_t v, int dtype,
     if (backward) {
         p.o_kn = take(rows_x * 12);
         p.o_gs = take(4);
-        p.o_px = a.nsx > 1 ? take(a.nsx * rows_x * a.cq * 4) : -1;
-        p.o_pw = a.nsw > 1 ? take(a.nsw * rows_w * a.cq * 4) : -1;
+        p.o_px = p.parts_x ? take(a.nsx * rows_x * a.cq * 4) : -1;
+        p.o_pw = p.parts_w ? take(a.nsw * rows_w * a.cq * 4) : -1;
         p.o_pb = take(4 * a.nsw * rows_w * 4);
     } else {
         p.o_pm = take(4 * a.nsx * n * 4);
@@ -1315,12 +1339,11 @@ static void label_fill(LabelPrep& q, const LabelPlan& p, unsigned char* s, const
 
 extern "C" {
 
-// Sets limit `which` (0: tries of a wait, 1: stages a producer fills) to `value`, a negative one to its default, for launches from
-// now on; returns the value before, or -1 for a limit that there is not.
+// Sets limit `which` of label_limits to `value`, a negative one to its default, for calls from now on; returns the value before, or
+// -1 for a limit that there is not.
 int64_t rgs_cuda_label_limit(int64_t which, int64_t value) {
-    if (which < 0 || which > 1) return -1;
-    if (value < 0) value = which ? 0xffffffffll : LWAIT;
-    return label_limits[which].exchange(value);
+    if (which < 0 || which > 2) return -1;
+    return label_limits[which].exchange(value < 0 ? label_defaults[which] : value);
 }
 
 // direct: bit 0 / 1: rows of x / w start on 16-byte boundaries
@@ -1331,11 +1354,12 @@ int64_t rgs_cuda_label_scratch_bytes(int64_t n, int64_t c, int64_t vocab, int64_
 }
 
 int rgs_cuda_label_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* labels, int64_t label_bytes,
-                       int64_t n, int64_t c, int64_t vocab, int64_t dtype, int64_t b_dtype, int64_t mean, void* scratch, float* lse,
-                       float* losses, float* result, float* count, void* stream) {
+                       int64_t n, int64_t c, int64_t vocab, int64_t dtype, int64_t b_dtype, int64_t mean, void* scratch, int64_t scratch_bytes,
+                       float* lse, float* losses, float* result, float* count, void* stream) {
     cudaStream_t st = (cudaStream_t)stream;
     LabelPlan p;
     label_plan(p, n, c, vocab, (int)dtype, label_direct(x, ldx, w, ldw), 0);
+    if (p.bytes > scratch_bytes) return 24;
     LabelArgs& a = p.a;
     unsigned char* s = reinterpret_cast<unsigned char*>(up((int64_t)reinterpret_cast<uintptr_t>(scratch), 1024));
     LabelPrep q{};
@@ -1362,10 +1386,11 @@ int rgs_cuda_label_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
 
 int rgs_cuda_label_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* labels, int64_t label_bytes,
                        int64_t n, int64_t c, int64_t vocab, int64_t dtype, int64_t b_dtype, const float* lse, const float* gout,
-                       int64_t per_row, int64_t mean, const float* count, void* scratch, void* dx, void* dw, void* db, void* stream) {
+                       int64_t per_row, int64_t mean, const float* count, void* scratch, int64_t scratch_bytes, void* dx, void* dw, void* db, void* stream) {
     cudaStream_t st = (cudaStream_t)stream;
     LabelPlan p;
     label_plan(p, n, c, vocab, (int)dtype, label_direct(x, ldx, w, ldw), 1);
+    if (p.bytes > scratch_bytes) return 24;
     LabelArgs& a = p.a;
     unsigned char* s = reinterpret_cast<unsigned char*>(up((int64_t)reinterpret_cast<uintptr_t>(scratch), 1024));
     LabelPrep q{};
@@ -1379,17 +1404,20 @@ int rgs_cuda_label_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     if (rc) return rc;
     label_prep(p, q, st);
     RGS_CUDA_CHECK(cudaGetLastError());
-    a.items_x = dx ? (unsigned)a.nmx * a.nrange * a.nsx : 0;
-    a.items_w = dw || db ? (unsigned)a.nmw * a.nrange * a.nsw : 0;
     a.kn = q.kn; a.lse = lse; a.gs = q.gs; a.per_row = (int)per_row;
     a.labels = labels; a.label_bytes = (int)label_bytes;
     a.flags = count;
-    a.part_x = dx && a.nsx > 1 ? reinterpret_cast<float*>(s + p.o_px) : nullptr;
-    a.part_w = dw && a.nsw > 1 ? reinterpret_cast<float*>(s + p.o_pw) : nullptr;
+    a.part_x = dx && p.parts_x ? reinterpret_cast<float*>(s + p.o_px) : nullptr;
+    a.part_w = dw && p.parts_w ? reinterpret_cast<float*>(s + p.o_pw) : nullptr;
     a.part_b = db ? reinterpret_cast<float*>(s + p.o_pb) : nullptr;
     a.dx = dx; a.dw = dw;
-    rc = label_run<true>(p, m, st);
-    if (rc) return rc;
+    const int subx = dx ? a.subx : 0, subw = dw || db ? a.subw : 0;
+    for (a.sub = 0; a.sub < subx || a.sub < subw; ++a.sub) {
+        a.items_x = a.sub < subx ? (unsigned)a.nmx * a.nrange * a.nsx : 0;
+        a.items_w = a.sub < subw ? (unsigned)a.nmw * a.nrange * a.nsw : 0;
+        rc = label_run<true>(p, m, st);
+        if (rc) return rc;
+    }
     if (a.part_x) rgs_label_reduce_x_kernel<<<label_grid(n * (a.cq / 4), RGS_SMS * 16), 256, 0, st>>>(a);
     const int64_t blocks_w = a.part_w ? (vocab * (a.cq / 4) + 31) / 32 : 0, blocks_b = db ? (vocab + 31) / 32 : 0;
     if (blocks_w + blocks_b) rgs_label_reduce_w_kernel<<<(unsigned)(blocks_w + blocks_b), 512, 0, st>>>(a, (int)blocks_w, db, (int)b_dtype);

@@ -44,8 +44,9 @@ class _LabelLoss(torch.autograd.Function):
         result = None if per_row else new((), dtype=torch.float32, device=dev)
         b_code = DTYPES[bias.dtype] if bias is not None else 0
         if n:
+            scratch = _scratch(x, ldx, w, ldw, 0)
             native.call("label_fwd", dev, x, ldx, w, ldw, bias, y, y.element_size(), n, c, v, DTYPES[x.dtype], b_code,
-                        int(reduction == "mean"), _scratch(x, ldx, w, ldw, 0), lse, losses, result, lse + 8 * n)
+                        int(reduction == "mean"), scratch, scratch.numel(), lse, losses, result, lse + 8 * n)
         ctx.save_for_backward(x, w, bias, y, state)
         ctx.args = (features.shape, weight.shape, saved_as(x, w, bias, y, state), b_code, reduction)
         return losses.view(features.shape[:-1]) if per_row else result
@@ -71,9 +72,10 @@ def _label_backward(ctx, gout):
     dw = new(w_shape, dtype=w.dtype, device=dev) if ctx.needs_input_grad[1] else None
     db = new(v, dtype=bias.dtype, device=dev) if ctx.needs_input_grad[2] else None
     if n and (dx is not None or dw is not None or db is not None):
+        scratch = _scratch(x, ldx, w, ldw, 1)
         native.call("label_bwd", dev, x, ldx, w, ldw, bias, y, y.element_size(), n, c, v, DTYPES[x.dtype], b_code, state, g,
                     int(reduction == "none"), int(reduction == "mean"), state.data_ptr() + 8 * n,
-                    _scratch(x, ldx, w, ldw, 1), dx, dw, db)
+                    scratch, scratch.numel(), dx, dw, db)
     return dx, dw, db, None, None
 
 

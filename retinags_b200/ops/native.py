@@ -45,8 +45,8 @@ SIGNATURES = {
     "densify_gather": "pppiippppppiipp",
     "records_pack": "pppipiipp",
     "records_unpack": "pipppiip",
-    "label_fwd": "pipippiiiiiiipppppp",
-    "label_bwd": "pipippiiiiiippiipppppp",
+    "label_fwd": "pipippiiiiiiipippppp",
+    "label_bwd": "pipippiiiiiippiippipppp",
     "norm_fwd": "piiippiiifpippp",
     "norm_bwd": "piiipppiipiiifppppp",
     "pack8": "piiiiippp",

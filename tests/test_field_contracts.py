@@ -5,7 +5,7 @@ import torch
 
 import retinags_b200 as R
 from retinags_b200.ops import native
-from field_reference import make_label_case
+from field_reference import assert_within, label_reference, make_label_case
 
 F32, BF16 = torch.float32, torch.bfloat16
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -175,10 +175,11 @@ def test_label_loss_scores_that_32_bits_hold_coarsely(device, dtype, spread, bia
 
 @pytest.fixture
 def label_limit():
-    """Sets a limit of the label kernel's waits (0: tries, 1: stages that a producer fills); defaults afterwards."""
+    """Sets a limit of the label kernel (0: tries of a wait, 1: stages that a producer fills, 2: bytes of partial sums); defaults
+    afterwards."""
     dev = torch.device("cuda")
     yield lambda which, value: native.size_of("label_limit", dev, which, value)
-    for which in (0, 1):
+    for which in (0, 1, 2):
         native.size_of("label_limit", dev, which, -1)
 
 
@@ -229,3 +230,77 @@ def test_label_loss_is_right_or_nan_when_waits_run_out(label_limit, n, c, v, dty
         assert all(torch.isnan(t).any() for t in (out, *torch.autograd.grad(out, leaves)))
     assert torch.equal(forward("none"), losses)
     assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(forward("mean"), leaves), grads["mean"]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("room", [-1, 0, 200000])
+@pytest.mark.parametrize("which", ["features", "weight"])
+def test_label_loss_32_bit_sums_of_one_sign_whatever_the_room(label_limit, which, room):
+    """Gradients that add 32768 numbers of one sign.  All scores are zero (so every p is 1/V) and the label's own row adds nothing.
+
+    The tensor core truncates where it adds, by less than 2^-23 of the sum a step.  Accumulators of eight tiles take 64 steps:
+    64 * 2^-23 = 7.7e-6 of the sum; the pieces of 256 tiles are 32 to 256 sums rounded to nearest, 288 * 2^-25 on average over a
+    growing sum = 8.6e-6 if all went one way; p is off by 2e-6 (logarithm, exponential).  With one accumulator for all, 2048
+    steps lose half of 2^-23.5 of a sum that grows to its end: 4e-5."""
+    label_limit(2, room)
+    gen = torch.Generator().manual_seed(7)
+    big, small, c = 32768, 130, 64
+    if which == "features":
+        x = torch.zeros(small, c, device="cuda", requires_grad=True)
+        w = (torch.rand(big, c, generator=gen) + 0.5).cuda()
+        w[0] = 0.0
+        leaf, y = x, torch.zeros(small, dtype=torch.long, device="cuda")
+    else:
+        x = (torch.rand(big, c, generator=gen) + 0.5).cuda()
+        w = torch.zeros(small, c, device="cuda", requires_grad=True)
+        leaf, y = w, torch.zeros(big, dtype=torch.long, device="cuda")
+    (g,) = torch.autograd.grad(R.label_loss(x, w, y, reduction="sum"), leaf)
+    if which == "features":
+        want = (w.double().sum(0) / big).expand(small, c)
+    else:
+        g, want = g[1:], (x.double().sum(0) / small).expand(small - 1, c)
+    err = ((g.double() - want) / want).abs().max().item()
+    assert err <= 7.7e-6 + 8.6e-6 + 2e-6, err
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,c,v,dtype", [(300, 64, 3000, F32), (3000, 200, 300, F32), (3000, 33, 2900, F32), (130, 64, 70000, BF16), (70000, 40, 130, BF16),
+                                         (70000, 300, 130, BF16)])
+def test_label_loss_pieces_that_follow_each_other(label_limit, n, c, v, dtype):
+    """No room for more than one partial sum: its pieces are added launch after launch; the same bits every time."""
+    x, w, y, b = make_label_case(n, c, v, dtype, seed=n, device="cuda")
+    count = max(int((y >= 0).sum()), 1)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    ref = label_reference(x.detach(), w.detach(), y, b.detach(), torch.full((n,), 1.0 / count, device="cuda"), dtype)
+    full = torch.autograd.grad(R.label_loss(x, w, y, bias=b), leaves)
+    label_limit(2, 0)
+    runs = [torch.autograd.grad(R.label_loss(x, w, y, bias=b), leaves) for _ in range(2)]
+    for name, got, again, r in zip(("dX", "dW", "db"), *runs, ref[1:]):
+        assert_within(got, r, name)
+        assert torch.equal(got, again)
+    for got, r in zip(full, ref[1:]):
+        assert_within(got, r)
+    for k in range(3):  # one gradient alone: the same bits
+        t = [p.detach() for p in leaves]
+        t[k].requires_grad_(True)
+        (g,) = torch.autograd.grad(R.label_loss(t[0], t[1], y, bias=t[2]), t[k])
+        assert torch.equal(g, runs[0][k])
+
+
+@pytest.mark.gpu
+def test_label_loss_refuses_a_workspace_that_is_too_small(label_limit):
+    """A workspace sized under another limit than the call's is refused, not overrun."""
+    x, w, y, b = make_label_case(3000, 64, 3000, F32, seed=1, device="cuda")
+    loss = R.label_loss(x.requires_grad_(True), w, y, bias=b)
+    want = torch.autograd.grad(loss, x, retain_graph=True)
+    from retinags_b200.ops import label_loss as module
+    sized = module._scratch
+    try:
+        module._scratch = lambda *a: sized(*a)[:-1]
+        with pytest.raises(RuntimeError, match="status 24"):
+            torch.autograd.grad(loss, x, retain_graph=True)
+        with pytest.raises(RuntimeError, match="status 24"):
+            R.label_loss(x, w, y, bias=b)
+    finally:
+        module._scratch = sized
+    assert torch.equal(torch.autograd.grad(loss, x)[0], want[0])
