@@ -851,7 +851,10 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 }
             } else if (it.dw && a.part_b && it.oc0 == 0) {
                 dead = __any_sync(0xffffffffu, dead || *fail);
-                float* p = a.part_b + ((int64_t)it.split * 4 + wg) * a.nmw * LT + r;
+                // which warpgroup takes the even tiles of an item hangs on the items before it: the sums go by even and odd, so
+                // that their order, and db, do not hang on what else is asked for
+                const int place = wg ^ (int)((t - (uint32_t)(it.j1 - it.j0)) & 1u);
+                float* p = a.part_b + ((int64_t)it.split * 4 + place) * a.nmw * LT + r;
                 *p = (dead ? nan : sum * gshare) + (a.sub ? *p : 0.f);
             }
         }

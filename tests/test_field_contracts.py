@@ -304,3 +304,16 @@ def test_label_loss_refuses_a_workspace_that_is_too_small(label_limit):
     finally:
         module._scratch = sized
     assert torch.equal(torch.autograd.grad(loss, x)[0], want[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,c,v,dtype", [(20000, 64, 3000, F32), (20000, 64, 3000, BF16), (30000, 200, 300, BF16), (9000, 100, 900, F32)])
+def test_label_loss_gradients_do_not_depend_on_what_else_is_asked_for(n, c, v, dtype):
+    x, w, y, b = make_label_case(n, c, v, dtype, seed=3, device="cuda")
+    out = {}
+    for wanted in ((0, 1, 2), (0,), (1,), (2,), (0, 2), (1, 2), (0, 1)):
+        t = [p.detach().requires_grad_(k in wanted) for k, p in enumerate((x, w, b))]
+        out[wanted] = dict(zip(wanted, torch.autograd.grad(R.label_loss(t[0], t[1], y, bias=t[2]), [t[k] for k in wanted])))
+    for wanted, grads in out.items():
+        for k, g in grads.items():
+            assert torch.equal(g, out[(0, 1, 2)][k]), (wanted, k)
