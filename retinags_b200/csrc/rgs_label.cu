@@ -1202,6 +1202,9 @@ struct LabelPlan {
 
 #define LJOIN 592  // most blocks of the joining kernel
 
+// what a backward pass is to give: bits of `backward`, 0 for the forward pass
+enum { LB_ANY = 1, LB_DX = 2, LB_DW = 4, LB_DB = 8 };
+
 static void label_plan(LabelPlan& p, int64_t n, int64_t c, int64_t v, int dtype, int direct, int backward) {
     LabelArgs& a = p.a;
     memset(&p, 0, sizeof(p));
@@ -1250,8 +1253,8 @@ static void label_plan(LabelPlan& p, int64_t n, int64_t c, int64_t v, int dtype,
     a.perx = a.nmw / px; a.restx = a.nmw % px;
     a.perw = a.nmx / pw; a.restw = a.nmx % pw;
     // one partial sum: 32-bit outputs are added up where they lie
-    p.parts_x = a.nsx > 1 || (a.subx > 1 && dtype == RGS_BF16);
-    p.parts_w = a.nsw > 1 || (a.subw > 1 && dtype == RGS_BF16);
+    p.parts_x = !(backward & LB_DX) ? 0 : a.nsx > 1 || (a.subx > 1 && dtype == RGS_BF16);
+    p.parts_w = !(backward & LB_DW) ? 0 : a.nsw > 1 || (a.subw > 1 && dtype == RGS_BF16);
     int64_t o = 0;
     auto take = [&](int64_t bytes) { const int64_t at = o; o = up(o + bytes, 1024); return at; };
     p.o_xs = p.direct_x ? -1 : take(n * p.cp * 2 * p.pieces);
@@ -1263,7 +1266,7 @@ static void label_plan(LabelPlan& p, int64_t n, int64_t c, int64_t v, int dtype,
         p.o_gs = take(4);
         p.o_px = p.parts_x ? take(a.nsx * rows_x * a.cq * 4) : -1;
         p.o_pw = p.parts_w ? take(a.nsw * rows_w * a.cq * 4) : -1;
-        p.o_pb = take(4 * a.nsw * rows_w * 4);
+        p.o_pb = backward & LB_DB ? take(4 * a.nsw * rows_w * 4) : -1;
     } else {
         p.o_pm = take(4 * a.nsx * n * 4);
         p.o_ps = take(4 * a.nsx * n * 4);
@@ -1349,7 +1352,7 @@ int64_t rgs_cuda_label_limit(int64_t which, int64_t value) {
     return label_limits[which].exchange(value < 0 ? label_defaults[which] : value);
 }
 
-// direct: bit 0 / 1: rows of x / w start on 16-byte boundaries
+// direct: bit 0 / 1: rows of x / w start on 16-byte boundaries; backward: 0, or LB_ bits of the gradients wanted
 int64_t rgs_cuda_label_scratch_bytes(int64_t n, int64_t c, int64_t vocab, int64_t dtype, int64_t direct, int64_t backward) {
     LabelPlan p;
     label_plan(p, n, c, vocab, (int)dtype, (int)direct, (int)backward);
@@ -1392,7 +1395,7 @@ int rgs_cuda_label_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
                        int64_t per_row, int64_t mean, const float* count, void* scratch, int64_t scratch_bytes, void* dx, void* dw, void* db, void* stream) {
     cudaStream_t st = (cudaStream_t)stream;
     LabelPlan p;
-    label_plan(p, n, c, vocab, (int)dtype, label_direct(x, ldx, w, ldw), 1);
+    label_plan(p, n, c, vocab, (int)dtype, label_direct(x, ldx, w, ldw), LB_ANY | (dx ? LB_DX : 0) | (dw ? LB_DW : 0) | (db ? LB_DB : 0));
     if (p.bytes > scratch_bytes) return 24;
     LabelArgs& a = p.a;
     unsigned char* s = reinterpret_cast<unsigned char*>(up((int64_t)reinterpret_cast<uintptr_t>(scratch), 1024));
@@ -1410,8 +1413,8 @@ int rgs_cuda_label_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     a.kn = q.kn; a.lse = lse; a.gs = q.gs; a.per_row = (int)per_row;
     a.labels = labels; a.label_bytes = (int)label_bytes;
     a.flags = count;
-    a.part_x = dx && p.parts_x ? reinterpret_cast<float*>(s + p.o_px) : nullptr;
-    a.part_w = dw && p.parts_w ? reinterpret_cast<float*>(s + p.o_pw) : nullptr;
+    a.part_x = p.parts_x ? reinterpret_cast<float*>(s + p.o_px) : nullptr;
+    a.part_w = p.parts_w ? reinterpret_cast<float*>(s + p.o_pw) : nullptr;
     a.part_b = db ? reinterpret_cast<float*>(s + p.o_pb) : nullptr;
     a.dx = dx; a.dw = dw;
     const int subx = dx ? a.subx : 0, subw = dw || db ? a.subw : 0;

@@ -19,7 +19,8 @@ _LIMIT = 2 ** 31 - 1
 
 
 def _scratch(x: torch.Tensor, ldx: int, w: torch.Tensor, ldw: int, backward: int) -> torch.Tensor:
-    """Workspace of one pass; it depends on whether the kernels can read the rows as they lie (16-byte boundaries)."""
+    """Workspace of one pass; it depends on whether the kernels can read the rows as they lie (16-byte boundaries) and on the
+    gradients that a backward pass is to give (1, and 2 for features, 4 for weight, 8 for bias)."""
     device = x.device
     direct = (ldx % 8 == 0 and x.data_ptr() % 16 == 0) + 2 * (ldw % 8 == 0 and w.data_ptr() % 16 == 0)
     size = native.size_of("label_scratch_bytes", device, x.shape[0], x.shape[1], w.shape[0], DTYPES[x.dtype], direct, backward)
@@ -72,7 +73,7 @@ def _label_backward(ctx, gout):
     dw = new(w_shape, dtype=w.dtype, device=dev) if ctx.needs_input_grad[1] else None
     db = new(v, dtype=bias.dtype, device=dev) if ctx.needs_input_grad[2] else None
     if n and (dx is not None or dw is not None or db is not None):
-        scratch = _scratch(x, ldx, w, ldw, 1)
+        scratch = _scratch(x, ldx, w, ldw, 1 + 2 * (dx is not None) + 4 * (dw is not None) + 8 * (db is not None))
         native.call("label_bwd", dev, x, ldx, w, ldw, bias, y, y.element_size(), n, c, v, DTYPES[x.dtype], b_code, state, g,
                     int(reduction == "none"), int(reduction == "mean"), state.data_ptr() + 8 * n,
                     scratch, scratch.numel(), dx, dw, db)

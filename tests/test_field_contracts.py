@@ -307,6 +307,29 @@ def test_label_loss_refuses_a_workspace_that_is_too_small(label_limit):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_label_loss_takes_room_for_the_gradients_asked_for(dtype, monkeypatch):
+    """Partial sums of dX and of dW are in the workspace only where that gradient is asked for; values do not depend on it."""
+    from retinags_b200.ops import label_loss as module
+    sized, sizes = module._scratch, []
+    monkeypatch.setattr(module, "_scratch", lambda *a: (lambda t: (sizes.append(t.numel()), t)[1])(sized(*a)))
+    n, c, v = 20000, 64, 3000
+    x, w, y, b = make_label_case(n, c, v, dtype, seed=3, device="cuda")
+    out, used = {}, {}
+    for wanted in ((0, 1, 2), (0,), (1,), (2,), (0, 2), (1, 2)):
+        t = [p.detach().requires_grad_(k in wanted) for k, p in enumerate((x, w, b))]
+        loss = R.label_loss(t[0], t[1], y, bias=t[2])
+        sizes.clear()
+        out[wanted] = dict(zip(wanted, torch.autograd.grad(loss, [t[k] for k in wanted])))
+        (used[wanted],) = sizes
+    for wanted, grads in out.items():
+        assert all(torch.equal(g, out[(0, 1, 2)][k]) for k, g in grads.items())
+    assert used[(0,)] < used[(0, 2)] < used[(0, 1, 2)] and used[(2,)] < used[(1, 2)] < used[(0, 1, 2)]
+    parts_w = used[(1, 2)] - used[(2,)]  # pieces of dW, rows of 128 labels
+    assert parts_w >= 3072 * 64 * 4 and used[(0, 1, 2)] - used[(0, 2)] == parts_w
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n,c,v,dtype", [(20000, 64, 3000, F32), (20000, 64, 3000, BF16), (30000, 200, 300, BF16), (9000, 100, 900, F32)])
 def test_label_loss_gradients_do_not_depend_on_what_else_is_asked_for(n, c, v, dtype):
     x, w, y, b = make_label_case(n, c, v, dtype, seed=3, device="cuda")
