@@ -60,7 +60,7 @@
 #define LWAIT (1u << 20)
 #define LOG2E 1.4426950408889634f
 
-enum { LF_DIRTY = 1,   // a pixel without a label holds something that is not finite
+enum { LF_DIRTY = 1,   // a pixel without a label has a score that is not finite (its features, or a row of the weight)
        LF_LARGE = 2 }; // a largest score above 2^10: m and log z are not added up, and m stays out of the product
 
 struct LabelArgs {
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             if (!dead) rgs_mbar_arrive(&sh->o_free[oc_.slot]);
             oc_.next(a.nob);
         };
-        const bool dirty = GRAD && P == 1 && WHOLE && (flags & LF_DIRTY);
+        const bool dirty = GRAD && (flags & LF_DIRTY);
         const bool rare = dirty || scaled;
         int next_label = row_label(blockIdx.x), out_label = 0;
         float next_scale = row_scale(blockIdx.x), out_scale = 1.f;  // out_: of the first item whose output is not written
@@ -818,7 +818,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 };
                 if (rare) gradient(std::true_type());
                 else gradient(std::false_type());
-                if (P == 1 && dirty && it.dw) {
+                if (P == 1 && WHOLE && dirty && it.dw) {
                     // pixels without a label whose features are not finite: 0 * inf must not reach dW, so their rows of the
                     // staged block are cleared (row n of every chunk, whole, whatever the swizzle)
                     if (__float_as_int(kb[row - half]) < 0) {

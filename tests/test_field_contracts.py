@@ -340,3 +340,17 @@ def test_label_loss_gradients_do_not_depend_on_what_else_is_asked_for(n, c, v, d
     for wanted, grads in out.items():
         for k, g in grads.items():
             assert torch.equal(g, out[(0, 1, 2)][k]), (wanted, k)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("c", [24, 64, 300])
+@pytest.mark.parametrize("device", DEVICES)
+def test_label_loss_without_labels_gives_zeros_whatever_the_classifier_holds(device, c, dtype):
+    x, w, y, b = make_label_case(150, c, 140, dtype, seed=5, device=device)
+    y[:] = -1
+    w[3, 1], w[139, 0], b[7] = float("nan"), float("inf"), float("nan")
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    for reduction in ("mean", "sum", "none"):
+        out = R.label_loss(x, w, y, bias=b, reduction=reduction)
+        assert (out == 0).all()
+        assert all((g == 0).all() for g in torch.autograd.grad(out.sum(), leaves))
