@@ -2,6 +2,8 @@
 #include <math.h>
 #include <stdint.h>
 #include <string.h>
+#include <new>
+#include <vector>
 #include "rgs_field_math.h"
 
 static inline int64_t field_at(int64_t n, int64_t c, int64_t ld, int64_t planes) { return planes ? c * ld + n : n * ld + c; }
@@ -100,17 +102,23 @@ int rgs_cpu_norm_bwd(const void* x, int64_t dtype, int64_t ld, int64_t planes, c
         }
     }
     if (dw || db) {
+        std::vector<double> ms;  // mean and rstd of every row, once (anew for every channel: quadratic in the channels)
+        if (dw) {
+            try {
+                ms.resize(2 * (size_t)n);
+            } catch (const std::exception&) {
+                return 12;
+            }
+#pragma omp parallel for schedule(static)
+            for (int64_t i = 0; i < n; ++i) stats(i, ms[2 * i], ms[2 * i + 1]);
+        }
 #pragma omp parallel for schedule(static)
         for (int64_t j = 0; j < c; ++j) {
             double sw = 0, sb = 0;
             for (int64_t i = 0; i < n; ++i) {
                 const double g = rgs_load_as_float(dy, i * ldy + j, (int)dy_dtype);
                 sb += g;
-                if (dw) {
-                    double mu, rstd;
-                    stats(i, mu, rstd);
-                    sw += g * (kept(i, j) - mu) * rstd;
-                }
+                if (dw) sw += g * (kept(i, j) - ms[2 * i]) * ms[2 * i + 1];
             }
             if (dw) rgs_store_float(dw, j, (int)p_dtype, (float)sw);
             if (db) rgs_store_float(db, j, (int)p_dtype, (float)sb);

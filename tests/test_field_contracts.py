@@ -1,5 +1,7 @@
 """Label loss, layer norm and 8-bit features where callers meet them from the side: saved-tensor hooks, layouts of gradients,
 limits inside the accepted ranges.  Every case runs on the CPU backend and on the GPU."""
+import time
+
 import pytest
 import torch
 
@@ -354,3 +356,20 @@ def test_label_loss_without_labels_gives_zeros_whatever_the_classifier_holds(dev
         out = R.label_loss(x, w, y, bias=b, reduction=reduction)
         assert (out == 0).all()
         assert all((g == 0).all() for g in torch.autograd.grad(out.sum(), leaves))
+
+
+def test_cpu_layer_norm_is_linear_in_the_channels():
+    """The weight's gradient takes a row's mean and variance once, not once a channel: 32 times the channels in the same number
+    of elements must not take 32 times as long (4 times is allowed for caches and a busy machine)."""
+    def seconds(n, c):
+        x, dy = torch.randn(n, c, generator=torch.Generator().manual_seed(1)), torch.ones(n, c)
+        w = torch.ones(c, requires_grad=True)
+        best = float("inf")
+        for _ in range(3):
+            y = R.layer_norm(x, w)
+            t = time.perf_counter()
+            torch.autograd.grad(y, w, dy)
+            best = min(best, time.perf_counter() - t)
+        return best
+    seconds(64, 32)
+    assert seconds(512, 1024) < 4 * seconds(16384, 32) + 0.05
