@@ -75,6 +75,9 @@ static inline int64_t rgs_sm_count() {
 }
 #define RGS_SMS rgs_sm_count()
 
+// Kernels launched by the label-field entry points (rgs_norm.cu holds the number); returns it with `more` added.
+extern "C" int64_t rgs_cuda_field_launches(int64_t more);
+
 #define RGS_CUDA_CHECK(expr)                          \
     do {                                              \
         cudaError_t _e = (expr);                      \

@@ -1298,6 +1298,7 @@ static int label_launch(const LabelMaps& m, LabelArgs a, cudaStream_t stream) {
     a.wait = (uint32_t)label_limits[0].load();
     a.loads = (uint32_t)label_limits[1].load();
     rgs_label_tc_kernel<P, GRAD, KC, CS, WHOLE><<<(unsigned)(items < sms ? items : sms), LTHREADS, LSMEM, stream>>>(m.x, m.w, m.ex, m.ew, a);
+    rgs_cuda_field_launches(1);
     return (int)cudaGetLastError();
 }
 
@@ -1330,6 +1331,7 @@ static int label_operands(const LabelPlan& p, const LabelPrep& q, LabelMaps* m) 
 static void label_prep(const LabelPlan& p, const LabelPrep& q, cudaStream_t stream) {
     const int64_t work = ((q.xs ? q.n : 0) + (q.ws ? q.v : 0)) * (q.cp / 8) + (int64_t)q.nmw * LT + (q.backward ? (int64_t)q.nmx * LT : LT);
     rgs_label_prep_kernel<<<label_grid(work, RGS_SMS * 16), 256, 0, stream>>>(q);
+    rgs_cuda_field_launches(1);
 }
 
 static void label_fill(LabelPrep& q, const LabelPlan& p, unsigned char* s, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
@@ -1387,6 +1389,7 @@ int rgs_cuda_label_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     rgs_label_join_kernel<<<label_grid(n, LJOIN), 256, 0, st>>>(a.pm, a.ps, a.at, labels, (int)label_bytes, n, vocab, 4 * a.nsx, (int)mean, lse, losses,
                                                                 result, count, reinterpret_cast<double*>(s + p.o_bsum),
                                                                 reinterpret_cast<unsigned long long*>(s + p.o_bcount), q.ticket);
+    rgs_cuda_field_launches(1);
     return (int)cudaGetLastError();
 }
 
@@ -1426,6 +1429,7 @@ int rgs_cuda_label_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     }
     if (a.part_x) rgs_label_reduce_x_kernel<<<label_grid(n * (a.cq / 4), RGS_SMS * 16), 256, 0, st>>>(a);
     const int64_t blocks_w = a.part_w ? (vocab * (a.cq / 4) + 31) / 32 : 0, blocks_b = db ? (vocab + 31) / 32 : 0;
+    rgs_cuda_field_launches((a.part_x ? 1 : 0) + (blocks_w + blocks_b ? 1 : 0));
     if (blocks_w + blocks_b) rgs_label_reduce_w_kernel<<<(unsigned)(blocks_w + blocks_b), 512, 0, st>>>(a, (int)blocks_w, db, (int)b_dtype);
     return (int)cudaGetLastError();
 }

@@ -990,6 +990,7 @@ static int norm_rows_launch(const NormArgs& a, bool backward, cudaStream_t st) {
         // a few rows: one block, no partial sums, one launch
         const int64_t grid = want <= 4 ? 1 : at_most(at_most(want, most), NORM_PARTS);
         rgs_norm_rows_bwd_kernel<VEC, NV, LANES, SHIFT><<<(unsigned)grid, NT, 0, st>>>(a);
+        rgs_cuda_field_launches(1);
         return (int)grid;
     }
     static std::atomic<int64_t> most[2];
@@ -999,6 +1000,7 @@ static int norm_rows_launch(const NormArgs& a, bool backward, cudaStream_t st) {
     const unsigned grid = (unsigned)at_most(want, most[pack]);
     if (pack) rgs_norm_rows_fwd_kernel<VEC, NV, LANES, SHIFT, !SHIFT><<<grid, NT, 0, st>>>(a);
     else rgs_norm_rows_fwd_kernel<VEC, NV, LANES, SHIFT, false><<<grid, NT, 0, st>>>(a);
+    rgs_cuda_field_launches(1);
     return 0;
 }
 
@@ -1046,6 +1048,7 @@ static int norm_planes_launch(const NormArgs& a, int* parts, cudaStream_t st) {
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, rgs_norm_planes_kernel<NV, V, Q, BWD>, V * 32, (size_t)smem) != cudaSuccess || per_sm < 1) per_sm = 1;
     *parts = (int)at_most(at_most((a.n + 32 * Q - 1) / (32 * Q), RGS_SMS * per_sm), NORM_PARTS);
     rgs_norm_planes_kernel<NV, V, Q, BWD><<<(unsigned)*parts, V * 32, smem, st>>>(a);
+    rgs_cuda_field_launches(1);
     return (int)cudaGetLastError();
 }
 
@@ -1062,6 +1065,11 @@ static int norm_planes(const NormArgs& a, int* parts, cudaStream_t st) {
 }
 
 extern "C" {
+
+int64_t rgs_cuda_field_launches(int64_t more) {
+    static std::atomic<int64_t> count{0};
+    return count.fetch_add(more) + more;
+}
 
 int64_t rgs_cuda_norm_scratch_bytes(int64_t n, int64_t c) { return (int64_t)NORM_PARTS * 2 * c * 4 + (c > NR_MAX ? n * 8 : 0) + 16; }
 
@@ -1084,6 +1092,7 @@ int rgs_cuda_pack8(const void* x, int64_t dtype, int64_t ld, int64_t planes, int
         if (a.src == SRC_BF16) rgs_pack8_rows_kernel<1, RGS_BF16><<<grid, NT, 0, st>>>(a, 0);
         else rgs_pack8_rows_kernel<1, RGS_F32><<<grid, NT, 0, st>>>(a, 0);
     }
+    rgs_cuda_field_launches(1);
     return (int)cudaGetLastError();
 }
 
@@ -1095,6 +1104,7 @@ int rgs_cuda_unpack8(const int8_t* codes, const uint8_t* expo, int64_t planes, i
         rgs_unpack8_kernel<4><<<(unsigned)norm_grid((n * c / 4 + NT * 4 - 1) / (NT * 4), 32), NT, 0, st>>>(a, !planes && c % 32 == 0, out, (int)dtype);
     else
         rgs_unpack8_kernel<1><<<(unsigned)norm_grid((n * c + NT * 4 - 1) / (NT * 4), 32), NT, 0, st>>>(a, 0, out, (int)dtype);
+    rgs_cuda_field_launches(1);
     return (int)cudaGetLastError();
 }
 
@@ -1110,6 +1120,7 @@ int rgs_cuda_norm_fwd(const void* x, int64_t dtype, int64_t ld, int64_t planes, 
     if (planes && c > NP_MAX) return 23;
     if (c > NR_MAX) {
         rgs_norm_wide_kernel<<<(unsigned)norm_grid((n + 7) / 8, 16), NT, 0, st>>>(a, 0, nullptr);
+        rgs_cuda_field_launches(1);
         RGS_CUDA_CHECK(cudaGetLastError());
         return codes ? rgs_cuda_pack8(x, dtype, ld, planes, n, c, codes, expo, stream) : 0;
     }
@@ -1145,9 +1156,11 @@ int rgs_cuda_norm_bwd(const void* x, int64_t dtype, int64_t ld, int64_t planes, 
     if (c > NR_MAX) {
         float2* stats = reinterpret_cast<float2*>(static_cast<float*>(scratch) + (int64_t)NORM_PARTS * 2 * c);
         rgs_norm_wide_kernel<<<(unsigned)norm_grid((n + 7) / 8, 16), NT, 0, st>>>(a, 1, stats);
+        rgs_cuda_field_launches(1);
         if (a.part) {
             parts = (int)norm_grid((n + 63) / 64, 1);
             rgs_norm_wide_sums_kernel<<<dim3((unsigned)((c + 31) / 32), (unsigned)parts), NT, 0, st>>>(a, stats);
+            rgs_cuda_field_launches(1);
         }
     } else if (planes) {
         const int rc = norm_planes<true>(a, &parts, st);
@@ -1160,8 +1173,10 @@ int rgs_cuda_norm_bwd(const void* x, int64_t dtype, int64_t ld, int64_t planes, 
         else parts = norm_rows_single(a, true, st);
     }
     RGS_CUDA_CHECK(cudaGetLastError());
-    if (a.part && (parts > 1 || c > NR_MAX))
+    if (a.part && (parts > 1 || c > NR_MAX)) {
         rgs_norm_reduce_kernel<<<dim3((unsigned)((c + 31) / 32), 2), 1024, 0, st>>>(a.part, parts, (int)c, dw, db, (int)p_dtype);
+        rgs_cuda_field_launches(1);
+    }
     return (int)cudaGetLastError();
 }
 

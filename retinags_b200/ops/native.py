@@ -168,7 +168,8 @@ def stream_ptr(device: torch.device):
 # kernels launched by one call of an entry point (the radix sort's count depends on the tile count)
 _KERNELS = {"project_slots": 1, "project_slots2": 2, "project_slots2_geom": 2, "colour_slab": 1, "tile_maps_or": 1, "tile_map_push": 1, "project_emit": 1, "blend_fwd": 1, "blend_bwd": 1, "geom_bwd": 1, "scatter_radii": 1, "adam": 1, "adam_rows": 2,
             "composite_fwd": 1, "composite_bwd": 1, "ssim_fwd": 1, "ssim_bwd": 1, "densify_classify": 2, "blend_fwd_slab": 1, "blend_bwd_slab": 1,
-            "label_fwd": 3, "label_bwd": 3, "norm_fwd": 1, "norm_bwd": 2, "pack8": 1, "unpack8": 1}
+            # these say how many they launch (the dispatch on sizes and layouts is theirs)
+            "label_fwd": 0, "label_bwd": 0, "norm_fwd": 0, "norm_bwd": 0, "pack8": 0, "unpack8": 0}
 _LAUNCHES = [0]
 _SORT_SWEEP = [os.environ.get("RGS_SORT", "") != "3k"]
 
@@ -196,7 +197,7 @@ def cuda_switch(name: str, on: bool) -> bool:
 
 def launch_count() -> int:
     """Number of kernels of the CUDA library launched so far by this process."""
-    return _LAUNCHES[0]
+    return _LAUNCHES[0] + (size_of("field_launches", torch.device("cuda"), 0) if "cuda" in _LIBS else 0)
 
 
 def _count_launches(name: str, args) -> int:

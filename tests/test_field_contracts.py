@@ -373,3 +373,41 @@ def test_cpu_layer_norm_is_linear_in_the_channels():
         return best
     seconds(64, 32)
     assert seconds(512, 1024) < 4 * seconds(16384, 32) + 0.05
+
+
+@pytest.mark.gpu
+def test_launch_count_is_that_of_the_profiler():
+    from torch.profiler import ProfilerActivity, profile
+    gen = torch.Generator().manual_seed(1)
+
+    def label(n, c, v, dtype, wanted, reduction="mean"):
+        t = [p.detach().requires_grad_(k in wanted) for k, p in enumerate(p for p in make_label_case(n, c, v, dtype, device="cuda") if p.dtype != torch.int64)]
+        y = torch.zeros(n, dtype=torch.long, device="cuda")
+        out = R.label_loss(t[0], t[1], y, bias=t[2], reduction=reduction)
+        up = torch.ones_like(out)
+        return lambda: torch.autograd.grad(out, [t[k] for k in wanted], up, retain_graph=True) if wanted else R.label_loss(t[0], t[1], y, bias=t[2])
+
+    def norm(n, c, keep, planes, backward):
+        x = torch.randn(n, c, generator=gen).cuda()
+        leaf = (x.t().contiguous().t() if planes else x).requires_grad_(True)
+        w = torch.ones(c, device="cuda", requires_grad=True)
+        y = R.layer_norm(leaf, w, keep=keep)
+        up = torch.ones_like(y)
+        return (lambda: torch.autograd.grad(y, [leaf, w], up, retain_graph=True)) if backward else (lambda: R.layer_norm(leaf, w, keep=keep))
+
+    packed = R.pack8(torch.randn(50, 40, generator=gen).cuda())
+    steps = [label(300, 64, 100, BF16, ()), label(300, 64, 100, BF16, (0,)), label(300, 64, 100, F32, (1,)), label(40000, 64, 100, F32, (0, 1, 2)),
+             label(40000, 64, 3000, F32, (0, 1, 2)), label(60000, 64, 100, BF16, (0,)), label(300, 64, 100, BF16, (2,), "none"),
+             norm(5, 64, "input", False, True), norm(5000, 64, "input", False, True), norm(500, 33, "int8", False, False),
+             norm(500, 64, "int8", False, False), norm(300, 1500, "int8", False, False), norm(300, 1500, "input", False, True),
+             norm(300, 64, "int8", True, True), lambda: packed.unpack(), lambda: R.pack8(packed.unpack())]
+    for k, step in enumerate(steps):
+        step()
+        torch.cuda.synchronize()
+        with profile(activities=[ProfilerActivity.CUDA]) as prof:
+            before = native.launch_count()
+            step()
+            torch.cuda.synchronize()
+            counted = native.launch_count() - before
+        seen = sum(e.count for e in prof.key_averages() if "rgs_" in e.key)
+        assert counted == seen > 0, (k, counted, seen)
