@@ -411,3 +411,80 @@ def test_launch_count_is_that_of_the_profiler():
             counted = native.launch_count() - before
         seen = sum(e.count for e in prof.key_averages() if "rgs_" in e.key)
         assert counted == seen > 0, (k, counted, seen)
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("keep", ["input", "int8"])
+@pytest.mark.parametrize("device", DEVICES)
+def test_layouts_of_the_norm_and_of_gradients(device, keep, out_dtype):
+    """The output is dense rows whatever the input; the kernels' gradient is dense, as planes where the input is planes (a slice of
+    them too), else as rows.  A leaf's own gradient then follows autograd's rule for leaves."""
+    base = torch.randn(40, 91, generator=torch.Generator().manual_seed(1)).to(device)
+    rows, planes = (24, 1), (1, 30)
+    for view, want in ((base[:30, :24], rows), (base[:30, 5:29], rows), (base[:30, ::3][:, :24], rows), (base[::1, :30].t()[:, 3:27], planes),
+                       (base[:24, 7:37].t(), planes), (base[:24, :30].t().contiguous(), rows), (base[0:1, :24].expand(30, 24), rows)):
+        assert view.shape == (30, 24)
+        seen = []
+        leaf = view.detach().requires_grad_(True)
+        y = R.layer_norm(leaf.view_as(leaf), keep=keep, out_dtype=out_dtype)
+        assert y.is_contiguous() and y.dtype == out_dtype
+        y.grad_fn.register_hook(lambda grads, _: seen.append(grads[0]))
+        (g,) = torch.autograd.grad(y, leaf, torch.ones_like(y))
+        assert seen[0].stride() == want and g.shape == leaf.shape
+        want_y = torch.nn.functional.layer_norm(view.double(), (24,))
+        # half a step of the output's type; a row of 24: 40 roundings of values below 4, times 1/sqrt(var) below 2
+        torch.testing.assert_close(y.double(), want_y, atol=40 * 2.0 ** -24 * 8, rtol=2.0 ** -24 if out_dtype == F32 else 2.0 ** -8)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("device", DEVICES)
+def test_label_field_on_rendered_planes(device, dtype):
+    """Planes as the rasteriser writes them, three channels a render, through norm and loss; gradients reach the splats' features and
+    are those of the plain formulas."""
+    from helpers import activated, small_scene
+    from retinags_b200.ops.rasterize import GaussianRasterizationSettings, GaussianRasterizer
+    from retinags_b200.utils import loss as plain
+    g, cams = small_scene(n=300, width=80, height=48)
+    cam = cams[0]
+    a = {k: v.to(device) for k, v in activated(g).items()}
+    mats = [torch.as_tensor(m).to(device) for m in (cam.world_view_transform, cam.full_proj_transform, cam.view_world_transform, cam.camera_center)]
+    st = GaussianRasterizationSettings(cam.height, cam.width, cam.tan_fovx, cam.tan_fovy, torch.zeros(3, device=device), 1.0, *mats[:3],
+                                       torch.full((3,), -1e9), torch.full((3,), 1e9), 0, mats[3])
+    gen = torch.Generator().manual_seed(3)
+    feats = (torch.rand(300, 4, 1, 3, generator=gen) * 2).to(device).requires_grad_(True)  # twelve channels
+    labels = torch.randint(-1, 7, (48, 80), generator=gen).to(device)
+    gain = torch.ones(12, device=device, requires_grad=True)
+    w = torch.randn(7, 12, generator=gen).to(device).to(dtype).requires_grad_(True)
+    raster, rest = GaussianRasterizer(st), torch.zeros(300, 15, 3, device=device)
+
+    def planes_of(f):
+        return torch.cat([raster(a["xyz"], torch.zeros_like(a["xyz"]), a["opacity"], shs=torch.cat([f[:, k], rest], 1), scales=a["scale"],
+                                 rotations=a["rot"])[0] for k in range(4)])
+
+    planes = planes_of(feats)
+    assert planes.shape == (12, 48, 80) and planes.is_contiguous()
+    # eps is that of features of size one: pixels without a splat keep a small scale
+    for keep in ("input", "int8"):
+        loss = R.label_loss(R.layer_norm(planes.permute(1, 2, 0), gain, eps=1e-2, out_dtype=dtype, keep=keep), w, labels)
+        gp, gg, gw = torch.autograd.grad(loss, [planes, gain, w], retain_graph=True)
+        kept = R.pack8(planes.detach().permute(1, 2, 0)).unpack().double() if keep == "int8" else planes.detach().permute(1, 2, 0).double()
+        p, gd = planes.detach().permute(1, 2, 0).double().requires_grad_(True), gain.detach().double().requires_grad_(True)
+        h = torch.nn.functional.layer_norm(p, (12,), gd, None, 1e-2)
+        hr = h.to(dtype).double()  # what the classifier reads
+        wd = w.detach().double().requires_grad_(True)
+        want = plain.label_loss(hr.detach().requires_grad_(True), wd, labels)
+        hl = hr.detach().requires_grad_(True)
+        gh, gwd = torch.autograd.grad(plain.label_loss(hl, wd, labels), [hl, wd])
+        k = kept.requires_grad_(True)
+        hk = torch.nn.functional.layer_norm(k, (12,), gd, None, 1e-2)
+        gk, ggd = torch.autograd.grad(hk, [k, gd], gh)
+        # 32 bits: some hundred roundings of sums; bf16: G, dh and dW are rounded (three halves of 2^-8), h may round to the other side
+        rel = 2e-5 if dtype == F32 else 4 * 2.0 ** -8
+        assert abs(loss.item() - want.item()) <= rel * want.item()
+        for got, ref in ((gp.permute(1, 2, 0), gk), (gg, ggd), (gw, gwd)):
+            assert (got.double() - ref).norm() <= rel * ref.norm()
+        # a render's backward pass is for one call, so each gradient has a render of its own.  Two renders on the GPU add a splat's
+        # gradient up in another order (some hundred pixels of a sum: 1e-4 is far above that), and h may round to the other side
+        (gf,) = torch.autograd.grad(R.label_loss(R.layer_norm(planes_of(feats).permute(1, 2, 0), gain, eps=1e-2, out_dtype=dtype, keep=keep), w, labels), feats)
+        (ref,) = torch.autograd.grad(planes_of(feats), feats, gp)
+        assert torch.isfinite(gf).all() and gf.abs().max() > 0 and (gf - ref).norm() <= max(rel, 1e-4) * ref.norm()
