@@ -27,12 +27,17 @@
 // products are kept; what is dropped is below 2^-24 of a product.  G is split the same way in registers.
 //
 // What bounds it, per 128 x 128 scores: 1024 clocks for the exponentials (16 per clock and SM) and 4 C clocks for a product,
-// so the exponentials up to about 128 channels (forward; two products backward), the products beyond.  Measured on 148 SMs:
-//   1657600 pixels x 64 channels x 1024 labels, bf16: forward 0.58 ms (1.4 times the exponentials alone), both gradients
-//     1.55 ms (2.1 times); the rest is waiting between the two products and the label terms
-//   66560 x 256 x 32771, bf16: forward 1.1 ms (1.0 PFLOP/s), gradients 3.8 ms (1.2 PFLOP/s of the 4.5 TFLOP done): the first
+// so the exponentials up to about 128 channels (forward; two products backward), the products beyond.  Measured on 148 SMs, whole
+// passes with preparation, joining and reduction (events, L2 flushed):
+//   1657600 pixels x 64 channels x 1024 labels, bf16: forward 0.62 ms (1.7 times the exponentials alone, 0.37 ms), both gradients
+//     1.54 ms (2.1 times); the rest is waiting between the two products and the label terms
+//   66560 x 256 x 32771, bf16: forward 1.09 ms (1.0 PFLOP/s), gradients 3.9 ms (1.1 PFLOP/s of the 4.5 TFLOP done): the first
 //     product reads 128 bytes of operands a clock, all that shared memory gives, while TMA writes the next block there
-//   1657600 x 32 x 512, 32 bits: forward 0.39 ms, gradients 1.4 ms: the split of G in three and six products for one
+//   1657600 x 32 x 512, 32 bits: forward 0.50 ms, gradients 1.47 ms: the split of G in three and six products for one; splitting the
+//     features into pieces is 0.1 ms of each pass
+// Gradients of wide features: an item gives 256 output channels (64 in 32 bits) and forms the scores anew, and beyond 8 chunks of
+// pieces A is fetched with every block of B.  66560 pixels x 4096 labels, a step: bf16 0.72 ms at 256 channels, 2.2 at 512, 9.3 at
+// 1024; 32 bits 0.90 at 64, 2.3 at 128, 7.4 at 256, 25 at 512, 106 at 1024 (products with the scores in memory: 18 and 31 ms).
 //
 // All waits are bounded.  A warp whose wait runs out says so in shared memory (fail) before anything else it does.  From then on
 // barriers may complete for work that is not whole: the MMA warp goes through its motions to the end of its item.  So the

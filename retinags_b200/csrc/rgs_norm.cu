@@ -15,11 +15,12 @@
 // Codes of such rows are read element by element throughout.  Channel planes (the renderer's images) are read with a lane to
 // a pixel and turned into rows in shared memory.  Beyond 1024 channels a warp re-reads its row.
 //
-// Measured (a copy moves 6.5 TB/s): 1657600 rows x 64 channels, float32 in, bf16 out: forward 107 us (5.9 TB/s), with the
-// 8-bit copy 128 us (5.8 TB/s), backward 198 us (5.4 TB/s), from codes 211 us (3.5 TB/s: the arithmetic of decoding shares
-// the time); the same from planes 194 and 309 us (instructions: two thirds of the issue slots, most of them addresses and
-// the sums over warps); 40003 x 771 bf16 46 and 136 us (backward: 255 registers, one block to an SM, a quarter of the issue
-// slots: waiting, although the next row is on its way); packing 92, unpacking 117 us.
+// Measured (a copy moves 6.5 TB/s): 1657600 rows x 64 channels, float32 in, bf16 out: forward 108 us (5.9 TB/s), with the
+// 8-bit copy 127 us (5.8 TB/s), backward 189 us (5.6 TB/s), from codes 206 us (3.6 TB/s: the arithmetic of decoding shares
+// the time); the same from planes 193 and 306 us, in 8 bits 317 and 364 us (instructions: two thirds of the issue slots, most of
+// them addresses and the sums over warps); 40003 x 771 bf16 47 and 134 us (backward: 255 registers, one block to an SM, a quarter
+// of the issue slots: waiting, with no registers left to fetch the next row ahead), in 8 bits, codes one by one, 103 and 439 us;
+// packing 95, unpacking 118 us.  Beyond 1024 channels nothing is kept in registers: 40003 x 2000, a step, 1.0 ms.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -215,7 +216,7 @@ __device__ __forceinline__ void row_stats(const float (&x)[NV][VEC], int l, int 
             const float d = !maybe_out<VEC, NV, LANES, SHIFT>(k) || in_row<VEC, LANES, SHIFT>(k, q, l, s0, c) ? x[k][q] - mu : 0.f;
             s = fmaf(d, d, s);
         }
-    rstd = rsqrtf(group_sum<LANES>(s) * inv_c + eps);  // within two units in the last place
+    rstd = rsqrtf(group_sum<LANES>(s) * inv_c + eps);  // within two units in the last place (the kernel of wide rows: root and quotient)
 }
 
 template <int VEC>

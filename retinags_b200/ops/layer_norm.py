@@ -2,8 +2,9 @@
 
 Blended features are weighted sums over the splats of a pixel, so their size follows the pixel's coverage; the norm
 takes that out ahead of a classifier (``ops.label_loss``).  The input may be rows (..., C) or, as the renderer writes an
-image, channel planes (``image.permute(1, 2, 0)`` of a (C,H,W) image), both read where they lie; the output is dense
-rows in ``out_dtype``.  Sums are held in 32 bits whatever the types.
+image, channel planes (``image.permute(1, 2, 0)`` of a (C,H,W) image), both read where they lie (planes of more than 512
+channels, and any other layout, are copied into rows); the output is dense rows in ``out_dtype``.  Sums are held in 32 bits
+whatever the types.
 """
 from __future__ import annotations
 
@@ -91,7 +92,10 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     ``x`` and ``out_dtype`` (default: that of ``x``) are float32 or bfloat16; ``weight`` and ``bias`` (C) are of one of
     these types, both of the same.  ``keep`` says what waits for the backward pass: ``"input"`` the tensor itself,
     ``"int8"`` its 8-bit form (``ops.pack8``); the gradients are then those of the norm at the restored values, and the
-    input's memory is free as soon as nothing else holds it.
+    input's memory is free as soon as nothing else holds it.  A step of the codes is 1/254 to 1/127 of the largest magnitude
+    among 32 channels, so the gradients suffer where channels differ little beside their size: with 64 channels of spread 0.1
+    the gradient of ``x`` is off by 0.2 % (in norm) around 0, by 1 % around 1, 4 % around 5 and 18 % around 20, that of
+    ``weight`` by about four times as much.
     """
     dtype_code(x, "layer_norm")
     out_dtype = x.dtype if out_dtype is None else out_dtype

@@ -137,7 +137,9 @@ def alloc_codes(shape, planes: int, device):
 
 
 def pack8(x: torch.Tensor) -> Packed8:
-    """Pack a float32 or bfloat16 tensor (..., C); rows or channel planes are read where they lie."""
+    """Pack a float32 or bfloat16 tensor (..., C); rows or channel planes are read where they lie.
+
+    A form to keep values in: no gradient passes through it (``pack8(x).unpack()`` is detached from ``x``)."""
     code = dtype_code(x, "pack8")
     flat, ld, planes = as_rows(x.detach(), "pack8")
     codes, exponents = alloc_codes(x.shape, planes, x.device)
