@@ -30,10 +30,10 @@
 // so the exponentials up to about 128 channels (forward; two products backward), the products beyond.  Measured on 148 SMs, whole
 // passes with preparation, joining and reduction (events, L2 flushed):
 //   1657600 pixels x 64 channels x 1024 labels, bf16: forward 0.62 ms (1.7 times the exponentials alone, 0.37 ms), both gradients
-//     1.54 ms (2.1 times); the rest is waiting between the two products and the label terms
-//   66560 x 256 x 32771, bf16: forward 1.09 ms (1.0 PFLOP/s), gradients 3.9 ms (1.1 PFLOP/s of the 4.5 TFLOP done): the first
+//     1.53 ms (2.1 times); the rest is waiting between the two products and the label terms
+//   66560 x 256 x 32771, bf16: forward 1.02 ms (1.1 PFLOP/s), gradients 3.9 ms (1.1 PFLOP/s of the 4.5 TFLOP done): the first
 //     product reads 128 bytes of operands a clock, all that shared memory gives, while TMA writes the next block there
-//   1657600 x 32 x 512, 32 bits: forward 0.50 ms, gradients 1.47 ms: the split of G in three and six products for one; splitting the
+//   1657600 x 32 x 512, 32 bits: forward 0.50 ms, gradients 1.41 ms: the split of G in three and six products for one; splitting the
 //     features into pieces is 0.1 ms of each pass
 // Gradients of wide features: an item gives 256 output channels (64 in 32 bits) and forms the scores anew, and beyond 8 chunks of
 // pieces A is fetched with every block of B.  66560 pixels x 4096 labels, a step: bf16 0.72 ms at 256 channels, 2.2 at 512, 9.3 at
@@ -119,10 +119,18 @@ __device__ __forceinline__ bool lb_wait_warp(unsigned long long* bar, uint32_t p
     return __all_sync(0xffffffffu, lb_wait(bar, parity, fail, limit));
 }
 // The MMA warp's.  It goes on either way: every answer that its loop looks at costs (votes 3 % of a pass, a lane that gives up
-// issuing 20 to 50 %).
+// issuing 20 to 50 %), and so does anything between a try that succeeds and the return (codebook forward 1033 -> 1093 us).
 __device__ __noinline__ void lb_wait_slow(unsigned long long* bar, uint32_t parity, volatile int* fail, uint32_t limit) {
-    if (*fail) __threadfence_block();
-    else lb_wait(bar, parity, fail, limit);
+    if (*fail) {
+        __threadfence_block();
+        return;
+    }
+    for (uint32_t it = 0; it < limit; ++it) {
+        if (lb_try(bar, parity)) return;
+        if ((it & 15u) == 15u && *fail) return;
+    }
+    *fail = 1;
+    __threadfence_block();  // seen before what this warp issues next
 }
 __device__ __forceinline__ void lb_wait_quiet(unsigned long long* bar, uint32_t parity, volatile int* fail, uint32_t limit) {
     if (!lb_try(bar, parity)) lb_wait_slow(bar, parity, fail, limit);
@@ -212,6 +220,7 @@ __device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 
 struct LabelItem { int dw, m, oc0, noc, split, j0, j1; };
 
 // single threads run this between products: no division where there is nothing to divide
+template <bool GRAD>
 __device__ __forceinline__ LabelItem lb_item(const LabelArgs& a, unsigned i) {
     LabelItem it;
     it.dw = i >= a.items_x;
@@ -225,7 +234,7 @@ __device__ __forceinline__ LabelItem lb_item(const LabelArgs& a, unsigned i) {
     it.oc0 = (int)range * a.noc;
     it.noc = min(a.noc, a.nk - it.oc0);
     it.split = (int)q;
-    q = q * (unsigned)(it.dw ? a.subw : a.subx) + (unsigned)a.sub;  // its piece
+    if (GRAD) q = q * (unsigned)(it.dw ? a.subw : a.subx) + (unsigned)a.sub;  // its piece
     it.j0 = (int)(q * base + min(q, rest));  // the first `rest` pieces are one tile longer
     it.j1 = it.j0 + (int)base + (q < rest);
     return it;
@@ -362,7 +371,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
             for (int oc = 0; oc < prev_noc && ok; oc += CS) load(prev_dw ? &map_x : &map_w, (prev_oc0 + oc) / CS, prev_j, nullptr);
         };
         for (unsigned i = blockIdx.x; i < items && ok; i += gridDim.x) {
-            const LabelItem it = lb_item(a, i);
+            const LabelItem it = lb_item<GRAD>(a, i);
             const CUtensorMap *ma = it.dw ? &map_w : &map_x, *mb = it.dw ? &map_x : &map_w;
             // (forward: the pixels' extra channels are the same for all, one tile of them)
             ok = lb_wait_warp(&sh->ea_empty[eac.slot], eac.phase ^ 1, fail, a.wait);
@@ -546,12 +555,12 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         unsigned si = blockIdx.x, oi = blockIdx.x;
         LabelItem is, io;
         int sj = 0, oj = 0;
-        if (si < items) { is = io = lb_item(a, si); sj = oj = is.j0; }
+        if (si < items) { is = io = lb_item<GRAD>(a, si); sj = oj = is.j0; }
         auto step_s = [&]() {
             issue_s(is, sj);
             if (++sj == is.j1) {
                 si += gridDim.x;
-                if (si < items) { is = lb_item(a, si); sj = is.j0; }
+                if (si < items) { is = lb_item<GRAD>(a, si); sj = is.j0; }
             }
         };
         auto failed = [&]() { return __any_sync(0xffffffffu, *fail); };
@@ -564,7 +573,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                 if (++oj == io.j1) {
                     if (failed()) break;
                     oi += gridDim.x;
-                    if (oi < items) { io = lb_item(a, oi); oj = io.j0; }
+                    if (oi < items) { io = lb_item<GRAD>(a, oi); oj = io.j0; }
                 }
             }
         } else {
@@ -596,7 +605,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         // what a row of A brings to an item, fetched an item ahead: from memory at its start it would cost as much as a score tile
         auto row_label = [&](unsigned i) -> int {
             if (i >= items) return -1;
-            const LabelItem it = lb_item(a, i);
+            const LabelItem it = lb_item<GRAD>(a, i);
             if (it.dw) return 0;
             if (GRAD) return __float_as_int(a.kn[(size_t)it.m * (3 * LT) + row]);
             const int64_t r = (int64_t)it.m * LT + row;
@@ -604,11 +613,11 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         };
         auto row_scale = [&](unsigned i) -> float {
             if (!GRAD || i >= items) return 1.f;
-            const LabelItem it = lb_item(a, i);
+            const LabelItem it = lb_item<GRAD>(a, i);
             return it.dw ? gshare : a.kn[(size_t)it.m * (3 * LT) + LT + row];
         };
         auto write_out = [&](unsigned i, float scale, int label) {
-            const LabelItem it = lb_item(a, i);
+            const LabelItem it = lb_item<GRAD>(a, i);
             if (!dead) dead = __any_sync(0xffffffffu, !lb_wait(&sh->o_full[oc_.slot], oc_.phase, fail, a.wait));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t o = tmem + lanes + OUT + oc_.slot * OB;
@@ -656,7 +665,7 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
         int next_label = row_label(blockIdx.x), out_label = 0;
         float next_scale = row_scale(blockIdx.x), out_scale = 1.f;  // out_: of the first item whose output is not written
         for (unsigned i = blockIdx.x; i < items; i += gridDim.x) {
-            const LabelItem it = lb_item(a, i);
+            const LabelItem it = lb_item<GRAD>(a, i);
             const int64_t r = (int64_t)it.m * LT + row;
             const int label = next_label;
             const float scale = next_scale;
