@@ -488,3 +488,27 @@ def test_label_field_on_rendered_planes(device, dtype):
         (gf,) = torch.autograd.grad(R.label_loss(R.layer_norm(planes_of(feats).permute(1, 2, 0), gain, eps=1e-2, out_dtype=dtype, keep=keep), w, labels), feats)
         (ref,) = torch.autograd.grad(planes_of(feats), feats, gp)
         assert torch.isfinite(gf).all() and gf.abs().max() > 0 and (gf - ref).norm() <= max(rel, 1e-4) * ref.norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("c", [8, 33, 64, 100, 200, 300, 700])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_label_loss_large_scores_at_every_width(c, dtype, reduction):
+    """Scores of thousands beside ordinary ones, pixels without a label among them, one with infinite features: how A and B are
+    staged hangs on the width, and m comes off in registers in each of these forms."""
+    x, w, y, b = make_label_case(270, c, 333, F32, seed=c, device="cuda")
+    x[:90] *= 1500.0
+    x, w, b = x.to(dtype), w.to(dtype), b.to(dtype)
+    free = int((y < 0).nonzero()[0])
+    count = int((y >= 0).sum())
+    up = torch.rand(270, generator=torch.Generator().manual_seed(1)).cuda() + 0.5 if reduction == "none" else torch.full((270,), 1.0 / count, device="cuda")
+    ref = label_reference(x, w, y, b, up, dtype)
+    x[free, c // 2] = float("inf")
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    out = R.label_loss(leaves[0], leaves[1], y, bias=leaves[2], reduction=reduction)
+    if reduction == "none":
+        assert_within(out.detach(), ref[0], "losses")
+    grads = torch.autograd.grad(out, leaves, up if reduction == "none" else None)
+    for name, got, r in zip(("dX", "dW", "db"), grads, ref[1:]):
+        assert_within(got, r, name)
