@@ -512,3 +512,34 @@ def test_label_loss_large_scores_at_every_width(c, dtype, reduction):
     grads = torch.autograd.grad(out, leaves, up if reduction == "none" else None)
     for name, got, r in zip(("dX", "dW", "db"), grads, ref[1:]):
         assert_within(got, r, name)
+
+
+def test_no_gradient_passes_through_the_8_bit_form():
+    x = torch.randn(5, 40, requires_grad=True)
+    assert not R.pack8(x).unpack().requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("planes", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_layer_norm_in_8_bits_at_every_width(dtype, planes):
+    """The kept codes are those of the 8-bit form at every number of channels (lanes, vectors and blocks of 32 follow from it), and
+    the gradients are those of the norm at their values."""
+    from field_reference import norm_reference
+    gen = torch.Generator().manual_seed(5)
+    x, dy = torch.randn(37, 1100, generator=gen).to(dtype), torch.randn(37, 1100, generator=gen).cuda()
+    w, b = (torch.rand(1100, generator=gen) + 0.5).cuda(), torch.randn(1100, generator=gen).cuda()
+    widths = list(range(1, 140)) + list(range(140, 530, 13)) + [511, 512, 513, 544, 575, 576, 640, 771, 772, 1000, 1018, 1019, 1023, 1024, 1025, 1056, 1100]
+    for c in widths:
+        part = x[:, :c].contiguous()
+        host = R.pack8(part)
+        leaf = part.cuda()
+        leaf = (leaf.t().contiguous().t() if planes else leaf).requires_grad_(True)
+        leaves = [leaf, w[:c].clone().requires_grad_(True), b[:c].clone().requires_grad_(True)]
+        up = dy[:, :c].contiguous()
+        y = R.layer_norm(*leaves, keep="int8", out_dtype=F32)
+        codes, exponents = (t for t in y.grad_fn.saved_tensors if t is not None and t.dtype in (torch.int8, torch.uint8))
+        assert torch.equal(codes.cpu(), host.codes) and torch.equal(exponents.cpu(), host.exponents), c
+        ref = norm_reference(part.cuda(), leaves[1].detach(), leaves[2].detach(), up, 1e-5, host.unpack(F32).cuda(), F32, dtype, F32)
+        for name, got, r in zip(("y", "dx", "dw", "db"), (y.detach(), *torch.autograd.grad(y, leaves, up)), ref):
+            assert_within(got, r, f"{name} of {c} channels")
