@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import native
-from .pack8 import DTYPES, as_rows, dtype_code, restored, saved_as
+from .pack8 import DTYPES, as_rows, dtype_code, restored
 
 MAX_CHANNELS = 1024
 _REDUCTIONS = ("mean", "sum", "none")
@@ -49,7 +49,7 @@ class _LabelLoss(torch.autograd.Function):
             native.call("label_fwd", dev, x, ldx, w, ldw, bias, y, y.element_size(), n, c, v, DTYPES[x.dtype], b_code,
                         int(reduction == "mean"), scratch, scratch.numel(), lse, losses, result, lse + 8 * n)
         ctx.save_for_backward(x, w, bias, y, state)
-        ctx.args = (features.shape, weight.shape, saved_as(x, w, bias, y, state), b_code, reduction)
+        ctx.args = (features.shape, n, c, v, features.dtype, bias.dtype if bias is not None else None, y.dtype, dev, b_code, reduction)
         return losses.view(features.shape[:-1]) if per_row else result
 
     @staticmethod
@@ -58,19 +58,24 @@ class _LabelLoss(torch.autograd.Function):
         return _label_backward_once(ctx, gout) if torch.is_grad_enabled() else _label_backward(ctx, gout)
 
 
+def _saved_rows(t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device):
+    restored(t, shape, dtype, device, "label_loss")
+    return (t, shape[1]) if t.is_contiguous() else as_rows(t, "label_loss", planes_ok=False)[:2]
+
+
 def _label_backward(ctx, gout):
-    x_shape, w_shape, kinds, b_code, reduction = ctx.args
-    x, w, bias, y, state = restored(ctx.saved_tensors, kinds, "label_loss")
-    x, ldx, _ = as_rows(x, "label_loss", planes_ok=False)
-    w, ldw, _ = as_rows(w, "label_loss", planes_ok=False)
-    bias, y, state = bias.contiguous() if bias is not None else None, y.contiguous(), state.contiguous()
-    dev = x.device
-    n, c = x.shape
-    v = w.shape[0]
+    x_shape, n, c, v, dtype, b_dtype, y_dtype, dev, b_code, reduction = ctx.args
+    x, w, bias, y, state = ctx.saved_tensors
+    x, ldx = _saved_rows(x, (n, c), dtype, dev)
+    w, ldw = _saved_rows(w, (v, c), dtype, dev)
+    y = restored(y, (n,), y_dtype, dev, "label_loss").contiguous()
+    state = restored(state, (2 * n + 2,), torch.float32, dev, "label_loss").contiguous()
+    if b_dtype is not None:
+        bias = restored(bias, (v,), b_dtype, dev, "label_loss").contiguous()
     g = gout if gout.dim() < 2 and gout.is_contiguous() else gout.reshape(-1).contiguous()
     new = torch.empty if n else torch.zeros
     dx = torch.empty(x_shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
-    dw = new(w_shape, dtype=w.dtype, device=dev) if ctx.needs_input_grad[1] else None
+    dw = new((v, c), dtype=w.dtype, device=dev) if ctx.needs_input_grad[1] else None
     db = new(v, dtype=bias.dtype, device=dev) if ctx.needs_input_grad[2] else None
     if n and (dx is not None or dw is not None or db is not None):
         scratch = _scratch(x, ldx, w, ldw, 1 + 2 * (dx is not None) + 4 * (dw is not None) + 8 * (db is not None))

@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import native
-from .pack8 import DTYPES, alloc_codes, as_rows, dense, dtype_code, empty_like_layout, restored, saved_as
+from .pack8 import BLOCK, DTYPES, alloc_codes, as_rows, dense, dtype_code, empty_like_layout, restored
 
 MAX_PLANES = 512  # channels up to which planes are read and written where they lie; more are copied into rows and back
 
@@ -20,21 +20,14 @@ def _scratch(device: torch.device, n: int, c: int) -> torch.Tensor:
     return torch.empty(native.size_of("norm_scratch_bytes", device, n, c), dtype=torch.uint8, device=device)
 
 
-def _rows_or_planes(x: torch.Tensor):
-    """(tensor (N,C), leading stride, planes) that the kernels read."""
-    flat, ld, planes = as_rows(x, "layer_norm")
-    if planes and flat.shape[1] > MAX_PLANES:
-        return flat.contiguous(), flat.shape[1], 0
-    return flat, ld, planes
-
-
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, out_dtype, keep):
         flat, ld, planes = as_rows(x, "layer_norm")
         n, c = flat.shape
         out_planes = planes
-        flat, ld, planes = _rows_or_planes(flat)
+        if planes and c > MAX_PLANES:
+            flat, ld, planes = flat.contiguous(), c, 0
         dev = x.device
         y = torch.empty(x.shape, dtype=out_dtype, device=dev)
         p_code = DTYPES[weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32]
@@ -45,9 +38,8 @@ class _LayerNorm(torch.autograd.Function):
         if n:
             native.call("norm_fwd", dev, flat, DTYPES[x.dtype], ld, planes, weight, bias, p_code, n, c, eps, y, DTYPES[out_dtype],
                         codes, exponents)
-        kept = (flat if codes is None else None, codes, exponents, weight)
-        ctx.save_for_backward(*kept)
-        ctx.layout = (saved_as(*kept), x.shape, x.dtype, planes, out_planes, n, c, p_code, eps, weight.dtype if weight is not None else None,
+        ctx.save_for_backward(flat if codes is None else None, codes, exponents, weight)
+        ctx.layout = (codes is not None, x.shape, x.dtype, planes, out_planes, n, c, p_code, eps, weight.dtype if weight is not None else None,
                       bias.dtype if bias is not None else None)
         return y
 
@@ -58,17 +50,21 @@ class _LayerNorm(torch.autograd.Function):
 
 
 def _norm_backward(ctx, dy):
-    kinds, shape, x_dtype, planes, out_planes, n, c, p_code, eps, w_dtype, b_dtype = ctx.layout
-    flat, codes, exponents, weight = restored(ctx.saved_tensors, kinds, "layer_norm")
-    ld = c
-    if codes is None:
-        flat, ld, planes = _rows_or_planes(flat)
+    coded, shape, x_dtype, planes, out_planes, n, c, p_code, eps, w_dtype, b_dtype = ctx.layout
+    flat, codes, exponents, weight = ctx.saved_tensors
+    dev, ld = dy.device, c
+    if coded:
+        codes = dense(restored(codes, shape, torch.int8, dev, "layer_norm"), planes)
+        exponents = dense(restored(exponents, (*shape[:-1], (c + BLOCK - 1) // BLOCK), torch.uint8, dev, "layer_norm"), planes)
+    elif restored(flat, (n, c), x_dtype, dev, "layer_norm").is_contiguous():
+        planes = 0
     else:
-        codes, exponents = dense(codes, planes), dense(exponents, planes)
-    if weight is not None:
-        weight = weight.contiguous()
+        flat, ld, planes = as_rows(flat, "layer_norm")
+        if planes and c > MAX_PLANES:
+            flat, ld, planes = flat.contiguous(), c, 0
+    if w_dtype is not None:
+        weight = restored(weight, (c,), w_dtype, dev, "layer_norm").contiguous()
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
-    dev = dy.device
     dyf, ldy, _ = as_rows(dy, "layer_norm", planes_ok=False)
     dx = empty_like_layout(shape, planes, x_dtype, dev) if need_x else None
     new = torch.empty if n else torch.zeros

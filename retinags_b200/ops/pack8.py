@@ -59,19 +59,13 @@ def as_rows(x: torch.Tensor, what: str, planes_ok: bool = True):
     return flat.contiguous(), c, 0
 
 
-def saved_as(*tensors):
-    """What ``restored`` asks of tensors kept for a backward pass."""
-    return tuple(None if t is None else (t.shape, t.dtype, t.device) for t in tensors)
-
-
-def restored(tensors, kinds, what: str):
-    """Tensors as autograd gives them back.  Saved-tensor hooks (offloading, compression) may restore them with other strides, so
-    nothing about their layout is kept across the passes; another shape, type or device is refused."""
-    for t, kind in zip(tensors, kinds):
-        if kind is not None and (t is None or (t.shape, t.dtype, t.device) != kind):
-            got = "nothing" if t is None else f"{t.dtype} of shape {tuple(t.shape)} on {t.device}"
-            raise RuntimeError(f"{what}: a saved tensor came back as {got}, {kind[1]} of shape {tuple(kind[0])} on {kind[2]} expected")
-    return tensors
+def restored(t, shape, dtype: torch.dtype, device: torch.device, what: str) -> torch.Tensor:
+    """A saved tensor as autograd gives it back.  Saved-tensor hooks (offloading, compression) may restore it with other strides, so
+    nothing about its layout is kept across the passes; another shape, type or device is refused."""
+    if t is None or t.shape != shape or t.dtype is not dtype or t.device != device:
+        got = "nothing" if t is None else f"{t.dtype} of shape {tuple(t.shape)} on {t.device}"
+        raise RuntimeError(f"{what}: a saved tensor came back as {got}, {dtype} of shape {tuple(shape)} on {device} expected")
+    return t
 
 
 def empty_like_layout(shape, planes: int, dtype, device) -> torch.Tensor:
