@@ -750,17 +750,16 @@ __global__ void __launch_bounds__(LTHREADS, 1) rgs_label_tc_kernel(const __grid_
                     __syncwarp();
                     tm_ld32(s + h, u);
                     tm_wait_ld32(u);
-                    if (RARE && large) {  // m of the row, or of the 32 pixels of the columns (none: -infinity stays)
-                        if (it.dw) {
-                            const int lab = reinterpret_cast<const int*>(kb)[h + lane];
-                            row_m = lab >= 0 ? a.lse[(int64_t)j * LT + half + h + lane] : 0.f;
-                        }
-#pragma unroll
-                        for (int q = 0; q < 32; ++q) u[q] = __float_as_uint(__uint_as_float(u[q]) - (it.dw ? __shfl_sync(0xffffffffu, row_m, q) : row_m));
+                    if (RARE && large && it.dw) {  // m of the pixels of the columns; of a row: above (no label: -infinity stays)
+                        const int lab = reinterpret_cast<const int*>(kb)[h + lane];
+                        row_m = lab >= 0 ? a.lse[(int64_t)j * LT + half + h + lane] : 0.f;
                     }
 #pragma unroll
                     for (int o = 0; o < 32; o += 16) {  // 16 columns: one step of the product's inner dimension
                         float e[16];
+                        if (RARE && large)  // (all 32 at once cost registers: codebook gradients 3.79 -> 3.95 ms, though never run there)
+#pragma unroll
+                            for (int q = 0; q < 16; ++q) u[o + q] = __float_as_uint(__uint_as_float(u[o + q]) - __shfl_sync(0xffffffffu, row_m, it.dw ? o + q : lane));
 #pragma unroll
                         for (int q = 0; q < 16; q += 2) {
                             un2(mul2(mk2u(u[o + q], u[o + q + 1]), log2e), e[q], e[q + 1]);
