@@ -31,7 +31,7 @@
 // passes with preparation, joining and reduction (events, L2 flushed):
 //   1657600 pixels x 64 channels x 1024 labels, bf16: forward 0.62 ms (1.7 times the exponentials alone, 0.37 ms), both gradients
 //     1.53 ms (2.1 times); the rest is waiting between the two products and the label terms
-//   66560 x 256 x 32771, bf16: forward 1.02 ms (1.1 PFLOP/s), gradients 3.9 ms (1.1 PFLOP/s of the 4.5 TFLOP done): the first
+//   66560 x 256 x 32771, bf16: forward 1.02 ms (1.1 PFLOP/s), gradients 3.8 ms (1.2 PFLOP/s of the 4.5 TFLOP done): the first
 //     product reads 128 bytes of operands a clock, all that shared memory gives, while TMA writes the next block there
 //   1657600 x 32 x 512, 32 bits: forward 0.50 ms, gradients 1.41 ms: the split of G in three and six products for one; splitting the
 //     features into pieces is 0.1 ms of each pass
