@@ -36,8 +36,8 @@
 //   1657600 x 32 x 512, 32 bits: forward 0.50 ms, gradients 1.41 ms: the split of G in three and six products for one; splitting the
 //     features into pieces is 0.1 ms of each pass
 // Gradients of wide features: an item gives 256 output channels (64 in 32 bits) and forms the scores anew, and beyond 8 chunks of
-// pieces A is fetched with every block of B.  66560 pixels x 4096 labels, a step: bf16 0.72 ms at 256 channels, 2.2 at 512, 9.3 at
-// 1024; 32 bits 0.90 at 64, 2.3 at 128, 7.4 at 256, 25 at 512, 106 at 1024 (products with the scores in memory: 18 and 31 ms).
+// pieces A is fetched with every block of B.  66560 pixels x 4096 labels, a step: bf16 0.69 ms at 256 channels, 2.1 at 512, 9.3 at
+// 1024; 32 bits 0.86 at 64, 2.2 at 128, 7.4 at 256, 26 at 512, 108 at 1024 (products with the scores in memory: 18 and 31 ms).
 //
 // All waits are bounded.  A warp whose wait runs out says so in shared memory (fail) before anything else it does.  From then on
 // barriers may complete for work that is not whole: the MMA warp goes through its motions to the end of its item.  So the

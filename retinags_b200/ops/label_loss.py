@@ -105,7 +105,7 @@ def label_loss(features: torch.Tensor, weight: torch.Tensor, labels: torch.Tenso
 
     Features are read as rows; planes (``image.permute(1, 2, 0)``) are copied into rows first.  Gradients form the scores anew
     for every 256 channels in bfloat16 and every 64 in float32, so wide features cost more than their width: 66560 pixels x
-    4096 labels take 0.39, 0.72, 2.2 and 9.3 ms a step at 64, 256, 512 and 1024 bfloat16 channels, and 0.9, 7.4, 25 and 106 ms in
+    4096 labels take 0.38, 0.69, 2.1 and 9.3 ms a step at 64, 256, 512 and 1024 bfloat16 channels, and 0.9, 7.4, 26 and 108 ms in
     float32 (where the scores fit, two products with them in memory are faster above 256 channels: 18 and 31 ms).
     Workspace beside the results: a copy of features or weight that do not start on 16 bytes (float32: 6 bytes a channel of
     each), some 50 bytes a pixel and a label, and for gradients partial sums in 32 bits, up to 2 GiB and one result each for features
