@@ -327,8 +327,8 @@ def test_label_loss_takes_room_for_the_gradients_asked_for(dtype, monkeypatch):
     for wanted, grads in out.items():
         assert all(torch.equal(g, out[(0, 1, 2)][k]) for k, g in grads.items())
     assert used[(0,)] < used[(0, 2)] < used[(0, 1, 2)] and used[(2,)] < used[(1, 2)] < used[(0, 1, 2)]
-    parts_w = used[(1, 2)] - used[(2,)]  # pieces of dW, rows of 128 labels
-    assert parts_w >= 3072 * 64 * 4 and used[(0, 1, 2)] - used[(0, 2)] == parts_w
+    parts_w = used[(1, 2)] - used[(2,)]  # pieces of dW, 24 tiles of 128 labels each
+    assert parts_w >= 24 * 128 * 64 * 4 and used[(0, 1, 2)] - used[(0, 2)] == parts_w
 
 
 @pytest.mark.gpu
